@@ -1,0 +1,159 @@
+/*
+ * symmetrix_node_ops.h -- C ABI of the node operators (libsymmetrix_mi355x.so):
+ * what a learned block over an evaluator's atoms is made of, forward and
+ * backward, for training it and for serving it.  The reference has no
+ * counterpart.
+ *
+ *   species embedding     out[t] = scale * table[types[t]], and its gradient
+ *   residual norm         y = x + a * sigmoid(g) * post * d / rms(d),
+ *                         h = next * y / rms(y), and their gradients
+ *   8-bit block product   y = x W^T with E4M3 operands, a scale for each block of
+ *                         128 values along the summed axis
+ *
+ * Conventions are those of symmetrix_mi355x.h (0 or a negative SMX_ERR_* code, no
+ * exceptions, smx_last_error() for the message), with these:
+ *   - every pointer is a device pointer; every call enqueues on `stream` (a
+ *     hipStream_t; NULL: the default stream) of the current device, keeps no
+ *     argument and does not wait, so a call may be captured into a HIP graph;
+ *   - nothing is allocated: a call that needs room between its kernels takes a
+ *     workspace of the size its _workspace function gives (16-byte aligned, the
+ *     caller's again when the enqueued work is done);
+ *   - row arrays are [rows][channels] with unit stride along the channels and
+ *     any stride >= channels (in elements) between rows; outputs must not
+ *     overlap inputs unless the comment says so;
+ *   - values are SMX_DTYPE_* (one type for all row arrays of a call); sums, norms and
+ *     products are held in FP32 and rounded once, to nearest even, when they are
+ *     stored;
+ *   - results do not depend on the order in which workgroups run.
+ */
+#ifndef SYMMETRIX_NODE_OPS_H
+#define SYMMETRIX_NODE_OPS_H
+
+#include <stdint.h>
+
+#include "symmetrix_mi355x.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+enum { SMX_DTYPE_F32 = 0, SMX_DTYPE_BF16 = 1, SMX_DTYPE_F16 = 2 };
+
+/* ---- species embedding ---- */
+
+/* out[t][c] = scale * table[types[t]][c].  A type outside [0, num_types) is no
+ * species (a masked or padding atom): its row is zero.  types: int32, or int64 when
+ * types_are_64bit.  tokens < 2^31. */
+SMX_API int32_t smx_embed(const void* types, int32_t types_are_64bit, int64_t tokens, const void* table,
+                          int64_t table_stride, int64_t num_types, int64_t channels, int32_t dtype, float scale,
+                          void* out, int64_t out_stride, void* stream);
+/* out[v][c] = scale * sum over the t with types[t] == v of grad[t][c], every row
+ * of out written (zeros for a type without atoms).  The atoms are sorted by type
+ * (stably) and each type's rows summed in a fixed order. */
+SMX_API int64_t smx_embed_gradient_workspace(int64_t tokens, int64_t num_types, int64_t channels);
+SMX_API int32_t smx_embed_gradient(const void* types, int32_t types_are_64bit, int64_t tokens, const void* grad,
+                                   int64_t grad_stride, int64_t num_types, int64_t channels, int32_t dtype,
+                                   float scale, void* out, int64_t out_stride, void* workspace,
+                                   int64_t workspace_bytes, void* stream);
+
+/* ---- residual norm ---- */
+
+/* How the gate logits are given: not at all (a gate of one), one for each
+ * value ([rows][channels], gate_stride between rows), for each channel
+ * ([channels]), or for each row ([rows], gate_stride between them). */
+enum { SMX_GATE_NONE = 0, SMX_GATE_FULL = 1, SMX_GATE_CHANNEL = 2, SMX_GATE_ROW = 3 };
+
+/* y = x + scale * sigmoid(gate) * post * d * r1,  r1 = 1 / sqrt(mean(d^2) + eps)
+ * h = next * y * r2,                              r2 = 1 / sqrt(mean(y^2) + eps)
+ * (means over a row's channels; h is formed from y before it is rounded).
+ * post, scale and next are FP32 [channels].  d NULL: y = x, and post, gate and
+ * scale are not read.  scale NULL: ones.  y NULL: not written.  next NULL: no h.
+ * y may be x.  With h_scales, h is written as 8-bit blocks (below) instead of
+ * `dtype`: h the values [rows][smx_block_stride(channels)] and h_scales
+ * [rows][smx_block_scale_stride(channels)].  channels <= 16384. */
+typedef struct SmxResidualNormArgs {
+    uint32_t struct_size;
+    int32_t dtype;
+    int64_t rows;
+    int64_t channels;
+    const void* x;
+    int64_t x_stride;
+    const void* d;
+    int64_t d_stride;
+    const void* gate;
+    int64_t gate_stride;
+    int32_t gate_kind;
+    float eps;
+    const float* post;
+    const float* scale;
+    const float* next;
+    void* y;
+    int64_t y_stride;
+    void* h;
+    int64_t h_stride; /* ignored with h_scales */
+    uint8_t* h_scales;
+} SmxResidualNormArgs;
+SMX_API int32_t smx_residual_norm(const SmxResidualNormArgs* args, void* stream);
+
+/* The gradients with respect to every input, from the inputs alone (nothing
+ * of the forward call is kept): of a loss whose gradients with respect to y and h
+ * are grad_y (NULL: zero) and grad_h (NULL: zero; needs next).  Each output may be NULL
+ * (not formed).  dx, dd and a full or row gate's dgate are `dtype`; a channel gate's
+ * dgate, dpost, dscale and dnext are FP32 [channels], summed over the rows in a fixed
+ * order.  dx may be grad_y. */
+typedef struct SmxResidualNormGradientArgs {
+    SmxResidualNormArgs forward; /* y, h and h_scales are not used */
+    const void* grad_y;
+    int64_t grad_y_stride;
+    const void* grad_h;
+    int64_t grad_h_stride;
+    void* dx;
+    int64_t dx_stride;
+    void* dd;
+    int64_t dd_stride;
+    void* dgate;
+    int64_t dgate_stride;
+    float* dpost;
+    float* dscale;
+    float* dnext;
+    void* workspace;
+    int64_t workspace_bytes;
+} SmxResidualNormGradientArgs;
+SMX_API int64_t smx_residual_norm_gradient_workspace(int64_t rows, int64_t channels);
+SMX_API int32_t smx_residual_norm_gradient(const SmxResidualNormGradientArgs* args, void* stream);
+
+/* ---- 8-bit block product ---- */
+
+/* A matrix [rows][cols] in 8-bit blocks: E4M3 values [rows][smx_block_stride(cols)]
+ * (cols rounded up to 128, the rest zeros) and one E8M0 scale byte b, the scale
+ * 2^(b-127), for each block of 128 values of a row: [rows][smx_block_scale_stride(cols)]
+ * (the number of blocks rounded up to 4, the rest zeros).  A block's scale is the
+ * least power of two >= 2^-127 that brings its largest finite magnitude to 448 or less; values
+ * round to nearest even; an infinity or NaN is stored as NaN.  Both arrays must be
+ * 16-byte aligned. */
+SMX_API int64_t smx_block_stride(int64_t cols);
+SMX_API int64_t smx_block_scale_stride(int64_t cols);
+/* x [rows][cols] in blocks along its rows (values, scales) and/or the blocks of
+ * its transpose, [cols][rows] in blocks along the rows of x (values_t, scales_t);
+ * either pair may be NULL. */
+SMX_API int32_t smx_block_quantize(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int64_t cols,
+                                   uint8_t* values, uint8_t* scales, uint8_t* values_t, uint8_t* scales_t,
+                                   void* stream);
+/* out[i][j] = sum over k of a[i][k] b[j][k], a [m][k] and b [n][k] in 8-bit blocks. */
+SMX_API int64_t smx_block_product_workspace(int64_t m, int64_t n, int64_t k);
+SMX_API int32_t smx_block_product(const uint8_t* a_values, const uint8_t* a_scales, const uint8_t* b_values,
+                                  const uint8_t* b_scales, int64_t m, int64_t n, int64_t k, int32_t dtype, void* out,
+                                  int64_t out_stride, void* workspace, int64_t workspace_bytes, void* stream);
+/* The same with a = x [m][k] of `dtype`, brought to blocks within the call;
+ * out is out_dtype. */
+SMX_API int64_t smx_block_linear_workspace(int64_t m, int64_t n, int64_t k);
+SMX_API int32_t smx_block_linear(const void* x, int64_t x_stride, int32_t dtype, const uint8_t* w_values,
+                                 const uint8_t* w_scales, int64_t m, int64_t n, int64_t k, int32_t out_dtype,
+                                 void* out, int64_t out_stride, void* workspace, int64_t workspace_bytes,
+                                 void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* SYMMETRIX_NODE_OPS_H */

@@ -1,0 +1,126 @@
+// What the node operators' sources share: value types, row access, checks of
+// arguments and the C boundary.
+#pragma once
+
+#include <cstdint>
+#include <new>
+#include <stdexcept>
+#include <string>
+
+#include "../../include/symmetrix_node_ops.h"
+#include "device_common.hpp"
+
+namespace smx {
+
+void set_last_error(const std::string& message);  // evaluator.cpp
+
+namespace node {
+
+using bf16 = __bf16;
+using f16 = _Float16;
+using i64 = long long;
+
+inline int size_of(int dtype) { return dtype == SMX_DTYPE_F32 ? 4 : 2; }
+
+// f(T{}) with the value type of an SMX_DTYPE_* code
+template <class F>
+void with_dtype(int dtype, F&& f) {
+    switch (dtype) {
+        case SMX_DTYPE_F32: f(float{}); break;
+        case SMX_DTYPE_BF16: f(bf16{}); break;
+        case SMX_DTYPE_F16: f(f16{}); break;
+        default: throw std::invalid_argument("unknown dtype code " + std::to_string(dtype));
+    }
+}
+
+// N values as they lie in memory
+template <class T, int N>
+struct alignas(sizeof(T) * N) Pack {
+    T v[N];
+};
+
+inline void require(bool ok, const char* what) {
+    if (!ok) throw std::invalid_argument(what);
+}
+
+inline bool aligned(const void* p, std::size_t to) { return reinterpret_cast<std::uintptr_t>(p) % to == 0; }
+
+// checks one row array; an empty one needs no memory
+inline void check_rows(const void* p, i64 stride, i64 rows, i64 channels, int dtype, const char* name) {
+    if (rows > 0 && channels > 0 && !p) throw std::invalid_argument(std::string(name) + " is NULL");
+    if (p && rows > 1 && stride < channels) throw std::invalid_argument(std::string(name) + ": the row stride is less than a row");
+    if (!aligned(p, static_cast<std::size_t>(size_of(dtype)))) throw std::invalid_argument(std::string(name) + " is not aligned to its values");
+}
+
+inline void check_workspace(const void* p, i64 bytes, i64 needed) {
+    if (needed == 0) return;
+    if (!p || bytes < needed)
+        throw std::invalid_argument("the workspace holds " + std::to_string(p ? bytes : 0) + " bytes, " + std::to_string(needed) +
+                                    " are needed");
+    require(aligned(p, 16), "the workspace is not 16-byte aligned");
+}
+
+template <class F>
+int32_t guarded(F&& fn) noexcept {
+    const auto failed = [](int32_t code, const char* what) {
+        try {
+            set_last_error(what);
+        } catch (...) {  // no memory for the message
+        }
+        return code;
+    };
+    try {
+        fn();
+        return SMX_OK;
+    } catch (const std::bad_alloc&) {
+        return failed(SMX_ERR_OUT_OF_MEMORY, "out of memory");
+    } catch (const std::domain_error& e) {
+        return failed(SMX_ERR_UNSUPPORTED, e.what());
+    } catch (const std::invalid_argument& e) {
+        return failed(SMX_ERR_INVALID_ARGUMENT, e.what());
+    } catch (const std::exception& e) {
+        return failed(SMX_ERR_RUNTIME, e.what());
+    } catch (...) {
+        return failed(SMX_ERR_RUNTIME, "unknown error");
+    }
+}
+
+// ---- 8-bit blocks ----
+
+constexpr int kBlock = 128;
+
+inline i64 block_stride(i64 cols) { return (cols + kBlock - 1) / kBlock * kBlock; }
+inline i64 block_scale_stride(i64 cols) { return (block_stride(cols) / kBlock + 3) / 4 * 4; }
+
+// The scale byte of a block whose largest finite magnitude is `top`: the
+// least e >= -127 with top <= 448 * 2^e = 1.75 * 2^(e + 8), plus 127.
+__device__ __forceinline__ int block_scale_byte(float top) {
+    const unsigned bits = __float_as_uint(top);
+    const int b = static_cast<int>(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return b < 0 ? 0 : b;
+}
+
+// 2^-(byte - 127), exact (bytes reach 247)
+__device__ __forceinline__ float block_inverse_scale(int byte) {
+    return __uint_as_float(static_cast<unsigned>(254 - byte) << 23);
+}
+
+// |v|, or 0 for an infinity or NaN
+__device__ __forceinline__ float finite_magnitude(float v) {
+    const float a = __builtin_fabsf(v);
+    return a < __builtin_inff() ? a : 0.0f;
+}
+
+// an infinity becomes NaN: E4M3 has none
+__device__ __forceinline__ float e4m3_input(float v, float inverse) {
+    return __builtin_fabsf(v) < __builtin_inff() ? v * inverse : __builtin_nanf("");
+}
+
+__device__ __forceinline__ unsigned e4m3_four(float a, float b, float c, float d, float inverse) {
+    int p = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_input(a, inverse), e4m3_input(b, inverse), 0, false);
+    p = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_input(c, inverse), e4m3_input(d, inverse), p, true);
+    return static_cast<unsigned>(p);
+}
+
+}  // namespace node
+}  // namespace smx

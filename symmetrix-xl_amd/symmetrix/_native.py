@@ -76,6 +76,27 @@ class SmxMh1Info(ctypes.Structure):
                 ("radial_size", ctypes.c_int32), ("has_zbl", ctypes.c_int32), ("r_cut", ctypes.c_double)]
 
 
+class SmxResidualNormArgs(ctypes.Structure):
+    """Arguments of smx_residual_norm (device pointers as integers)."""
+    _fields_ = [("struct_size", ctypes.c_uint32), ("dtype", ctypes.c_int32), ("rows", ctypes.c_int64),
+                ("channels", ctypes.c_int64), ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64),
+                ("d", ctypes.c_void_p), ("d_stride", ctypes.c_int64), ("gate", ctypes.c_void_p),
+                ("gate_stride", ctypes.c_int64), ("gate_kind", ctypes.c_int32), ("eps", ctypes.c_float),
+                ("post", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("next", ctypes.c_void_p),
+                ("y", ctypes.c_void_p), ("y_stride", ctypes.c_int64), ("h", ctypes.c_void_p),
+                ("h_stride", ctypes.c_int64), ("h_scales", ctypes.c_void_p)]
+
+
+class SmxResidualNormGradientArgs(ctypes.Structure):
+    """Arguments of smx_residual_norm_gradient (device pointers as integers)."""
+    _fields_ = [("forward", SmxResidualNormArgs), ("grad_y", ctypes.c_void_p), ("grad_y_stride", ctypes.c_int64),
+                ("grad_h", ctypes.c_void_p), ("grad_h_stride", ctypes.c_int64), ("dx", ctypes.c_void_p),
+                ("dx_stride", ctypes.c_int64), ("dd", ctypes.c_void_p), ("dd_stride", ctypes.c_int64),
+                ("dgate", ctypes.c_void_p), ("dgate_stride", ctypes.c_int64), ("dpost", ctypes.c_void_p),
+                ("dscale", ctypes.c_void_p), ("dnext", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_int64)]
+
+
 class SmxLammpsArgsV2(ctypes.Structure):
     """SmxLammpsArgsV1 followed by the caller's hipStream_t: the call waits
     for the work the caller queued there instead of synchronising the device."""
@@ -86,6 +107,7 @@ class SmxLammpsArgsV2(ctypes.Structure):
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _u64 = ctypes.c_uint64
+_f32 = ctypes.c_float
 _dbl = ctypes.c_double
 _vp = ctypes.c_void_p
 _cp = ctypes.c_char_p
@@ -183,6 +205,20 @@ SIGNATURES = [
     ("smx_mh1_debug_stage", _i32, [_vp, _cp, _vp, _i64, _p_i64]),
     ("smx_mh1_set_kernel_timing", _i32, [_vp, _i32]),
     ("smx_mh1_kernel_timing", _i32, [_vp, _i32, ctypes.POINTER(_cp), _p_dbl, _p_i64]),
+    # node operators, include/symmetrix_node_ops.h
+    ("smx_embed", _i32, [_vp, _i32, _i64, _vp, _i64, _i64, _i64, _i32, _f32, _vp, _i64, _vp]),
+    ("smx_embed_gradient_workspace", _i64, [_i64, _i64, _i64]),
+    ("smx_embed_gradient", _i32, [_vp, _i32, _i64, _vp, _i64, _i64, _i64, _i32, _f32, _vp, _i64, _vp, _i64, _vp]),
+    ("smx_residual_norm", _i32, [ctypes.POINTER(SmxResidualNormArgs), _vp]),
+    ("smx_residual_norm_gradient_workspace", _i64, [_i64, _i64]),
+    ("smx_residual_norm_gradient", _i32, [ctypes.POINTER(SmxResidualNormGradientArgs), _vp]),
+    ("smx_block_stride", _i64, [_i64]),
+    ("smx_block_scale_stride", _i64, [_i64]),
+    ("smx_block_quantize", _i32, [_vp, _i64, _i32, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
+    ("smx_block_product_workspace", _i64, [_i64, _i64, _i64]),
+    ("smx_block_product", _i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp]),
+    ("smx_block_linear_workspace", _i64, [_i64, _i64, _i64]),
+    ("smx_block_linear", _i32, [_vp, _i64, _i32, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp]),
 ]
 
 

@@ -9,6 +9,7 @@ import os
 import sys
 
 import pytest
+import torch  # noqa: F401  (first: the library then shares torch's HIP runtime, which symmetrix.node_ops asks for)
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 for p in (ROOT, os.path.join(ROOT, "symmetrix-xl_amd")):
