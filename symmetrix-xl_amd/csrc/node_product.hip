@@ -23,54 +23,148 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 constexpr i64 kShortSum = 512;
 
-// Blocks along the rows: one wave per block.
-template <class T>
-__global__ void __launch_bounds__(256) k_quantize_rows(const T* __restrict__ x, i64 x_stride, i64 rows, i64 cols,
-                                                       std::uint8_t* __restrict__ values,
-                                                       std::uint8_t* __restrict__ scales, i64 pitch, i64 scale_pitch) {
-    const int lane = threadIdx.x % 64;
-    const i64 total = rows * scale_pitch;
-    for (i64 b = static_cast<i64>(blockIdx.x) * 4 + threadIdx.x / 64; b < total; b += static_cast<i64>(gridDim.x) * 4) {
-        const i64 r = b / scale_pitch, k = b % scale_pitch;
-        if (k * kBlock >= pitch) {
-            if (lane == 0) scales[b] = 0;
-            continue;
+// max(v, v of the lane that the DPP control CTRL names)
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float v) {
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false)));
+}
+
+// the largest of each row of 16 lanes, in all of them
+__device__ __forceinline__ float row_max(float v) {
+    v = dpp_max<0xb1>(v);
+    v = dpp_max<0x4e>(v);
+    v = dpp_max<0x141>(v);
+    return dpp_max<0x140>(v);
+}
+
+// Eight values from column c on; zeros past the end.  VEC: rows are 16-byte aligned.
+template <class T, bool VEC>
+__device__ __forceinline__ void load_eight(const T* row, i64 c, i64 cols, float (&v)[8]) {
+    if (VEC && c + 8 <= cols) {
+        constexpr int N = 16 / sizeof(T);
+#pragma unroll
+        for (int h = 0; h < 8; h += N) {
+            const Pack<T, N> p = *reinterpret_cast<const Pack<T, N>*>(row + c + h);
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[h + i] = static_cast<float>(p.v[i]);
         }
-        const i64 c = k * kBlock + 2 * lane;
-        const float v0 = c < cols ? static_cast<float>(x[r * x_stride + c]) : 0.0f;
-        const float v1 = c + 1 < cols ? static_cast<float>(x[r * x_stride + c + 1]) : 0.0f;
-        float top = fmaxf(finite_magnitude(v0), finite_magnitude(v1));
-        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-        const int byte = block_scale_byte(top);
-        const unsigned q = e4m3_four(v0, v1, 0.0f, 0.0f, block_inverse_scale(byte));
-        *reinterpret_cast<std::uint16_t*>(values + r * pitch + c) = static_cast<std::uint16_t>(q);
-        if (lane == 0) scales[b] = static_cast<std::uint8_t>(byte);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? static_cast<float>(row[c + i]) : 0.0f;
     }
 }
 
-// Blocks along the columns, stored as rows of the transpose: one wave per block.
-template <class T>
-__global__ void __launch_bounds__(256) k_quantize_columns(const T* __restrict__ x, i64 x_stride, i64 rows, i64 cols,
-                                                          std::uint8_t* __restrict__ values,
-                                                          std::uint8_t* __restrict__ scales, i64 pitch,
-                                                          i64 scale_pitch) {
-    const int lane = threadIdx.x % 64;
-    const i64 total = cols * scale_pitch;
-    for (i64 b = static_cast<i64>(blockIdx.x) * 4 + threadIdx.x / 64; b < total; b += static_cast<i64>(gridDim.x) * 4) {
-        const i64 c = b / scale_pitch, k = b % scale_pitch;
-        if (k * kBlock >= pitch) {
-            if (lane == 0) scales[b] = 0;
-            continue;
+__device__ __forceinline__ float top_of(const float (&v)[8]) {
+    float top = finite_magnitude(v[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, finite_magnitude(v[i]));
+    return top;
+}
+
+__device__ __forceinline__ uint2 e4m3_eight(const float (&v)[8], float inverse) {
+    return make_uint2(e4m3_four(v[0], v[1], v[2], v[3], inverse), e4m3_four(v[4], v[5], v[6], v[7], inverse));
+}
+
+// Blocks along the rows: 16 lanes a block, eight values each, so a row's loads
+// and stores are whole lines.  One read of x and one write of a byte a value.
+template <class T, bool VEC>
+__global__ void __launch_bounds__(256) k_quantize_rows(const T* __restrict__ x, i64 x_stride, i64 rows, i64 cols,
+                                                       std::uint8_t* __restrict__ values,
+                                                       std::uint8_t* __restrict__ scales, i64 pitch, i64 scale_pitch) {
+    const int sub = threadIdx.x % 16;
+    const unsigned blocks = static_cast<unsigned>(pitch / kBlock);
+    for (i64 g = static_cast<i64>(blockIdx.x) * 16 + threadIdx.x / 16; g < rows * blocks;
+         g += static_cast<i64>(gridDim.x) * 16) {
+        const i64 r = g < (1LL << 32) ? static_cast<unsigned>(g) / blocks : g / blocks;
+        const int k = static_cast<int>(g - r * blocks);
+        const i64 c = static_cast<i64>(k) * kBlock + 8 * sub;
+        float v[8];
+        load_eight<T, VEC>(x + r * x_stride, c, cols, v);
+        const int byte = block_scale_byte(row_max(top_of(v)));
+        *reinterpret_cast<uint2*>(values + r * pitch + c) = e4m3_eight(v, block_inverse_scale(byte));
+        std::uint8_t* const sc = scales + r * scale_pitch + k;
+        if (sub == 0) *sc = static_cast<std::uint8_t>(byte);
+        if (k + 1 == static_cast<int>(blocks) && sub > 0 && k + sub < scale_pitch) sc[sub] = 0;
+    }
+}
+
+// One tile of 128 x 128 a workgroup: blocks along its columns, stored as rows of
+// the transpose, and along its rows too (ROWS) in the same reading.  A thread
+// holds 8 x 8 values; the transposed bytes cross LDS in pieces of eight, each column's
+// pieces permuted by the column so that the 16 lanes that write at once meet 16 places.
+template <class T, bool VEC, bool ROWS>
+__global__ void __launch_bounds__(256) k_quantize_tile(const T* __restrict__ x, i64 x_stride, i64 rows, i64 cols,
+                                                       std::uint8_t* __restrict__ values,
+                                                       std::uint8_t* __restrict__ scales, i64 pitch, i64 scale_pitch,
+                                                       std::uint8_t* __restrict__ values_t,
+                                                       std::uint8_t* __restrict__ scales_t, i64 pitch_t,
+                                                       i64 scale_pitch_t) {
+    __shared__ float tops[16][kBlock + 4];
+    __shared__ int bytes[kBlock];
+    __shared__ uint2 turned[kBlock][16];
+    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    const i64 blocks_c = (cols + kBlock - 1) / kBlock;
+    const i64 tr = blockIdx.x / blocks_c, tc = blockIdx.x % blocks_c;
+    const i64 r0 = tr * kBlock + 8 * ty, c0 = tc * kBlock + 8 * tx;
+    float v[8][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (r0 + i < rows)
+            load_eight<T, VEC>(x + (r0 + i) * x_stride, c0, cols, v[i]);
+        else
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+    }
+    if constexpr (ROWS) {
+        const int k = static_cast<int>(tc);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int byte = block_scale_byte(row_max(top_of(v[i])));
+            if (r0 + i >= rows) continue;
+            *reinterpret_cast<uint2*>(values + (r0 + i) * pitch + c0) = e4m3_eight(v[i], block_inverse_scale(byte));
+            std::uint8_t* const sc = scales + (r0 + i) * scale_pitch + k;
+            if (tx == 0) *sc = static_cast<std::uint8_t>(byte);
+            if (tc + 1 == blocks_c && tx > 0 && k + tx < scale_pitch) sc[tx] = 0;
         }
-        const i64 r = k * kBlock + 2 * lane;
-        const float v0 = r < rows ? static_cast<float>(x[r * x_stride + c]) : 0.0f;
-        const float v1 = r + 1 < rows ? static_cast<float>(x[(r + 1) * x_stride + c]) : 0.0f;
-        float top = fmaxf(finite_magnitude(v0), finite_magnitude(v1));
-        for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, finite_magnitude(v[i][j]));
+        tops[ty][8 * tx + j] = top;
+    }
+    __syncthreads();
+    if (threadIdx.x < kBlock) {
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, tops[i][threadIdx.x]);
         const int byte = block_scale_byte(top);
-        const unsigned q = e4m3_four(v0, v1, 0.0f, 0.0f, block_inverse_scale(byte));
-        *reinterpret_cast<std::uint16_t*>(values + c * pitch + r) = static_cast<std::uint16_t>(q);
-        if (lane == 0) scales[b] = static_cast<std::uint8_t>(byte);
+        bytes[threadIdx.x] = byte;
+        const i64 c = tc * kBlock + threadIdx.x;
+        if (c < cols) {
+            std::uint8_t* const sc = scales_t + c * scale_pitch_t + tr;
+            *sc = static_cast<std::uint8_t>(byte);
+            if ((tr + 1) * kBlock >= rows)
+                for (i64 z = tr + 1; z < scale_pitch_t; ++z) sc[z - tr] = 0;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        float w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = v[i][j];
+        turned[8 * tx + j][ty ^ tx] = e4m3_eight(w, block_inverse_scale(bytes[8 * tx + j]));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int p = q * 256 + threadIdx.x, c = p / 8, piece = p % 8 * 2;
+        const uint2 lo = turned[c][piece ^ (c / 8)], hi = turned[c][(piece + 1) ^ (c / 8)];
+        if (tc * kBlock + c < cols)
+            *reinterpret_cast<uint4*>(values_t + (tc * kBlock + c) * pitch_t + tr * kBlock + 8 * piece) =
+                make_uint4(lo.x, lo.y, hi.x, hi.y);
     }
 }
 
@@ -98,55 +192,259 @@ __device__ __forceinline__ float scale_of(int byte) {
     return byte ? __uint_as_float(static_cast<unsigned>(byte) << 23) : 0x1p-127f;
 }
 
-// 16 x 16 outputs a wave, operands straight from memory.  Lane l holds row
-// l % 16 of both operands and bytes 32 (l / 16) on of the block (the order of
-// k inside a block is the operands' own affair, as one scale covers it); the
-// accumulator's lane l holds column l % 16 of rows 4 (l / 16) on, so with b as the first
-// operand a lane's four values lie side by side in a row of the output.
-template <class O, bool WIDE>
-__global__ void __launch_bounds__(256) k_product_simple(const std::uint8_t* __restrict__ a,
-                                                        const std::uint8_t* __restrict__ as,
-                                                        const std::uint8_t* __restrict__ b,
-                                                        const std::uint8_t* __restrict__ bs, i64 m, i64 n, i64 k,
-                                                        i64 pitch, i64 scale_pitch, O* __restrict__ out,
-                                                        i64 out_stride) {
-    const int lane = threadIdx.x % 64;
-    const i64 tiles_n = (n + 15) / 16, tiles = (m + 15) / 16 * tiles_n;
-    const i64 tile = static_cast<i64>(blockIdx.x) * 4 + threadIdx.x / 64;
-    if (tile >= tiles) return;
-    const i64 i0 = tile / tiles_n * 16, j0 = tile % tiles_n * 16;
-    const i64 i = i0 + lane % 16, j = j0 + lane % 16;
-    const i64 ia = i < m ? i : m - 1, jb = j < n ? j : n - 1;
-    const std::uint8_t* pa = a + ia * pitch + 32 * (lane / 16);
-    const std::uint8_t* pb = b + jb * pitch + 32 * (lane / 16);
-    acc4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (i64 kb = 0; kb < pitch / kBlock; ++kb) {
-        i32x8 va, vb;
-        for (int h = 0; h < 2; ++h) {
-            const i32x4 ha = *reinterpret_cast<const i32x4*>(pa + kb * kBlock + 16 * h);
-            const i32x4 hb = *reinterpret_cast<const i32x4*>(pb + kb * kBlock + 16 * h);
-            for (int q = 0; q < 4; ++q) va[4 * h + q] = ha[q], vb[4 * h + q] = hb[q];
-        }
-        const int sa = as[ia * scale_pitch + kb], sb = bs[jb * scale_pitch + kb];
-        if constexpr (WIDE) {
-            for (int q = 0; q < 4; ++q)
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16(vb[2 * q], vb[2 * q + 1], scale_of(sb)),
-                                                              to_bf16(va[2 * q], va[2 * q + 1], scale_of(sa)), acc, 0, 0, 0);
+// Operands and output of one product, the rows of both operands in 8-bit blocks.
+template <class O>
+struct Product {
+    const std::uint8_t *a, *as, *b, *bs;
+    int m, n;
+    int blocks;  // of 128 along the summed axis
+    i64 pitch, scale_pitch;
+    O* out;
+    i64 out_stride;
+    bool vec;        // four outputs of a row may be stored at once
+    float* partial;  // [splits][m][n] when the sum is split, else NULL
+    int split_blocks;
+    int tiles_m, tiles_n;
+};
+
+// A lane's four neighbouring outputs of row i from column j on.
+template <class O>
+__device__ __forceinline__ void store_four(const Product<O>& p, int i, int j, acc4 v, int split) {
+    if (i >= p.m) return;
+    if (p.partial) {
+        float* const at = p.partial + (static_cast<i64>(split) * p.m + i) * p.n + j;
+        if (p.n % 4 == 0 && j + 4 <= p.n) {
+            *reinterpret_cast<acc4*>(at) = v;
         } else {
-            acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vb, va, acc, 0, 0, 0, sb, 0, sa);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (j + q < p.n) at[q] = v[q];
         }
+        return;
     }
-    mfma_settle();
-    if (i >= m) return;
-    for (int v = 0; v < 4; ++v) {
-        const i64 col = j0 + 4 * (lane / 16) + v;
-        if (col < n) out[i * out_stride + col] = static_cast<O>(acc[v]);
+    O* const at = p.out + i * p.out_stride + j;
+    if (p.vec && j + 4 <= p.n) {
+        Pack<O, 4> o;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o.v[q] = static_cast<O>(v[q]);
+        *reinterpret_cast<Pack<O, 4>*>(at) = o;
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (j + q < p.n) at[q] = static_cast<O>(v[q]);
     }
 }
+
+// 1 KB of LDS at byte `lds` (the wave's own, uniform) from 64 lanes' 16 bytes at their offsets `at`
+// into the buffer: memory to LDS without registers.  The compiler does not count it: dma_wait.
+__device__ __forceinline__ void dma(__amdgpu_buffer_rsrc_t from, unsigned lds, int at, int also) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :
+                 : "s"(lds), "v"(at), "s"(from), "s"(also)
+                 : "memory");
+}
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// BM x BN outputs a workgroup of WM x WN waves.  Both operands' blocks of 128
+// go to LDS by dma, two stages deep: while one block is multiplied, the next arrives.  A row's
+// eight 16-byte pieces are permuted by half the row's number (in the global
+// addresses, within one line), so that the 16 rows that a fragment read meets at once lie in
+// 16 different places of the 64 banks.  Lane l holds row l % 16 of a fragment and pieces l / 16 and
+// l / 16 + 4 of the block: the order of k inside a block is the operands' own affair, as one
+// scale covers it.  The accumulator's lane l holds column l % 16 of rows 4 (l / 16) on; with b as the first operand its
+// four values lie side by side in a row of the output.
+template <class O, bool WIDE, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN, (BM + BN) * kBlock * 2 > 81920 ? 1 : 2) k_product_tile(Product<O> p) {
+    constexpr int WAVES = WM * WN, MF = BM / WM / 16, NF = BN / WN / 16, LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;
+    constexpr unsigned kStage = (BM + BN) * kBlock;
+    static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0);
+    __shared__ __attribute__((aligned(1024))) std::uint8_t lds[2 * kStage];
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    // bands of eight tile rows, each band column by column: the tiles that one XCD works on
+    // share their rows of both operands in its L2
+    const int id = xcd_remap(blockIdx.x, gridDim.x);
+    const int band = id / (8 * p.tiles_n), in_band = id % (8 * p.tiles_n);
+    const int high = p.tiles_m - 8 * band < 8 ? p.tiles_m - 8 * band : 8;
+    const int i0 = (8 * band + in_band % high) * BM, j0 = in_band / high * BN;
+    const int first = blockIdx.y * p.split_blocks;
+    const int last = first + p.split_blocks < p.blocks ? first + p.split_blocks : p.blocks;
+
+    const int rows_a = p.m - i0 < BM ? p.m - i0 : BM, rows_b = p.n - j0 < BN ? p.n - j0 : BN;
+    const int pitch = static_cast<int>(p.pitch);
+    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<std::uint8_t*>(p.a + i0 * p.pitch), 0, rows_a * pitch, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<std::uint8_t*>(p.b + j0 * p.pitch), 0, rows_b * pitch, 0x00020000);
+    int at_a[LA], at_b[LB];
+#pragma unroll
+    for (int q = 0; q < LA; ++q) {
+        const int r = 8 * (wave + WAVES * q) + lane / 8;
+        at_a[q] = (r < rows_a ? r : rows_a - 1) * pitch + ((lane % 8) ^ (r / 2 % 8)) * 16;
+    }
+#pragma unroll
+    for (int q = 0; q < LB; ++q) {
+        const int r = 8 * (wave + WAVES * q) + lane / 8;
+        at_b[q] = (r < rows_b ? r : rows_b - 1) * pitch + ((lane % 8) ^ (r / 2 % 8)) * 16;
+    }
+    const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<std::uintptr_t>(
+        (__attribute__((address_space(3))) std::uint8_t*)lds));
+    const auto stage = [&](int kb) {
+        const unsigned to = __builtin_amdgcn_readfirstlane(lds0 + (kb & 1) * kStage + wave * 1024);
+#pragma unroll
+        for (int q = 0; q < LA; ++q) dma(ra, to + q * WAVES * 1024, at_a[q], kb * kBlock);
+#pragma unroll
+        for (int q = 0; q < LB; ++q) dma(rb, to + BM * kBlock + q * WAVES * 1024, at_b[q], kb * kBlock);
+    };
+
+    // the scales of four blocks are one dword; a wave holds those of its rows, and the next four's
+    const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+    const unsigned *sa_at[MF], *sb_at[NF];
+    unsigned sa[MF], sb[NF], sa_next[MF], sb_next[NF];
+#pragma unroll
+    for (int f = 0; f < MF; ++f) {
+        const int r = i0 + wm + 16 * f + lane % 16;
+        sa_at[f] = reinterpret_cast<const unsigned*>(p.as + (r < p.m ? r : p.m - 1) * p.scale_pitch);
+        sa_next[f] = sa_at[f][first / 4];
+    }
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+        const int r = j0 + wn + 16 * f + lane % 16;
+        sb_at[f] = reinterpret_cast<const unsigned*>(p.bs + (r < p.n ? r : p.n - 1) * p.scale_pitch);
+        sb_next[f] = sb_at[f][first / 4];
+    }
+
+    acc4 acc[MF][NF];
+#pragma unroll
+    for (int f = 0; f < MF; ++f)
+#pragma unroll
+        for (int g = 0; g < NF; ++g) acc[f][g] = acc4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    const int piece = (lane % 16) * kBlock + ((lane / 16) ^ (lane % 16 / 2)) * 16;
+    stage(first);
+    for (int kb = first; kb < last; ++kb) {
+        dma_wait();
+        __syncthreads();
+        if (kb % 4 == 0) {
+#pragma unroll
+            for (int f = 0; f < MF; ++f) sa[f] = sa_next[f];
+#pragma unroll
+            for (int f = 0; f < NF; ++f) sb[f] = sb_next[f];
+            const int more = (kb + 4 < last ? kb + 4 : kb) / 4;
+#pragma unroll
+            for (int f = 0; f < MF; ++f) sa_next[f] = sa_at[f][more];
+#pragma unroll
+            for (int f = 0; f < NF; ++f) sb_next[f] = sb_at[f][more];
+        }
+        if (kb + 1 < last) stage(kb + 1);
+        const std::uint8_t* const ta = lds + (kb & 1) * kStage + wm * kBlock + piece;
+        const std::uint8_t* const tb = lds + (kb & 1) * kStage + (BM + wn) * kBlock + piece;
+        const std::uint8_t* const ta2 = lds + (kb & 1) * kStage + wm * kBlock + (piece ^ 64);
+        const std::uint8_t* const tb2 = lds + (kb & 1) * kStage + (BM + wn) * kBlock + (piece ^ 64);
+        const auto fragment = [](const std::uint8_t* lo, const std::uint8_t* hi, int f) {
+            const i32x4 x = *reinterpret_cast<const i32x4*>(lo + 16 * kBlock * f);
+            const i32x4 y = *reinterpret_cast<const i32x4*>(hi + 16 * kBlock * f);
+            return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+        };
+        i32x8 vb[NF];
+#pragma unroll
+        for (int g = 0; g < NF; ++g) vb[g] = fragment(tb, tb2, g);
+        if constexpr (!WIDE) {
+#pragma unroll
+            for (int f = 0; f < MF; ++f) {
+                const i32x8 va = fragment(ta, ta2, f);
+#pragma unroll
+                for (int g = 0; g < NF; ++g)
+                    acc[f][g] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vb[g], va, acc[f][g], 0, 0, 0, sb[g],
+                                                                                0, sa[f]);
+            }
+        } else {
+            i32x8 va[MF];
+#pragma unroll
+            for (int f = 0; f < MF; ++f) va[f] = fragment(ta, ta2, f);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                bf16x8 wb[NF];
+#pragma unroll
+                for (int g = 0; g < NF; ++g) wb[g] = to_bf16(vb[g][2 * q], vb[g][2 * q + 1], scale_of(sb[g] & 0xff));
+#pragma unroll
+                for (int f = 0; f < MF; ++f) {
+                    const bf16x8 wa = to_bf16(va[f][2 * q], va[f][2 * q + 1], scale_of(sa[f] & 0xff));
+#pragma unroll
+                    for (int g = 0; g < NF; ++g)
+                        acc[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[g], wa, acc[f][g], 0, 0, 0);
+                }
+            }
+        }
+#pragma unroll
+        for (int f = 0; f < MF; ++f) sa[f] >>= 8;
+#pragma unroll
+        for (int g = 0; g < NF; ++g) sb[g] >>= 8;
+    }
+    mfma_settle();
+#pragma unroll
+    for (int f = 0; f < MF; ++f)
+#pragma unroll
+        for (int g = 0; g < NF; ++g)
+            store_four(p, i0 + wm + 16 * f + lane % 16, j0 + wn + 16 * g + 4 * (lane / 16), acc[f][g], blockIdx.y);
+}
+
+// Joins the parts of a split sum, in their order.
+template <class O>
+__global__ void __launch_bounds__(256) k_product_join(Product<O> p, int splits) {
+    const i64 total = static_cast<i64>(p.m) * p.n;
+    for (i64 e = static_cast<i64>(blockIdx.x) * 256 + threadIdx.x; e < total; e += static_cast<i64>(gridDim.x) * 256) {
+        float sum = p.partial[e];
+        for (int s = 1; s < splits; ++s) sum += p.partial[s * total + e];
+        p.out[e / p.n * p.out_stride + e % p.n] = static_cast<O>(sum);
+    }
+}
+
+template <class O>
+__global__ void __launch_bounds__(256) k_product_zero(O* __restrict__ out, i64 out_stride, i64 m, i64 n) {
+    for (i64 e = static_cast<i64>(blockIdx.x) * 256 + threadIdx.x; e < m * n; e += static_cast<i64>(gridDim.x) * 256)
+        out[e / n * out_stride + e % n] = static_cast<O>(0.0f);
+}
+
+// How a product is cut: the tile, and parts of the summed axis.
+struct Plan {
+    int tile;  // 256, 128 or 64
+    int splits;
+    i64 split_blocks;
+};
+
+constexpr int kUnits = 256;  // compute units
+
+Plan plan_product(i64 m, i64 n, i64 k) {
+    const auto tiles = [&](i64 t) { return (m + t - 1) / t * ((n + t - 1) / t); };
+    const i64 blocks = (k + kBlock - 1) / kBlock;
+    Plan p{tiles(256) >= kUnits ? 256 : tiles(128) >= kUnits / 2 ? 128 : 64, 1, blocks};
+    const i64 count = tiles(p.tile);
+    if (p.tile == 64 && count < kUnits && blocks >= 8) {
+        const i64 want = (2 * kUnits + count - 1) / count, most = blocks / 4;
+        const i64 parts = want < most ? want : most;
+        p.split_blocks = ((blocks + parts - 1) / parts + 3) / 4 * 4;  // scales are read four blocks at a time
+        p.splits = static_cast<int>((blocks + p.split_blocks - 1) / p.split_blocks);
+    }
+    return p;
+}
+
+i64 split_bytes(i64 m, i64 n, i64 k) {
+    if (m <= 0 || n <= 0 || k <= 0) return 0;
+    const Plan p = plan_product(m, n, k);
+    return p.splits > 1 ? 4 * p.splits * m * n : 0;
+}
+
+// bytes of a matrix's blocks, scales included, as the workspace holds them
+i64 block_bytes(i64 rows, i64 cols) { return rows * block_stride(cols) + (rows * block_scale_stride(cols) + 15) / 16 * 16; }
 
 void check_sizes(i64 m, i64 n, i64 k) {
     require(m >= 0 && m < (1LL << 31) && n >= 0 && n < (1LL << 31) && k >= 0 && k < (1LL << 31),
             "sizes must be in [0, 2^31)");
+}
+
+// a tile of 256 rows is addressed with 31 bits
+void check_summed(i64 k) {
+    if (k > (1LL << 23) - kBlock) throw std::domain_error("products sum over up to 2^23 - 128 values");
 }
 
 void check_blocks(const void* values, const void* scales, i64 rows, i64 cols, const char* name) {
@@ -156,32 +454,73 @@ void check_blocks(const void* values, const void* scales, i64 rows, i64 cols, co
         throw std::invalid_argument(std::string(name) + ": 8-bit blocks must be 16-byte aligned");
 }
 
-template <class T>
-void launch_quantize(const void* x, i64 x_stride, i64 rows, i64 cols, std::uint8_t* values, std::uint8_t* scales,
+template <class T, bool VEC>
+void launch_quantize(const T* x, i64 x_stride, i64 rows, i64 cols, std::uint8_t* values, std::uint8_t* scales,
                      std::uint8_t* values_t, std::uint8_t* scales_t, hipStream_t stream) {
-    const auto grid = [](i64 blocks) { return static_cast<unsigned>(blocks < 4 * 65536 ? (blocks + 3) / 4 : 65536); };
-    if (values && rows > 0 && cols > 0) {
-        const i64 pitch = block_stride(cols), scale_pitch = block_scale_stride(cols);
-        k_quantize_rows<T><<<grid(rows * scale_pitch), 256, 0, stream>>>(static_cast<const T*>(x), x_stride, rows, cols,
-                                                                       values, scales, pitch, scale_pitch);
+    const i64 pitch = block_stride(cols), scale_pitch = block_scale_stride(cols);
+    if (!values_t) {
+        const i64 groups = (rows * (pitch / kBlock) + 15) / 16;
+        k_quantize_rows<T, VEC><<<static_cast<unsigned>(groups < 65536 ? groups : 65536), 256, 0, stream>>>(
+            x, x_stride, rows, cols, values, scales, pitch, scale_pitch);
         SMX_LAUNCH_CHECK("k_quantize_rows");
+        return;
     }
-    if (values_t && rows > 0 && cols > 0) {
-        const i64 pitch = block_stride(rows), scale_pitch = block_scale_stride(rows);
-        k_quantize_columns<T><<<grid(cols * scale_pitch), 256, 0, stream>>>(static_cast<const T*>(x), x_stride, rows,
-                                                                          cols, values_t, scales_t, pitch, scale_pitch);
-        SMX_LAUNCH_CHECK("k_quantize_columns");
+    const i64 tiles = block_stride(rows) / kBlock * (pitch / kBlock);
+    require(tiles < (1LL << 31), "the matrix has too many tiles");
+    (values ? k_quantize_tile<T, VEC, true> : k_quantize_tile<T, VEC, false>)<<<static_cast<unsigned>(tiles), 256, 0,
+                                                                                stream>>>(
+        x, x_stride, rows, cols, values, scales, pitch, scale_pitch, values_t, scales_t, block_stride(rows),
+        block_scale_stride(rows));
+    SMX_LAUNCH_CHECK("k_quantize_tile");
+}
+
+void quantize(const void* x, i64 x_stride, int dtype, i64 rows, i64 cols, std::uint8_t* values, std::uint8_t* scales,
+              std::uint8_t* values_t, std::uint8_t* scales_t, hipStream_t stream) {
+    if (rows == 0 || cols == 0 || (!values && !values_t)) return;
+    const bool vec = aligned(x, 16) && (rows == 1 || x_stride * size_of(dtype) % 16 == 0);
+    with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        (vec ? launch_quantize<T, true> : launch_quantize<T, false>)(static_cast<const T*>(x), x_stride, rows, cols,
+                                                                    values, scales, values_t, scales_t, stream);
+    });
+}
+
+template <class O, bool WIDE>
+void launch_tiles(const Product<O>& p, const Plan& plan, hipStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(p.tiles_m * p.tiles_n), static_cast<unsigned>(plan.splits));
+    switch (plan.tile) {
+        case 256: k_product_tile<O, WIDE, 256, 256, 2, 4><<<grid, 512, 0, stream>>>(p); break;
+        case 128: k_product_tile<O, WIDE, 128, 128, 2, 2><<<grid, 256, 0, stream>>>(p); break;
+        default: k_product_tile<O, WIDE, 64, 64, 2, 2><<<grid, 256, 0, stream>>>(p); break;
     }
+    SMX_LAUNCH_CHECK("k_product_tile");
 }
 
 template <class O>
 void launch_product(const std::uint8_t* a, const std::uint8_t* as, const std::uint8_t* b, const std::uint8_t* bs, i64 m,
-                    i64 n, i64 k, O* out, i64 out_stride, hipStream_t stream) {
-    const i64 tiles = (m + 15) / 16 * ((n + 15) / 16);
+                    i64 n, i64 k, O* out, i64 out_stride, float* partial, hipStream_t stream) {
+    if (k == 0) {
+        k_product_zero<O><<<static_cast<unsigned>(m * n < 256 * 4096 ? (m * n + 255) / 256 : 4096), 256, 0, stream>>>(
+            out, out_stride, m, n);
+        SMX_LAUNCH_CHECK("k_product_zero");
+        return;
+    }
+    const Plan plan = plan_product(m, n, k);
+    const i64 tiles_m = (m + plan.tile - 1) / plan.tile, tiles_n = (n + plan.tile - 1) / plan.tile;
+    require(tiles_m * tiles_n < (1LL << 31) && 8 * tiles_n < (1LL << 31), "the product has too many tiles");
+    const bool vec = aligned(out, 4 * sizeof(O)) && (m == 1 || out_stride % 4 == 0);
+    const Product<O> p{a,   as,         b,   bs,
+                       static_cast<int>(m), static_cast<int>(n), static_cast<int>(block_stride(k) / kBlock),
+                       block_stride(k),     block_scale_stride(k), out, out_stride, vec,
+                       plan.splits > 1 ? partial : nullptr, static_cast<int>(plan.split_blocks),
+                       static_cast<int>(tiles_m), static_cast<int>(tiles_n)};
     const bool wide = sizeof(O) == 4 || k <= kShortSum;
-    (wide ? k_product_simple<O, true> : k_product_simple<O, false>)<<<blocks_for(tiles, 4), 256, 0, stream>>>(
-        a, as, b, bs, m, n, k, block_stride(k), block_scale_stride(k), out, out_stride);
-    SMX_LAUNCH_CHECK("k_product_simple");
+    (wide ? launch_tiles<O, true> : launch_tiles<O, false>)(p, plan, stream);
+    if (plan.splits > 1) {
+        k_product_join<O><<<static_cast<unsigned>(m * n < 256 * 4096 ? (m * n + 255) / 256 : 4096), 256, 0, stream>>>(
+            p, plan.splits);
+        SMX_LAUNCH_CHECK("k_product_join");
+    }
 }
 
 }  // namespace
@@ -206,14 +545,11 @@ int32_t smx_block_quantize(const void* x, int64_t x_stride, int32_t dtype, int64
         require(values || values_t || rows == 0 || cols == 0, "no output is asked for");
         if (values) check_blocks(values, scales, rows, cols, "values");
         if (values_t) check_blocks(values_t, scales_t, rows, cols, "values_t");
-        with_dtype(dtype, [&](auto t) {
-            launch_quantize<decltype(t)>(x, x_stride, rows, cols, values, scales, values_t, scales_t,
-                                         static_cast<hipStream_t>(stream));
-        });
+        quantize(x, x_stride, dtype, rows, cols, values, scales, values_t, scales_t, static_cast<hipStream_t>(stream));
     });
 }
 
-int64_t smx_block_product_workspace(int64_t, int64_t, int64_t) { return 0; }
+int64_t smx_block_product_workspace(int64_t m, int64_t n, int64_t k) { return split_bytes(m, n, k); }
 
 int32_t smx_block_product(const uint8_t* a_values, const uint8_t* a_scales, const uint8_t* b_values,
                           const uint8_t* b_scales, int64_t m, int64_t n, int64_t k, int32_t dtype, void* out,
@@ -224,19 +560,20 @@ int32_t smx_block_product(const uint8_t* a_values, const uint8_t* a_scales, cons
         check_blocks(a_values, a_scales, m, k, "a");
         check_blocks(b_values, b_scales, n, k, "b");
         check_rows(out, out_stride, m, n, dtype, "out");
+        check_summed(k);
         check_workspace(workspace, workspace_bytes, smx_block_product_workspace(m, n, k));
         if (m == 0 || n == 0) return;
         with_dtype(dtype, [&](auto o) {
             using O = decltype(o);
             launch_product<O>(a_values, a_scales, b_values, b_scales, m, n, k, static_cast<O*>(out), out_stride,
-                              static_cast<hipStream_t>(stream));
+                              static_cast<float*>(workspace), static_cast<hipStream_t>(stream));
         });
     });
 }
 
 int64_t smx_block_linear_workspace(int64_t m, int64_t n, int64_t k) {
     if (m <= 0 || n <= 0 || k <= 0) return 0;
-    return m * block_stride(k) + (m * block_scale_stride(k) + 15) / 16 * 16;
+    return block_bytes(m, k) + split_bytes(m, n, k);
 }
 
 int32_t smx_block_linear(const void* x, int64_t x_stride, int32_t dtype, const uint8_t* w_values,
@@ -249,18 +586,16 @@ int32_t smx_block_linear(const void* x, int64_t x_stride, int32_t dtype, const u
         check_rows(x, x_stride, m, k, dtype, "x");
         check_blocks(w_values, w_scales, n, k, "w");
         check_rows(out, out_stride, m, n, out_dtype, "out");
+        check_summed(k);
         check_workspace(workspace, workspace_bytes, smx_block_linear_workspace(m, n, k));
         if (m == 0 || n == 0) return;
         auto* const values = static_cast<std::uint8_t*>(workspace);
         std::uint8_t* const scales = k > 0 ? values + m * block_stride(k) : nullptr;
-        if (k > 0)
-            with_dtype(dtype, [&](auto t) {
-                launch_quantize<decltype(t)>(x, x_stride, m, k, values, scales, nullptr, nullptr,
-                                             static_cast<hipStream_t>(stream));
-            });
+        auto* const partial = k > 0 ? reinterpret_cast<float*>(values + block_bytes(m, k)) : nullptr;
+        quantize(x, x_stride, dtype, m, k, values, scales, nullptr, nullptr, static_cast<hipStream_t>(stream));
         with_dtype(out_dtype, [&](auto o) {
             using O = decltype(o);
-            launch_product<O>(values, scales, w_values, w_scales, m, n, k, static_cast<O*>(out), out_stride,
+            launch_product<O>(values, scales, w_values, w_scales, m, n, k, static_cast<O*>(out), out_stride, partial,
                               static_cast<hipStream_t>(stream));
         });
     });
