@@ -7,6 +7,8 @@
 //   q  = H next,     dx = G + r2 (q - v mean(q v)),              dnext  = sum H v
 //   dg = dx a n s (1 - s),   da = sum dx s n,   p = dx a s,      dpost  = sum p u
 //   t  = p post,     dd = r1 (t - u mean(t u))
+#include <type_traits>
+
 #include "node_ops.hpp"
 
 namespace smx {
@@ -33,181 +35,379 @@ struct Norm {
     float *dgate_channel, *dpost, *dscale, *dnext;
 };
 
-__device__ __forceinline__ float sigmoid(float g) { return 1.0f / (1.0f + __expf(-g)); }
+// 1 / (1 + e^-g) on the hardware exponential and reciprocal, about 2^-22 of it
+__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
 
-template <class T>
-__device__ __forceinline__ float gate_of(const Norm<T>& a, i64 r, int c) {
-    switch (a.gate_kind) {
-        case SMX_GATE_FULL: return sigmoid(static_cast<float>(a.gate[r * a.gate_stride + c]));
-        case SMX_GATE_CHANNEL: return sigmoid(static_cast<float>(a.gate[c]));
-        case SMX_GATE_ROW: return sigmoid(static_cast<float>(a.gate[r * a.gate_stride]));
-        default: return 1.0f;
-    }
-}
+// Threads of a workgroup with G lanes a row: several rows' lanes up to a wave each, one row's above
+// (whose sums wait at barriers, so no other row may share the workgroup).
+constexpr int threads_of(int g) { return g > 64 ? g : 256; }
 
-template <class T>
-__device__ __forceinline__ float y_of(const Norm<T>& a, i64 r, int c, float r1) {
-    const float x = static_cast<float>(a.x[r * a.x_stride + c]);
-    if (!a.d) return x;
-    const float n = a.post[c] * static_cast<float>(a.d[r * a.d_stride + c]) * r1;
-    return x + (a.scale ? a.scale[c] : 1.0f) * gate_of(a, r, c) * n;
-}
-
-// Sum over a workgroup of 256 threads; every thread gets it.
-__device__ __forceinline__ float group_sum(float v, float* room) {
-    v = wave_total<64>(v);
-    __syncthreads();
-    if (threadIdx.x % 64 == 0) room[threadIdx.x / 64] = v;
-    __syncthreads();
-    return (room[0] + room[1]) + (room[2] + room[3]);
-}
-
-template <class T>
-__device__ __forceinline__ float d_norm(const Norm<T>& a, i64 r, float* room) {
-    if (!a.d) return 0.0f;
-    float s = 0.0f;
-    for (int c = threadIdx.x; c < a.channels; c += 256) {
-        const float d = static_cast<float>(a.d[r * a.d_stride + c]);
-        s += d * d;
-    }
-    return 1.0f / sqrtf(group_sum(s, room) / static_cast<float>(a.channels) + a.eps);
-}
-
-template <class T>
-__device__ __forceinline__ float y_norm(const Norm<T>& a, i64 r, float r1, float* room) {
-    float s = 0.0f;
-    for (int c = threadIdx.x; c < a.channels; c += 256) {
-        const float y = y_of(a, r, c, r1);
-        s += y * y;
-    }
-    return 1.0f / sqrtf(group_sum(s, room) / static_cast<float>(a.channels) + a.eps);
-}
-
-// One workgroup per row, reading the row again for each of its sums.
-template <class T>
-__global__ void __launch_bounds__(256) k_residual_norm(Norm<T> a) {
-    __shared__ float room[4], blocks[4];
-    for (i64 r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const float r1 = d_norm(a, r, room);
-        const float r2 = a.next ? y_norm(a, r, r1, room) : 0.0f;
-        const int padded = a.h8 ? (a.channels + 255) / 256 * 256 : a.channels;
-        for (int c0 = 0; c0 < padded; c0 += 256) {
-            const int c = c0 + threadIdx.x;
-            const bool in = c < a.channels;
-            const float y = in ? y_of(a, r, c, r1) : 0.0f;
-            const float h = in && a.next ? a.next[c] * y * r2 : 0.0f;
-            if (a.h8) {
-                float top = finite_magnitude(h);
-                for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-                __syncthreads();
-                if (threadIdx.x % 64 == 0) blocks[threadIdx.x / 64] = top;
-                __syncthreads();
-                const int w = threadIdx.x / 128 * 2;
-                const int byte = block_scale_byte(fmaxf(blocks[w], blocks[w + 1]));
-                const int width = (a.channels + 127) / 128 * 128;
-                if (c < width) {
-                    a.h8[r * width + c] = static_cast<std::uint8_t>(
-                        e4m3_four(h, 0.0f, 0.0f, 0.0f, block_inverse_scale(byte)) & 0xff);
-                    const int pitch = (width / 128 + 3) / 4 * 4;
-                    if (c % 128 == 0) a.h_scales[r * pitch + c / 128] = static_cast<std::uint8_t>(byte);
-                    if (c == 0)
-                        for (int b = width / 128; b < pitch; ++b) a.h_scales[r * pitch + b] = 0;
-                }
-            } else if (in && a.next) {
-                a.h[r * a.h_stride + c] = static_cast<T>(h);
+// The sums of K values over G lanes, in all of them; G a power of two from 16 on, lanes side by
+// side, above a wave the whole workgroup (one barrier: consecutive calls take
+// the two halves of `room` in turn).
+template <int G, int K>
+struct GroupSum {
+    static constexpr int kWaves = G > 64 ? G / 64 : 1;
+    struct Room {
+        float v[2][K][kWaves];
+    };
+    __device__ __forceinline__ static void sum(float (&v)[K], Room& room, int& turn) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            v[k] = row_total(v[k]);
+            if constexpr (G >= 32) v[k] += __shfl_xor(v[k], 16);
+            if constexpr (G >= 64) v[k] += __shfl_xor(v[k], 32);
+        }
+        if constexpr (G > 64) {
+            turn ^= 1;
+            if (threadIdx.x % 64 == 0)
+#pragma unroll
+                for (int k = 0; k < K; ++k) room.v[turn][k][threadIdx.x / 64] = v[k];
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                float s = room.v[turn][k][0];
+#pragma unroll
+                for (int w = 1; w < kWaves; ++w) s += room.v[turn][k][w];
+                v[k] = s;
             }
-            if (in && a.y) a.y[r * a.y_stride + c] = static_cast<T>(y);
         }
     }
+};
+
+// What a lane keeps of the channels it holds, for all its rows.
+struct Channels {
+    float post[8], scale[8], next[8], gate[8];  // gate: its sigmoid where no row has another
+};
+
+template <class T>
+__device__ __forceinline__ void load_channels(const Norm<T>& a, int c, Channels& w) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w.post[i] = w.scale[i] = w.next[i] = 0.0f, w.gate[i] = 1.0f;
+    if (a.d) {
+        load_eight(a.post, c, a.channels, w.post);
+        if (a.scale) {
+            load_eight(a.scale, c, a.channels, w.scale);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w.scale[i] = 1.0f;
+        }
+        if (a.gate_kind == SMX_GATE_CHANNEL) {
+            load_eight(a.gate, c, a.channels, w.gate);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w.gate[i] = sigmoid(w.gate[i]);
+        }
+    }
+    if (a.next) load_eight(a.next, c, a.channels, w.next);
 }
 
-// One workgroup per row: its outputs, and the row's r1, r2 and mean(q v) for
-// the sums over rows.
+// A lane's share of a row as it lies in memory.
 template <class T>
-__global__ void __launch_bounds__(256) k_norm_gradient_rows(Norm<T> a, float* __restrict__ stats) {
-    __shared__ float room[4];
+struct Share {
+    Pack<T, 8> x, d, g;
+};
+
+template <class T>
+__device__ __forceinline__ void load_share(const Norm<T>& a, i64 r, int c, Share<T>& s) {
+    s.x = load_pack(a.x + r * a.x_stride, c, a.channels);
+    if (!a.d) return;
+    s.d = load_pack(a.d + r * a.d_stride, c, a.channels);
+    if (a.gate_kind == SMX_GATE_FULL) s.g = load_pack(a.gate + r * a.gate_stride, c, a.channels);
+}
+
+template <class T>
+__device__ __forceinline__ float gate_at(const Norm<T>& a, const Share<T>& s, const Channels& w, float row_gate, int i) {
+    return a.gate_kind == SMX_GATE_FULL ? sigmoid(static_cast<float>(s.g.v[i]))
+           : a.gate_kind == SMX_GATE_ROW ? row_gate : w.gate[i];
+}
+
+template <class T>
+__device__ __forceinline__ float row_gate_of(const Norm<T>& a, i64 r) {
+    return a.gate_kind == SMX_GATE_ROW ? sigmoid(static_cast<float>(a.gate[r * a.gate_stride])) : 1.0f;
+}
+
+// y of eight channels from column c on; zeros past the end.
+template <class T>
+__device__ __forceinline__ void y_of(const Norm<T>& a, const Share<T>& s, const Channels& w, float r1, float row_gate, int c,
+                                     float (&y)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = static_cast<float>(s.x.v[i]);
+    if (!a.d) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float step = w.scale[i] * gate_at(a, s, w, row_gate, i) * (w.post[i] * (static_cast<float>(s.d.v[i]) * r1));
+        y[i] += c + i < a.channels ? step : 0.0f;
+    }
+}
+
+// G lanes a row, each N times eight neighbouring values in registers, so that
+// a row is read once and its two sums stay between lanes; a lane keeps its channels'
+// weights for all its rows.  A group of 128 channels is 16 lanes, which is where an 8-bit block's
+// scale is found.
+template <class T, int G, int N>
+__global__ void __launch_bounds__(threads_of(G)) k_residual_norm(Norm<T> a) {
+    constexpr int kThreads = threads_of(G), kGroups = kThreads / G;
+    __shared__ typename GroupSum<G, 1>::Room room;
+    const int lane = threadIdx.x % G;
     const float inv = 1.0f / static_cast<float>(a.channels);
-    for (i64 r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const float r1 = d_norm(a, r, room);
-        float r2 = 0.0f, m2 = 0.0f;
-        if (a.gh) {
-            r2 = y_norm(a, r, r1, room);
-            float s = 0.0f;
-            for (int c = threadIdx.x; c < a.channels; c += 256)
-                s += static_cast<float>(a.gh[r * a.gh_stride + c]) * a.next[c] * y_of(a, r, c, r1) * r2;
-            m2 = group_sum(s, room) * inv;
+    Channels w[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) load_channels(a, 8 * (lane + G * n), w[n]);
+    int turn = 0;
+    for (i64 r = static_cast<i64>(blockIdx.x) * kGroups + threadIdx.x / G; r < a.rows;
+         r += static_cast<i64>(gridDim.x) * kGroups) {
+        Share<T> s[N];
+        float sum[1] = {0.0f};
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            load_share(a, r, 8 * (lane + G * n), s[n]);
+            if (a.d)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum[0] += static_cast<float>(s[n].d.v[i]) * static_cast<float>(s[n].d.v[i]);
         }
-        const auto dx_of = [&](int c) {
-            float g = a.gy ? static_cast<float>(a.gy[r * a.gy_stride + c]) : 0.0f;
-            if (a.gh)
-                g += r2 * (static_cast<float>(a.gh[r * a.gh_stride + c]) * a.next[c] - y_of(a, r, c, r1) * r2 * m2);
-            return g;
-        };
-        float m1 = 0.0f, row_gate = 0.0f;
+        float r1 = 0.0f, row_gate = 1.0f;
         if (a.d) {
-            float s = 0.0f, k = 0.0f;
-            for (int c = threadIdx.x; c < a.channels; c += 256) {
-                const float dx = dx_of(c), u = static_cast<float>(a.d[r * a.d_stride + c]) * r1;
-                const float sc = a.scale ? a.scale[c] : 1.0f, sg = gate_of(a, r, c);
-                s += dx * sc * sg * a.post[c] * u;
-                k += dx * sc * a.post[c] * u * sg * (1.0f - sg);
-            }
-            m1 = group_sum(s, room) * inv;
-            row_gate = group_sum(k, room);
+            row_gate = row_gate_of(a, r);
+            GroupSum<G, 1>::sum(sum, room, turn);
+            r1 = rsqrtf(sum[0] * inv + a.eps);
         }
-        __syncthreads();  // dx may lie where gy does
-        for (int c = threadIdx.x; c < a.channels; c += 256) {
-            const float dx = dx_of(c);
-            if (a.d) {
-                const float u = static_cast<float>(a.d[r * a.d_stride + c]) * r1;
-                const float sc = a.scale ? a.scale[c] : 1.0f, sg = gate_of(a, r, c);
-                if (a.dd) a.dd[r * a.dd_stride + c] = static_cast<T>(r1 * (dx * sc * sg * a.post[c] - u * m1));
-                if (a.dgate && a.gate_kind == SMX_GATE_FULL)
-                    a.dgate[r * a.dgate_stride + c] = static_cast<T>(dx * sc * a.post[c] * u * sg * (1.0f - sg));
-            }
-            if (a.dx) a.dx[r * a.dx_stride + c] = static_cast<T>(dx);
+        float y[N][8];
+        sum[0] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int c = 8 * (lane + G * n);
+            y_of(a, s[n], w[n], r1, row_gate, c, y[n]);
+            if (a.y) store_eight(a.y + r * a.y_stride, c, a.channels, y[n]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[0] += y[n][i] * y[n][i];
         }
-        if (threadIdx.x == 0) {
-            if (a.dgate && a.gate_kind == SMX_GATE_ROW) a.dgate[r * a.dgate_stride] = static_cast<T>(row_gate);
-            stats[3 * r] = r1;
-            stats[3 * r + 1] = r2;
-            stats[3 * r + 2] = m2;
+        if (!a.next) continue;
+        GroupSum<G, 1>::sum(sum, room, turn);
+        const float r2 = rsqrtf(sum[0] * inv + a.eps);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int c = 8 * (lane + G * n);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[n][i] = c + i < a.channels ? w[n].next[i] * (y[n][i] * r2) : 0.0f;
+            if (a.h8) {
+                const int pitch = (a.channels + kBlock - 1) / kBlock * kBlock, blocks = pitch / kBlock;
+                const int scale_pitch = (blocks + 3) / 4 * 4, k = c / kBlock;
+                const int byte = block_scale_byte(row_max(top_of(y[n])));
+                if (c < pitch) {
+                    *reinterpret_cast<uint2*>(a.h8 + r * pitch + c) = e4m3_eight(y[n], block_inverse_scale(byte));
+                    std::uint8_t* const at = a.h_scales + r * scale_pitch + k;
+                    const int sub = lane % 16;
+                    if (sub == 0) *at = static_cast<std::uint8_t>(byte);
+                    if (k + 1 == blocks && sub > 0 && k + sub < scale_pitch) at[sub] = 0;
+                }
+            } else {
+                store_eight(a.h + r * a.h_stride, c, a.channels, y[n]);
+            }
         }
     }
 }
 
-// The sums over rows: 64 channels a workgroup, sixteen of its waves' rows at a time.
-template <class T>
-__global__ void __launch_bounds__(1024) k_norm_gradient_channels(Norm<T> a, const float* __restrict__ stats) {
-    __shared__ float part[16][4][64];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = blockIdx.x * 64 + lane;
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (c < a.channels)
-        for (i64 r = wave; r < a.rows; r += 16) {
-            const float r1 = stats[3 * r], r2 = stats[3 * r + 1], m2 = stats[3 * r + 2];
-            float dx = a.gy ? static_cast<float>(a.gy[r * a.gy_stride + c]) : 0.0f;
-            if (a.gh) {
-                const float gh = static_cast<float>(a.gh[r * a.gh_stride + c]), v = y_of(a, r, c, r1) * r2;
-                dx += r2 * (gh * a.next[c] - v * m2);
-                s[3] += gh * v;
-            }
-            if (a.d) {
-                const float u = static_cast<float>(a.d[r * a.d_stride + c]) * r1;
-                const float sc = a.scale ? a.scale[c] : 1.0f, sg = gate_of(a, r, c);
-                s[0] += dx * sc * a.post[c] * u * sg * (1.0f - sg);
-                s[1] += dx * sc * sg * u;
-                s[2] += dx * sg * a.post[c] * u;
-            }
+// What a workgroup adds up over its rows: dgate (of a channel gate), dpost, dscale, dnext.
+constexpr int kSums = 4;
+
+// The gradient of a row in one reading of it, as above.  The sums over rows stay
+// in registers over all rows of a group, are joined in LDS for the workgroup's groups, and leave as one
+// part [kSums][channels] a workgroup.
+template <class T, int G, int N>
+__global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, float* __restrict__ parts) {
+    constexpr int kThreads = threads_of(G), kGroups = kThreads / G;
+    __shared__ union {
+        typename GroupSum<G, 2>::Room room;
+        float join[kGroups > 1 ? kGroups : 1][kGroups > 1 ? G * 8 * N : 1];
+    } lds;
+    const int lane = threadIdx.x % G;
+    const float inv = 1.0f / static_cast<float>(a.channels);
+    Channels w[N];
+    float acc[kSums][N][8];
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        load_channels(a, 8 * (lane + G * n), w[n]);
+#pragma unroll
+        for (int k = 0; k < kSums; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[k][n][i] = 0.0f;
+    }
+    int turn = 0;
+    for (i64 r = static_cast<i64>(blockIdx.x) * kGroups + threadIdx.x / G; r < a.rows;
+         r += static_cast<i64>(gridDim.x) * kGroups) {
+        Share<T> s[N];
+        Pack<T, 8> gy[N], gh[N];
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int c = 8 * (lane + G * n);
+            load_share(a, r, c, s[n]);
+            if (a.gy) gy[n] = load_pack(a.gy + r * a.gy_stride, c, a.channels);
+            if (a.gh) gh[n] = load_pack(a.gh + r * a.gh_stride, c, a.channels);
+            if (a.d)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum[0] += static_cast<float>(s[n].d.v[i]) * static_cast<float>(s[n].d.v[i]);
         }
-    for (int k = 0; k < 4; ++k) part[wave][k][lane] = s[k];
-    __syncthreads();
-    if (wave >= 4 || c >= a.channels) return;
-    float* const out = wave == 0 ? (a.gate_kind == SMX_GATE_CHANNEL ? a.dgate_channel : nullptr)
-                                 : wave == 1 ? a.dpost : wave == 2 ? a.dscale : a.dnext;
+        float r1 = 0.0f, row_gate = 1.0f;
+        if (a.d) {
+            row_gate = row_gate_of(a, r);
+            GroupSum<G, 2>::sum(sum, lds.room, turn);
+            r1 = rsqrtf(sum[0] * inv + a.eps);
+        }
+        float dx[N][8];
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dx[n][i] = a.gy ? static_cast<float>(gy[n].v[i]) : 0.0f;
+        if (a.gh) {
+            float y[N][8];
+            sum[0] = sum[1] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                y_of(a, s[n], w[n], r1, row_gate, 8 * (lane + G * n), y[n]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    sum[0] += y[n][i] * y[n][i];
+                    sum[1] += static_cast<float>(gh[n].v[i]) * w[n].next[i] * y[n][i];
+                }
+            }
+            GroupSum<G, 2>::sum(sum, lds.room, turn);
+            const float r2 = rsqrtf(sum[0] * inv + a.eps), m2 = sum[1] * inv * r2;
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float v = y[n][i] * r2, g = static_cast<float>(gh[n].v[i]);
+                    dx[n][i] += r2 * (g * w[n].next[i] - v * m2);
+                    acc[3][n][i] += g * v;
+                }
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+            if (a.dx) store_eight(a.dx + r * a.dx_stride, 8 * (lane + G * n), a.channels, dx[n]);
+        if (!a.d) continue;
+        float u[N][8], t[N][8];
+        sum[0] = sum[1] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int c = 8 * (lane + G * n);
+            float dg[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float sg = gate_at(a, s[n], w[n], row_gate, i);
+                u[n][i] = static_cast<float>(s[n].d.v[i]) * r1;
+                const float p = dx[n][i] * sg, un = u[n][i] * w[n].post[i];
+                t[n][i] = p * w[n].scale[i] * w[n].post[i];
+                acc[1][n][i] += p * w[n].scale[i] * u[n][i];
+                acc[2][n][i] += p * un;
+                dg[i] = p * w[n].scale[i] * un * (1.0f - sg);
+                acc[0][n][i] += dg[i];
+                sum[0] += t[n][i] * u[n][i];
+                sum[1] += c + i < a.channels ? dg[i] : 0.0f;
+            }
+            if (a.dgate && a.gate_kind == SMX_GATE_FULL) store_eight(a.dgate + r * a.dgate_stride, c, a.channels, dg);
+        }
+        GroupSum<G, 2>::sum(sum, lds.room, turn);
+        const float m1 = sum[0] * inv;
+        if (a.dd)
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t[n][i] = r1 * (t[n][i] - u[n][i] * m1);
+                store_eight(a.dd + r * a.dd_stride, 8 * (lane + G * n), a.channels, t[n]);
+            }
+        if (a.dgate && a.gate_kind == SMX_GATE_ROW && lane == 0)
+            a.dgate[r * a.dgate_stride] = static_cast<T>(sum[1]);
+    }
+    if (!parts) return;
+    float* const part = parts + static_cast<i64>(blockIdx.x) * kSums * a.channels;
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) {
+        if constexpr (kGroups > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) lds.join[threadIdx.x / G][8 * (lane + G * n) + i] = acc[k][n][i];
+            __syncthreads();
+            for (int c = threadIdx.x; c < a.channels; c += kThreads) {
+                float v = lds.join[0][c];
+#pragma unroll
+                for (int g = 1; g < kGroups; ++g) v += lds.join[g][c];
+                part[k * a.channels + c] = v;
+            }
+        } else {
+#pragma unroll
+            for (int n = 0; n < N; ++n) store_eight(part + k * a.channels, 8 * (lane + G * n), a.channels, acc[k][n]);
+        }
+    }
+}
+
+// Adds the workgroups' parts up: 64 channels of one sum a workgroup, its sixteen
+// waves every sixteenth part.
+template <class T>
+__global__ void __launch_bounds__(1024) k_norm_gradient_join(Norm<T> a, const float* __restrict__ parts, int count) {
+    __shared__ float room[16][64];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = blockIdx.x * 64 + lane, k = blockIdx.y;
+    float* const out = k == 0 ? a.dgate_channel : k == 1 ? a.dpost : k == 2 ? a.dscale : a.dnext;
     if (!out) return;
     float sum = 0.0f;
-    for (int w = 0; w < 16; ++w) sum += part[w][wave][lane];
+    if (c < a.channels)
+        for (int p = wave; p < count; p += 16) sum += parts[(static_cast<i64>(p) * kSums + k) * a.channels + c];
+    room[wave][lane] = sum;
+    __syncthreads();
+    if (wave || c >= a.channels) return;
+    for (int w = 1; w < 16; ++w) sum += room[w][lane];
     out[c] = sum;
+}
+
+// f(lanes a row, times eight values a lane) for the forward kernel: up to 16 values
+// a lane, whose row then is in at most 64 lanes up to 1,024 channels.
+template <class F>
+void with_forward_shape(int channels, F&& f) {
+    using std::integral_constant;
+    const auto go = [&](auto g, auto n) { f(g, n); };
+#define SMX_SHAPE(MOST, G, N) \
+    if (channels <= MOST) return go(integral_constant<int, G>{}, integral_constant<int, N>{});
+    SMX_SHAPE(128, 16, 1)
+    SMX_SHAPE(256, 32, 1)
+    SMX_SHAPE(512, 64, 1)
+    SMX_SHAPE(1024, 64, 2)
+    SMX_SHAPE(2048, 256, 1)
+    SMX_SHAPE(4096, 512, 1)
+    SMX_SHAPE(8192, 1024, 1)
+    SMX_SHAPE(16384, 1024, 2)
+}
+
+// For the gradient, which holds five rows and four sums besides: eight values a lane as far as a
+// workgroup goes.
+template <class F>
+void with_gradient_shape(int channels, F&& f) {
+    using std::integral_constant;
+    const auto go = [&](auto g, auto n) { f(g, n); };
+    SMX_SHAPE(128, 16, 1)
+    SMX_SHAPE(256, 32, 1)
+    SMX_SHAPE(512, 64, 1)
+    SMX_SHAPE(1024, 128, 1)
+    SMX_SHAPE(2048, 256, 1)
+    SMX_SHAPE(4096, 512, 1)
+    SMX_SHAPE(8192, 1024, 1)
+    SMX_SHAPE(16384, 1024, 2)
+#undef SMX_SHAPE
+}
+
+constexpr i64 kUnits = 256;  // compute units
+
+// Workgroups of a gradient call, each of which leaves a part: enough to fill the
+// card, and at least four rows a group, so that the parts stay below an eighth of the rows.
+i64 gradient_groups(i64 rows, i64 channels) {
+    i64 groups = 1, threads = 256;
+    with_gradient_shape(static_cast<int>(channels), [&](auto g, auto) {
+        threads = threads_of(g.value);
+        groups = threads / g.value;
+    });
+    const i64 full = kUnits * (threads >= 1024 ? 2 : threads == 512 ? 2 : 4), want = (rows + 4 * groups - 1) / (4 * groups);
+    return want < full ? want : full;
 }
 
 void check_norm(const SmxResidualNormArgs& a) {
@@ -281,14 +481,22 @@ int32_t smx_residual_norm(const SmxResidualNormArgs* args, void* stream) {
                 n.h = static_cast<T*>(a.h);
                 n.h_stride = a.h_stride;
             }
-            k_residual_norm<T><<<static_cast<unsigned>(a.rows < 65536 ? a.rows : 65536), 256, 0,
-                                 static_cast<hipStream_t>(stream)>>>(n);
+            with_forward_shape(n.channels, [&](auto g, auto times) {
+                constexpr int G = decltype(g)::value, N = decltype(times)::value;
+                constexpr int threads = threads_of(G), groups = threads / G;
+                const i64 want = (a.rows + groups - 1) / groups, full = kUnits * (2048 / threads);
+                k_residual_norm<T, G, N><<<static_cast<unsigned>(want < full ? want : full), threads, 0,
+                                           static_cast<hipStream_t>(stream)>>>(n);
+            });
             SMX_LAUNCH_CHECK("k_residual_norm");
         });
     });
 }
 
-int64_t smx_residual_norm_gradient_workspace(int64_t rows, int64_t) { return rows > 0 ? 12 * rows : 0; }
+int64_t smx_residual_norm_gradient_workspace(int64_t rows, int64_t channels) {
+    if (rows <= 0 || channels <= 0 || channels > 16384) return 0;
+    return 4 * kSums * channels * gradient_groups(rows, channels);
+}
 
 int32_t smx_residual_norm_gradient(const SmxResidualNormGradientArgs* args, void* stream) {
     return guarded([&] {
@@ -330,16 +538,21 @@ int32_t smx_residual_norm_gradient(const SmxResidualNormGradientArgs* args, void
             n.dpost = g.dpost;
             n.dscale = g.dscale;
             n.dnext = g.dnext;
-            float* const stats = static_cast<float*>(g.workspace);
+            const bool sums = n.dgate_channel || n.dpost || n.dscale || n.dnext;
+            float* const parts = sums ? static_cast<float*>(g.workspace) : nullptr;
+            const i64 count = a.rows > 0 ? gradient_groups(a.rows, a.channels) : 0;
             if (a.rows > 0) {
-                k_norm_gradient_rows<T><<<static_cast<unsigned>(a.rows < 65536 ? a.rows : 65536), 256, 0,
-                                          static_cast<hipStream_t>(stream)>>>(n, stats);
-                SMX_LAUNCH_CHECK("k_norm_gradient_rows");
+                with_gradient_shape(n.channels, [&](auto lanes, auto times) {
+                    constexpr int G = decltype(lanes)::value, N = decltype(times)::value;
+                    k_norm_gradient<T, G, N><<<static_cast<unsigned>(count), threads_of(G), 0,
+                                               static_cast<hipStream_t>(stream)>>>(n, parts);
+                });
+                SMX_LAUNCH_CHECK("k_norm_gradient");
             }
-            if (n.dgate_channel || n.dpost || n.dscale || n.dnext) {
-                k_norm_gradient_channels<T><<<blocks_for(a.channels, 64), 1024, 0, static_cast<hipStream_t>(stream)>>>(
-                    n, stats);
-                SMX_LAUNCH_CHECK("k_norm_gradient_channels");
+            if (sums) {
+                k_norm_gradient_join<T><<<dim3(blocks_for(a.channels, 64), kSums), 1024, 0,
+                                          static_cast<hipStream_t>(stream)>>>(n, parts, static_cast<int>(count));
+                SMX_LAUNCH_CHECK("k_norm_gradient_join");
             }
         });
     });

@@ -33,11 +33,44 @@ void with_dtype(int dtype, F&& f) {
     }
 }
 
-// N values as they lie in memory
+// N values as they lie in memory, aligned to one of them: global loads and
+// stores of 16 bytes take any alignment on this target.
 template <class T, int N>
-struct alignas(sizeof(T) * N) Pack {
+struct __attribute__((packed, aligned(sizeof(T)))) Pack {
     T v[N];
 };
+
+// Eight values from column c on, zeros past the end.
+template <class T>
+__device__ __forceinline__ Pack<T, 8> load_pack(const T* row, int c, int cols) {
+    if (c + 8 <= cols) return *reinterpret_cast<const Pack<T, 8>*>(row + c);
+    Pack<T, 8> p;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p.v[i] = c + i < cols ? row[c + i] : static_cast<T>(0.0f);
+    return p;
+}
+
+template <class T>
+__device__ __forceinline__ void load_eight(const T* row, int c, int cols, float (&v)[8]) {
+    const Pack<T, 8> p = load_pack(row, c, cols);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(p.v[i]);
+}
+
+// Eight values from column c on, up to the end.
+template <class T>
+__device__ __forceinline__ void store_eight(T* row, int c, int cols, const float (&v)[8]) {
+    Pack<T, 8> p;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p.v[i] = static_cast<T>(v[i]);
+    if (c + 8 <= cols) {
+        *reinterpret_cast<Pack<T, 8>*>(row + c) = p;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c + i < cols) row[c + i] = p.v[i];
+    }
+}
 
 inline void require(bool ok, const char* what) {
     if (!ok) throw std::invalid_argument(what);
@@ -120,6 +153,31 @@ __device__ __forceinline__ unsigned e4m3_four(float a, float b, float c, float d
     int p = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_input(a, inverse), e4m3_input(b, inverse), 0, false);
     p = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_input(c, inverse), e4m3_input(d, inverse), p, true);
     return static_cast<unsigned>(p);
+}
+
+// max(v, v of the lane that the DPP control CTRL names)
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float v) {
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false)));
+}
+
+// the largest of each row of 16 lanes, in all of them
+__device__ __forceinline__ float row_max(float v) {
+    v = dpp_max<0xb1>(v);
+    v = dpp_max<0x4e>(v);
+    v = dpp_max<0x141>(v);
+    return dpp_max<0x140>(v);
+}
+
+__device__ __forceinline__ float top_of(const float (&v)[8]) {
+    float top = finite_magnitude(v[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, finite_magnitude(v[i]));
+    return top;
+}
+
+__device__ __forceinline__ uint2 e4m3_eight(const float (&v)[8], float inverse) {
+    return make_uint2(e4m3_four(v[0], v[1], v[2], v[3], inverse), e4m3_four(v[4], v[5], v[6], v[7], inverse));
 }
 
 }  // namespace node

@@ -23,51 +23,9 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 constexpr i64 kShortSum = 512;
 
-// max(v, v of the lane that the DPP control CTRL names)
-template <int CTRL>
-__device__ __forceinline__ float dpp_max(float v) {
-    return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false)));
-}
-
-// the largest of each row of 16 lanes, in all of them
-__device__ __forceinline__ float row_max(float v) {
-    v = dpp_max<0xb1>(v);
-    v = dpp_max<0x4e>(v);
-    v = dpp_max<0x141>(v);
-    return dpp_max<0x140>(v);
-}
-
-// Eight values from column c on; zeros past the end.  VEC: rows are 16-byte aligned.
-template <class T, bool VEC>
-__device__ __forceinline__ void load_eight(const T* row, i64 c, i64 cols, float (&v)[8]) {
-    if (VEC && c + 8 <= cols) {
-        constexpr int N = 16 / sizeof(T);
-#pragma unroll
-        for (int h = 0; h < 8; h += N) {
-            const Pack<T, N> p = *reinterpret_cast<const Pack<T, N>*>(row + c + h);
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[h + i] = static_cast<float>(p.v[i]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? static_cast<float>(row[c + i]) : 0.0f;
-    }
-}
-
-__device__ __forceinline__ float top_of(const float (&v)[8]) {
-    float top = finite_magnitude(v[0]);
-#pragma unroll
-    for (int i = 1; i < 8; ++i) top = fmaxf(top, finite_magnitude(v[i]));
-    return top;
-}
-
-__device__ __forceinline__ uint2 e4m3_eight(const float (&v)[8], float inverse) {
-    return make_uint2(e4m3_four(v[0], v[1], v[2], v[3], inverse), e4m3_four(v[4], v[5], v[6], v[7], inverse));
-}
-
 // Blocks along the rows: 16 lanes a block, eight values each, so a row's loads
 // and stores are whole lines.  One read of x and one write of a byte a value.
-template <class T, bool VEC>
+template <class T>
 __global__ void __launch_bounds__(256) k_quantize_rows(const T* __restrict__ x, i64 x_stride, i64 rows, i64 cols,
                                                        std::uint8_t* __restrict__ values,
                                                        std::uint8_t* __restrict__ scales, i64 pitch, i64 scale_pitch) {
@@ -77,9 +35,9 @@ __global__ void __launch_bounds__(256) k_quantize_rows(const T* __restrict__ x, 
          g += static_cast<i64>(gridDim.x) * 16) {
         const i64 r = g < (1LL << 32) ? static_cast<unsigned>(g) / blocks : g / blocks;
         const int k = static_cast<int>(g - r * blocks);
-        const i64 c = static_cast<i64>(k) * kBlock + 8 * sub;
+        const int c = k * kBlock + 8 * sub;
         float v[8];
-        load_eight<T, VEC>(x + r * x_stride, c, cols, v);
+        load_eight(x + r * x_stride, c, static_cast<int>(cols), v);
         const int byte = block_scale_byte(row_max(top_of(v)));
         *reinterpret_cast<uint2*>(values + r * pitch + c) = e4m3_eight(v, block_inverse_scale(byte));
         std::uint8_t* const sc = scales + r * scale_pitch + k;
@@ -92,7 +50,7 @@ __global__ void __launch_bounds__(256) k_quantize_rows(const T* __restrict__ x, 
 // the transpose, and along its rows too (ROWS) in the same reading.  A thread
 // holds 8 x 8 values; the transposed bytes cross LDS in pieces of eight, each column's
 // pieces permuted by the column so that the 16 lanes that write at once meet 16 places.
-template <class T, bool VEC, bool ROWS>
+template <class T, bool ROWS>
 __global__ void __launch_bounds__(256) k_quantize_tile(const T* __restrict__ x, i64 x_stride, i64 rows, i64 cols,
                                                        std::uint8_t* __restrict__ values,
                                                        std::uint8_t* __restrict__ scales, i64 pitch, i64 scale_pitch,
@@ -110,7 +68,7 @@ __global__ void __launch_bounds__(256) k_quantize_tile(const T* __restrict__ x, 
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         if (r0 + i < rows)
-            load_eight<T, VEC>(x + (r0 + i) * x_stride, c0, cols, v[i]);
+            load_eight(x + (r0 + i) * x_stride, static_cast<int>(c0), static_cast<int>(cols), v[i]);
         else
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
@@ -201,7 +159,6 @@ struct Product {
     i64 pitch, scale_pitch;
     O* out;
     i64 out_stride;
-    bool vec;        // four outputs of a row may be stored at once
     float* partial;  // [splits][m][n] when the sum is split, else NULL
     int split_blocks;
     int tiles_m, tiles_n;
@@ -223,7 +180,7 @@ __device__ __forceinline__ void store_four(const Product<O>& p, int i, int j, ac
         return;
     }
     O* const at = p.out + i * p.out_stride + j;
-    if (p.vec && j + 4 <= p.n) {
+    if (j + 4 <= p.n) {
         Pack<O, 4> o;
 #pragma unroll
         for (int q = 0; q < 4; ++q) o.v[q] = static_cast<O>(v[q]);
@@ -438,8 +395,8 @@ i64 split_bytes(i64 m, i64 n, i64 k) {
 i64 block_bytes(i64 rows, i64 cols) { return rows * block_stride(cols) + (rows * block_scale_stride(cols) + 15) / 16 * 16; }
 
 void check_sizes(i64 m, i64 n, i64 k) {
-    require(m >= 0 && m < (1LL << 31) && n >= 0 && n < (1LL << 31) && k >= 0 && k < (1LL << 31),
-            "sizes must be in [0, 2^31)");
+    constexpr i64 most = (1LL << 31) - 512;  // indexes of a tile past the end stay in 31 bits
+    require(m >= 0 && m <= most && n >= 0 && n <= most && k >= 0 && k <= most, "sizes must be in [0, 2^31 - 512]");
 }
 
 // a tile of 256 rows is addressed with 31 bits
@@ -454,20 +411,20 @@ void check_blocks(const void* values, const void* scales, i64 rows, i64 cols, co
         throw std::invalid_argument(std::string(name) + ": 8-bit blocks must be 16-byte aligned");
 }
 
-template <class T, bool VEC>
+template <class T>
 void launch_quantize(const T* x, i64 x_stride, i64 rows, i64 cols, std::uint8_t* values, std::uint8_t* scales,
                      std::uint8_t* values_t, std::uint8_t* scales_t, hipStream_t stream) {
     const i64 pitch = block_stride(cols), scale_pitch = block_scale_stride(cols);
     if (!values_t) {
         const i64 groups = (rows * (pitch / kBlock) + 15) / 16;
-        k_quantize_rows<T, VEC><<<static_cast<unsigned>(groups < 65536 ? groups : 65536), 256, 0, stream>>>(
+        k_quantize_rows<T><<<static_cast<unsigned>(groups < 65536 ? groups : 65536), 256, 0, stream>>>(
             x, x_stride, rows, cols, values, scales, pitch, scale_pitch);
         SMX_LAUNCH_CHECK("k_quantize_rows");
         return;
     }
     const i64 tiles = block_stride(rows) / kBlock * (pitch / kBlock);
     require(tiles < (1LL << 31), "the matrix has too many tiles");
-    (values ? k_quantize_tile<T, VEC, true> : k_quantize_tile<T, VEC, false>)<<<static_cast<unsigned>(tiles), 256, 0,
+    (values ? k_quantize_tile<T, true> : k_quantize_tile<T, false>)<<<static_cast<unsigned>(tiles), 256, 0,
                                                                                 stream>>>(
         x, x_stride, rows, cols, values, scales, pitch, scale_pitch, values_t, scales_t, block_stride(rows),
         block_scale_stride(rows));
@@ -477,11 +434,9 @@ void launch_quantize(const T* x, i64 x_stride, i64 rows, i64 cols, std::uint8_t*
 void quantize(const void* x, i64 x_stride, int dtype, i64 rows, i64 cols, std::uint8_t* values, std::uint8_t* scales,
               std::uint8_t* values_t, std::uint8_t* scales_t, hipStream_t stream) {
     if (rows == 0 || cols == 0 || (!values && !values_t)) return;
-    const bool vec = aligned(x, 16) && (rows == 1 || x_stride * size_of(dtype) % 16 == 0);
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        (vec ? launch_quantize<T, true> : launch_quantize<T, false>)(static_cast<const T*>(x), x_stride, rows, cols,
-                                                                    values, scales, values_t, scales_t, stream);
+        launch_quantize(static_cast<const T*>(x), x_stride, rows, cols, values, scales, values_t, scales_t, stream);
     });
 }
 
@@ -508,10 +463,9 @@ void launch_product(const std::uint8_t* a, const std::uint8_t* as, const std::ui
     const Plan plan = plan_product(m, n, k);
     const i64 tiles_m = (m + plan.tile - 1) / plan.tile, tiles_n = (n + plan.tile - 1) / plan.tile;
     require(tiles_m * tiles_n < (1LL << 31) && 8 * tiles_n < (1LL << 31), "the product has too many tiles");
-    const bool vec = aligned(out, 4 * sizeof(O)) && (m == 1 || out_stride % 4 == 0);
     const Product<O> p{a,   as,         b,   bs,
                        static_cast<int>(m), static_cast<int>(n), static_cast<int>(block_stride(k) / kBlock),
-                       block_stride(k),     block_scale_stride(k), out, out_stride, vec,
+                       block_stride(k),     block_scale_stride(k), out, out_stride,
                        plan.splits > 1 ? partial : nullptr, static_cast<int>(plan.split_blocks),
                        static_cast<int>(tiles_m), static_cast<int>(tiles_n)};
     const bool wide = sizeof(O) == 4 || k <= kShortSum;
