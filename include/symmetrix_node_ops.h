@@ -98,9 +98,8 @@ SMX_API int32_t smx_residual_norm(const SmxResidualNormArgs* args, void* stream)
 /* The gradients with respect to every input, from the inputs alone (nothing
  * of the forward call is kept): of a loss whose gradients with respect to y and h
  * are grad_y (NULL: zero) and grad_h (NULL: zero; needs next).  Each output may be NULL
- * (not formed).  dx, dd and a full or row gate's dgate are `dtype`; a channel gate's
- * dgate, dpost, dscale and dnext are FP32 [channels], summed over the rows in a fixed
- * order.  dx may be grad_y. */
+ * (not formed).  dx, dd and dgate (of the gate's shape) are `dtype`; dpost, dscale and dnext are FP32
+ * [channels].  Sums over the rows have a fixed order.  dx may be grad_y. */
 typedef struct SmxResidualNormGradientArgs {
     SmxResidualNormArgs forward; /* y, h and h_scales are not used */
     const void* grad_y;

@@ -7,8 +7,6 @@
 //   q  = H next,     dx = G + r2 (q - v mean(q v)),              dnext  = sum H v
 //   dg = dx a n s (1 - s),   da = sum dx s n,   p = dx a s,      dpost  = sum p u
 //   t  = p post,     dd = r1 (t - u mean(t u))
-#include <type_traits>
-
 #include "node_ops.hpp"
 
 namespace smx {
@@ -32,7 +30,8 @@ struct Norm {
     i64 gy_stride, gh_stride;
     T *dx, *dd, *dgate;
     i64 dx_stride, dd_stride, dgate_stride;
-    float *dgate_channel, *dpost, *dscale, *dnext;
+    T* dgate_channel;
+    float *dpost, *dscale, *dnext;
 };
 
 // 1 / (1 + e^-g) on the hardware exponential and reciprocal, about 2^-22 of it
@@ -64,47 +63,40 @@ struct GroupSum {
 #pragma unroll
                 for (int k = 0; k < K; ++k) room.v[turn][k][threadIdx.x / 64] = v[k];
             __syncthreads();
+            const int w = threadIdx.x % 16;
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                float s = room.v[turn][k][0];
-#pragma unroll
-                for (int w = 1; w < kWaves; ++w) s += room.v[turn][k][w];
-                v[k] = s;
-            }
+            for (int k = 0; k < K; ++k) v[k] = row_total(w < kWaves ? room.v[turn][k][w] : 0.0f);
         }
     }
 };
 
-// What a lane keeps of the channels it holds, for all its rows.
-struct Channels {
-    float post[8], scale[8], next[8], gate[8];  // gate: its sigmoid where no row has another
-};
-
+// What a lane keeps of the channels it holds, for all its rows: scale * post (times the gate, where
+// it is the channel's) and next.
 template <class T>
-__device__ __forceinline__ void load_channels(const Norm<T>& a, int c, Channels& w) {
+__device__ __forceinline__ void load_channels(const Norm<T>& a, int c, float (&step)[8], float (&next)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w.post[i] = w.scale[i] = w.next[i] = 0.0f, w.gate[i] = 1.0f;
+    for (int i = 0; i < 8; ++i) step[i] = next[i] = 0.0f;
     if (a.d) {
-        load_eight(a.post, c, a.channels, w.post);
+        float v[8];
+        load_eight(a.post, c, a.channels, step);
         if (a.scale) {
-            load_eight(a.scale, c, a.channels, w.scale);
-        } else {
+            load_eight(a.scale, c, a.channels, v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w.scale[i] = 1.0f;
+            for (int i = 0; i < 8; ++i) step[i] *= v[i];
         }
         if (a.gate_kind == SMX_GATE_CHANNEL) {
-            load_eight(a.gate, c, a.channels, w.gate);
+            load_eight(a.gate, c, a.channels, v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w.gate[i] = sigmoid(w.gate[i]);
+            for (int i = 0; i < 8; ++i) step[i] *= sigmoid(v[i]);
         }
     }
-    if (a.next) load_eight(a.next, c, a.channels, w.next);
+    if (a.next) load_eight(a.next, c, a.channels, next);
 }
 
 // A lane's share of a row as it lies in memory.
 template <class T>
 struct Share {
-    Pack<T, 8> x, d, g;
+    Eight<T> x, d, g;
 };
 
 template <class T>
@@ -116,28 +108,27 @@ __device__ __forceinline__ void load_share(const Norm<T>& a, i64 r, int c, Share
 }
 
 template <class T>
-__device__ __forceinline__ float gate_at(const Norm<T>& a, const Share<T>& s, const Channels& w, float row_gate, int i) {
-    return a.gate_kind == SMX_GATE_FULL ? sigmoid(static_cast<float>(s.g.v[i]))
-           : a.gate_kind == SMX_GATE_ROW ? row_gate : w.gate[i];
+__device__ __forceinline__ T row_gate_of(const Norm<T>& a, i64 r) {
+    return a.gate_kind == SMX_GATE_ROW ? a.gate[r * a.gate_stride] : static_cast<T>(0.0f);
 }
 
+// scale * post * gate of eight channels; zeros past the end.
 template <class T>
-__device__ __forceinline__ float row_gate_of(const Norm<T>& a, i64 r) {
-    return a.gate_kind == SMX_GATE_ROW ? sigmoid(static_cast<float>(a.gate[r * a.gate_stride])) : 1.0f;
-}
-
-// y of eight channels from column c on; zeros past the end.
-template <class T>
-__device__ __forceinline__ void y_of(const Norm<T>& a, const Share<T>& s, const Channels& w, float r1, float row_gate, int c,
-                                     float (&y)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = static_cast<float>(s.x.v[i]);
-    if (!a.d) return;
+__device__ __forceinline__ void steps_of(const Norm<T>& a, const Share<T>& s, const float (&step)[8], float row_gate,
+                                         float (&gate)[8], float (&f)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float step = w.scale[i] * gate_at(a, s, w, row_gate, i) * (w.post[i] * (static_cast<float>(s.d.v[i]) * r1));
-        y[i] += c + i < a.channels ? step : 0.0f;
+        gate[i] = a.gate_kind == SMX_GATE_FULL ? sigmoid(s.g[i]) : row_gate;
+        f[i] = step[i] * gate[i];
     }
+}
+
+template <class T>
+__device__ __forceinline__ float square_sum(const Eight<T>& d) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += d[i] * d[i];
+    return s;
 }
 
 // G lanes a row, each N times eight neighbouring values in registers, so that
@@ -150,9 +141,9 @@ __global__ void __launch_bounds__(threads_of(G)) k_residual_norm(Norm<T> a) {
     __shared__ typename GroupSum<G, 1>::Room room;
     const int lane = threadIdx.x % G;
     const float inv = 1.0f / static_cast<float>(a.channels);
-    Channels w[N];
+    float step[N][8], next[N][8];
 #pragma unroll
-    for (int n = 0; n < N; ++n) load_channels(a, 8 * (lane + G * n), w[n]);
+    for (int n = 0; n < N; ++n) load_channels(a, 8 * (lane + G * n), step[n], next[n]);
     int turn = 0;
     for (i64 r = static_cast<i64>(blockIdx.x) * kGroups + threadIdx.x / G; r < a.rows;
          r += static_cast<i64>(gridDim.x) * kGroups) {
@@ -161,13 +152,11 @@ __global__ void __launch_bounds__(threads_of(G)) k_residual_norm(Norm<T> a) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             load_share(a, r, 8 * (lane + G * n), s[n]);
-            if (a.d)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sum[0] += static_cast<float>(s[n].d.v[i]) * static_cast<float>(s[n].d.v[i]);
+            if (a.d) sum[0] += square_sum(s[n].d);
         }
         float r1 = 0.0f, row_gate = 1.0f;
         if (a.d) {
-            row_gate = row_gate_of(a, r);
+            if (a.gate_kind == SMX_GATE_ROW) row_gate = sigmoid(static_cast<float>(row_gate_of(a, r)));
             GroupSum<G, 1>::sum(sum, room, turn);
             r1 = rsqrtf(sum[0] * inv + a.eps);
         }
@@ -176,10 +165,17 @@ __global__ void __launch_bounds__(threads_of(G)) k_residual_norm(Norm<T> a) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int c = 8 * (lane + G * n);
-            y_of(a, s[n], w[n], r1, row_gate, c, y[n]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[n][i] = s[n].x[i];
+            if (a.d) {
+                float gate[8], f[8];
+                steps_of(a, s[n], step[n], row_gate, gate, f);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) y[n][i] += f[i] * (s[n].d[i] * r1);
+            }
             if (a.y) store_eight(a.y + r * a.y_stride, c, a.channels, y[n]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum[0] += y[n][i] * y[n][i];
+            for (int i = 0; i < 8; ++i) sum[0] += c + i < a.channels ? y[n][i] * y[n][i] : 0.0f;
         }
         if (!a.next) continue;
         GroupSum<G, 1>::sum(sum, room, turn);
@@ -188,7 +184,7 @@ __global__ void __launch_bounds__(threads_of(G)) k_residual_norm(Norm<T> a) {
         for (int n = 0; n < N; ++n) {
             const int c = 8 * (lane + G * n);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[n][i] = c + i < a.channels ? w[n].next[i] * (y[n][i] * r2) : 0.0f;
+            for (int i = 0; i < 8; ++i) y[n][i] = c + i < a.channels ? next[n][i] * (y[n][i] * r2) : 0.0f;
             if (a.h8) {
                 const int pitch = (a.channels + kBlock - 1) / kBlock * kBlock, blocks = pitch / kBlock;
                 const int scale_pitch = (blocks + 3) / 4 * 4, k = c / kBlock;
@@ -207,117 +203,133 @@ __global__ void __launch_bounds__(threads_of(G)) k_residual_norm(Norm<T> a) {
     }
 }
 
-// What a workgroup adds up over its rows: dgate (of a channel gate), dpost, dscale, dnext.
-constexpr int kSums = 4;
+// What a workgroup adds up over its rows: S = sum dx s u and dnext.  Where the gate is the
+// channel's, or there is none, every other gradient of a channel vector is S times
+// constants of the channel, and dpost = a S, dscale = post S always.
+constexpr int kSums = 2;
 
-// The gradient of a row in one reading of it, as above.  The sums over rows stay
-// in registers over all rows of a group, are joined in LDS for the workgroup's groups, and leave as one
-// part [kSums][channels] a workgroup.
+// The gradient of a row in one reading of it, as above, in two rounds of sums: mean(d^2), and then,
+// with f = a post s and dx = G + r2 q - r2^2 m y, m = r2 mean(q y), those of y^2, q y and the three parts of
+//   sum t u = sum G f u + r2 sum q f u - r2^2 m sum y f u,
+// which is also a row gate's gradient over 1 - s.  The next row is read while
+// one is worked on.  The sums over rows stay in registers over all rows of a group, are joined in LDS for the
+// workgroup's groups, and leave as one part [kSums][channels] a workgroup.
 template <class T, int G, int N>
 __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, float* __restrict__ parts) {
     constexpr int kThreads = threads_of(G), kGroups = kThreads / G;
     __shared__ union {
-        typename GroupSum<G, 2>::Room room;
+        typename GroupSum<G, 5>::Room room;
         float join[kGroups > 1 ? kGroups : 1][kGroups > 1 ? G * 8 * N : 1];
     } lds;
+    struct Row {
+        Share<T> s[N];
+        Eight<T> gy[N], gh[N];
+        T gate;
+    };
     const int lane = threadIdx.x % G;
     const float inv = 1.0f / static_cast<float>(a.channels);
-    Channels w[N];
-    float acc[kSums][N][8];
+    float step[N][8], next[N][8], acc[kSums][N][8];
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        load_channels(a, 8 * (lane + G * n), w[n]);
+        load_channels(a, 8 * (lane + G * n), step[n], next[n]);
 #pragma unroll
         for (int k = 0; k < kSums; ++k)
 #pragma unroll
             for (int i = 0; i < 8; ++i) acc[k][n][i] = 0.0f;
     }
-    int turn = 0;
-    for (i64 r = static_cast<i64>(blockIdx.x) * kGroups + threadIdx.x / G; r < a.rows;
-         r += static_cast<i64>(gridDim.x) * kGroups) {
-        Share<T> s[N];
-        Pack<T, 8> gy[N], gh[N];
-        float sum[2] = {0.0f, 0.0f};
+    const auto read = [&](i64 r, Row& row) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int c = 8 * (lane + G * n);
-            load_share(a, r, c, s[n]);
-            if (a.gy) gy[n] = load_pack(a.gy + r * a.gy_stride, c, a.channels);
-            if (a.gh) gh[n] = load_pack(a.gh + r * a.gh_stride, c, a.channels);
-            if (a.d)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sum[0] += static_cast<float>(s[n].d.v[i]) * static_cast<float>(s[n].d.v[i]);
+            load_share(a, r, c, row.s[n]);
+            if (a.gy) row.gy[n] = load_pack(a.gy + r * a.gy_stride, c, a.channels);
+            if (a.gh) row.gh[n] = load_pack(a.gh + r * a.gh_stride, c, a.channels);
         }
-        float r1 = 0.0f, row_gate = 1.0f;
+        row.gate = row_gate_of(a, r);
+    };
+    // (a workgroup of 16 waves has half the registers a lane: other waves' work covers its reading)
+    constexpr bool kAhead = threads_of(G) <= 512;
+    const i64 hop = static_cast<i64>(gridDim.x) * kGroups;
+    int turn = 0;
+    i64 r = static_cast<i64>(blockIdx.x) * kGroups + threadIdx.x / G;
+    Row row, ahead;
+    if (kAhead && r < a.rows) read(r, row);
+    for (; r < a.rows; r += hop) {
+        if constexpr (!kAhead)
+            read(r, row);
+        else if (r + hop < a.rows)
+            read(r + hop, ahead);
+        float r1 = 0.0f;
+        const float row_gate = a.gate_kind == SMX_GATE_ROW ? sigmoid(static_cast<float>(row.gate)) : 1.0f;
         if (a.d) {
-            row_gate = row_gate_of(a, r);
-            GroupSum<G, 2>::sum(sum, lds.room, turn);
+            float sum[1] = {0.0f};
+#pragma unroll
+            for (int n = 0; n < N; ++n) sum[0] += square_sum(row.s[n].d);
+            GroupSum<G, 1>::sum(sum, *reinterpret_cast<typename GroupSum<G, 1>::Room*>(&lds.room), turn);
             r1 = rsqrtf(sum[0] * inv + a.eps);
         }
-        float dx[N][8];
+        float y[N][8], sum[5] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int n = 0; n < N; ++n)
+        for (int n = 0; n < N; ++n) {
+            const int c = 8 * (lane + G * n);
+            float gate[8], f[8];
+            if (a.d) steps_of(a, row.s[n], step[n], row_gate, gate, f);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) dx[n][i] = a.gy ? static_cast<float>(gy[n].v[i]) : 0.0f;
-        if (a.gh) {
-            float y[N][8];
-            sum[0] = sum[1] = 0.0f;
-#pragma unroll
-            for (int n = 0; n < N; ++n) {
-                y_of(a, s[n], w[n], r1, row_gate, 8 * (lane + G * n), y[n]);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    sum[0] += y[n][i] * y[n][i];
-                    sum[1] += static_cast<float>(gh[n].v[i]) * w[n].next[i] * y[n][i];
+            for (int i = 0; i < 8; ++i) {
+                y[n][i] = row.s[n].x[i];
+                const float q = a.gh ? row.gh[n][i] * next[n][i] : 0.0f;
+                if (a.d) {
+                    const float fu = f[i] * (row.s[n].d[i] * r1);
+                    y[n][i] += fu;
+                    sum[2] += a.gy ? row.gy[n][i] * fu : 0.0f;
+                    sum[3] += q * fu;
+                    sum[4] += y[n][i] * fu;
                 }
+                sum[0] += c + i < a.channels ? y[n][i] * y[n][i] : 0.0f;
+                sum[1] += q * y[n][i];
             }
-            GroupSum<G, 2>::sum(sum, lds.room, turn);
-            const float r2 = rsqrtf(sum[0] * inv + a.eps), m2 = sum[1] * inv * r2;
+        }
+        GroupSum<G, 5>::sum(sum, lds.room, turn);
+        const float r2 = a.gh ? rsqrtf(sum[0] * inv + a.eps) : 0.0f;
+        if constexpr (!kAhead) {
+            // work gate and step out again below: sixteen registers less over the sums' barrier
 #pragma unroll
             for (int n = 0; n < N; ++n)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float v = y[n][i] * r2, g = static_cast<float>(gh[n].v[i]);
-                    dx[n][i] += r2 * (g * w[n].next[i] - v * m2);
-                    acc[3][n][i] += g * v;
+                for (int i = 0; i < Eight<T>::kWords; ++i) {
+                    if (a.gate_kind == SMX_GATE_FULL) asm volatile("" : "+v"(row.s[n].g.w[i]));
+                    asm volatile("" : "+v"(row.s[n].d.w[i]));
+                    asm volatile("" : "+v"(row.gh[n].w[i]));
                 }
         }
-#pragma unroll
-        for (int n = 0; n < N; ++n)
-            if (a.dx) store_eight(a.dx + r * a.dx_stride, 8 * (lane + G * n), a.channels, dx[n]);
-        if (!a.d) continue;
-        float u[N][8], t[N][8];
-        sum[0] = sum[1] = 0.0f;
+        const float ry = r2 * r2 * (r2 * (sum[1] * inv)), tu = sum[2] + r2 * sum[3] - ry * sum[4], m1 = tu * inv;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int c = 8 * (lane + G * n);
-            float dg[8];
+            float gate[8], f[8], dx[8], dd[8], dg[8];
+            if (a.d) steps_of(a, row.s[n], step[n], row_gate, gate, f);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float sg = gate_at(a, s[n], w[n], row_gate, i);
-                u[n][i] = static_cast<float>(s[n].d.v[i]) * r1;
-                const float p = dx[n][i] * sg, un = u[n][i] * w[n].post[i];
-                t[n][i] = p * w[n].scale[i] * w[n].post[i];
-                acc[1][n][i] += p * w[n].scale[i] * u[n][i];
-                acc[2][n][i] += p * un;
-                dg[i] = p * w[n].scale[i] * un * (1.0f - sg);
-                acc[0][n][i] += dg[i];
-                sum[0] += t[n][i] * u[n][i];
-                sum[1] += c + i < a.channels ? dg[i] : 0.0f;
+                dx[i] = a.gy ? row.gy[n][i] : 0.0f;
+                if (a.gh) {
+                    const float g = row.gh[n][i];
+                    dx[i] += r2 * (g * next[n][i]) - ry * y[n][i];
+                    acc[1][n][i] += g * (y[n][i] * r2);
+                }
+                if (a.d) {
+                    const float u = row.s[n].d[i] * r1, t = dx[i] * f[i];
+                    acc[0][n][i] += dx[i] * (gate[i] * u);
+                    dd[i] = r1 * (t - u * m1);
+                    dg[i] = t * u * (1.0f - gate[i]);
+                }
             }
+            if (a.dx) store_eight(a.dx + r * a.dx_stride, c, a.channels, dx);
+            if (a.dd) store_eight(a.dd + r * a.dd_stride, c, a.channels, dd);
             if (a.dgate && a.gate_kind == SMX_GATE_FULL) store_eight(a.dgate + r * a.dgate_stride, c, a.channels, dg);
         }
-        GroupSum<G, 2>::sum(sum, lds.room, turn);
-        const float m1 = sum[0] * inv;
-        if (a.dd)
-#pragma unroll
-            for (int n = 0; n < N; ++n) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) t[n][i] = r1 * (t[n][i] - u[n][i] * m1);
-                store_eight(a.dd + r * a.dd_stride, 8 * (lane + G * n), a.channels, t[n]);
-            }
         if (a.dgate && a.gate_kind == SMX_GATE_ROW && lane == 0)
-            a.dgate[r * a.dgate_stride] = static_cast<T>(sum[1]);
+            a.dgate[r * a.dgate_stride] = static_cast<T>(tu * (1.0f - row_gate));
+        if constexpr (kAhead) row = ahead;
     }
     if (!parts) return;
     float* const part = parts + static_cast<i64>(blockIdx.x) * kSums * a.channels;
@@ -349,8 +361,7 @@ template <class T>
 __global__ void __launch_bounds__(1024) k_norm_gradient_join(Norm<T> a, const float* __restrict__ parts, int count) {
     __shared__ float room[16][64];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = blockIdx.x * 64 + lane, k = blockIdx.y;
-    float* const out = k == 0 ? a.dgate_channel : k == 1 ? a.dpost : k == 2 ? a.dscale : a.dnext;
-    if (!out) return;
+    if (k == 0 ? !a.d && a.rows > 0 : !a.dnext) return;
     float sum = 0.0f;
     if (c < a.channels)
         for (int p = wave; p < count; p += 16) sum += parts[(static_cast<i64>(p) * kSums + k) * a.channels + c];
@@ -358,7 +369,18 @@ __global__ void __launch_bounds__(1024) k_norm_gradient_join(Norm<T> a, const fl
     __syncthreads();
     if (wave || c >= a.channels) return;
     for (int w = 1; w < 16; ++w) sum += room[w][lane];
-    out[c] = sum;
+    if (k == 1) {
+        a.dnext[c] = sum;
+        return;
+    }
+    const float scale = a.scale ? a.scale[c] : 1.0f;
+    float gate = 1.0f;
+    if (a.gate_kind == SMX_GATE_CHANNEL) {  // S was summed without the channel's gate
+        gate = sigmoid(static_cast<float>(a.gate[c]));
+        if (a.dgate_channel) a.dgate_channel[c] = static_cast<T>(sum * a.post[c] * scale * gate * (1.0f - gate));
+    }
+    if (a.dpost) a.dpost[c] = sum * scale * gate;
+    if (a.dscale) a.dscale[c] = sum * a.post[c] * gate;
 }
 
 // f(lanes a row, times eight values a lane) for the forward kernel: up to 16 values
@@ -398,15 +420,15 @@ void with_gradient_shape(int channels, F&& f) {
 
 constexpr i64 kUnits = 256;  // compute units
 
-// Workgroups of a gradient call, each of which leaves a part: enough to fill the
-// card, and at least four rows a group, so that the parts stay below an eighth of the rows.
+// Workgroups of a gradient call, each of which leaves a part: as many as the card holds at once (two
+// waves a SIMD), and at least two rows a group.
 i64 gradient_groups(i64 rows, i64 channels) {
     i64 groups = 1, threads = 256;
     with_gradient_shape(static_cast<int>(channels), [&](auto g, auto) {
         threads = threads_of(g.value);
         groups = threads / g.value;
     });
-    const i64 full = kUnits * (threads >= 1024 ? 2 : threads == 512 ? 2 : 4), want = (rows + 4 * groups - 1) / (4 * groups);
+    const i64 full = kUnits * (threads < 512 ? 512 / threads : 1), want = (rows + 2 * groups - 1) / (2 * groups);
     return want < full ? want : full;
 }
 
@@ -517,7 +539,7 @@ int32_t smx_residual_norm_gradient(const SmxResidualNormGradientArgs* args, void
         if (g.dgate && a.gate_kind == SMX_GATE_FULL)
             check_rows(g.dgate, g.dgate_stride, a.rows, a.channels, a.dtype, "dgate");
         if (g.dgate && a.gate_kind == SMX_GATE_ROW) check_rows(g.dgate, g.dgate_stride, a.rows, 1, a.dtype, "dgate");
-        if (g.dgate && a.gate_kind == SMX_GATE_CHANNEL) require(aligned(g.dgate, 4), "dgate is not aligned to its values");
+        if (g.dgate && a.gate_kind == SMX_GATE_CHANNEL) check_rows(g.dgate, a.channels, 1, a.channels, a.dtype, "dgate");
         check_workspace(g.workspace, g.workspace_bytes, smx_residual_norm_gradient_workspace(a.rows, a.channels));
         with_dtype(a.dtype, [&](auto t) {
             using T = decltype(t);
@@ -531,7 +553,7 @@ int32_t smx_residual_norm_gradient(const SmxResidualNormGradientArgs* args, void
             n.dx_stride = g.dx_stride;
             n.dd_stride = g.dd_stride;
             if (a.gate_kind == SMX_GATE_CHANNEL)
-                n.dgate_channel = static_cast<float*>(g.dgate);
+                n.dgate_channel = static_cast<T*>(g.dgate);
             else
                 n.dgate = static_cast<T*>(g.dgate);
             n.dgate_stride = g.dgate_stride;

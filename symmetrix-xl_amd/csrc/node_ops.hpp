@@ -6,6 +6,7 @@
 #include <new>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "../../include/symmetrix_node_ops.h"
 #include "device_common.hpp"
@@ -40,21 +41,57 @@ struct __attribute__((packed, aligned(sizeof(T)))) Pack {
     T v[N];
 };
 
+// Eight values as the 32-bit words that hold them, so that 16-bit ones wait two in a register.
+template <class T>
+struct Eight {
+    static constexpr int kWords = sizeof(T) * 2;
+    std::uint32_t w[kWords];
+    __device__ __forceinline__ float operator[](int i) const {
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(w[i]);
+        } else if constexpr (std::is_same_v<T, bf16>) {
+            return __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+        } else {
+            return static_cast<float>(__builtin_bit_cast(f16, static_cast<std::uint16_t>(w[i / 2] >> (16 * (i % 2)))));
+        }
+    }
+};
+
+template <class T>
+__device__ __forceinline__ std::uint32_t bits_of(T v) {
+    if constexpr (sizeof(T) == 4)
+        return __builtin_bit_cast(std::uint32_t, v);
+    else
+        return __builtin_bit_cast(std::uint16_t, v);
+}
+
 // Eight values from column c on, zeros past the end.
 template <class T>
-__device__ __forceinline__ Pack<T, 8> load_pack(const T* row, int c, int cols) {
-    if (c + 8 <= cols) return *reinterpret_cast<const Pack<T, 8>*>(row + c);
-    Pack<T, 8> p;
+__device__ __forceinline__ Eight<T> load_pack(const T* row, int c, int cols) {
+    struct __attribute__((packed, aligned(sizeof(T)))) Words {
+        std::uint32_t w[Eight<T>::kWords];
+    };
+    Eight<T> e;
+    if (c + 8 <= cols) {
+        const Words p = *reinterpret_cast<const Words*>(row + c);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p.v[i] = c + i < cols ? row[c + i] : static_cast<T>(0.0f);
-    return p;
+        for (int i = 0; i < Eight<T>::kWords; ++i) e.w[i] = p.w[i];
+        return e;
+    }
+    constexpr int kPer = 4 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < Eight<T>::kWords; ++i) {
+        e.w[i] = c + kPer * i < cols ? bits_of(row[c + kPer * i]) : 0u;
+        if constexpr (kPer == 2) e.w[i] |= c + 2 * i + 1 < cols ? bits_of(row[c + 2 * i + 1]) << 16 : 0u;
+    }
+    return e;
 }
 
 template <class T>
 __device__ __forceinline__ void load_eight(const T* row, int c, int cols, float (&v)[8]) {
-    const Pack<T, 8> p = load_pack(row, c, cols);
+    const Eight<T> p = load_pack(row, c, cols);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(p.v[i]);
+    for (int i = 0; i < 8; ++i) v[i] = p[i];
 }
 
 // Eight values from column c on, up to the end.

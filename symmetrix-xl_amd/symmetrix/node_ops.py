@@ -225,7 +225,7 @@ def _norm_outputs(a, x, y, next_weight, quantized):
 def residual_norm_gradient(x, d, post, gate, scale, next_weight, grad_y, grad_h, eps=1e-6):
     """Gradients ``(x, d, gate, post, scale, next_weight)`` of ``residual_norm`` from its inputs
     and the gradients of ``y`` and ``h`` (either may be None); None for inputs that are None.
-    Those of channel vectors are float32 (a channel gate's in the gate's type)."""
+    Those of ``post``, ``scale`` and ``next_weight`` are float32."""
     a = _norm_args(x, d, post, gate, scale, next_weight, eps)
     r, c = x.shape
     g = _native.SmxResidualNormGradientArgs(a)
@@ -242,7 +242,7 @@ def residual_norm_gradient(x, d, post, gate, scale, next_weight, grad_y, grad_h,
     g.dx, g.dx_stride = dx.data_ptr(), c
     dd = dg = dpost = dscale = dnext = None
     # the channel vectors' gradients share one allocation
-    vectors = torch.empty((4, c), dtype=torch.float32, device=x.device)
+    vectors = torch.empty((3, c), dtype=torch.float32, device=x.device)
     if d is not None:
         dd = torch.empty((r, c), dtype=x.dtype, device=x.device)
         g.dd, g.dd_stride = dd.data_ptr(), c
@@ -252,12 +252,8 @@ def residual_norm_gradient(x, d, post, gate, scale, next_weight, grad_y, grad_h,
             dscale = vectors[1]
             g.dscale = dscale.data_ptr()
         if gate is not None:
-            if a.gate_kind == 2:
-                dg = vectors[3]
-                g.dgate = dg.data_ptr()
-            else:
-                dg = torch.empty(gate.shape, dtype=x.dtype, device=x.device)
-                g.dgate, g.dgate_stride = dg.data_ptr(), gate.shape[1]
+            dg = torch.empty(gate.shape, dtype=x.dtype, device=x.device)
+            g.dgate, g.dgate_stride = dg.data_ptr(), gate.shape[-1]
     if next_weight is not None:
         dnext = vectors[2]
         g.dnext = dnext.data_ptr()
@@ -265,8 +261,6 @@ def residual_norm_gradient(x, d, post, gate, scale, next_weight, grad_y, grad_h,
     room = _workspace(size, x)
     g.workspace, g.workspace_bytes = _at(room), size
     check(lib.smx_residual_norm_gradient(ctypes.byref(g), stream))
-    if dg is not None and dg.dtype is not x.dtype:
-        dg = dg.to(x.dtype)
     return dx, dd, dg, dpost, dscale, dnext
 
 
