@@ -43,7 +43,7 @@ enum { SMX_DTYPE_F32 = 0, SMX_DTYPE_BF16 = 1, SMX_DTYPE_F16 = 2 };
 
 /* out[t][c] = scale * table[types[t]][c].  A type outside [0, num_types) is no
  * species (a masked or padding atom): its row is zero.  types: int32, or int64 when
- * types_are_64bit.  tokens < 2^31. */
+ * types_are_64bit.  Up to 2^31 - 65536 tokens and types. */
 SMX_API int32_t smx_embed(const void* types, int32_t types_are_64bit, int64_t tokens, const void* table,
                           int64_t table_stride, int64_t num_types, int64_t channels, int32_t dtype, float scale,
                           void* out, int64_t out_stride, void* stream);

@@ -13,43 +13,432 @@ __device__ __forceinline__ int type_of(const I* types, i64 t, i64 num_types) {
     return z >= 0 && static_cast<i64>(z) < num_types ? static_cast<int>(z) : -1;
 }
 
-// One thread per value.
+// Lanes that share a row, eight channels each: a power of two up to a wave, which takes wider rows
+// in slabs of 512.
+inline int lanes_of(i64 channels) {
+    int g = 8;
+    while (g < 64 && 8 * g < channels) g *= 2;
+    return g;
+}
+
 template <class T, class I>
 __global__ void __launch_bounds__(256) k_embed(const I* __restrict__ types, i64 tokens, const T* __restrict__ table,
-                                               i64 table_stride, i64 num_types, i64 channels, float scale,
-                                               T* __restrict__ out, i64 out_stride) {
-    for (i64 t = blockIdx.x; t < tokens; t += gridDim.x) {
+                                               i64 table_stride, i64 num_types, int channels, float scale,
+                                               T* __restrict__ out, i64 out_stride, int lanes) {
+    const int groups = 256 / lanes;
+    const int c = 8 * (blockIdx.y * lanes + threadIdx.x % lanes);
+    if (c >= channels) return;
+    for (i64 t = static_cast<i64>(blockIdx.x) * groups + threadIdx.x / lanes; t < tokens;
+         t += static_cast<i64>(gridDim.x) * groups) {
         const int z = type_of(types, t, num_types);
-        for (i64 c = threadIdx.x; c < channels; c += blockDim.x)
-            out[t * out_stride + c] =
-                z < 0 ? static_cast<T>(0.0f) : static_cast<T>(scale * static_cast<float>(table[z * table_stride + c]));
+        float v[8];
+        if (z >= 0) load_eight(table + z * table_stride, c, channels, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = z < 0 ? 0.0f : scale * v[i];
+        store_eight(out + t * out_stride, c, channels, v);
     }
 }
 
-// One workgroup per type and 256 channels: it goes over the atoms' types and
-// adds the rows of its own, in their order.
-template <class T, class I>
-__global__ void __launch_bounds__(256) k_embed_gradient(const I* __restrict__ types, i64 tokens,
-                                                        const T* __restrict__ grad, i64 grad_stride, i64 num_types,
-                                                        i64 channels, float scale, T* __restrict__ out,
-                                                        i64 out_stride) {
-    __shared__ unsigned long long mine[4];
-    const int v = static_cast<int>(blockIdx.x);
-    const i64 c = static_cast<i64>(blockIdx.y) * 256 + threadIdx.x;
-    float sum = 0.0f;
-    for (i64 t0 = 0; t0 < tokens; t0 += 256) {
-        const i64 t = t0 + threadIdx.x;
-        const unsigned long long m = __ballot(t < tokens && type_of(types, t, num_types) == v);
-        if (threadIdx.x % 64 == 0) mine[threadIdx.x / 64] = m;
+// ---- the gradient: atoms sorted by type, then runs of one type added up ----
+//
+// The sort is a stable radix sort of (type, atom), eight bits a pass, least first; types outside the
+// table sort last as num_types.  Up to kSmall atoms one workgroup sorts in LDS; above, tiles of
+// kTile atoms (times up to 512 tiles) are counted, and each pass places a tile's atoms by the counts of all tiles
+// before it and counts the next pass's digits where they land.
+
+constexpr int kDigits = 256, kTile = 2048, kMostTiles = 512, kSmall = 4096;
+
+// the lanes of the wave that are `in` and hold the same digit
+__device__ __forceinline__ unsigned long long same_digit(int digit, bool in) {
+    unsigned long long m = __ballot(in);
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+        const bool one = digit >> b & 1;
+        const unsigned long long w = __ballot(one);
+        m &= one ? w : ~w;
+    }
+    return m;
+}
+
+// What a workgroup of WAVES waves ranks its atoms with.
+template <int WAVES>
+struct RankRoom {
+    int count[WAVES][kDigits];  // of each wave, then the place of each wave's first
+    int total[kDigits];
+    int wave_total[4];
+};
+
+// Exclusive sums over the 256 digits: thread d < 256 gives its value and gets the sum of those before it.
+// Every thread of the workgroup calls it.
+template <int WAVES>
+__device__ __forceinline__ int digits_before(int v, RankRoom<WAVES>& room) {
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    int sum = v;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const int below = __shfl_up(sum, o);
+        if (lane >= o) sum += below;
+    }
+    if (threadIdx.x < kDigits && lane == 63) room.wave_total[wave] = sum;
+    __syncthreads();
+    int before = sum - v;
+    for (int w = 0; w < wave && w < 4; ++w) before += room.wave_total[w];
+    __syncthreads();
+    return before;
+}
+
+// Ranks N atoms a lane (64 neighbouring ones a round, a wave's rounds neighbouring): rank[k] among the wave's
+// atoms of the same digit, the waves' counts in room.count.
+template <int WAVES, int N>
+__device__ __forceinline__ void rank_in_wave(const int (&digit)[N], const bool (&in)[N], int (&rank)[N],
+                                             RankRoom<WAVES>& room) {
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    for (int d = lane; d < kDigits; d += 64) room.count[wave][d] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const unsigned long long same = same_digit(digit[k], in[k]);
+        const int before = __popcll(same & ((1ull << lane) - 1));
+        const int had = in[k] ? room.count[wave][digit[k]] : 0;
+        rank[k] = had + before;
+        __builtin_amdgcn_wave_barrier();
+        if (in[k] && before == 0) room.count[wave][digit[k]] = had + __popcll(same);
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+}
+
+template <class I>
+__device__ __forceinline__ int sort_key(const I* types, i64 t, i64 num_types) {
+    const int z = type_of(types, t, num_types);
+    return z < 0 ? static_cast<int>(num_types) : z;
+}
+
+// One workgroup sorts up to kSmall atoms; the others clear `seen`.
+template <class I>
+__global__ void __launch_bounds__(1024) k_sort_small(const I* __restrict__ types, int tokens, i64 num_types, int bits,
+                                                     int* __restrict__ keys, int* __restrict__ order,
+                                                     std::uint8_t* __restrict__ seen) {
+    constexpr int kWaves = 16, N = kSmall / 1024;
+    __shared__ RankRoom<kWaves> room;
+    __shared__ int skey[kSmall], satom[kSmall];
+    if (blockIdx.x > 0) {
+        for (i64 v = static_cast<i64>(blockIdx.x - 1) * 1024 + threadIdx.x; v < num_types;
+             v += static_cast<i64>(gridDim.x - 1) * 1024)
+            seen[v] = 0;
+        return;
+    }
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    int key[N], atom[N], digit[N], rank[N];
+    bool in[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        atom[k] = wave * 64 * N + 64 * k + lane;
+        in[k] = atom[k] < tokens;
+        key[k] = in[k] ? sort_key(types, atom[k], num_types) : 0;
+    }
+    for (int shift = 0; shift < bits; shift += 8) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) digit[k] = key[k] >> shift & (kDigits - 1);
+        rank_in_wave<kWaves, N>(digit, in, rank, room);
+        int total = 0;
+        if (threadIdx.x < kDigits)
+            for (int w = 0; w < kWaves; ++w) total += room.count[w][threadIdx.x];
+        int place = digits_before<kWaves>(threadIdx.x < kDigits ? total : 0, room);
+        if (threadIdx.x < kDigits)
+            for (int w = 0; w < kWaves; ++w) {
+                const int n = room.count[w][threadIdx.x];
+                room.count[w][threadIdx.x] = place;
+                place += n;
+            }
         __syncthreads();
-        for (int w = 0; w < 4; ++w)
-            for (unsigned long long left = mine[w]; left; left &= left - 1) {
-                const i64 row = t0 + 64 * w + __builtin_ctzll(left);
-                if (c < channels) sum += static_cast<float>(grad[row * grad_stride + c]);
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (in[k]) {
+                const int to = room.count[wave][digit[k]] + rank[k];
+                skey[to] = key[k];
+                satom[to] = atom[k];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int p = wave * 64 * N + 64 * k + lane;
+            if (in[k]) key[k] = skey[p], atom[k] = satom[p];  // (in[k] is that of the place as well)
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+        if (in[k]) keys[wave * 64 * N + 64 * k + lane] = key[k], order[wave * 64 * N + 64 * k + lane] = atom[k];
+}
+
+// Counts the lowest digits of a tile's types; clears the later passes' counts and `seen`.
+template <class I>
+__global__ void __launch_bounds__(256) k_sort_count(const I* __restrict__ types, i64 tokens, i64 num_types, int tile,
+                                                    int* __restrict__ counts, i64 later, std::uint8_t* __restrict__ seen) {
+    __shared__ int count[kDigits];
+    count[threadIdx.x] = 0;
+    __syncthreads();
+    const i64 first = static_cast<i64>(blockIdx.x) * tile, last = first + tile < tokens ? first + tile : tokens;
+    for (i64 t = first + threadIdx.x; t < last; t += 256)
+        atomicAdd(&count[sort_key(types, t, num_types) & (kDigits - 1)], 1);
+    __syncthreads();
+    const i64 hop = static_cast<i64>(gridDim.x) * 256, me = static_cast<i64>(blockIdx.x) * 256 + threadIdx.x;
+    counts[me] = count[threadIdx.x];
+    for (i64 i = hop + me; i < hop + later; i += hop) counts[i] = 0;
+    for (i64 v = me; v < num_types; v += hop) seen[v] = 0;
+}
+
+// One pass: a tile's atoms to their places.  counts: this pass's [tiles][256]; next: the following
+// pass's, or NULL.  The first pass (types given) reads the types themselves.
+template <class I>
+__global__ void __launch_bounds__(256) k_sort_place(const I* __restrict__ types, const int* __restrict__ keys_in,
+                                                    const int* __restrict__ order_in, i64 tokens, i64 num_types, int tile,
+                                                    int shift, const int* __restrict__ counts, int* __restrict__ next,
+                                                    int* __restrict__ keys, int* __restrict__ order) {
+    constexpr int kWaves = 4, N = kTile / 256;
+    __shared__ RankRoom<kWaves> room;
+    __shared__ int base[kDigits];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    int before = 0, total = 0;
+    for (int b = 0; b < static_cast<int>(gridDim.x); ++b) {
+        const int n = counts[b * kDigits + threadIdx.x];
+        before += b < static_cast<int>(blockIdx.x) ? n : 0;
+        total += n;
+    }
+    base[threadIdx.x] = digits_before<kWaves>(total, room) + before;
+    const i64 first = static_cast<i64>(blockIdx.x) * tile, last = first + tile < tokens ? first + tile : tokens;
+    for (i64 at = first; at < last; at += kTile) {
+        int key[N], atom[N], digit[N], rank[N];
+        bool in[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const i64 p = at + wave * 64 * N + 64 * k + lane;
+            in[k] = p < last;
+            key[k] = !in[k] ? 0 : types ? sort_key(types, p, num_types) : keys_in[p];
+            atom[k] = !in[k] ? 0 : types ? static_cast<int>(p) : order_in[p];
+            digit[k] = key[k] >> shift & (kDigits - 1);
+        }
+        rank_in_wave<kWaves, N>(digit, in, rank, room);
+        int place = base[threadIdx.x];
+        for (int w = 0; w < kWaves; ++w) {
+            const int n = room.count[w][threadIdx.x];
+            room.count[w][threadIdx.x] = place;
+            place += n;
+        }
+        base[threadIdx.x] = place;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (in[k]) {
+                const int to = room.count[wave][digit[k]] + rank[k];
+                keys[to] = key[k];
+                order[to] = atom[k];
+                // (a sum of ones: its order does not matter)
+                if (next) atomicAdd(&next[to / tile * kDigits + (key[k] >> (shift + 8) & (kDigits - 1))], 1);
             }
         __syncthreads();
     }
-    if (c < channels) out[v * out_stride + c] = static_cast<T>(scale * sum);
+}
+
+constexpr int kRun = 16;  // sorted atoms a group of lanes adds up
+
+// 256 / lanes groups a workgroup, each kRun sorted atoms of 8 lanes' channels.  A type whose atoms lie
+// within a group is done there; the first and last runs of the groups are joined in LDS, in order; what crosses
+// the workgroup's ends leaves as a part: [0] of a run that goes on from the workgroup before, [1] of one that starts here
+// and goes on in the next.
+template <class T>
+__global__ void __launch_bounds__(256) k_embed_runs(const int* __restrict__ keys, const int* __restrict__ order, i64 tokens,
+                                                    const T* __restrict__ grad, i64 grad_stride, int num_types,
+                                                    int channels, float scale, T* __restrict__ out, i64 out_stride,
+                                                    float* __restrict__ parts, std::uint8_t* __restrict__ seen, int lanes) {
+    __shared__ int piece_key[2 * 32];
+    __shared__ float piece[2 * 256 * 8];
+    const int groups = 256 / lanes, width = 8 * lanes, group = threadIdx.x / lanes, lane = threadIdx.x % lanes;
+    const int c0 = blockIdx.y * width, c = c0 + 8 * lane;
+    const i64 chunk = static_cast<i64>(groups) * kRun, start = blockIdx.x * chunk;
+    const i64 end = start + chunk < tokens ? start + chunk : tokens;
+    const i64 first = start + group * kRun;
+    float acc[8], head[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = head[i] = 0.0f;
+    int current = -1, head_key = -1;  // no run yet
+    bool in_head = true;
+    const auto close = [&]() {
+        if (in_head) {
+            head_key = current;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) head[i] = acc[i];
+            in_head = false;
+        } else if (c < channels) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = scale * acc[i];
+            store_eight(out + static_cast<i64>(current) * out_stride, c, channels, v);
+        }
+        if (lane == 0 && blockIdx.y == 0) seen[current] = 1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
+    };
+#pragma unroll
+    for (int b = 0; b < kRun; b += 8) {
+        int key[8];
+        Eight<T> row[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const i64 p = first + b + j;
+            key[j] = p < end ? keys[p] : num_types;
+            const int atom = p < end ? order[p] : 0;
+#pragma unroll
+            for (int i = 0; i < Eight<T>::kWords; ++i) row[j].w[i] = 0;
+            if (key[j] < num_types && c < channels)
+                row[j] = load_pack(grad + static_cast<i64>(atom) * grad_stride, c, channels);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (key[j] >= num_types) continue;  // past the end, or no species: these sort last
+            if (key[j] != current) {
+                if (current >= 0) close();
+                current = key[j];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) acc[i] += row[j][i];
+        }
+    }
+    // a group's pieces: its first run and, where it has another, its last
+    const bool one = in_head;
+    if (lane == 0) {
+        piece_key[2 * group] = one ? current : head_key;
+        piece_key[2 * group + 1] = one ? -1 : current;
+        if (current >= 0 && blockIdx.y == 0) seen[current] = 1;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        piece[2 * group * width + 8 * lane + i] = one ? acc[i] : head[i];
+        piece[(2 * group + 1) * width + 8 * lane + i] = acc[i];
+    }
+    __syncthreads();
+    const int before = start > 0 ? keys[start - 1] : -1, after = end < tokens ? keys[end] : num_types;
+    for (int w = threadIdx.x; w < width && c0 + w < channels; w += 256) {
+        float sum = 0.0f;
+        int run = -1;
+        bool from_before = false;
+        for (int q = 0; q < 2 * groups; ++q) {
+            const int key = piece_key[q];
+            if (key < 0) continue;
+            if (key != run) {
+                if (run >= 0) {
+                    if (from_before)
+                        parts[(2 * static_cast<i64>(blockIdx.x)) * channels + c0 + w] = sum;
+                    else
+                        out[run * out_stride + c0 + w] = static_cast<T>(scale * sum);
+                }
+                from_before = run < 0 && key == before;
+                run = key;
+                sum = 0.0f;
+            }
+            sum += piece[q * width + w];
+        }
+        if (run < 0) continue;
+        if (from_before)
+            parts[(2 * static_cast<i64>(blockIdx.x)) * channels + c0 + w] = sum;
+        else if (run == after)
+            parts[(2 * static_cast<i64>(blockIdx.x) + 1) * channels + c0 + w] = sum;
+        else
+            out[run * out_stride + c0 + w] = static_cast<T>(scale * sum);
+    }
+}
+
+// Zeros for the types without atoms (workgroups from `chunks` on, a wave a row), and the joins of runs
+// that cross workgroups: workgroup b's, if a run starts in b's atoms and goes on.
+template <class T>
+__global__ void __launch_bounds__(256) k_embed_finish(const int* __restrict__ keys, i64 tokens, int num_types, int channels,
+                                                      float scale, T* __restrict__ out, i64 out_stride,
+                                                      const float* __restrict__ parts,
+                                                      const std::uint8_t* __restrict__ seen, i64 chunk, int chunks) {
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    if (static_cast<int>(blockIdx.x) >= chunks) {
+        const i64 hop = (static_cast<i64>(gridDim.x) - chunks) * 4;
+        for (i64 v = (static_cast<i64>(blockIdx.x) - chunks) * 4 + wave; v < num_types; v += hop) {
+            if (seen[v]) continue;
+            const float zeros[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            for (int c = 8 * lane; c < channels; c += 512) store_eight(out + v * out_stride, c, channels, zeros);
+        }
+        return;
+    }
+    __shared__ float room[4][64];
+    const i64 start = blockIdx.x * chunk, end = start + chunk;
+    if (end >= tokens) return;
+    const int run = keys[end - 1];
+    if (run >= num_types || keys[end] != run) return;
+    if (keys[start] == run && start > 0 && keys[start - 1] == run) return;  // it started before
+    // the first place past the run: the 64 lanes narrow the range down together
+    i64 low = end, high = tokens;
+    while (high - low > 1) {  // keys[low] == run, and keys[high] != run where it exists
+        const i64 hop = (high - low + 63) / 64, p = low + (lane + 1) * hop;
+        const int same = __popcll(__ballot(p < high && keys[p] == run));
+        const i64 up = low + (same + 1) * hop;
+        low += same * hop;
+        high = up < high ? up : high;
+    }
+    const i64 past = low + 1, last = (past - 1) / chunk;  // the workgroup of the run's last atom
+    for (int c0 = 0; c0 < channels; c0 += 64) {
+        const int c = c0 + lane;
+        float sum = 0.0f;
+        if (c < channels) {
+            if (wave == 0) sum = parts[(2 * static_cast<i64>(blockIdx.x) + 1) * channels + c];
+            i64 b = blockIdx.x + 1 + wave;
+            for (; b + 28 <= last; b += 32) {
+                float v[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[k] = parts[2 * (b + 4 * k) * channels + c];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) sum += v[k];
+            }
+            for (; b <= last; b += 4) sum += parts[2 * b * channels + c];
+        }
+        room[wave][lane] = sum;
+        __syncthreads();
+        if (wave == 0 && c < channels)
+            out[run * out_stride + c] = static_cast<T>(scale * ((room[0][lane] + room[1][lane]) + (room[2][lane] + room[3][lane])));
+        __syncthreads();
+    }
+}
+
+// The parts of a gradient call's workspace, in bytes from its start.
+struct Workspace {
+    i64 keys[2], order[2], counts, seen, parts, size;
+    int passes, tile, tiles, lanes, chunks;
+    i64 chunk;
+};
+
+Workspace plan_gradient(i64 tokens, i64 num_types, i64 channels) {
+    Workspace w{};
+    int bits = 1;
+    while (num_types >> bits) ++bits;  // keys run to num_types
+    w.passes = (bits + 7) / 8;
+    w.tile = kTile * static_cast<int>((tokens + static_cast<i64>(kTile) * kMostTiles - 1) / (static_cast<i64>(kTile) * kMostTiles));
+    if (w.tile == 0) w.tile = kTile;
+    w.tiles = static_cast<int>((tokens + w.tile - 1) / w.tile);
+    w.lanes = lanes_of(channels);
+    w.chunk = static_cast<i64>(256 / w.lanes) * kRun;
+    w.chunks = static_cast<int>((tokens + w.chunk - 1) / w.chunk);
+    const auto take = [&](i64 bytes) {
+        const i64 at = w.size;
+        w.size += (bytes + 15) / 16 * 16;
+        return at;
+    };
+    const bool small = tokens <= kSmall;
+    w.keys[0] = take(4 * tokens);
+    w.order[0] = take(4 * tokens);
+    if (!small) {
+        w.keys[1] = take(4 * tokens);
+        w.order[1] = take(4 * tokens);
+        w.counts = take(4LL * kDigits * w.tiles * w.passes);
+    }
+    w.seen = take(num_types);
+    w.parts = take(8LL * w.chunks * channels);
+    return w;
 }
 
 template <class F>
@@ -61,9 +450,10 @@ void with_index(int32_t wide, F&& f) {
 }
 
 void check_embed(const void* types, i64 tokens, i64 num_types, i64 channels, int dtype) {
-    require(tokens >= 0 && tokens < (1LL << 31), "tokens must be in [0, 2^31)");
-    require(num_types >= 0 && num_types < (1LL << 31), "num_types must be in [0, 2^31)");
-    require(channels >= 0 && channels < (1LL << 31), "channels must be in [0, 2^31)");
+    constexpr i64 most = (1LL << 31) - 65536;  // indexes of a tile past the end stay in 31 bits
+    require(tokens >= 0 && tokens <= most, "tokens must be in [0, 2^31 - 65536]");
+    require(num_types >= 0 && num_types <= most, "num_types must be in [0, 2^31 - 65536]");
+    require(channels >= 0 && channels <= 65535 * 512, "channels must be in [0, 65535 * 512]");
     require(dtype >= SMX_DTYPE_F32 && dtype <= SMX_DTYPE_F16, "unknown dtype code");
     require(tokens == 0 || types, "types is NULL");
 }
@@ -89,17 +479,22 @@ int32_t smx_embed(const void* types, int32_t types_are_64bit, int64_t tokens, co
             using T = decltype(t);
             with_index(types_are_64bit, [&](auto i) {
                 using I = decltype(i);
-                k_embed<T, I><<<static_cast<unsigned>(tokens < 65536 ? tokens : 65536), 256, 0,
-                                static_cast<hipStream_t>(stream)>>>(
+                const int lanes = lanes_of(channels), groups = 256 / lanes;
+                const i64 want = (tokens + groups - 1) / groups;
+                k_embed<T, I><<<dim3(static_cast<unsigned>(want < 65536 ? want : 65536), blocks_for(channels, 8 * lanes)), 256,
+                                0, static_cast<hipStream_t>(stream)>>>(
                     static_cast<const I*>(types), tokens, static_cast<const T*>(table), table_stride, num_types,
-                    channels, scale, static_cast<T*>(out), out_stride);
+                    static_cast<int>(channels), scale, static_cast<T*>(out), out_stride, lanes);
                 SMX_LAUNCH_CHECK("k_embed");
             });
         });
     });
 }
 
-int64_t smx_embed_gradient_workspace(int64_t, int64_t, int64_t) { return 0; }
+int64_t smx_embed_gradient_workspace(int64_t tokens, int64_t num_types, int64_t channels) {
+    if (tokens < 0 || num_types <= 0 || channels <= 0) return 0;
+    return plan_gradient(tokens, num_types, channels).size;
+}
 
 int32_t smx_embed_gradient(const void* types, int32_t types_are_64bit, int64_t tokens, const void* grad,
                            int64_t grad_stride, int64_t num_types, int64_t channels, int32_t dtype, float scale,
@@ -110,17 +505,51 @@ int32_t smx_embed_gradient(const void* types, int32_t types_are_64bit, int64_t t
         check_rows(out, out_stride, num_types, channels, dtype, "out");
         check_workspace(workspace, workspace_bytes, smx_embed_gradient_workspace(tokens, num_types, channels));
         if (num_types == 0 || channels == 0) return;
+        const Workspace w = plan_gradient(tokens, num_types, channels);
+        const auto queue = static_cast<hipStream_t>(stream);
+        auto* const base = static_cast<std::uint8_t*>(workspace);
+        const auto ints = [&](i64 at) { return reinterpret_cast<int*>(base + at); };
+        std::uint8_t* const seen = base + w.seen;
+        int at = 0;  // which of the two buffers holds the sorted atoms
+        with_index(types_are_64bit, [&](auto i) {
+            using I = decltype(i);
+            const I* const z = static_cast<const I*>(types);
+            if (tokens <= kSmall) {
+                const unsigned clear = blocks_for(num_types, 16 * 1024);
+                k_sort_small<I><<<1 + (clear < 255 ? clear : 255), 1024, 0, queue>>>(
+                    z, static_cast<int>(tokens), num_types, 8 * w.passes, ints(w.keys[0]), ints(w.order[0]), seen);
+                SMX_LAUNCH_CHECK("k_sort_small");
+                return;
+            }
+            const i64 pass = static_cast<i64>(w.tiles) * kDigits;
+            k_sort_count<I><<<w.tiles, 256, 0, queue>>>(z, tokens, num_types, w.tile, ints(w.counts), (w.passes - 1) * pass,
+                                                        seen);
+            SMX_LAUNCH_CHECK("k_sort_count");
+            for (int p = 0; p < w.passes; ++p, at ^= 1) {
+                int* const counts = ints(w.counts) + p * pass;
+                k_sort_place<I><<<w.tiles, 256, 0, queue>>>(p ? nullptr : z, ints(w.keys[at ^ 1]), ints(w.order[at ^ 1]), tokens,
+                                                            num_types, w.tile, 8 * p, counts,
+                                                            p + 1 < w.passes ? counts + pass : nullptr, ints(w.keys[at]),
+                                                            ints(w.order[at]));
+                SMX_LAUNCH_CHECK("k_sort_place");
+            }
+            at ^= 1;
+        });
         with_dtype(dtype, [&](auto t) {
             using T = decltype(t);
-            with_index(types_are_64bit, [&](auto i) {
-                using I = decltype(i);
-                k_embed_gradient<T, I>
-                    <<<dim3(static_cast<unsigned>(num_types), blocks_for(channels, 256)), 256, 0,
-                       static_cast<hipStream_t>(stream)>>>(static_cast<const I*>(types), tokens,
-                                                           static_cast<const T*>(grad), grad_stride, num_types,
-                                                           channels, scale, static_cast<T*>(out), out_stride);
-                SMX_LAUNCH_CHECK("k_embed_gradient");
-            });
+            auto* const parts = reinterpret_cast<float*>(base + w.parts);
+            if (tokens > 0) {
+                k_embed_runs<T><<<dim3(static_cast<unsigned>(w.chunks), blocks_for(channels, 8 * w.lanes)), 256, 0, queue>>>(
+                    ints(w.keys[at]), ints(w.order[at]), tokens, static_cast<const T*>(grad), grad_stride,
+                    static_cast<int>(num_types), static_cast<int>(channels), scale, static_cast<T*>(out), out_stride, parts,
+                    seen, w.lanes);
+                SMX_LAUNCH_CHECK("k_embed_runs");
+            }
+            const unsigned rows = blocks_for(num_types, 4);
+            k_embed_finish<T><<<static_cast<unsigned>(w.chunks) + (rows < 8192 ? rows : 8192), 256, 0, queue>>>(
+                ints(w.keys[at]), tokens, static_cast<int>(num_types), static_cast<int>(channels), scale,
+                static_cast<T*>(out), out_stride, parts, seen, w.chunk, w.chunks);
+            SMX_LAUNCH_CHECK("k_embed_finish");
         });
     });
 }

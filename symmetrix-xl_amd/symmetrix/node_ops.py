@@ -51,10 +51,41 @@ class BlockValues:
     """A matrix in 8-bit blocks along its rows: E4M3 ``values`` [rows][columns rounded up to
     128] and E8M0 ``scales`` (a byte for each block, four-aligned)."""
 
-    __slots__ = ("values", "scales", "shape")
+    __slots__ = ("shape", "_room", "_at")
 
     def __init__(self, values, scales, shape):
-        self.values, self.scales, self.shape = values, scales, shape
+        self.shape, self._room = tuple(shape), (values, scales)
+        self._at = values.data_ptr(), scales.data_ptr()
+
+    @classmethod
+    def _empty(cls, rows, cols, like):
+        """Room for a matrix: values and then scales in one allocation."""
+        self = cls.__new__(cls)
+        pitch, scale_pitch = _pitches(cols)
+        room = torch.empty(rows * (pitch + scale_pitch), dtype=torch.uint8, device=like.device)
+        self.shape, self._room = (rows, cols), room
+        at = room.data_ptr()
+        self._at = at, at + rows * pitch
+        return self
+
+    def _split(self):
+        if not isinstance(self._room, tuple):
+            rows, cols = self.shape
+            pitch, scale_pitch = _pitches(cols)
+            self._room = (self._room[:rows * pitch].view(torch.float8_e4m3fn).view(rows, pitch),
+                          self._room[rows * pitch:].view(rows, scale_pitch))
+        return self._room
+
+    @property
+    def values(self):
+        return self._split()[0]
+
+    @property
+    def scales(self):
+        return self._split()[1]
+
+    def _device(self):
+        return (self._room[0] if isinstance(self._room, tuple) else self._room).get_device()
 
     def float(self):
         """The values that the blocks stand for, in float32."""
@@ -65,35 +96,53 @@ class BlockValues:
         return torch.ldexp(v, e[:, :, None]).reshape(r, blocks * _BLOCK)[:, :c]
 
 
-def _stream(t):
-    if not t.is_cuda:
+def _pitches(cols):
+    blocks = -(-cols // _BLOCK)
+    return blocks * _BLOCK, -(-blocks // 4) * 4
+
+
+# the current stream's handle without the Stream object around it, which costs more than some of the calls here
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+def _stream(device):
+    if device < 0:
         raise ValueError("node operators take tensors on a HIP device")
-    if t.device.index != torch.cuda.current_device():
+    if device != torch.cuda.current_device():
         raise ValueError("node operators take tensors of the current device")
-    return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(device)
 
 
-def _rows(t, name, like=None, channels=None, rows=None):
-    """Checks a row tensor; its row stride in elements."""
-    if t.dim() != 2:
-        raise ValueError("%s must be two-dimensional" % name)
-    if t.dtype not in _DTYPES:
+def _rows(t, name):
+    """Checks a row tensor; (type code, rows, channels, row stride in elements)."""
+    code = _DTYPES.get(t.dtype)
+    if code is None:
         raise ValueError("%s must be float32, bfloat16 or float16" % name)
-    if like is not None and (t.dtype is not like.dtype or t.device != like.device):
-        raise ValueError("%s must have the type and device of the other rows" % name)
-    r, c = t.shape
-    if (channels is not None and c != channels) or (rows is not None and r != rows):
-        raise ValueError("%s has the wrong shape" % name)
+    shape = t.shape
+    if len(shape) != 2:
+        raise ValueError("%s must be two-dimensional" % name)
+    r, c = shape
     stride, unit = t.stride()
-    if (unit != 1 and c > 1) or (r > 1 and stride < c):
+    if (unit != 1 and c > 1) or (stride < c and r > 1):
         raise ValueError("%s must have unit stride along its channels and rows that do not overlap" % name)
-    return stride if r > 1 else max(stride, c)
+    return code, r, c, stride if r > 1 else c
 
 
-def _vector(t, name, like, channels):
+def _like(t, name, x, shape):
+    """Checks another row tensor of x's type and device; its row stride in elements."""
+    if t.dtype is not x.dtype or t.get_device() != x.get_device():
+        raise ValueError("%s must have the type and device of the other rows" % name)
+    if t.shape != shape:
+        raise ValueError("%s has the wrong shape" % name)
+    return _rows(t, name)[3]
+
+
+def _vector(t, name, x, channels):
     if t is None:
         return None
-    if t.dtype is not torch.float32 or t.device != like.device or t.shape != (channels,) or not t.is_contiguous():
+    if t.dtype is not torch.float32 or t.get_device() != x.get_device() or t.shape != (channels,) \
+            or not t.is_contiguous():
         raise ValueError("%s must be a contiguous float32 vector of the channels, on the rows' device" % name)
     return t.data_ptr()
 
@@ -110,78 +159,81 @@ def _at(t):
 
 
 def _types(types, like):
-    if types.dim() != 1 or types.dtype not in (torch.int32, torch.int64) or not types.is_contiguous() \
-            or types.device != like.device:
+    wide = types.dtype is torch.int64
+    if (not wide and types.dtype is not torch.int32) or types.dim() != 1 or not types.is_contiguous() \
+            or types.get_device() != like.get_device():
         raise ValueError("types must be a contiguous int32 or int64 vector on the rows' device")
-    return 1 if types.dtype is torch.int64 else 0
+    return wide
 
 
 def embed(types, table, scale=1.0):
     """``scale * table[types]``; a type outside the table gives a row of zeros."""
-    stride = _rows(table, "table")
+    code, v, c, stride = _rows(table, "table")
     wide = _types(types, table)
-    stream = _stream(table)
-    t, (v, c) = types.shape[0], table.shape
-    out = torch.empty((t, c), dtype=table.dtype, device=table.device)
-    check(lib.smx_embed(types.data_ptr(), wide, t, table.data_ptr(), stride, v, c, _DTYPES[table.dtype], scale,
-                        out.data_ptr(), c, stream))
+    stream = _stream(table.get_device())
+    t = types.shape[0]
+    out = table.new_empty((t, c))
+    check(lib.smx_embed(types.data_ptr(), wide, t, table.data_ptr(), stride, v, c, code, scale, out.data_ptr(), c,
+                        stream))
     return out
 
 
 def embed_gradient(types, grad, num_types, scale=1.0):
     """The table's gradient [num_types][channels]: for each type, ``scale`` times the sum of
     its atoms' rows of ``grad``, in a fixed order."""
-    stride = _rows(grad, "grad", rows=types.shape[0])
+    code, t, c, stride = _rows(grad, "grad")
+    if types.shape[0] != t:
+        raise ValueError("grad has the wrong shape")
     wide = _types(types, grad)
-    stream = _stream(grad)
-    t, c = grad.shape
-    out = torch.empty((num_types, c), dtype=grad.dtype, device=grad.device)
+    stream = _stream(grad.get_device())
+    out = grad.new_empty((num_types, c))
     size = lib.smx_embed_gradient_workspace(t, num_types, c)
     room = _workspace(size, grad)
-    check(lib.smx_embed_gradient(types.data_ptr(), wide, t, grad.data_ptr(), stride, num_types, c,
-                                 _DTYPES[grad.dtype], scale, out.data_ptr(), c, _at(room), size, stream))
+    check(lib.smx_embed_gradient(types.data_ptr(), wide, t, grad.data_ptr(), stride, num_types, c, code, scale,
+                                 out.data_ptr(), c, _at(room), size, stream))
     return out
 
 
 # ---- residual norm ----
 
 
-def _gate(gate, x):
+def _gate(gate, x, shape):
     """(kind, row stride) of the gate logits."""
-    if gate is None:
-        return 0, 0
-    if gate.dtype is not x.dtype or gate.device != x.device:
+    if gate.dtype is not x.dtype or gate.get_device() != x.get_device():
         raise ValueError("gate must have the type and device of the rows")
-    r, c = x.shape
-    if gate.dim() == 1 and gate.shape[0] == c:
+    r, c = shape
+    given = gate.shape
+    if len(given) == 2 and given == shape and c > 1:
+        return 1, _rows(gate, "gate")[3]
+    if len(given) == 1 and given[0] == c:
         if c > 1 and gate.stride(0) != 1:
             raise ValueError("a channel gate must be contiguous")
         return 2, 0
-    if gate.dim() == 2 and gate.shape == (r, c) and c > 1:
-        return 1, _rows(gate, "gate", x)
-    if gate.dim() == 2 and gate.shape == (r, 1):
+    if len(given) == 2 and given == (r, 1):
         if r > 1 and gate.stride(0) < 1:
             raise ValueError("the rows of a gate must not overlap")
         return 3, max(gate.stride(0), 1)
     raise ValueError("gate must be [rows][channels], [channels] or [rows][1]")
 
 
+_NORM_ARGS = ctypes.sizeof(_native.SmxResidualNormArgs)
+
+
 def _norm_args(x, d, post, gate, scale, next_weight, eps):
-    xs = _rows(x, "x")
-    r, c = x.shape
+    code, r, c, xs = _rows(x, "x")
     if d is None:
         if gate is not None or post is not None or scale is not None:
             raise ValueError("post, gate and scale go with d")
-        ds, kind, gs = 0, 0, 0
-    else:
-        ds = _rows(d, "d", x, c, r)
-        if post is None:
-            raise ValueError("post must be given with d")
-        kind, gs = _gate(gate, x)
-    a = _native.SmxResidualNormArgs(
-        ctypes.sizeof(_native.SmxResidualNormArgs), _DTYPES[x.dtype], r, c, x.data_ptr(), xs, _at(d), ds, _at(gate), gs,
-        kind, eps, _vector(post, "post", x, c), _vector(scale, "scale", x, c), _vector(next_weight, "next_weight", x, c))
-    return a
+        return _native.SmxResidualNormArgs(_NORM_ARGS, code, r, c, x.data_ptr(), xs, None, 0, None, 0, 0, eps, None, None,
+                                           _vector(next_weight, "next_weight", x, c))
+    shape = x.shape
+    ds = _like(d, "d", x, shape)
+    if post is None:
+        raise ValueError("post must be given with d")
+    kind, gs = (0, 0) if gate is None else _gate(gate, x, shape)
+    return _native.SmxResidualNormArgs(
+        _NORM_ARGS, code, r, c, x.data_ptr(), xs, d.data_ptr(), ds, None if gate is None else gate.data_ptr(), gs, kind,
+        eps, _vector(post, "post", x, c), _vector(scale, "scale", x, c), _vector(next_weight, "next_weight", x, c))
 
 
 def residual_norm(x, d, post, gate=None, scale=None, next_weight=None, eps=1e-6, quantized=False):
@@ -191,34 +243,30 @@ def residual_norm(x, d, post, gate=None, scale=None, next_weight=None, eps=1e-6,
     ``gate``: logits, one for each value ([rows][channels]), channel ([channels]) or row
     ([rows][1]); ``post``, ``scale`` and ``next_weight``: float32 [channels]."""
     a = _norm_args(x, d, post, gate, scale, next_weight, eps)
-    stream = _stream(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    h = _norm_outputs(a, x, y, next_weight, quantized)
-    check(lib.smx_residual_norm(ctypes.byref(a), stream))
+    stream = _stream(x.get_device())
+    y = x.new_empty(x.shape)
+    a.y, a.y_stride = y.data_ptr(), a.channels
+    h = None if next_weight is None else _norm_output(a, x, quantized)
+    check(lib.smx_residual_norm(a, stream))
     return y, h
 
 
 def norm(x, weight, eps=1e-6, quantized=False):
     """``weight * x / rms(x)``, as ``BlockValues`` when ``quantized``."""
     a = _norm_args(x, None, None, None, None, weight, eps)
-    stream = _stream(x)
-    h = _norm_outputs(a, x, None, weight, quantized)
-    check(lib.smx_residual_norm(ctypes.byref(a), stream))
+    stream = _stream(x.get_device())
+    h = _norm_output(a, x, quantized)
+    check(lib.smx_residual_norm(a, stream))
     return h
 
 
-def _norm_outputs(a, x, y, next_weight, quantized):
-    r, c = x.shape
-    if y is not None:
-        a.y, a.y_stride = y.data_ptr(), c
-    if next_weight is None:
-        return None
-    if not quantized:
-        h = torch.empty((r, c), dtype=x.dtype, device=x.device)
-        a.h, a.h_stride = h.data_ptr(), c
-        return h
-    h = _empty_blocks(r, c, x.device)
-    a.h, a.h_scales = h.values.data_ptr(), h.scales.data_ptr()
+def _norm_output(a, x, quantized):
+    if quantized:
+        h = BlockValues._empty(a.rows, a.channels, x)
+        a.h, a.h_scales = h._at
+    else:
+        h = x.new_empty(x.shape)
+        a.h, a.h_stride = h.data_ptr(), a.channels
     return h
 
 
@@ -227,95 +275,80 @@ def residual_norm_gradient(x, d, post, gate, scale, next_weight, grad_y, grad_h,
     and the gradients of ``y`` and ``h`` (either may be None); None for inputs that are None.
     Those of ``post``, ``scale`` and ``next_weight`` are float32."""
     a = _norm_args(x, d, post, gate, scale, next_weight, eps)
-    r, c = x.shape
-    g = _native.SmxResidualNormGradientArgs(a)
+    r, c, shape = a.rows, a.channels, x.shape
+    gys = ghs = 0
     if grad_y is not None:
-        g.grad_y_stride = _rows(grad_y, "grad_y", x, c, r)
-        g.grad_y = grad_y.data_ptr()
+        gys = _like(grad_y, "grad_y", x, shape)
     if grad_h is not None:
         if next_weight is None:
             raise ValueError("grad_h without next_weight")
-        g.grad_h_stride = _rows(grad_h, "grad_h", x, c, r)
-        g.grad_h = grad_h.data_ptr()
-    stream = _stream(x)
-    dx = torch.empty((r, c), dtype=x.dtype, device=x.device)
-    g.dx, g.dx_stride = dx.data_ptr(), c
+        ghs = _like(grad_h, "grad_h", x, shape)
+    stream = _stream(x.get_device())
+    dx = x.new_empty(shape)
     dd = dg = dpost = dscale = dnext = None
-    # the channel vectors' gradients share one allocation
-    vectors = torch.empty((3, c), dtype=torch.float32, device=x.device)
     if d is not None:
-        dd = torch.empty((r, c), dtype=x.dtype, device=x.device)
-        g.dd, g.dd_stride = dd.data_ptr(), c
-        dpost = vectors[0]
-        g.dpost = dpost.data_ptr()
+        dd, dpost = x.new_empty(shape), torch.empty_like(post)
         if scale is not None:
-            dscale = vectors[1]
-            g.dscale = dscale.data_ptr()
+            dscale = torch.empty_like(scale)
         if gate is not None:
-            dg = torch.empty(gate.shape, dtype=x.dtype, device=x.device)
-            g.dgate, g.dgate_stride = dg.data_ptr(), gate.shape[-1]
+            dg = x.new_empty(gate.shape)
     if next_weight is not None:
-        dnext = vectors[2]
-        g.dnext = dnext.data_ptr()
+        dnext = torch.empty_like(next_weight)
     size = lib.smx_residual_norm_gradient_workspace(r, c)
     room = _workspace(size, x)
-    g.workspace, g.workspace_bytes = _at(room), size
-    check(lib.smx_residual_norm_gradient(ctypes.byref(g), stream))
+    g = _native.SmxResidualNormGradientArgs(
+        a, _at(grad_y), gys, _at(grad_h), ghs, dx.data_ptr(), c, _at(dd), c, _at(dg),
+        1 if a.gate_kind == 3 else c, _at(dpost), _at(dscale), _at(dnext), _at(room), size)
+    check(lib.smx_residual_norm_gradient(g, stream))
     return dx, dd, dg, dpost, dscale, dnext
 
 
 # ---- 8-bit block product ----
 
 
-def _empty_blocks(rows, cols, device):
-    pitch = -(-cols // _BLOCK) * _BLOCK
-    blocks = pitch // _BLOCK
-    return BlockValues(torch.empty((rows, pitch), dtype=torch.float8_e4m3fn, device=device),
-                       torch.empty((rows, -(-blocks // 4) * 4), dtype=torch.uint8, device=device), (rows, cols))
-
-
 def quantize(x, rows=True, columns=False):
     """``x`` in 8-bit blocks along its rows, or (``columns``) its transpose in blocks along
     x's columns; both, in one pass, as a pair."""
-    stride = _rows(x, "x")
+    code, r, c, stride = _rows(x, "x")
     if not (rows or columns):
         raise ValueError("neither rows nor columns are asked for")
-    stream = _stream(x)
-    r, c = x.shape
-    a = _empty_blocks(r, c, x.device) if rows else None
-    b = _empty_blocks(c, r, x.device) if columns else None
-    check(lib.smx_block_quantize(x.data_ptr(), stride, _DTYPES[x.dtype], r, c, _at(a and a.values),
-                                 _at(a and a.scales), _at(b and b.values), _at(b and b.scales), stream))
+    stream = _stream(x.get_device())
+    a = BlockValues._empty(r, c, x) if rows else None
+    b = BlockValues._empty(c, r, x) if columns else None
+    av, asc = a._at if rows else (None, None)
+    bv, bsc = b._at if columns else (None, None)
+    check(lib.smx_block_quantize(x.data_ptr(), stride, code, r, c, av, asc, bv, bsc, stream))
     return (a, b) if rows and columns else a if rows else b
 
 
 def _check_blocks(b, name, k, device):
     if not isinstance(b, BlockValues):
         raise ValueError("%s must be BlockValues (symmetrix.node_ops.quantize)" % name)
-    if b.shape[1] != k or b.values.device != device:
+    if b.shape[1] != k or b._device() != device:
         raise ValueError("%s must have as many columns as the other operand, on its device" % name)
 
 
 def _product_dtype(dtype):
-    if dtype not in _DTYPES:
+    code = _DTYPES.get(dtype)
+    if code is None:
         raise ValueError("products are float32, bfloat16 or float16")
-    return _DTYPES[dtype]
+    return code
 
 
 def block_product(a, b, dtype=torch.float32):
     """``a @ b.T`` of two ``BlockValues``, [m][k] and [n][k]."""
     if not isinstance(a, BlockValues):
         raise ValueError("a must be BlockValues (symmetrix.node_ops.quantize)")
-    (m, k), n = a.shape, b.shape[0]
-    device = a.values.device
+    m, k = a.shape
+    device = a._device()
     _check_blocks(b, "b", k, device)
+    n = b.shape[0]
     code = _product_dtype(dtype)
-    stream = _stream(a.values)
+    stream = _stream(device)
     out = torch.empty((m, n), dtype=dtype, device=device)
     size = lib.smx_block_product_workspace(m, n, k)
-    room = _workspace(size, a.values)
-    check(lib.smx_block_product(_at(a.values), _at(a.scales), _at(b.values), _at(b.scales), m, n, k, code,
-                                out.data_ptr(), n, _at(room), size, stream))
+    room = _workspace(size, out)
+    check(lib.smx_block_product(*a._at, *b._at, m, n, k, code, out.data_ptr(), n, _at(room), size, stream))
     return out
 
 
@@ -323,22 +356,20 @@ def block_linear(x, w, dtype=None, keep=False):
     """``x @ w.T`` with x [m][k] brought to 8-bit blocks within the call and ``w`` the weights'
     ``BlockValues`` [n][k]; in x's type unless ``dtype`` is given.  With ``keep`` the pair of the
     product and x's column blocks, which ``block_linear_gradient`` takes."""
-    stride = _rows(x, "x")
-    m, k = x.shape
-    _check_blocks(w, "w", k, x.device)
-    if dtype is None:
-        dtype = x.dtype
+    code, m, k, stride = _rows(x, "x")
+    device = x.get_device()
+    _check_blocks(w, "w", k, device)
     if keep:
         rows, columns = quantize(x, columns=True)
-        return block_product(rows, w, dtype), columns
-    code = _product_dtype(dtype)
-    stream = _stream(x)
+        return block_product(rows, w, x.dtype if dtype is None else dtype), columns
+    out_code = code if dtype is None else _product_dtype(dtype)
+    current = _stream(device)
     n = w.shape[0]
-    out = torch.empty((m, n), dtype=dtype, device=x.device)
+    out = x.new_empty((m, n)) if dtype is None else x.new_empty((m, n), dtype=dtype)
     size = lib.smx_block_linear_workspace(m, n, k)
     room = _workspace(size, x)
-    check(lib.smx_block_linear(x.data_ptr(), stride, _DTYPES[x.dtype], _at(w.values), _at(w.scales), m, n, k, code,
-                               out.data_ptr(), n, _at(room), size, stream))
+    check(lib.smx_block_linear(x.data_ptr(), stride, code, *w._at, m, n, k, out_code, out.data_ptr(), n, _at(room), size,
+                               current))
     return out
 
 
