@@ -200,6 +200,13 @@ __device__ __forceinline__ void dma(__amdgpu_buffer_rsrc_t from, unsigned lds, i
                  : "s"(lds), "v"(at), "s"(from), "s"(also)
                  : "memory");
 }
+// 256 bytes, four a lane, as above.
+__device__ __forceinline__ void dma_words(__amdgpu_buffer_rsrc_t from, unsigned lds, int at, int also) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+                 :
+                 : "s"(lds), "v"(at), "s"(from), "s"(also)
+                 : "memory");
+}
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // BM x BN outputs a workgroup of WM x WN waves.  Both operands' blocks of 128
@@ -212,10 +219,11 @@ __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" :
 // four values lie side by side in a row of the output.
 template <class O, bool WIDE, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, (BM + BN) * kBlock * 2 > 81920 ? 1 : 2) k_product_tile(Product<O> p) {
-    constexpr int WAVES = WM * WN, MF = BM / WM / 16, NF = BN / WN / 16, LA = BM / 8 / WAVES, LB = BN / 8 / WAVES;
+    constexpr int WAVES = WM * WN, MF = BM / WM / 16, NF = BN / WN / 16, LA = BM / 8 / WAVES, LB = BN / 8 / WAVES,
+                  LS = ((BM + BN) / 64 + WAVES - 1) / WAVES;
     constexpr unsigned kStage = (BM + BN) * kBlock;
-    static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0);
-    __shared__ __attribute__((aligned(1024))) std::uint8_t lds[2 * kStage];
+    static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && BM % 64 == 0 && BN % 64 == 0);
+    __shared__ __attribute__((aligned(1024))) std::uint8_t lds[2 * kStage + 8 * (BM + BN)];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     // bands of eight tile rows, each band column by column: the tiles that one XCD works on
     // share their rows of both operands in its L2
@@ -253,22 +261,31 @@ __global__ void __launch_bounds__(64 * WM * WN, (BM + BN) * kBlock * 2 > 81920 ?
         for (int q = 0; q < LB; ++q) dma(rb, to + BM * kBlock + q * WAVES * 1024, at_b[q], kb * kBlock);
     };
 
-    // the scales of four blocks are one dword; a wave holds those of its rows, and the next four's
+    // The scales of four blocks are one dword a row, which goes to LDS the same way, 64 rows an
+    // instruction, while the four blocks before are worked on.
     const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
-    const unsigned *sa_at[MF], *sb_at[NF];
-    unsigned sa[MF], sb[NF], sa_next[MF], sb_next[NF];
+    const int scale_pitch = static_cast<int>(p.scale_pitch);
+    __amdgpu_buffer_rsrc_t rs[LS];
+    int at_s[LS];
 #pragma unroll
-    for (int f = 0; f < MF; ++f) {
-        const int r = i0 + wm + 16 * f + lane % 16;
-        sa_at[f] = reinterpret_cast<const unsigned*>(p.as + (r < p.m ? r : p.m - 1) * p.scale_pitch);
-        sa_next[f] = sa_at[f][first / 4];
+    for (int q = 0; q < LS; ++q) {
+        const int w = wave + WAVES * q, rows = w < BM / 64 ? rows_a : rows_b;
+        rs[q] = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<std::uint8_t*>(w < BM / 64 ? p.as + i0 * p.scale_pitch : p.bs + j0 * p.scale_pitch), 0,
+            rows * scale_pitch, 0x00020000);
+        const int r = 64 * (w < BM / 64 ? w : w - BM / 64) + lane;
+        at_s[q] = (r < rows ? r : rows - 1) * scale_pitch;
     }
+    const auto stage_scales = [&](int group) {
 #pragma unroll
-    for (int f = 0; f < NF; ++f) {
-        const int r = j0 + wn + 16 * f + lane % 16;
-        sb_at[f] = reinterpret_cast<const unsigned*>(p.bs + (r < p.n ? r : p.n - 1) * p.scale_pitch);
-        sb_next[f] = sb_at[f][first / 4];
-    }
+        for (int q = 0; q < LS; ++q)
+            if (wave + WAVES * q < (BM + BN) / 64)
+                dma_words(rs[q],
+                          __builtin_amdgcn_readfirstlane(lds0 + 2 * kStage +
+                                                         ((group & 1) * (BM + BN) + 64 * (wave + WAVES * q)) * 4),
+                          at_s[q], 4 * group);
+    };
+    unsigned sa[MF], sb[NF];
 
     acc4 acc[MF][NF];
 #pragma unroll
@@ -277,20 +294,18 @@ __global__ void __launch_bounds__(64 * WM * WN, (BM + BN) * kBlock * 2 > 81920 ?
         for (int g = 0; g < NF; ++g) acc[f][g] = acc4{0.0f, 0.0f, 0.0f, 0.0f};
 
     const int piece = (lane % 16) * kBlock + ((lane / 16) ^ (lane % 16 / 2)) * 16;
+    stage_scales(first / 4);
     stage(first);
     for (int kb = first; kb < last; ++kb) {
         dma_wait();
         __syncthreads();
         if (kb % 4 == 0) {
+            const unsigned* const now = reinterpret_cast<const unsigned*>(lds + 2 * kStage) + (kb / 4 & 1) * (BM + BN) + lane % 16;
 #pragma unroll
-            for (int f = 0; f < MF; ++f) sa[f] = sa_next[f];
+            for (int f = 0; f < MF; ++f) sa[f] = now[wm + 16 * f];
 #pragma unroll
-            for (int f = 0; f < NF; ++f) sb[f] = sb_next[f];
-            const int more = (kb + 4 < last ? kb + 4 : kb) / 4;
-#pragma unroll
-            for (int f = 0; f < MF; ++f) sa_next[f] = sa_at[f][more];
-#pragma unroll
-            for (int f = 0; f < NF; ++f) sb_next[f] = sb_at[f][more];
+            for (int g = 0; g < NF; ++g) sb[g] = now[BM + wn + 16 * g];
+            if (kb + 4 < last) stage_scales(kb / 4 + 1);
         }
         if (kb + 1 < last) stage(kb + 1);
         const std::uint8_t* const ta = lds + (kb & 1) * kStage + wm * kBlock + piece;
@@ -371,10 +386,16 @@ struct Plan {
 
 constexpr int kUnits = 256;  // compute units
 
+// The tile is the one whose rounds over the card take least: a unit holds one tile of 256 at a
+// time, two of 128 or four of 64, whose rates on large products are as 1 : 1/1.12 : 1/1.86 (2,607, 2,322 and
+// 1,401 TFLOP/s at 8192 x 8192 x 8192).  20000 x 1024 x 512: 38.9 us in 316 tiles of 256, two rounds, 28.5 in 1,256 of
+// 128; 4096 x 2048 x 8192 to FP32: 176 and 118 us.
 Plan plan_product(i64 m, i64 n, i64 k) {
     const auto tiles = [&](i64 t) { return (m + t - 1) / t * ((n + t - 1) / t); };
+    const auto rounds = [&](i64 t, i64 held) { return (tiles(t) + held * kUnits - 1) / (held * kUnits); };
     const i64 blocks = (k + kBlock - 1) / kBlock;
-    Plan p{tiles(256) >= kUnits ? 256 : tiles(128) >= kUnits / 2 ? 128 : 64, 1, blocks};
+    const double t256 = 1.0 * rounds(256, 1), t128 = 1.12 / 2 * rounds(128, 2), t64 = 1.86 / 4 * rounds(64, 4);
+    Plan p{t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64, 1, blocks};
     const i64 count = tiles(p.tile);
     if (p.tile == 64 && count < kUnits && blocks >= 8) {
         const i64 want = (2 * kUnits + count - 1) / count, most = blocks / 4;
