@@ -9,8 +9,8 @@
 //   - bf16: an E4M3 value times its scale is a bf16 value exactly (v_cvt_scalef32_pk_bf16_fp8), and
 //     v_mfma_f32_16x16x32_bf16 sums as FP32 does, at half the rate.  (Values below 2^-126 count as zero there.)
 // FP32 outputs take the bf16 form, so that their sums are FP32 sums.  16-bit outputs, which are rounded
-// to 2^-9 or 2^-12 anyway, take the 8-bit form, but for short sums (up to 512), where a call is bound by its
-// memory and the bf16 form costs nothing.
+// to 2^-9 or 2^-12 anyway, take the 8-bit form, but for short sums (up to 256), whose FP32 error is below what the
+// adder drops (20000 x 1024 x 512: 28.9 us in the bf16 form, 22.9 in the 8-bit one).
 #include "node_ops.hpp"
 
 namespace smx {
@@ -21,7 +21,7 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
-constexpr i64 kShortSum = 512;
+constexpr i64 kShortSum = 256;
 
 // Blocks along the rows: 16 lanes a block, eight values each, so a row's loads
 // and stores are whole lines.  One read of x and one write of a byte a value.
@@ -207,24 +207,32 @@ __device__ __forceinline__ void dma_words(__amdgpu_buffer_rsrc_t from, unsigned 
                  : "s"(lds), "v"(at), "s"(from), "s"(also)
                  : "memory");
 }
-__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// until at most N of the wave's memory operations are under way (they end in order)
+template <int N>
+__device__ __forceinline__ void dma_wait() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
 
-// BM x BN outputs a workgroup of WM x WN waves.  Both operands' blocks of 128
-// go to LDS by dma, two stages deep: while one block is multiplied, the next arrives.  A row's
-// eight 16-byte pieces are permuted by half the row's number (in the global
+// BM x BN outputs a workgroup of WM x WN x KG waves.  Both operands' blocks of 128
+// go to LDS by dma, KG blocks at a time and STAGES deep: while some are multiplied, the next ones
+// arrive.  A row's eight 16-byte pieces are permuted by half the row's number (in the global
 // addresses, within one line), so that the 16 rows that a fragment read meets at once lie in
 // 16 different places of the 64 banks.  Lane l holds row l % 16 of a fragment and pieces l / 16 and
 // l / 16 + 4 of the block: the order of k inside a block is the operands' own affair, as one
 // scale covers it.  The accumulator's lane l holds column l % 16 of rows 4 (l / 16) on; with b as the first operand its
-// four values lie side by side in a row of the output.
-template <class O, bool WIDE, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN, (BM + BN) * kBlock * 2 > 81920 ? 1 : 2) k_product_tile(Product<O> p) {
-    constexpr int WAVES = WM * WN, MF = BM / WM / 16, NF = BN / WN / 16, LA = BM / 8 / WAVES, LB = BN / 8 / WAVES,
-                  LS = ((BM + BN) / 64 + WAVES - 1) / WAVES;
-    constexpr unsigned kStage = (BM + BN) * kBlock;
-    static_assert(BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0 && BM % 64 == 0 && BN % 64 == 0);
-    __shared__ __attribute__((aligned(1024))) std::uint8_t lds[2 * kStage + 8 * (BM + BN)];
+// four values lie side by side in a row of the output.  With KG > 1, for few tiles, KG groups of waves
+// take every KG-th block each, so that their waits overlap, and their sums are joined in LDS.
+template <class O, bool WIDE, int BM, int BN, int WM, int WN, int KG, int STAGES>
+__global__ void __launch_bounds__(64 * WM * WN * KG, (BM + BN) * kBlock * KG * STAGES > 81920 ? 1 : 2)
+k_product_tile(Product<O> p) {
+    constexpr int WAVES = WM * WN * KG, MF = BM / WM / 16, NF = BN / WN / 16, LA = BM / 8 * KG / WAVES,
+                  LB = BN / 8 * KG / WAVES, LS = ((BM + BN) / 64 + WAVES - 1) / WAVES;
+    constexpr unsigned kOne = (BM + BN) * kBlock, kStage = kOne * KG;
+    static_assert(BM * KG % (8 * WAVES) == 0 && BN * KG % (8 * WAVES) == 0 && BM % 64 == 0 && BN % 64 == 0 && 4 % KG == 0);
+    static_assert(KG == 1 || STAGES * kStage >= WAVES * MF * NF * 1024);
+    __shared__ __attribute__((aligned(1024))) std::uint8_t lds[STAGES * kStage + 8 * (BM + BN)];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int kg = wave / (WM * WN), in_group = wave % (WM * WN);
     // bands of eight tile rows, each band column by column: the tiles that one XCD works on
     // share their rows of both operands in its L2
     const int id = xcd_remap(blockIdx.x, gridDim.x);
@@ -234,36 +242,39 @@ __global__ void __launch_bounds__(64 * WM * WN, (BM + BN) * kBlock * 2 > 81920 ?
     const int first = blockIdx.y * p.split_blocks;
     const int last = first + p.split_blocks < p.blocks ? first + p.split_blocks : p.blocks;
 
+    // (what a group reads past the last block, within the buffers' ranges, is not used)
     const int rows_a = p.m - i0 < BM ? p.m - i0 : BM, rows_b = p.n - j0 < BN ? p.n - j0 : BN;
     const int pitch = static_cast<int>(p.pitch);
     const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<std::uint8_t*>(p.a + i0 * p.pitch), 0, rows_a * pitch, 0x00020000);
     const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<std::uint8_t*>(p.b + j0 * p.pitch), 0, rows_b * pitch, 0x00020000);
-    int at_a[LA], at_b[LB];
+    int at_a[LA], at_b[LB], to_a[LA], to_b[LB];
 #pragma unroll
     for (int q = 0; q < LA; ++q) {
-        const int r = 8 * (wave + WAVES * q) + lane / 8;
-        at_a[q] = (r < rows_a ? r : rows_a - 1) * pitch + ((lane % 8) ^ (r / 2 % 8)) * 16;
+        const int w = wave + WAVES * q, b = w / (BM / 8), r = 8 * (w % (BM / 8)) + lane / 8;
+        at_a[q] = (r < rows_a ? r : rows_a - 1) * pitch + ((lane % 8) ^ (r / 2 % 8)) * 16 + b * kBlock;
+        to_a[q] = b * kOne + w % (BM / 8) * 1024;
     }
 #pragma unroll
     for (int q = 0; q < LB; ++q) {
-        const int r = 8 * (wave + WAVES * q) + lane / 8;
-        at_b[q] = (r < rows_b ? r : rows_b - 1) * pitch + ((lane % 8) ^ (r / 2 % 8)) * 16;
+        const int w = wave + WAVES * q, b = w / (BN / 8), r = 8 * (w % (BN / 8)) + lane / 8;
+        at_b[q] = (r < rows_b ? r : rows_b - 1) * pitch + ((lane % 8) ^ (r / 2 % 8)) * 16 + b * kBlock;
+        to_b[q] = b * kOne + BM * kBlock + w % (BN / 8) * 1024;
     }
     const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<std::uintptr_t>(
         (__attribute__((address_space(3))) std::uint8_t*)lds));
-    const auto stage = [&](int kb) {
-        const unsigned to = __builtin_amdgcn_readfirstlane(lds0 + (kb & 1) * kStage + wave * 1024);
+    const auto stage = [&](int kb, int slot) {
+        const unsigned to = __builtin_amdgcn_readfirstlane(lds0 + slot * kStage);
 #pragma unroll
-        for (int q = 0; q < LA; ++q) dma(ra, to + q * WAVES * 1024, at_a[q], kb * kBlock);
+        for (int q = 0; q < LA; ++q) dma(ra, to + to_a[q], at_a[q], kb * kBlock);
 #pragma unroll
-        for (int q = 0; q < LB; ++q) dma(rb, to + BM * kBlock + q * WAVES * 1024, at_b[q], kb * kBlock);
+        for (int q = 0; q < LB; ++q) dma(rb, to + to_b[q], at_b[q], kb * kBlock);
     };
 
     // The scales of four blocks are one dword a row, which goes to LDS the same way, 64 rows an
     // instruction, while the four blocks before are worked on.
-    const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+    const int wm = in_group / WN * (BM / WM), wn = in_group % WN * (BN / WN);
     const int scale_pitch = static_cast<int>(p.scale_pitch);
     __amdgpu_buffer_rsrc_t rs[LS];
     int at_s[LS];
@@ -281,7 +292,7 @@ __global__ void __launch_bounds__(64 * WM * WN, (BM + BN) * kBlock * 2 > 81920 ?
         for (int q = 0; q < LS; ++q)
             if (wave + WAVES * q < (BM + BN) / 64)
                 dma_words(rs[q],
-                          __builtin_amdgcn_readfirstlane(lds0 + 2 * kStage +
+                          __builtin_amdgcn_readfirstlane(lds0 + STAGES * kStage +
                                                          ((group & 1) * (BM + BN) + 64 * (wave + WAVES * q)) * 4),
                           at_s[q], 4 * group);
     };
@@ -295,69 +306,102 @@ __global__ void __launch_bounds__(64 * WM * WN, (BM + BN) * kBlock * 2 > 81920 ?
 
     const int piece = (lane % 16) * kBlock + ((lane / 16) ^ (lane % 16 / 2)) * 16;
     stage_scales(first / 4);
-    stage(first);
-    for (int kb = first; kb < last; ++kb) {
-        dma_wait();
+#pragma unroll
+    for (int q = 0; q < STAGES - 1; ++q)
+        if (first + q * KG < last) stage(first + q * KG, q);
+    int slot = 0;
+    for (int kb = first; kb < last; kb += KG) {
+        // a stage is there when only the stages after it are under way (scales under way besides are
+        // counted as if they were blocks': the wait is then for more)
+        if (kb + (STAGES - 2) * KG < last)
+            dma_wait<(STAGES - 2) * (LA + LB)>();
+        else
+            dma_wait<0>();
         __syncthreads();
         if (kb % 4 == 0) {
-            const unsigned* const now = reinterpret_cast<const unsigned*>(lds + 2 * kStage) + (kb / 4 & 1) * (BM + BN) + lane % 16;
+            const unsigned* const now = reinterpret_cast<const unsigned*>(lds + STAGES * kStage) + (kb / 4 & 1) * (BM + BN) + lane % 16;
 #pragma unroll
-            for (int f = 0; f < MF; ++f) sa[f] = now[wm + 16 * f];
+            for (int f = 0; f < MF; ++f) sa[f] = now[wm + 16 * f] >> (8 * kg);
 #pragma unroll
-            for (int g = 0; g < NF; ++g) sb[g] = now[BM + wn + 16 * g];
+            for (int g = 0; g < NF; ++g) sb[g] = now[BM + wn + 16 * g] >> (8 * kg);
             if (kb + 4 < last) stage_scales(kb / 4 + 1);
         }
-        if (kb + 1 < last) stage(kb + 1);
-        const std::uint8_t* const ta = lds + (kb & 1) * kStage + wm * kBlock + piece;
-        const std::uint8_t* const tb = lds + (kb & 1) * kStage + (BM + wn) * kBlock + piece;
-        const std::uint8_t* const ta2 = lds + (kb & 1) * kStage + wm * kBlock + (piece ^ 64);
-        const std::uint8_t* const tb2 = lds + (kb & 1) * kStage + (BM + wn) * kBlock + (piece ^ 64);
-        const auto fragment = [](const std::uint8_t* lo, const std::uint8_t* hi, int f) {
-            const i32x4 x = *reinterpret_cast<const i32x4*>(lo + 16 * kBlock * f);
-            const i32x4 y = *reinterpret_cast<const i32x4*>(hi + 16 * kBlock * f);
-            return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-        };
-        i32x8 vb[NF];
+        const int before = slot == 0 ? STAGES - 1 : slot - 1;  // read by all before the barrier
+        if (kb + (STAGES - 1) * KG < last) stage(kb + (STAGES - 1) * KG, before);
+        if (KG == 1 || kb + kg < last) {
+            const std::uint8_t* const tile = lds + slot * kStage + kg * kOne;
+            const auto fragment = [&](int row) {
+                const i32x4 x = *reinterpret_cast<const i32x4*>(tile + row * kBlock + piece);
+                const i32x4 y = *reinterpret_cast<const i32x4*>(tile + row * kBlock + (piece ^ 64));
+                return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+            };
+            i32x8 vb[NF];
 #pragma unroll
-        for (int g = 0; g < NF; ++g) vb[g] = fragment(tb, tb2, g);
-        if constexpr (!WIDE) {
-#pragma unroll
-            for (int f = 0; f < MF; ++f) {
-                const i32x8 va = fragment(ta, ta2, f);
-#pragma unroll
-                for (int g = 0; g < NF; ++g)
-                    acc[f][g] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vb[g], va, acc[f][g], 0, 0, 0, sb[g],
-                                                                                0, sa[f]);
-            }
-        } else {
-            i32x8 va[MF];
-#pragma unroll
-            for (int f = 0; f < MF; ++f) va[f] = fragment(ta, ta2, f);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                bf16x8 wb[NF];
-#pragma unroll
-                for (int g = 0; g < NF; ++g) wb[g] = to_bf16(vb[g][2 * q], vb[g][2 * q + 1], scale_of(sb[g] & 0xff));
+            for (int g = 0; g < NF; ++g) vb[g] = fragment(BM + wn + 16 * g);
+            if constexpr (!WIDE) {
 #pragma unroll
                 for (int f = 0; f < MF; ++f) {
-                    const bf16x8 wa = to_bf16(va[f][2 * q], va[f][2 * q + 1], scale_of(sa[f] & 0xff));
+                    const i32x8 va = fragment(wm + 16 * f);
 #pragma unroll
                     for (int g = 0; g < NF; ++g)
-                        acc[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[g], wa, acc[f][g], 0, 0, 0);
+                        acc[f][g] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vb[g], va, acc[f][g], 0, 0, 0,
+                                                                                    sb[g], 0, sa[f]);
+                }
+            } else {
+                i32x8 va[MF];
+#pragma unroll
+                for (int f = 0; f < MF; ++f) va[f] = fragment(wm + 16 * f);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    bf16x8 wb[NF];
+#pragma unroll
+                    for (int g = 0; g < NF; ++g)
+                        wb[g] = to_bf16(vb[g][2 * q], vb[g][2 * q + 1], scale_of(sb[g] & 0xff));
+#pragma unroll
+                    for (int f = 0; f < MF; ++f) {
+                        const bf16x8 wa = to_bf16(va[f][2 * q], va[f][2 * q + 1], scale_of(sa[f] & 0xff));
+#pragma unroll
+                        for (int g = 0; g < NF; ++g)
+                            acc[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[g], wa, acc[f][g], 0, 0, 0);
+                    }
                 }
             }
+            if constexpr (KG > 1) mfma_settle();  // (the block is conditional)
         }
 #pragma unroll
-        for (int f = 0; f < MF; ++f) sa[f] >>= 8;
+        for (int f = 0; f < MF; ++f) sa[f] = KG < 4 ? sa[f] >> (8 * KG) : 0;
 #pragma unroll
-        for (int g = 0; g < NF; ++g) sb[g] >>= 8;
+        for (int g = 0; g < NF; ++g) sb[g] = KG < 4 ? sb[g] >> (8 * KG) : 0;
+        slot = slot + 1 == STAGES ? 0 : slot + 1;
     }
     mfma_settle();
+    const auto put = [&](int f, int g, acc4 v) {
+        store_four(p, i0 + wm + 16 * f + lane % 16, j0 + wn + 16 * g + 4 * (lane / 16), v, blockIdx.y);
+    };
+    if constexpr (KG == 1) {
 #pragma unroll
-    for (int f = 0; f < MF; ++f)
+        for (int f = 0; f < MF; ++f)
 #pragma unroll
-        for (int g = 0; g < NF; ++g)
-            store_four(p, i0 + wm + 16 * f + lane % 16, j0 + wn + 16 * g + 4 * (lane / 16), acc[f][g], blockIdx.y);
+            for (int g = 0; g < NF; ++g) put(f, g, acc[f][g]);
+    } else {
+        // fragment q of every group is added up, in the groups' order, by group q % KG
+        acc4* const room = reinterpret_cast<acc4*>(lds);
+        const auto at = [&](int group, int q) {
+            return room + ((group * WM * WN + in_group) * MF * NF + q) * 64 + lane;
+        };
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < MF * NF; ++q) *at(kg, q) = acc[q / NF][q % NF];
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < MF * NF; ++q) {
+            if (q % KG != kg) continue;
+            acc4 sum = *at(0, q);
+#pragma unroll
+            for (int h = 1; h < KG; ++h) sum += *at(h, q);
+            put(q / NF, q % NF, sum);
+        }
+    }
 }
 
 // Joins the parts of a split sum, in their order.
@@ -379,7 +423,8 @@ __global__ void __launch_bounds__(256) k_product_zero(O* __restrict__ out, i64 o
 
 // How a product is cut: the tile, and parts of the summed axis.
 struct Plan {
-    int tile;  // 256, 128 or 64
+    int tile;    // 256, 128 or 64
+    int groups;  // of waves that share a tile's blocks: 1, or 4 for few tiles of 64
     int splits;
     i64 split_blocks;
 };
@@ -395,13 +440,16 @@ Plan plan_product(i64 m, i64 n, i64 k) {
     const auto rounds = [&](i64 t, i64 held) { return (tiles(t) + held * kUnits - 1) / (held * kUnits); };
     const i64 blocks = (k + kBlock - 1) / kBlock;
     const double t256 = 1.0 * rounds(256, 1), t128 = 1.12 / 2 * rounds(128, 2), t64 = 1.86 / 4 * rounds(64, 4);
-    Plan p{t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64, 1, blocks};
+    Plan p{t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64, 1, 1, blocks};
     const i64 count = tiles(p.tile);
-    if (p.tile == 64 && count < kUnits && blocks >= 8) {
-        const i64 want = (2 * kUnits + count - 1) / count, most = blocks / 4;
-        const i64 parts = want < most ? want : most;
-        p.split_blocks = ((blocks + parts - 1) / parts + 3) / 4 * 4;  // scales are read four blocks at a time
-        p.splits = static_cast<int>((blocks + p.split_blocks - 1) / p.split_blocks);
+    if (p.tile == 64 && count <= 2 * kUnits && blocks >= 4) {
+        p.groups = 4;
+        // parts of at least eight blocks, up to a tile for each unit
+        const i64 want = kUnits / count, most = blocks / 8, parts = want < most ? want : most;
+        if (parts > 1) {
+            p.split_blocks = ((blocks + parts - 1) / parts + 3) / 4 * 4;  // scales are read four blocks at a time
+            p.splits = static_cast<int>((blocks + p.split_blocks - 1) / p.split_blocks);
+        }
     }
     return p;
 }
@@ -465,9 +513,13 @@ template <class O, bool WIDE>
 void launch_tiles(const Product<O>& p, const Plan& plan, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>(p.tiles_m * p.tiles_n), static_cast<unsigned>(plan.splits));
     switch (plan.tile) {
-        case 256: k_product_tile<O, WIDE, 256, 256, 2, 4><<<grid, 512, 0, stream>>>(p); break;
-        case 128: k_product_tile<O, WIDE, 128, 128, 2, 2><<<grid, 256, 0, stream>>>(p); break;
-        default: k_product_tile<O, WIDE, 64, 64, 2, 2><<<grid, 256, 0, stream>>>(p); break;
+        case 256: k_product_tile<O, WIDE, 256, 256, 2, 4, 1, 2><<<grid, 512, 0, stream>>>(p); break;
+        case 128: k_product_tile<O, WIDE, 128, 128, 2, 2, 1, 2><<<grid, 256, 0, stream>>>(p); break;
+        default:
+            if (plan.groups == 1)
+                k_product_tile<O, WIDE, 64, 64, 2, 2, 1, 2><<<grid, 256, 0, stream>>>(p);
+            else
+                k_product_tile<O, WIDE, 64, 64, 2, 2, 4, 2><<<grid, 1024, 0, stream>>>(p);
     }
     SMX_LAUNCH_CHECK("k_product_tile");
 }
