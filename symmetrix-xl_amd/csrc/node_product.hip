@@ -404,6 +404,113 @@ k_product_tile(Product<O> p) {
     }
 }
 
+// Rows that k_product_rows takes, and those up to which its waves bring x to 8 bits themselves: that
+// work is done again for every 16 or 32 columns.
+constexpr i64 kFewRows = 16;
+constexpr int kRawRows = 4;
+
+// Up to 16 rows of a: 16 NF columns a workgroup, its KS waves every KS-th block each, joined in LDS.  The
+// weights' bytes are all of it, so they go straight to registers, kAhead blocks of them under way at once; a
+// wave brings its blocks of x to 8 bits itself (RAW: up to kRawRows rows of x as they are given), eight values a lane, which
+// cross LDS to the lanes of the fragment.  Fragment rows past the last row hold some row again and are not stored.
+template <class T, class O, bool RAW, bool WIDE, int NF, int KS>
+__global__ void __launch_bounds__(64 * KS) k_product_rows(Product<O> p, const T* __restrict__ x, i64 x_stride, int k) {
+    constexpr int kAhead = 4;
+    __shared__ acc4 room[KS][NF][64];
+    __shared__ __attribute__((aligned(16))) std::uint8_t brought[RAW ? KS : 1][RAW ? kAhead : 1][kRawRows * kBlock];
+    __shared__ int brought_scale[RAW ? KS : 1][RAW ? kAhead : 1][kRawRows];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, row = lane % 16, at = lane / 16 * 16;
+    const int j0 = xcd_remap(blockIdx.x, gridDim.x) * 16 * NF;
+    const std::uint8_t *b[NF], *bs[NF];
+#pragma unroll
+    for (int g = 0; g < NF; ++g) {
+        const int j = j0 + 16 * g + row < p.n ? j0 + 16 * g + row : p.n - 1;
+        b[g] = p.b + j * p.pitch + at;
+        bs[g] = p.bs + j * p.scale_pitch;
+    }
+    const int ia = row < p.m ? row : p.m - 1;
+    const int from = lane / 16 < p.m ? lane / 16 : p.m - 1;  // RAW: the row and values that this lane brings
+    const T* const xr = RAW ? x + from * x_stride : nullptr;
+    const std::uint8_t* const ar = RAW ? nullptr : p.a + ia * p.pitch + at;
+    acc4 acc[NF];
+#pragma unroll
+    for (int g = 0; g < NF; ++g) acc[g] = acc4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int kb0 = wave; kb0 < p.blocks; kb0 += KS * kAhead) {
+        i32x4 wb[kAhead][NF][2], wa[kAhead][2];
+        int sb[kAhead][NF], sa[kAhead];
+        Eight<T> v[kAhead];
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {
+            const int kb = kb0 + q * KS < p.blocks ? kb0 + q * KS : kb0;  // (a block read twice is used once)
+#pragma unroll
+            for (int g = 0; g < NF; ++g) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    wb[q][g][h] = *reinterpret_cast<const i32x4*>(b[g] + static_cast<i64>(kb) * kBlock + 64 * h);
+                sb[q][g] = bs[g][kb];
+            }
+            if constexpr (RAW) {
+                v[q] = load_pack(xr, kb * kBlock + 8 * row, k);
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    wa[q][h] = *reinterpret_cast<const i32x4*>(ar + static_cast<i64>(kb) * kBlock + 64 * h);
+                sa[q] = p.as[ia * p.scale_pitch + kb];
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {
+            if constexpr (RAW) {
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[i] = v[q][i];
+                const int byte = block_scale_byte(row_max(top_of(f)));
+                *reinterpret_cast<uint2*>(&brought[wave][q][8 * lane]) = e4m3_eight(f, block_inverse_scale(byte));
+                if (row == 0) brought_scale[wave][q][lane / 16] = byte;
+            }
+        }
+        if constexpr (RAW) {
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int q = 0; q < kAhead; ++q) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    wa[q][h] = *reinterpret_cast<const i32x4*>(&brought[wave][q][row % kRawRows * kBlock + at + 64 * h]);
+                sa[q] = brought_scale[wave][q][row % kRawRows];
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {
+            if (kb0 + q * KS >= p.blocks) break;
+            const i32x8 va = __builtin_shufflevector(wa[q][0], wa[q][1], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+            for (int g = 0; g < NF; ++g) {
+                const i32x8 vb = __builtin_shufflevector(wb[q][g][0], wb[q][g][1], 0, 1, 2, 3, 4, 5, 6, 7);
+                if constexpr (WIDE) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            to_bf16(vb[2 * e], vb[2 * e + 1], scale_of(sb[q][g])),
+                            to_bf16(va[2 * e], va[2 * e + 1], scale_of(sa[q])), acc[g], 0, 0, 0);
+                } else {
+                    acc[g] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vb, va, acc[g], 0, 0, 0, sb[q][g], 0, sa[q]);
+                }
+            }
+            mfma_settle();  // (the next block is conditional)
+        }
+    }
+    mfma_settle();
+#pragma unroll
+    for (int g = 0; g < NF; ++g) room[wave][g][lane] = acc[g];
+    __syncthreads();
+    if (wave >= NF) return;
+    acc4 sum = room[0][wave][lane];
+#pragma unroll
+    for (int w = 1; w < KS; ++w) sum += room[w][wave][lane];
+    store_four(p, row, j0 + 16 * wave + 4 * (lane / 16), sum, 0);
+}
+
 // Joins the parts of a split sum, in their order.
 template <class O>
 __global__ void __launch_bounds__(256) k_product_join(Product<O> p, int splits) {
@@ -455,7 +562,7 @@ Plan plan_product(i64 m, i64 n, i64 k) {
 }
 
 i64 split_bytes(i64 m, i64 n, i64 k) {
-    if (m <= 0 || n <= 0 || k <= 0) return 0;
+    if (m <= kFewRows || n <= 0 || k <= 0) return 0;
     const Plan p = plan_product(m, n, k);
     return p.splits > 1 ? 4 * p.splits * m * n : 0;
 }
@@ -524,6 +631,41 @@ void launch_tiles(const Product<O>& p, const Plan& plan, hipStream_t stream) {
     SMX_LAUNCH_CHECK("k_product_tile");
 }
 
+template <class T, class O, bool RAW>
+void launch_rows(Product<O> p, const T* x, i64 x_stride, i64 k, hipStream_t stream) {
+    const bool wide = sizeof(O) == 4 || k <= kShortSum;
+    // 32 columns a workgroup where that is one for each unit, else 16
+    const auto go = [&](auto w, auto nf) {
+        constexpr int NF = decltype(nf)::value, KS = 8;
+        k_product_rows<T, O, RAW, decltype(w)::value, NF, KS><<<blocks_for(p.n, 16 * NF), 64 * KS, 0, stream>>>(
+            p, x, x_stride, static_cast<int>(k));
+    };
+    const auto with_form = [&](auto w) {
+        using std::integral_constant;
+        if (p.n >= 32 * kUnits)
+            go(w, integral_constant<int, 2>{});
+        else
+            go(w, integral_constant<int, 1>{});
+    };
+    if (wide)
+        with_form(std::true_type{});
+    else
+        with_form(std::false_type{});
+    SMX_LAUNCH_CHECK("k_product_rows");
+}
+
+template <class O>
+Product<O> product_of(const std::uint8_t* a, const std::uint8_t* as, const std::uint8_t* b, const std::uint8_t* bs, i64 m,
+                      i64 n, i64 k, O* out, i64 out_stride) {
+    Product<O> p{};
+    p.a = a, p.as = as, p.b = b, p.bs = bs;
+    p.m = static_cast<int>(m), p.n = static_cast<int>(n);
+    p.blocks = static_cast<int>(block_stride(k) / kBlock);
+    p.pitch = block_stride(k), p.scale_pitch = block_scale_stride(k);
+    p.out = out, p.out_stride = out_stride;
+    return p;
+}
+
 template <class O>
 void launch_product(const std::uint8_t* a, const std::uint8_t* as, const std::uint8_t* b, const std::uint8_t* bs, i64 m,
                     i64 n, i64 k, O* out, i64 out_stride, float* partial, hipStream_t stream) {
@@ -533,14 +675,17 @@ void launch_product(const std::uint8_t* a, const std::uint8_t* as, const std::ui
         SMX_LAUNCH_CHECK("k_product_zero");
         return;
     }
+    Product<O> p = product_of(a, as, b, bs, m, n, k, out, out_stride);
+    if (m <= kFewRows) {
+        launch_rows<O, O, false>(p, nullptr, 0, k, stream);
+        return;
+    }
     const Plan plan = plan_product(m, n, k);
     const i64 tiles_m = (m + plan.tile - 1) / plan.tile, tiles_n = (n + plan.tile - 1) / plan.tile;
     require(tiles_m * tiles_n < (1LL << 31) && 8 * tiles_n < (1LL << 31), "the product has too many tiles");
-    const Product<O> p{a,   as,         b,   bs,
-                       static_cast<int>(m), static_cast<int>(n), static_cast<int>(block_stride(k) / kBlock),
-                       block_stride(k),     block_scale_stride(k), out, out_stride,
-                       plan.splits > 1 ? partial : nullptr, static_cast<int>(plan.split_blocks),
-                       static_cast<int>(tiles_m), static_cast<int>(tiles_n)};
+    p.partial = plan.splits > 1 ? partial : nullptr;
+    p.split_blocks = static_cast<int>(plan.split_blocks);
+    p.tiles_m = static_cast<int>(tiles_m), p.tiles_n = static_cast<int>(tiles_n);
     const bool wide = sizeof(O) == 4 || k <= kShortSum;
     (wide ? launch_tiles<O, true> : launch_tiles<O, false>)(p, plan, stream);
     if (plan.splits > 1) {
@@ -599,7 +744,7 @@ int32_t smx_block_product(const uint8_t* a_values, const uint8_t* a_scales, cons
 }
 
 int64_t smx_block_linear_workspace(int64_t m, int64_t n, int64_t k) {
-    if (m <= 0 || n <= 0 || k <= 0) return 0;
+    if (m <= kRawRows || n <= 0 || k <= 0) return 0;
     return block_bytes(m, k) + split_bytes(m, n, k);
 }
 
@@ -616,6 +761,18 @@ int32_t smx_block_linear(const void* x, int64_t x_stride, int32_t dtype, const u
         check_summed(k);
         check_workspace(workspace, workspace_bytes, smx_block_linear_workspace(m, n, k));
         if (m == 0 || n == 0) return;
+        if (m <= kRawRows && k > 0) {
+            with_dtype(dtype, [&](auto t) {
+                with_dtype(out_dtype, [&](auto o) {
+                    using T = decltype(t);
+                    using O = decltype(o);
+                    launch_rows<T, O, true>(product_of<O>(nullptr, nullptr, w_values, w_scales, m, n, k, static_cast<O*>(out),
+                                                          out_stride),
+                                            static_cast<const T*>(x), x_stride, k, static_cast<hipStream_t>(stream));
+                });
+            });
+            return;
+        }
         auto* const values = static_cast<std::uint8_t*>(workspace);
         std::uint8_t* const scales = k > 0 ? values + m * block_stride(k) : nullptr;
         auto* const partial = k > 0 ? reinterpret_cast<float*>(values + block_bytes(m, k)) : nullptr;
