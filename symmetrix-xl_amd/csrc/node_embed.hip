@@ -189,24 +189,32 @@ __global__ void __launch_bounds__(256) k_sort_count(const I* __restrict__ types,
     for (i64 v = me; v < num_types; v += hop) seen[v] = 0;
 }
 
-// One pass: a tile's atoms to their places.  counts: this pass's [tiles][256]; next: the following
+// One pass: a tile's atoms to their places, sixteen waves a workgroup (a pass is latency: its reads of the
+// counts, its scan and its scattered stores).  counts: this pass's [tiles][256]; next: the following
 // pass's, or NULL.  The first pass (types given) reads the types themselves.
 template <class I>
-__global__ void __launch_bounds__(256) k_sort_place(const I* __restrict__ types, const int* __restrict__ keys_in,
-                                                    const int* __restrict__ order_in, i64 tokens, i64 num_types, int tile,
-                                                    int shift, const int* __restrict__ counts, int* __restrict__ next,
-                                                    int* __restrict__ keys, int* __restrict__ order) {
-    constexpr int kWaves = 4, N = kTile / 256;
+__global__ void __launch_bounds__(1024) k_sort_place(const I* __restrict__ types, const int* __restrict__ keys_in,
+                                                     const int* __restrict__ order_in, i64 tokens, i64 num_types, int tile,
+                                                     int shift, const int* __restrict__ counts, int* __restrict__ next,
+                                                     int* __restrict__ keys, int* __restrict__ order) {
+    constexpr int kWaves = 16, N = kTile / 1024;
     __shared__ RankRoom<kWaves> room;
-    __shared__ int base[kDigits];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    __shared__ int base[kDigits], part[2][4][kDigits];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, mine = threadIdx.x % kDigits, quarter = threadIdx.x / kDigits;
     int before = 0, total = 0;
-    for (int b = 0; b < static_cast<int>(gridDim.x); ++b) {
-        const int n = counts[b * kDigits + threadIdx.x];
+#pragma unroll 8
+    for (int b = quarter; b < static_cast<int>(gridDim.x); b += 4) {
+        const int n = counts[b * kDigits + mine];
         before += b < static_cast<int>(blockIdx.x) ? n : 0;
         total += n;
     }
-    base[threadIdx.x] = digits_before<kWaves>(total, room) + before;
+    part[0][quarter][mine] = before;
+    part[1][quarter][mine] = total;
+    __syncthreads();
+    before = part[0][0][mine] + part[0][1][mine] + part[0][2][mine] + part[0][3][mine];
+    total = part[1][0][mine] + part[1][1][mine] + part[1][2][mine] + part[1][3][mine];
+    const int start = digits_before<kWaves>(total, room) + before;
+    if (threadIdx.x < kDigits) base[mine] = start;
     const i64 first = static_cast<i64>(blockIdx.x) * tile, last = first + tile < tokens ? first + tile : tokens;
     for (i64 at = first; at < last; at += kTile) {
         int key[N], atom[N], digit[N], rank[N];
@@ -220,13 +228,15 @@ __global__ void __launch_bounds__(256) k_sort_place(const I* __restrict__ types,
             digit[k] = key[k] >> shift & (kDigits - 1);
         }
         rank_in_wave<kWaves, N>(digit, in, rank, room);
-        int place = base[threadIdx.x];
-        for (int w = 0; w < kWaves; ++w) {
-            const int n = room.count[w][threadIdx.x];
-            room.count[w][threadIdx.x] = place;
-            place += n;
+        if (threadIdx.x < kDigits) {
+            int place = base[mine];
+            for (int w = 0; w < kWaves; ++w) {
+                const int n = room.count[w][mine];
+                room.count[w][mine] = place;
+                place += n;
+            }
+            base[mine] = place;
         }
-        base[threadIdx.x] = place;
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < N; ++k)
@@ -350,23 +360,26 @@ __global__ void __launch_bounds__(256) k_embed_runs(const int* __restrict__ keys
 }
 
 // Zeros for the types without atoms (workgroups from `chunks` on, a wave a row), and the joins of runs
-// that cross workgroups: workgroup b's, if a run starts in b's atoms and goes on.
+// that cross workgroups: workgroup b's, if a run starts in b's atoms and goes on.  A run of few parts is
+// added up by a thread a channel; one of many (thousands of atoms of a species) by sixteen waves, four channels
+// a lane, a sixteenth of the parts each.
 template <class T>
-__global__ void __launch_bounds__(256) k_embed_finish(const int* __restrict__ keys, i64 tokens, int num_types, int channels,
-                                                      float scale, T* __restrict__ out, i64 out_stride,
-                                                      const float* __restrict__ parts,
-                                                      const std::uint8_t* __restrict__ seen, i64 chunk, int chunks) {
+__global__ void __launch_bounds__(1024) k_embed_finish(const int* __restrict__ keys, i64 tokens, int num_types, int channels,
+                                                       float scale, T* __restrict__ out, i64 out_stride,
+                                                       const float* __restrict__ parts,
+                                                       const std::uint8_t* __restrict__ seen, i64 chunk, int chunks) {
+    constexpr int kWaves = 16;
+    __shared__ Pack<float, 4> room[kWaves][64];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     if (static_cast<int>(blockIdx.x) >= chunks) {
-        const i64 hop = (static_cast<i64>(gridDim.x) - chunks) * 4;
-        for (i64 v = (static_cast<i64>(blockIdx.x) - chunks) * 4 + wave; v < num_types; v += hop) {
+        const i64 hop = (static_cast<i64>(gridDim.x) - chunks) * kWaves;
+        for (i64 v = (static_cast<i64>(blockIdx.x) - chunks) * kWaves + wave; v < num_types; v += hop) {
             if (seen[v]) continue;
             const float zeros[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
             for (int c = 8 * lane; c < channels; c += 512) store_eight(out + v * out_stride, c, channels, zeros);
         }
         return;
     }
-    __shared__ float room[4][64];
     const i64 start = blockIdx.x * chunk, end = start + chunk;
     if (end >= tokens) return;
     const int run = keys[end - 1];
@@ -381,26 +394,43 @@ __global__ void __launch_bounds__(256) k_embed_finish(const int* __restrict__ ke
         low += same * hop;
         high = up < high ? up : high;
     }
-    const i64 past = low + 1, last = (past - 1) / chunk;  // the workgroup of the run's last atom
-    for (int c0 = 0; c0 < channels; c0 += 64) {
-        const int c = c0 + lane;
-        float sum = 0.0f;
-        if (c < channels) {
-            if (wave == 0) sum = parts[(2 * static_cast<i64>(blockIdx.x) + 1) * channels + c];
-            i64 b = blockIdx.x + 1 + wave;
-            for (; b + 28 <= last; b += 32) {
-                float v[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) v[k] = parts[2 * (b + 4 * k) * channels + c];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) sum += v[k];
-            }
-            for (; b <= last; b += 4) sum += parts[2 * b * channels + c];
+    const i64 last = low / chunk;  // the workgroup of the run's last atom
+    const float* const mine = parts + (2 * static_cast<i64>(blockIdx.x) + 1) * channels;
+    const i64 hop = 2LL * channels;
+    if (last - blockIdx.x <= 2 * kWaves) {
+        for (int c = threadIdx.x; c < channels; c += 1024) {
+            float sum = mine[c];
+            const float* at = parts + (static_cast<i64>(blockIdx.x) + 1) * hop + c;
+            for (i64 b = blockIdx.x + 1; b <= last; ++b, at += hop) sum += *at;
+            out[run * out_stride + c] = static_cast<T>(scale * sum);
         }
-        room[wave][lane] = sum;
+        return;
+    }
+    for (int c0 = 0; c0 < channels; c0 += 256) {
+        const int c = c0 + 4 * lane;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const auto add = [&](const float* part) {
+            if (c + 4 <= channels) {
+                const Pack<float, 4> v = *reinterpret_cast<const Pack<float, 4>*>(part + c);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] += v.v[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] += c + i < channels ? part[c + i] : 0.0f;
+            }
+        };
+        if (wave == 0) add(mine);
+#pragma unroll 8
+        for (i64 b = blockIdx.x + 1 + wave; b <= last; b += kWaves) add(parts + b * hop);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) room[wave][lane].v[i] = sum[i];
         __syncthreads();
-        if (wave == 0 && c < channels)
-            out[run * out_stride + c] = static_cast<T>(scale * ((room[0][lane] + room[1][lane]) + (room[2][lane] + room[3][lane])));
+        if (threadIdx.x < 256 && c0 + static_cast<int>(threadIdx.x) < channels) {
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) s += room[w][threadIdx.x / 4].v[threadIdx.x % 4];
+            out[run * out_stride + c0 + threadIdx.x] = static_cast<T>(scale * s);
+        }
         __syncthreads();
     }
 }
@@ -527,7 +557,7 @@ int32_t smx_embed_gradient(const void* types, int32_t types_are_64bit, int64_t t
             SMX_LAUNCH_CHECK("k_sort_count");
             for (int p = 0; p < w.passes; ++p, at ^= 1) {
                 int* const counts = ints(w.counts) + p * pass;
-                k_sort_place<I><<<w.tiles, 256, 0, queue>>>(p ? nullptr : z, ints(w.keys[at ^ 1]), ints(w.order[at ^ 1]), tokens,
+                k_sort_place<I><<<w.tiles, 1024, 0, queue>>>(p ? nullptr : z, ints(w.keys[at ^ 1]), ints(w.order[at ^ 1]), tokens,
                                                             num_types, w.tile, 8 * p, counts,
                                                             p + 1 < w.passes ? counts + pass : nullptr, ints(w.keys[at]),
                                                             ints(w.order[at]));
@@ -545,8 +575,8 @@ int32_t smx_embed_gradient(const void* types, int32_t types_are_64bit, int64_t t
                     seen, w.lanes);
                 SMX_LAUNCH_CHECK("k_embed_runs");
             }
-            const unsigned rows = blocks_for(num_types, 4);
-            k_embed_finish<T><<<static_cast<unsigned>(w.chunks) + (rows < 8192 ? rows : 8192), 256, 0, queue>>>(
+            const unsigned rows = blocks_for(num_types, 16);
+            k_embed_finish<T><<<static_cast<unsigned>(w.chunks) + (rows < 2048 ? rows : 2048), 1024, 0, queue>>>(
                 ints(w.keys[at]), tokens, static_cast<int>(num_types), static_cast<int>(channels), scale,
                 static_cast<T*>(out), out_stride, parts, seen, w.chunk, w.chunks);
             SMX_LAUNCH_CHECK("k_embed_finish");

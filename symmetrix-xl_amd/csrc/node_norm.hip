@@ -364,6 +364,7 @@ __global__ void __launch_bounds__(1024) k_norm_gradient_join(Norm<T> a, const fl
     if (k == 0 ? !a.d && a.rows > 0 : !a.dnext) return;
     float sum = 0.0f;
     if (c < a.channels)
+#pragma unroll 8
         for (int p = wave; p < count; p += 16) sum += parts[(static_cast<i64>(p) * kSums + k) * a.channels + c];
     room[wave][lane] = sum;
     __syncthreads();
