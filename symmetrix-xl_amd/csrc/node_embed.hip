@@ -31,10 +31,11 @@ __global__ void __launch_bounds__(256) k_embed(const I* __restrict__ types, i64 
     for (i64 t = static_cast<i64>(blockIdx.x) * groups + threadIdx.x / lanes; t < tokens;
          t += static_cast<i64>(gridDim.x) * groups) {
         const int z = type_of(types, t, num_types);
+        Eight<T> row;
+        if (z >= 0) row = load_pack(table + z * table_stride, c, channels);
         float v[8];
-        if (z >= 0) load_eight(table + z * table_stride, c, channels, v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = z < 0 ? 0.0f : scale * v[i];
+        for (int i = 0; i < 8; ++i) v[i] = z < 0 ? 0.0f : scale * row[i];
         store_eight(out + t * out_stride, c, channels, v);
     }
 }
@@ -46,7 +47,8 @@ __global__ void __launch_bounds__(256) k_embed(const I* __restrict__ types, i64 
 // kTile atoms (times up to 512 tiles) are counted, and each pass places a tile's atoms by the counts of all tiles
 // before it and counts the next pass's digits where they land.
 
-constexpr int kDigits = 256, kTile = 2048, kMostTiles = 512, kSmall = 4096;
+constexpr int kUnits = 256;  // compute units
+constexpr int kDigits = 256, kTile = 1024, kMostTiles = 512, kSmall = 4096;
 
 // the lanes of the wave that are `in` and hold the same digit
 __device__ __forceinline__ unsigned long long same_digit(int digit, bool in) {
@@ -251,9 +253,11 @@ __global__ void __launch_bounds__(1024) k_sort_place(const I* __restrict__ types
     }
 }
 
-constexpr int kRun = 16;  // sorted atoms a group of lanes adds up
+// Sorted atoms that a group of lanes adds up: as many, with as few parts to join, as still fill the
+// card (300,000 atoms of 5 species x 447: 326 us at 16, 270 at 64).
+constexpr int kRuns[3] = {64, 16, 8};
 
-// 256 / lanes groups a workgroup, each kRun sorted atoms of 8 lanes' channels.  A type whose atoms lie
+// 256 / lanes groups a workgroup, each `length` sorted atoms of 8 lanes' channels.  A type whose atoms lie
 // within a group is done there; the first and last runs of the groups are joined in LDS, in order; what crosses
 // the workgroup's ends leaves as a part: [0] of a run that goes on from the workgroup before, [1] of one that starts here
 // and goes on in the next.
@@ -261,14 +265,14 @@ template <class T>
 __global__ void __launch_bounds__(256) k_embed_runs(const int* __restrict__ keys, const int* __restrict__ order, i64 tokens,
                                                     const T* __restrict__ grad, i64 grad_stride, int num_types,
                                                     int channels, float scale, T* __restrict__ out, i64 out_stride,
-                                                    float* __restrict__ parts, std::uint8_t* __restrict__ seen, int lanes) {
+                                                    float* __restrict__ parts, std::uint8_t* __restrict__ seen, int lanes, int length) {
     __shared__ int piece_key[2 * 32];
     __shared__ float piece[2 * 256 * 8];
     const int groups = 256 / lanes, width = 8 * lanes, group = threadIdx.x / lanes, lane = threadIdx.x % lanes;
     const int c0 = blockIdx.y * width, c = c0 + 8 * lane;
-    const i64 chunk = static_cast<i64>(groups) * kRun, start = blockIdx.x * chunk;
+    const i64 chunk = static_cast<i64>(groups) * length, start = blockIdx.x * chunk;
     const i64 end = start + chunk < tokens ? start + chunk : tokens;
-    const i64 first = start + group * kRun;
+    const i64 first = start + group * length;
     float acc[8], head[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] = head[i] = 0.0f;
@@ -290,26 +294,32 @@ __global__ void __launch_bounds__(256) k_embed_runs(const int* __restrict__ keys
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
     };
+    const int before = start > 0 ? keys[start - 1] : -1, after = end < tokens ? keys[end] : num_types;
+    int key[8], atom[8];
+    const auto read = [&](int b) {
 #pragma unroll
-    for (int b = 0; b < kRun; b += 8) {
-        int key[8];
+        for (int j = 0; j < 8; ++j) {
+            const i64 p = first + b + j < end ? first + b + j : end - 1;
+            key[j] = first + b + j < end ? keys[p] : num_types;
+            atom[j] = order[p];
+        }
+    };
+    read(0);
+    for (int b = 0; b < length; b += 8) {
+        int here[8];
         Eight<T> row[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const i64 p = first + b + j;
-            key[j] = p < end ? keys[p] : num_types;
-            const int atom = p < end ? order[p] : 0;
-#pragma unroll
-            for (int i = 0; i < Eight<T>::kWords; ++i) row[j].w[i] = 0;
-            if (key[j] < num_types && c < channels)
-                row[j] = load_pack(grad + static_cast<i64>(atom) * grad_stride, c, channels);
+            here[j] = key[j];
+            if (here[j] < num_types && c < channels) row[j] = load_pack(grad + static_cast<i64>(atom[j]) * grad_stride, c, channels);
         }
+        if (b + 8 < length) read(b + 8);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            if (key[j] >= num_types) continue;  // past the end, or no species: these sort last
-            if (key[j] != current) {
+            if (here[j] >= num_types) continue;  // past the end, or no species: these sort last
+            if (here[j] != current) {
                 if (current >= 0) close();
-                current = key[j];
+                current = here[j];
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) acc[i] += row[j][i];
@@ -328,26 +338,31 @@ __global__ void __launch_bounds__(256) k_embed_runs(const int* __restrict__ keys
         piece[(2 * group + 1) * width + 8 * lane + i] = acc[i];
     }
     __syncthreads();
-    const int before = start > 0 ? keys[start - 1] : -1, after = end < tokens ? keys[end] : num_types;
     for (int w = threadIdx.x; w < width && c0 + w < channels; w += 256) {
         float sum = 0.0f;
         int run = -1;
         bool from_before = false;
-        for (int q = 0; q < 2 * groups; ++q) {
-            const int key = piece_key[q];
-            if (key < 0) continue;
-            if (key != run) {
-                if (run >= 0) {
-                    if (from_before)
-                        parts[(2 * static_cast<i64>(blockIdx.x)) * channels + c0 + w] = sum;
-                    else
-                        out[run * out_stride + c0 + w] = static_cast<T>(scale * sum);
+        for (int q0 = 0; q0 < 2 * groups; q0 += 8) {  // (at least four groups)
+            int next[8];
+            float value[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) next[j] = piece_key[q0 + j], value[j] = piece[(q0 + j) * width + w];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (next[j] < 0) continue;
+                if (next[j] != run) {
+                    if (run >= 0) {
+                        if (from_before)
+                            parts[(2 * static_cast<i64>(blockIdx.x)) * channels + c0 + w] = sum;
+                        else
+                            out[run * out_stride + c0 + w] = static_cast<T>(scale * sum);
+                    }
+                    from_before = run < 0 && next[j] == before;
+                    run = next[j];
+                    sum = 0.0f;
                 }
-                from_before = run < 0 && key == before;
-                run = key;
-                sum = 0.0f;
+                sum += value[j];
             }
-            sum += piece[q * width + w];
         }
         if (run < 0) continue;
         if (from_before)
@@ -361,14 +376,14 @@ __global__ void __launch_bounds__(256) k_embed_runs(const int* __restrict__ keys
 
 // Zeros for the types without atoms (workgroups from `chunks` on, a wave a row), and the joins of runs
 // that cross workgroups: workgroup b's, if a run starts in b's atoms and goes on.  A run of few parts is
-// added up by a thread a channel; one of many (thousands of atoms of a species) by sixteen waves, four channels
-// a lane, a sixteenth of the parts each.
+// added up by a thread a channel; one of many (thousands of atoms of a species) by eight waves, four channels
+// a lane, an eighth of the parts each.
 template <class T>
-__global__ void __launch_bounds__(1024) k_embed_finish(const int* __restrict__ keys, i64 tokens, int num_types, int channels,
+__global__ void __launch_bounds__(512) k_embed_finish(const int* __restrict__ keys, i64 tokens, int num_types, int channels,
                                                        float scale, T* __restrict__ out, i64 out_stride,
                                                        const float* __restrict__ parts,
                                                        const std::uint8_t* __restrict__ seen, i64 chunk, int chunks) {
-    constexpr int kWaves = 16;
+    constexpr int kWaves = 8;
     __shared__ Pack<float, 4> room[kWaves][64];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     if (static_cast<int>(blockIdx.x) >= chunks) {
@@ -398,7 +413,7 @@ __global__ void __launch_bounds__(1024) k_embed_finish(const int* __restrict__ k
     const float* const mine = parts + (2 * static_cast<i64>(blockIdx.x) + 1) * channels;
     const i64 hop = 2LL * channels;
     if (last - blockIdx.x <= 2 * kWaves) {
-        for (int c = threadIdx.x; c < channels; c += 1024) {
+        for (int c = threadIdx.x; c < channels; c += 512) {
             float sum = mine[c];
             const float* at = parts + (static_cast<i64>(blockIdx.x) + 1) * hop + c;
             for (i64 b = blockIdx.x + 1; b <= last; ++b, at += hop) sum += *at;
@@ -438,7 +453,7 @@ __global__ void __launch_bounds__(1024) k_embed_finish(const int* __restrict__ k
 // The parts of a gradient call's workspace, in bytes from its start.
 struct Workspace {
     i64 keys[2], order[2], counts, seen, parts, size;
-    int passes, tile, tiles, lanes, chunks;
+    int passes, tile, tiles, lanes, length, chunks;
     i64 chunk;
 };
 
@@ -451,7 +466,12 @@ Workspace plan_gradient(i64 tokens, i64 num_types, i64 channels) {
     if (w.tile == 0) w.tile = kTile;
     w.tiles = static_cast<int>((tokens + w.tile - 1) / w.tile);
     w.lanes = lanes_of(channels);
-    w.chunk = static_cast<i64>(256 / w.lanes) * kRun;
+    const i64 groups = 256 / w.lanes;
+    for (const int run : kRuns) {
+        w.length = run;
+        if (tokens >= groups * run * (run == 64 ? 4 : 1) * kUnits) break;
+    }
+    w.chunk = groups * w.length;
     w.chunks = static_cast<int>((tokens + w.chunk - 1) / w.chunk);
     const auto take = [&](i64 bytes) {
         const i64 at = w.size;
@@ -511,7 +531,7 @@ int32_t smx_embed(const void* types, int32_t types_are_64bit, int64_t tokens, co
                 using I = decltype(i);
                 const int lanes = lanes_of(channels), groups = 256 / lanes;
                 const i64 want = (tokens + groups - 1) / groups;
-                k_embed<T, I><<<dim3(static_cast<unsigned>(want < 65536 ? want : 65536), blocks_for(channels, 8 * lanes)), 256,
+                k_embed<T, I><<<dim3(static_cast<unsigned>(want < (1 << 20) ? want : 1 << 20), blocks_for(channels, 8 * lanes)), 256,
                                 0, static_cast<hipStream_t>(stream)>>>(
                     static_cast<const I*>(types), tokens, static_cast<const T*>(table), table_stride, num_types,
                     static_cast<int>(channels), scale, static_cast<T*>(out), out_stride, lanes);
@@ -572,11 +592,11 @@ int32_t smx_embed_gradient(const void* types, int32_t types_are_64bit, int64_t t
                 k_embed_runs<T><<<dim3(static_cast<unsigned>(w.chunks), blocks_for(channels, 8 * w.lanes)), 256, 0, queue>>>(
                     ints(w.keys[at]), ints(w.order[at]), tokens, static_cast<const T*>(grad), grad_stride,
                     static_cast<int>(num_types), static_cast<int>(channels), scale, static_cast<T*>(out), out_stride, parts,
-                    seen, w.lanes);
+                    seen, w.lanes, w.length);
                 SMX_LAUNCH_CHECK("k_embed_runs");
             }
-            const unsigned rows = blocks_for(num_types, 16);
-            k_embed_finish<T><<<static_cast<unsigned>(w.chunks) + (rows < 2048 ? rows : 2048), 1024, 0, queue>>>(
+            const unsigned rows = blocks_for(num_types, 8);
+            k_embed_finish<T><<<static_cast<unsigned>(w.chunks) + (rows < 4096 ? rows : 4096), 512, 0, queue>>>(
                 ints(w.keys[at]), tokens, static_cast<int>(num_types), static_cast<int>(channels), scale,
                 static_cast<T*>(out), out_stride, parts, seen, w.chunk, w.chunks);
             SMX_LAUNCH_CHECK("k_embed_finish");

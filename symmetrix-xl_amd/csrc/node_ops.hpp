@@ -94,18 +94,33 @@ __device__ __forceinline__ void load_eight(const T* row, int c, int cols, float 
     for (int i = 0; i < 8; ++i) v[i] = p[i];
 }
 
+// v, as another value to the compiler.  Where a whole store of neighbouring values and one value by value are two
+// branches, the compiler makes the first value's store common to both and cuts the whole one into pieces.
+__device__ __forceinline__ float apart(float v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 // Eight values from column c on, up to the end.
 template <class T>
 __device__ __forceinline__ void store_eight(T* row, int c, int cols, const float (&v)[8]) {
-    Pack<T, 8> p;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) p.v[i] = static_cast<T>(v[i]);
+    struct __attribute__((packed, aligned(sizeof(T)))) Words {
+        std::uint32_t w[Eight<T>::kWords];
+    };
     if (c + 8 <= cols) {
-        *reinterpret_cast<Pack<T, 8>*>(row + c) = p;
+        Words p;
+#pragma unroll
+        for (int i = 0; i < Eight<T>::kWords; ++i) {
+            if constexpr (sizeof(T) == 4)
+                p.w[i] = bits_of(static_cast<T>(v[i]));
+            else
+                p.w[i] = bits_of(static_cast<T>(v[2 * i])) | bits_of(static_cast<T>(v[2 * i + 1])) << 16;
+        }
+        *reinterpret_cast<Words*>(row + c) = p;
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (c + i < cols) row[c + i] = p.v[i];
+            if (c + i < cols) row[c + i] = static_cast<T>(apart(v[i]));
     }
 }
 

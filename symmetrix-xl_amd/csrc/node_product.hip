@@ -175,7 +175,7 @@ __device__ __forceinline__ void store_four(const Product<O>& p, int i, int j, ac
         } else {
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                if (j + q < p.n) at[q] = v[q];
+                if (j + q < p.n) at[q] = apart(v[q]);
         }
         return;
     }
@@ -188,7 +188,7 @@ __device__ __forceinline__ void store_four(const Product<O>& p, int i, int j, ac
     } else {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-            if (j + q < p.n) at[q] = static_cast<O>(v[q]);
+            if (j + q < p.n) at[q] = static_cast<O>(apart(v[q]));
     }
 }
 
