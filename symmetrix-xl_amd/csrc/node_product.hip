@@ -207,199 +207,197 @@ __device__ __forceinline__ void dma_words(__amdgpu_buffer_rsrc_t from, unsigned 
                  : "s"(lds), "v"(at), "s"(from), "s"(also)
                  : "memory");
 }
-// until at most N of the wave's memory operations are under way (they end in order)
-template <int N>
-__device__ __forceinline__ void dma_wait() {
-    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
-}
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // BM x BN outputs a workgroup of WM x WN x KG waves.  Both operands' blocks of 128
-// go to LDS by dma, KG blocks at a time and STAGES deep: while some are multiplied, the next ones
+// go to LDS by dma, KG blocks at a time: while some are multiplied, the next ones
 // arrive.  A row's eight 16-byte pieces are permuted by half the row's number (in the global
 // addresses, within one line), so that the 16 rows that a fragment read meets at once lie in
 // 16 different places of the 64 banks.  Lane l holds row l % 16 of a fragment and pieces l / 16 and
 // l / 16 + 4 of the block: the order of k inside a block is the operands' own affair, as one
 // scale covers it.  The accumulator's lane l holds column l % 16 of rows 4 (l / 16) on; with b as the first operand its
-// four values lie side by side in a row of the output.  With KG > 1, for few tiles, KG groups of waves
-// take every KG-th block each, so that their waits overlap, and their sums are joined in LDS.
-template <class O, bool WIDE, int BM, int BN, int WM, int WN, int KG, int STAGES>
-__global__ void __launch_bounds__(64 * WM * WN * KG, (BM + BN) * kBlock * KG * STAGES > 81920 ? 1 : 2)
+// four values lie side by side in a row of the output.  With KG == 1 a workgroup goes through every gridDim.x-th
+// tile, and the next one's first blocks arrive while this one's last are multiplied and stored.  With KG > 1, for
+// few tiles, KG groups of waves take every KG-th block each, so that their waits overlap, and their sums are joined in LDS.
+template <class O, bool WIDE, int BM, int BN, int WM, int WN, int KG>
+__global__ void __launch_bounds__(64 * WM * WN * KG, (BM + BN) * kBlock * KG * 2 > 81920 ? 1 : 2)
 k_product_tile(Product<O> p) {
     constexpr int WAVES = WM * WN * KG, MF = BM / WM / 16, NF = BN / WN / 16, LA = BM / 8 * KG / WAVES,
                   LB = BN / 8 * KG / WAVES, LS = ((BM + BN) / 64 + WAVES - 1) / WAVES;
-    constexpr unsigned kOne = (BM + BN) * kBlock, kStage = kOne * KG;
+    constexpr unsigned kOne = (BM + BN) * kBlock, kStage = kOne * KG, kScales = 2 * kStage;
     static_assert(BM * KG % (8 * WAVES) == 0 && BN * KG % (8 * WAVES) == 0 && BM % 64 == 0 && BN % 64 == 0 && 4 % KG == 0);
-    static_assert(KG == 1 || STAGES * kStage >= WAVES * MF * NF * 1024);
-    __shared__ __attribute__((aligned(1024))) std::uint8_t lds[STAGES * kStage + 8 * (BM + BN)];
+    static_assert(KG == 1 || 2 * kStage >= WAVES * MF * NF * 1024);
+    __shared__ __attribute__((aligned(1024))) std::uint8_t lds[2 * kStage + 8 * (BM + BN)];
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int kg = wave / (WM * WN), in_group = wave % (WM * WN);
-    // bands of eight tile rows, each band column by column: the tiles that one XCD works on
-    // share their rows of both operands in its L2
-    const int id = xcd_remap(blockIdx.x, gridDim.x);
-    const int band = id / (8 * p.tiles_n), in_band = id % (8 * p.tiles_n);
-    const int high = p.tiles_m - 8 * band < 8 ? p.tiles_m - 8 * band : 8;
-    const int i0 = (8 * band + in_band % high) * BM, j0 = in_band / high * BN;
+    const int wm = in_group / WN * (BM / WM), wn = in_group % WN * (BN / WN);
+    const int tiles = p.tiles_m * p.tiles_n;
     const int first = blockIdx.y * p.split_blocks;
     const int last = first + p.split_blocks < p.blocks ? first + p.split_blocks : p.blocks;
-
-    // (what a group reads past the last block, within the buffers' ranges, is not used)
-    const int rows_a = p.m - i0 < BM ? p.m - i0 : BM, rows_b = p.n - j0 < BN ? p.n - j0 : BN;
-    const int pitch = static_cast<int>(p.pitch);
-    const __amdgpu_buffer_rsrc_t ra = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<std::uint8_t*>(p.a + i0 * p.pitch), 0, rows_a * pitch, 0x00020000);
-    const __amdgpu_buffer_rsrc_t rb = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<std::uint8_t*>(p.b + j0 * p.pitch), 0, rows_b * pitch, 0x00020000);
-    int at_a[LA], at_b[LB], to_a[LA], to_b[LB];
-#pragma unroll
-    for (int q = 0; q < LA; ++q) {
-        const int w = wave + WAVES * q, b = w / (BM / 8), r = 8 * (w % (BM / 8)) + lane / 8;
-        at_a[q] = (r < rows_a ? r : rows_a - 1) * pitch + ((lane % 8) ^ (r / 2 % 8)) * 16 + b * kBlock;
-        to_a[q] = b * kOne + w % (BM / 8) * 1024;
-    }
-#pragma unroll
-    for (int q = 0; q < LB; ++q) {
-        const int w = wave + WAVES * q, b = w / (BN / 8), r = 8 * (w % (BN / 8)) + lane / 8;
-        at_b[q] = (r < rows_b ? r : rows_b - 1) * pitch + ((lane % 8) ^ (r / 2 % 8)) * 16 + b * kBlock;
-        to_b[q] = b * kOne + BM * kBlock + w % (BN / 8) * 1024;
-    }
+    const int pitch = static_cast<int>(p.pitch), scale_pitch = static_cast<int>(p.scale_pitch);
     const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<std::uintptr_t>(
         (__attribute__((address_space(3))) std::uint8_t*)lds));
+
+    // The tile whose blocks are being read.  Bands of eight tile rows, each band column by column: the
+    // tiles that one XCD works on share their rows of both operands in its L2.  (What a group reads past the
+    // last block, within the buffers' ranges, is not used.)
+    __amdgpu_buffer_rsrc_t ra, rb, rs[LS];
+    int i0, j0, at_a[LA], at_b[LB], at_s[LS];
+    const auto turn_to = [&](int turn) {
+        const int id = xcd_remap(turn, tiles);
+        const int band = id / (8 * p.tiles_n), in_band = id % (8 * p.tiles_n);
+        const int high = p.tiles_m - 8 * band < 8 ? p.tiles_m - 8 * band : 8;
+        i0 = (8 * band + in_band % high) * BM, j0 = in_band / high * BN;
+        const int rows_a = p.m - i0 < BM ? p.m - i0 : BM, rows_b = p.n - j0 < BN ? p.n - j0 : BN;
+        ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<std::uint8_t*>(p.a + i0 * p.pitch), 0, rows_a * pitch, 0x00020000);
+        rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<std::uint8_t*>(p.b + j0 * p.pitch), 0, rows_b * pitch, 0x00020000);
+#pragma unroll
+        for (int q = 0; q < LA; ++q) {
+            const int w = wave + WAVES * q, r = 8 * (w % (BM / 8)) + lane / 8;
+            at_a[q] = (r < rows_a ? r : rows_a - 1) * pitch + ((lane % 8) ^ (r / 2 % 8)) * 16 + w / (BM / 8) * kBlock;
+        }
+#pragma unroll
+        for (int q = 0; q < LB; ++q) {
+            const int w = wave + WAVES * q, r = 8 * (w % (BN / 8)) + lane / 8;
+            at_b[q] = (r < rows_b ? r : rows_b - 1) * pitch + ((lane % 8) ^ (r / 2 % 8)) * 16 + w / (BN / 8) * kBlock;
+        }
+        // The scales of four blocks are one dword a row, which goes to LDS the same way, 64 rows an
+        // instruction, while the four blocks before are worked on.
+#pragma unroll
+        for (int q = 0; q < LS; ++q) {
+            const int w = wave + WAVES * q, rows = w < BM / 64 ? rows_a : rows_b;
+            rs[q] = __builtin_amdgcn_make_buffer_rsrc(
+                const_cast<std::uint8_t*>(w < BM / 64 ? p.as + i0 * p.scale_pitch : p.bs + j0 * p.scale_pitch), 0,
+                rows * scale_pitch, 0x00020000);
+            const int r = 64 * (w < BM / 64 ? w : w - BM / 64) + lane;
+            at_s[q] = (r < rows ? r : rows - 1) * scale_pitch;
+        }
+    };
     const auto stage = [&](int kb, int slot) {
         const unsigned to = __builtin_amdgcn_readfirstlane(lds0 + slot * kStage);
 #pragma unroll
-        for (int q = 0; q < LA; ++q) dma(ra, to + to_a[q], at_a[q], kb * kBlock);
+        for (int q = 0; q < LA; ++q) {
+            const int w = wave + WAVES * q;
+            dma(ra, to + w / (BM / 8) * kOne + w % (BM / 8) * 1024, at_a[q], kb * kBlock);
+        }
 #pragma unroll
-        for (int q = 0; q < LB; ++q) dma(rb, to + to_b[q], at_b[q], kb * kBlock);
+        for (int q = 0; q < LB; ++q) {
+            const int w = wave + WAVES * q;
+            dma(rb, to + w / (BN / 8) * kOne + BM * kBlock + w % (BN / 8) * 1024, at_b[q], kb * kBlock);
+        }
     };
-
-    // The scales of four blocks are one dword a row, which goes to LDS the same way, 64 rows an
-    // instruction, while the four blocks before are worked on.
-    const int wm = in_group / WN * (BM / WM), wn = in_group % WN * (BN / WN);
-    const int scale_pitch = static_cast<int>(p.scale_pitch);
-    __amdgpu_buffer_rsrc_t rs[LS];
-    int at_s[LS];
-#pragma unroll
-    for (int q = 0; q < LS; ++q) {
-        const int w = wave + WAVES * q, rows = w < BM / 64 ? rows_a : rows_b;
-        rs[q] = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<std::uint8_t*>(w < BM / 64 ? p.as + i0 * p.scale_pitch : p.bs + j0 * p.scale_pitch), 0,
-            rows * scale_pitch, 0x00020000);
-        const int r = 64 * (w < BM / 64 ? w : w - BM / 64) + lane;
-        at_s[q] = (r < rows ? r : rows - 1) * scale_pitch;
-    }
-    const auto stage_scales = [&](int group) {
+    const auto stage_scales = [&](int group, int slot) {
+        const unsigned to = __builtin_amdgcn_readfirstlane(lds0 + kScales + slot * (BM + BN) * 4);
 #pragma unroll
         for (int q = 0; q < LS; ++q)
-            if (wave + WAVES * q < (BM + BN) / 64)
-                dma_words(rs[q],
-                          __builtin_amdgcn_readfirstlane(lds0 + STAGES * kStage +
-                                                         ((group & 1) * (BM + BN) + 64 * (wave + WAVES * q)) * 4),
-                          at_s[q], 4 * group);
+            if (wave + WAVES * q < (BM + BN) / 64) dma_words(rs[q], to + 256 * (wave + WAVES * q), at_s[q], 4 * group);
     };
-    unsigned sa[MF], sb[NF];
-
-    acc4 acc[MF][NF];
-#pragma unroll
-    for (int f = 0; f < MF; ++f)
-#pragma unroll
-        for (int g = 0; g < NF; ++g) acc[f][g] = acc4{0.0f, 0.0f, 0.0f, 0.0f};
 
     const int piece = (lane % 16) * kBlock + ((lane / 16) ^ (lane % 16 / 2)) * 16;
-    stage_scales(first / 4);
-#pragma unroll
-    for (int q = 0; q < STAGES - 1; ++q)
-        if (first + q * KG < last) stage(first + q * KG, q);
-    int slot = 0;
-    for (int kb = first; kb < last; kb += KG) {
-        // a stage is there when only the stages after it are under way (scales under way besides are
-        // counted as if they were blocks': the wait is then for more)
-        if (kb + (STAGES - 2) * KG < last)
-            dma_wait<(STAGES - 2) * (LA + LB)>();
-        else
-            dma_wait<0>();
-        __syncthreads();
-        if (kb % 4 == 0) {
-            const unsigned* const now = reinterpret_cast<const unsigned*>(lds + STAGES * kStage) + (kb / 4 & 1) * (BM + BN) + lane % 16;
-#pragma unroll
-            for (int f = 0; f < MF; ++f) sa[f] = now[wm + 16 * f] >> (8 * kg);
-#pragma unroll
-            for (int g = 0; g < NF; ++g) sb[g] = now[BM + wn + 16 * g] >> (8 * kg);
-            if (kb + 4 < last) stage_scales(kb / 4 + 1);
-        }
-        const int before = slot == 0 ? STAGES - 1 : slot - 1;  // read by all before the barrier
-        if (kb + (STAGES - 1) * KG < last) stage(kb + (STAGES - 1) * KG, before);
-        if (KG == 1 || kb + kg < last) {
-            const std::uint8_t* const tile = lds + slot * kStage + kg * kOne;
-            const auto fragment = [&](int row) {
-                const i32x4 x = *reinterpret_cast<const i32x4*>(tile + row * kBlock + piece);
-                const i32x4 y = *reinterpret_cast<const i32x4*>(tile + row * kBlock + (piece ^ 64));
-                return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-            };
-            i32x8 vb[NF];
-#pragma unroll
-            for (int g = 0; g < NF; ++g) vb[g] = fragment(BM + wn + 16 * g);
-            if constexpr (!WIDE) {
-#pragma unroll
-                for (int f = 0; f < MF; ++f) {
-                    const i32x8 va = fragment(wm + 16 * f);
-#pragma unroll
-                    for (int g = 0; g < NF; ++g)
-                        acc[f][g] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vb[g], va, acc[f][g], 0, 0, 0,
-                                                                                    sb[g], 0, sa[f]);
-                }
-            } else {
-                i32x8 va[MF];
-#pragma unroll
-                for (int f = 0; f < MF; ++f) va[f] = fragment(wm + 16 * f);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    bf16x8 wb[NF];
-#pragma unroll
-                    for (int g = 0; g < NF; ++g)
-                        wb[g] = to_bf16(vb[g][2 * q], vb[g][2 * q + 1], scale_of(sb[g] & 0xff));
-#pragma unroll
-                    for (int f = 0; f < MF; ++f) {
-                        const bf16x8 wa = to_bf16(va[f][2 * q], va[f][2 * q + 1], scale_of(sa[f] & 0xff));
-#pragma unroll
-                        for (int g = 0; g < NF; ++g)
-                            acc[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[g], wa, acc[f][g], 0, 0, 0);
-                    }
-                }
-            }
-            if constexpr (KG > 1) mfma_settle();  // (the block is conditional)
-        }
-#pragma unroll
-        for (int f = 0; f < MF; ++f) sa[f] = KG < 4 ? sa[f] >> (8 * KG) : 0;
-#pragma unroll
-        for (int g = 0; g < NF; ++g) sb[g] = KG < 4 ? sb[g] >> (8 * KG) : 0;
-        slot = slot + 1 == STAGES ? 0 : slot + 1;
-    }
-    mfma_settle();
-    const auto put = [&](int f, int g, acc4 v) {
-        store_four(p, i0 + wm + 16 * f + lane % 16, j0 + wn + 16 * g + 4 * (lane / 16), v, blockIdx.y);
-    };
-    if constexpr (KG == 1) {
+    int slot = 0, scale_slot = 0;
+    turn_to(blockIdx.x);
+    stage_scales(first / 4, 0);
+    stage(first, 0);
+    for (int turn = blockIdx.x; turn < tiles; turn += gridDim.x) {
+        const int i_now = i0, j_now = j0;
+        acc4 acc[MF][NF];
 #pragma unroll
         for (int f = 0; f < MF; ++f)
 #pragma unroll
-            for (int g = 0; g < NF; ++g) put(f, g, acc[f][g]);
-    } else {
-        // fragment q of every group is added up, in the groups' order, by group q % KG
-        acc4* const room = reinterpret_cast<acc4*>(lds);
-        const auto at = [&](int group, int q) {
-            return room + ((group * WM * WN + in_group) * MF * NF + q) * 64 + lane;
+            for (int g = 0; g < NF; ++g) acc[f][g] = acc4{0.0f, 0.0f, 0.0f, 0.0f};
+        unsigned sa[MF], sb[NF];
+        for (int kb = first; kb < last; kb += KG) {
+            dma_wait();
+            __syncthreads();  // the blocks are there, and all have read the ones before
+            if (kb % 4 == 0) {
+                const unsigned* const now = reinterpret_cast<const unsigned*>(lds + kScales) + scale_slot * (BM + BN) + lane % 16;
+#pragma unroll
+                for (int f = 0; f < MF; ++f) sa[f] = now[wm + 16 * f] >> (8 * kg);
+#pragma unroll
+                for (int g = 0; g < NF; ++g) sb[g] = now[BM + wn + 16 * g] >> (8 * kg);
+                scale_slot ^= 1;
+                if (kb + 4 < last) stage_scales(kb / 4 + 1, scale_slot);
+            }
+            const std::uint8_t* const tile = lds + slot * kStage + kg * kOne;
+            slot ^= 1;
+            if (kb + KG < last) {
+                stage(kb + KG, slot);
+            } else if (KG == 1 && turn + static_cast<int>(gridDim.x) < tiles) {
+                turn_to(turn + gridDim.x);
+                stage_scales(first / 4, scale_slot);
+                stage(first, slot);
+            }
+            if (KG == 1 || kb + kg < last) {
+                const auto fragment = [&](int row) {
+                    const i32x4 x = *reinterpret_cast<const i32x4*>(tile + row * kBlock + piece);
+                    const i32x4 y = *reinterpret_cast<const i32x4*>(tile + row * kBlock + (piece ^ 64));
+                    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+                };
+                i32x8 vb[NF];
+#pragma unroll
+                for (int g = 0; g < NF; ++g) vb[g] = fragment(BM + wn + 16 * g);
+                if constexpr (!WIDE) {
+#pragma unroll
+                    for (int f = 0; f < MF; ++f) {
+                        const i32x8 va = fragment(wm + 16 * f);
+#pragma unroll
+                        for (int g = 0; g < NF; ++g)
+                            acc[f][g] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vb[g], va, acc[f][g], 0, 0, 0,
+                                                                                        sb[g], 0, sa[f]);
+                    }
+                } else {
+                    i32x8 va[MF];
+#pragma unroll
+                    for (int f = 0; f < MF; ++f) va[f] = fragment(wm + 16 * f);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        bf16x8 wb[NF];
+#pragma unroll
+                        for (int g = 0; g < NF; ++g)
+                            wb[g] = to_bf16(vb[g][2 * q], vb[g][2 * q + 1], scale_of(sb[g] & 0xff));
+#pragma unroll
+                        for (int f = 0; f < MF; ++f) {
+                            const bf16x8 wa = to_bf16(va[f][2 * q], va[f][2 * q + 1], scale_of(sa[f] & 0xff));
+#pragma unroll
+                            for (int g = 0; g < NF; ++g)
+                                acc[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[g], wa, acc[f][g], 0, 0, 0);
+                        }
+                    }
+                }
+                if constexpr (KG > 1) mfma_settle();  // (the block is conditional)
+            }
+#pragma unroll
+            for (int f = 0; f < MF; ++f) sa[f] = KG < 4 ? sa[f] >> (8 * KG) : 0;
+#pragma unroll
+            for (int g = 0; g < NF; ++g) sb[g] = KG < 4 ? sb[g] >> (8 * KG) : 0;
+        }
+        mfma_settle();
+        const auto put = [&](int f, int g, acc4 v) {
+            store_four(p, i_now + wm + 16 * f + lane % 16, j_now + wn + 16 * g + 4 * (lane / 16), v, blockIdx.y);
         };
-        __syncthreads();
+        if constexpr (KG == 1) {
 #pragma unroll
-        for (int q = 0; q < MF * NF; ++q) *at(kg, q) = acc[q / NF][q % NF];
-        __syncthreads();
+            for (int f = 0; f < MF; ++f)
 #pragma unroll
-        for (int q = 0; q < MF * NF; ++q) {
-            if (q % KG != kg) continue;
-            acc4 sum = *at(0, q);
+                for (int g = 0; g < NF; ++g) put(f, g, acc[f][g]);
+        } else {
+            // fragment q of every group is added up, in the groups' order, by group q % KG
+            acc4* const room = reinterpret_cast<acc4*>(lds);
+            const auto at = [&](int group, int q) {
+                return room + ((group * WM * WN + in_group) * MF * NF + q) * 64 + lane;
+            };
+            __syncthreads();
 #pragma unroll
-            for (int h = 1; h < KG; ++h) sum += *at(h, q);
-            put(q / NF, q % NF, sum);
+            for (int q = 0; q < MF * NF; ++q) *at(kg, q) = acc[q / NF][q % NF];
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < MF * NF; ++q) {
+                if (q % KG != kg) continue;
+                acc4 sum = *at(0, q);
+#pragma unroll
+                for (int h = 1; h < KG; ++h) sum += *at(h, q);
+                put(q / NF, q % NF, sum);
+            }
         }
     }
 }
@@ -618,15 +616,19 @@ void quantize(const void* x, i64 x_stride, int dtype, i64 rows, i64 cols, std::u
 
 template <class O, bool WIDE>
 void launch_tiles(const Product<O>& p, const Plan& plan, hipStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(p.tiles_m * p.tiles_n), static_cast<unsigned>(plan.splits));
+    // as many workgroups as the card holds of a tile that goes on to the next, all otherwise
+    const auto grid = [&](int held) {
+        const int tiles = p.tiles_m * p.tiles_n, most = held * static_cast<int>(kUnits);
+        return dim3(static_cast<unsigned>(tiles < most || held == 0 ? tiles : most), static_cast<unsigned>(plan.splits));
+    };
     switch (plan.tile) {
-        case 256: k_product_tile<O, WIDE, 256, 256, 2, 4, 1, 2><<<grid, 512, 0, stream>>>(p); break;
-        case 128: k_product_tile<O, WIDE, 128, 128, 2, 2, 1, 2><<<grid, 256, 0, stream>>>(p); break;
+        case 256: k_product_tile<O, WIDE, 256, 256, 2, 4, 1><<<grid(1), 512, 0, stream>>>(p); break;
+        case 128: k_product_tile<O, WIDE, 128, 128, 2, 2, 1><<<grid(2), 256, 0, stream>>>(p); break;
         default:
             if (plan.groups == 1)
-                k_product_tile<O, WIDE, 64, 64, 2, 2, 1, 2><<<grid, 256, 0, stream>>>(p);
+                k_product_tile<O, WIDE, 64, 64, 2, 2, 1><<<grid(4), 256, 0, stream>>>(p);
             else
-                k_product_tile<O, WIDE, 64, 64, 2, 2, 4, 2><<<grid, 1024, 0, stream>>>(p);
+                k_product_tile<O, WIDE, 64, 64, 2, 2, 4><<<grid(0), 1024, 0, stream>>>(p);
     }
     SMX_LAUNCH_CHECK("k_product_tile");
 }
