@@ -3,16 +3,17 @@
 
 An instruction other than an MFMA that reads or overwrites a register written
 by v_mfma_f32_16x16x4_f32 (8 passes) must issue at least ten wait states after
-it, on every path, and after v_mfma_f32_16x16x32_bf16 (4 passes) at least eight;
-the hardware does not interlock.  The compiler inserts the waits, but in kernels
+it, on every path, and after v_mfma_f32_16x16x32_bf16 (4 passes) at least eight,
+and after v_mfma_scale_f32_16x16x128_f8f6f4 (8 passes) at least eleven; the hardware does not interlock.  The compiler inserts the waits, but in kernels
 whose MFMA chains sat in runtime-conditional blocks it padded only the
 fall-through path into a join, and a read on the taken branch came one
 instruction after its MFMA (a stale accumulator element, silently wrong).
 This walks each kernel's control-flow graph backwards from every instruction
 that touches a register (VALU operands, memory addresses and data) and reports
 those with fewer than MIN wait states since an MFMA that writes the register,
-over any path (a bf16 MFMA counts two more); an s_nop N counts N + 1, other
-instructions one.
+over any path (a bf16 MFMA counts two more, a scaled one one less); an s_nop N counts N + 1, other
+instructions one.  A scaled MFMA whose result overlaps an operand, which it would overwrite while it still reads
+it, is reported with no wait states: the compiler allocates that where accumulator and result are different values.
 
     python3 check_mfma_waits.py file.s [--min 10]      (exit 1 on findings)
 
@@ -31,7 +32,9 @@ _SINGLE = re.compile(r"([av])(\d+)$")
 
 
 # wait states an MFMA asks for less than the default (16x16x4 FP32, 8 passes)
-_SLACK = {"v_mfma_f32_16x16x32_bf16": 2}  # 4 passes
+_SLACK = {"v_mfma_f32_16x16x32_bf16": 2,  # 4 passes
+          "v_mfma_scale_f32_16x16x128_f8f6f4": -1}
+_MORE = 1  # wait states that some ask for above the default
 
 
 def _regs(token):
@@ -117,12 +120,16 @@ def findings(body, minimum):
     out = []
     for bi, b in enumerate(blocks):
         for k, t in enumerate(b["ins"]):
+            if t.startswith("v_mfma_scale"):
+                to, *of = [_regs(o) for o in t.split(None, 1)[1].split(",")[:3]]
+                for reg in sorted(to & set().union(*of)):
+                    out.append((b["label"], t, "%s%d" % reg, 0))
             if t.startswith("v_mfma") or t.startswith("s_") or " " not in t:
                 continue
             ops = t.split(None, 1)[1].split(",")
             for op in ops:
                 for reg in _regs(op):
-                    d = since_mfma(bi, k, reg, minimum, frozenset())
+                    d = since_mfma(bi, k, reg, minimum + _MORE, frozenset())
                     if d < minimum:  # (a bf16 MFMA's distance counts its slack)
                         out.append((b["label"], t, "%s%d" % reg, d))
     return out

@@ -417,7 +417,9 @@ __global__ void __launch_bounds__(64 * KS) k_product_rows(Product<O> p, const T*
     __shared__ acc4 room[KS][NF][64];
     __shared__ __attribute__((aligned(16))) std::uint8_t brought[RAW ? KS : 1][RAW ? kAhead : 1][kRawRows * kBlock];
     __shared__ int brought_scale[RAW ? KS : 1][RAW ? kAhead : 1][kRawRows];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, row = lane % 16, at = lane / 16 * 16;
+    // (a wave's branches have to be the whole wave's to the compiler too: matrix instructions run for all lanes)
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int row = lane % 16, at = lane / 16 * 16;
     const int j0 = xcd_remap(blockIdx.x, gridDim.x) * 16 * NF;
     const std::uint8_t *b[NF], *bs[NF];
 #pragma unroll
