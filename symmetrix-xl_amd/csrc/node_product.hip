@@ -238,16 +238,16 @@ k_product_tile(Product<O> p) {
     const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<std::uintptr_t>(
         (__attribute__((address_space(3))) std::uint8_t*)lds));
 
-    // The tile whose blocks are being read.  Bands of eight tile rows, each band column by column: the
+    // The tile whose blocks are being read.  Bands of four tile rows, each band column by column: the
     // tiles that one XCD works on share their rows of both operands in its L2.  (What a group reads past the
     // last block, within the buffers' ranges, is not used.)
     __amdgpu_buffer_rsrc_t ra, rb, rs[LS];
     int i0, j0, at_a[LA], at_b[LB], at_s[LS];
     const auto turn_to = [&](int turn) {
         const int id = xcd_remap(turn, tiles);
-        const int band = id / (8 * p.tiles_n), in_band = id % (8 * p.tiles_n);
-        const int high = p.tiles_m - 8 * band < 8 ? p.tiles_m - 8 * band : 8;
-        i0 = (8 * band + in_band % high) * BM, j0 = in_band / high * BN;
+        const int band = id / (4 * p.tiles_n), in_band = id % (4 * p.tiles_n);
+        const int high = p.tiles_m - 4 * band < 4 ? p.tiles_m - 4 * band : 4;
+        i0 = (4 * band + in_band % high) * BM, j0 = in_band / high * BN;
         const int rows_a = p.m - i0 < BM ? p.m - i0 : BM, rows_b = p.n - j0 < BN ? p.n - j0 : BN;
         ra = __builtin_amdgcn_make_buffer_rsrc(const_cast<std::uint8_t*>(p.a + i0 * p.pitch), 0, rows_a * pitch, 0x00020000);
         rb = __builtin_amdgcn_make_buffer_rsrc(const_cast<std::uint8_t*>(p.b + j0 * p.pitch), 0, rows_b * pitch, 0x00020000);
@@ -320,13 +320,6 @@ k_product_tile(Product<O> p) {
             }
             const std::uint8_t* const tile = lds + slot * kStage + kg * kOne;
             slot ^= 1;
-            if (kb + KG < last) {
-                stage(kb + KG, slot);
-            } else if (KG == 1 && turn + static_cast<int>(gridDim.x) < tiles) {
-                turn_to(turn + gridDim.x);
-                stage_scales(first / 4, scale_slot);
-                stage(first, slot);
-            }
             if (KG == 1 || kb + kg < last) {
                 const auto fragment = [&](int row) {
                     const i32x4 x = *reinterpret_cast<const i32x4*>(tile + row * kBlock + piece);
@@ -336,6 +329,13 @@ k_product_tile(Product<O> p) {
                 i32x8 vb[NF];
 #pragma unroll
                 for (int g = 0; g < NF; ++g) vb[g] = fragment(BM + wn + 16 * g);
+            if (kb + KG < last) {
+                stage(kb + KG, slot);
+            } else if (KG == 1 && turn + static_cast<int>(gridDim.x) < tiles) {
+                turn_to(turn + gridDim.x);
+                stage_scales(first / 4, scale_slot);
+                stage(first, slot);
+            }
                 if constexpr (!WIDE) {
 #pragma unroll
                     for (int f = 0; f < MF; ++f) {

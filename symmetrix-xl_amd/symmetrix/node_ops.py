@@ -138,13 +138,18 @@ def _like(t, name, x, shape):
     return _rows(t, name)[3]
 
 
-def _vector(t, name, x, channels):
+def _vector(t, name, device, channels):
     if t is None:
         return None
-    if t.dtype is not torch.float32 or t.get_device() != x.get_device() or t.shape != (channels,) \
+    if t.dtype is not torch.float32 or t.dim() != 1 or t.numel() != channels or t.get_device() != device \
             or not t.is_contiguous():
         raise ValueError("%s must be a contiguous float32 vector of the channels, on the rows' device" % name)
     return t.data_ptr()
+
+
+def _same(x):
+    """Room for rows like x's, packed."""
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
 
 
 def _workspace(size, like):
@@ -219,21 +224,27 @@ def _gate(gate, x, shape):
 _NORM_ARGS = ctypes.sizeof(_native.SmxResidualNormArgs)
 
 
-def _norm_args(x, d, post, gate, scale, next_weight, eps):
+def _norm_inputs(x, d, post, gate, scale, next_weight, eps):
+    """Checks; the fields of SmxResidualNormArgs up to its outputs."""
     code, r, c, xs = _rows(x, "x")
+    device = x.get_device()
     if d is None:
         if gate is not None or post is not None or scale is not None:
             raise ValueError("post, gate and scale go with d")
-        return _native.SmxResidualNormArgs(_NORM_ARGS, code, r, c, x.data_ptr(), xs, None, 0, None, 0, 0, eps, None, None,
-                                           _vector(next_weight, "next_weight", x, c))
+        return (_NORM_ARGS, code, r, c, x.data_ptr(), xs, None, 0, None, 0, 0, eps, None, None,
+                _vector(next_weight, "next_weight", device, c))
     shape = x.shape
     ds = _like(d, "d", x, shape)
     if post is None:
         raise ValueError("post must be given with d")
-    kind, gs = (0, 0) if gate is None else _gate(gate, x, shape)
-    return _native.SmxResidualNormArgs(
-        _NORM_ARGS, code, r, c, x.data_ptr(), xs, d.data_ptr(), ds, None if gate is None else gate.data_ptr(), gs, kind,
-        eps, _vector(post, "post", x, c), _vector(scale, "scale", x, c), _vector(next_weight, "next_weight", x, c))
+    if gate is None:
+        kind, at, gs = 0, None, 0
+    else:
+        kind, gs = _gate(gate, x, shape)
+        at = gate.data_ptr()
+    return (_NORM_ARGS, code, r, c, x.data_ptr(), xs, d.data_ptr(), ds, at, gs, kind, eps,
+            _vector(post, "post", device, c), _vector(scale, "scale", device, c),
+            _vector(next_weight, "next_weight", device, c))
 
 
 def residual_norm(x, d, post, gate=None, scale=None, next_weight=None, eps=1e-6, quantized=False):
@@ -242,40 +253,44 @@ def residual_norm(x, d, post, gate=None, scale=None, next_weight=None, eps=1e-6,
 
     ``gate``: logits, one for each value ([rows][channels]), channel ([channels]) or row
     ([rows][1]); ``post``, ``scale`` and ``next_weight``: float32 [channels]."""
-    a = _norm_args(x, d, post, gate, scale, next_weight, eps)
+    inputs = _norm_inputs(x, d, post, gate, scale, next_weight, eps)
     stream = _stream(x.get_device())
-    y = x.new_empty(x.shape)
-    a.y, a.y_stride = y.data_ptr(), a.channels
-    h = None if next_weight is None else _norm_output(a, x, quantized)
-    check(lib.smx_residual_norm(a, stream))
+    c = inputs[3]
+    y = _same(x)
+    h, at, scales = (None, None, None) if next_weight is None else _norm_output(x, quantized)
+    rc = lib.smx_residual_norm(_native.SmxResidualNormArgs(*inputs, y.data_ptr(), c, at, c, scales), stream)
+    if rc:
+        check(rc)
     return y, h
 
 
 def norm(x, weight, eps=1e-6, quantized=False):
     """``weight * x / rms(x)``, as ``BlockValues`` when ``quantized``."""
-    a = _norm_args(x, None, None, None, None, weight, eps)
+    inputs = _norm_inputs(x, None, None, None, None, weight, eps)
     stream = _stream(x.get_device())
-    h = _norm_output(a, x, quantized)
-    check(lib.smx_residual_norm(a, stream))
+    c = inputs[3]
+    h, at, scales = _norm_output(x, quantized)
+    rc = lib.smx_residual_norm(_native.SmxResidualNormArgs(*inputs, None, 0, at, c, scales), stream)
+    if rc:
+        check(rc)
     return h
 
 
-def _norm_output(a, x, quantized):
+def _norm_output(x, quantized):
+    """(h, its address, its scales' address)"""
     if quantized:
-        h = BlockValues._empty(a.rows, a.channels, x)
-        a.h, a.h_scales = h._at
-    else:
-        h = x.new_empty(x.shape)
-        a.h, a.h_stride = h.data_ptr(), a.channels
-    return h
+        h = BlockValues._empty(x.shape[0], x.shape[1], x)
+        return (h, *h._at)
+    h = _same(x)
+    return h, h.data_ptr(), None
 
 
 def residual_norm_gradient(x, d, post, gate, scale, next_weight, grad_y, grad_h, eps=1e-6):
     """Gradients ``(x, d, gate, post, scale, next_weight)`` of ``residual_norm`` from its inputs
     and the gradients of ``y`` and ``h`` (either may be None); None for inputs that are None.
     Those of ``post``, ``scale`` and ``next_weight`` are float32."""
-    a = _norm_args(x, d, post, gate, scale, next_weight, eps)
-    r, c, shape = a.rows, a.channels, x.shape
+    inputs = _norm_inputs(x, d, post, gate, scale, next_weight, eps)
+    r, c, shape = inputs[2], inputs[3], x.shape
     gys = ghs = 0
     if grad_y is not None:
         gys = _like(grad_y, "grad_y", x, shape)
@@ -284,22 +299,24 @@ def residual_norm_gradient(x, d, post, gate, scale, next_weight, grad_y, grad_h,
             raise ValueError("grad_h without next_weight")
         ghs = _like(grad_h, "grad_h", x, shape)
     stream = _stream(x.get_device())
-    dx = x.new_empty(shape)
+    dx = _same(x)
     dd = dg = dpost = dscale = dnext = None
     if d is not None:
-        dd, dpost = x.new_empty(shape), torch.empty_like(post)
+        dd, dpost = _same(x), torch.empty_like(post)
         if scale is not None:
             dscale = torch.empty_like(scale)
         if gate is not None:
-            dg = x.new_empty(gate.shape)
+            dg = _same(gate)
     if next_weight is not None:
         dnext = torch.empty_like(next_weight)
     size = lib.smx_residual_norm_gradient_workspace(r, c)
     room = _workspace(size, x)
     g = _native.SmxResidualNormGradientArgs(
-        a, _at(grad_y), gys, _at(grad_h), ghs, dx.data_ptr(), c, _at(dd), c, _at(dg),
-        1 if a.gate_kind == 3 else c, _at(dpost), _at(dscale), _at(dnext), _at(room), size)
-    check(lib.smx_residual_norm_gradient(g, stream))
+        _native.SmxResidualNormArgs(*inputs), _at(grad_y), gys, _at(grad_h), ghs, dx.data_ptr(), c, _at(dd), c, _at(dg),
+        1 if inputs[10] == 3 else c, _at(dpost), _at(dscale), _at(dnext), _at(room), size)
+    rc = lib.smx_residual_norm_gradient(g, stream)
+    if rc:
+        check(rc)
     return dx, dd, dg, dpost, dscale, dnext
 
 

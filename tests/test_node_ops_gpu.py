@@ -286,8 +286,7 @@ def test_norm_outputs_in_place_of_inputs(gen):
     import ctypes
     x, dd, post, g, scale, nxt = _norm_inputs(gen, 50, 200, "row", BF16)
     y, _ = ops.residual_norm(x, dd, post, g, scale)
-    a = ops._norm_args(x, dd, post, g, scale, None, 1e-6)
-    a.y, a.y_stride = x.data_ptr(), 200
+    a = _native.SmxResidualNormArgs(*ops._norm_inputs(x, dd, post, g, scale, None, 1e-6), x.data_ptr(), 200)
     _native.check(_native.lib.smx_residual_norm(ctypes.byref(a), torch.cuda.current_stream().cuda_stream))
     assert torch.equal(x, y)
 
