@@ -7,6 +7,8 @@
 //   q  = H next,     dx = G + r2 (q - v mean(q v)),              dnext  = sum H v
 //   dg = dx a n s (1 - s),   da = sum dx s n,   p = dx a s,      dpost  = sum p u
 //   t  = p post,     dd = r1 (t - u mean(t u))
+#include <variant>
+
 #include "node_ops.hpp"
 
 namespace smx {
@@ -93,18 +95,20 @@ __device__ __forceinline__ void load_channels(const Norm<T>& a, int c, float (&s
     if (a.next) load_eight(a.next, c, a.channels, next);
 }
 
-// A lane's share of a row as it lies in memory.
-template <class T>
+// A lane's share of a row as it lies in memory; FULL: a gate for each value, which takes registers that the other
+// kernels do without (8192 x 8192 FP32 gradient without it: 424 -> 314 us).
+template <class T, bool FULL>
 struct Share {
-    Eight<T> x, d, g;
+    Eight<T> x, d;
+    std::conditional_t<FULL, Eight<T>, std::monostate> g;
 };
 
-template <class T>
-__device__ __forceinline__ void load_share(const Norm<T>& a, i64 r, int c, Share<T>& s) {
+template <class T, bool FULL>
+__device__ __forceinline__ void load_share(const Norm<T>& a, i64 r, int c, Share<T, FULL>& s) {
     s.x = load_pack(a.x + r * a.x_stride, c, a.channels);
     if (!a.d) return;
     s.d = load_pack(a.d + r * a.d_stride, c, a.channels);
-    if (a.gate_kind == SMX_GATE_FULL) s.g = load_pack(a.gate + r * a.gate_stride, c, a.channels);
+    if constexpr (FULL) s.g = load_pack(a.gate + r * a.gate_stride, c, a.channels);
 }
 
 template <class T>
@@ -113,12 +117,15 @@ __device__ __forceinline__ T row_gate_of(const Norm<T>& a, i64 r) {
 }
 
 // scale * post * gate of eight channels; zeros past the end.
-template <class T>
-__device__ __forceinline__ void steps_of(const Norm<T>& a, const Share<T>& s, const float (&step)[8], float row_gate,
-                                         float (&gate)[8], float (&f)[8]) {
+template <class T, bool FULL>
+__device__ __forceinline__ void steps_of(const Share<T, FULL>& s, const float (&step)[8], float row_gate, float (&gate)[8],
+                                         float (&f)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        gate[i] = a.gate_kind == SMX_GATE_FULL ? sigmoid(s.g[i]) : row_gate;
+        if constexpr (FULL)
+            gate[i] = sigmoid(s.g[i]);
+        else
+            gate[i] = row_gate;
         f[i] = step[i] * gate[i];
     }
 }
@@ -135,7 +142,7 @@ __device__ __forceinline__ float square_sum(const Eight<T>& d) {
 // a row is read once and its two sums stay between lanes; a lane keeps its channels'
 // weights for all its rows.  A group of 128 channels is 16 lanes, which is where an 8-bit block's
 // scale is found.
-template <class T, int G, int N>
+template <class T, bool FULL, int G, int N>
 __global__ void __launch_bounds__(threads_of(G)) k_residual_norm(Norm<T> a) {
     constexpr int kThreads = threads_of(G), kGroups = kThreads / G;
     __shared__ typename GroupSum<G, 1>::Room room;
@@ -147,7 +154,7 @@ __global__ void __launch_bounds__(threads_of(G)) k_residual_norm(Norm<T> a) {
     int turn = 0;
     for (i64 r = static_cast<i64>(blockIdx.x) * kGroups + threadIdx.x / G; r < a.rows;
          r += static_cast<i64>(gridDim.x) * kGroups) {
-        Share<T> s[N];
+        Share<T, FULL> s[N];
         float sum[1] = {0.0f};
 #pragma unroll
         for (int n = 0; n < N; ++n) {
@@ -169,7 +176,7 @@ __global__ void __launch_bounds__(threads_of(G)) k_residual_norm(Norm<T> a) {
             for (int i = 0; i < 8; ++i) y[n][i] = s[n].x[i];
             if (a.d) {
                 float gate[8], f[8];
-                steps_of(a, s[n], step[n], row_gate, gate, f);
+                steps_of(s[n], step[n], row_gate, gate, f);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[n][i] += f[i] * (s[n].d[i] * r1);
             }
@@ -214,7 +221,7 @@ constexpr int kSums = 2;
 // which is also a row gate's gradient over 1 - s.  The next row is read while
 // one is worked on.  The sums over rows stay in registers over all rows of a group, are joined in LDS for the
 // workgroup's groups, and leave as one part [kSums][channels] a workgroup.
-template <class T, int G, int N>
+template <class T, bool FULL, int G, int N>
 __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, float* __restrict__ parts) {
     constexpr int kThreads = threads_of(G), kGroups = kThreads / G;
     __shared__ union {
@@ -222,7 +229,7 @@ __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, floa
         float join[kGroups > 1 ? kGroups : 1][kGroups > 1 ? G * 8 * N : 1];
     } lds;
     struct Row {
-        Share<T> s[N];
+        Share<T, FULL> s[N];
         Eight<T> gy[N], gh[N];
         T gate;
     };
@@ -273,7 +280,7 @@ __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, floa
         for (int n = 0; n < N; ++n) {
             const int c = 8 * (lane + G * n);
             float gate[8], f[8];
-            if (a.d) steps_of(a, row.s[n], step[n], row_gate, gate, f);
+            if (a.d) steps_of(row.s[n], step[n], row_gate, gate, f);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 y[n][i] = row.s[n].x[i];
@@ -297,7 +304,7 @@ __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, floa
             for (int n = 0; n < N; ++n)
 #pragma unroll
                 for (int i = 0; i < Eight<T>::kWords; ++i) {
-                    if (a.gate_kind == SMX_GATE_FULL) asm volatile("" : "+v"(row.s[n].g.w[i]));
+                    if constexpr (FULL) asm volatile("" : "+v"(row.s[n].g.w[i]));
                     asm volatile("" : "+v"(row.s[n].d.w[i]));
                     asm volatile("" : "+v"(row.gh[n].w[i]));
                 }
@@ -307,7 +314,7 @@ __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, floa
         for (int n = 0; n < N; ++n) {
             const int c = 8 * (lane + G * n);
             float gate[8], f[8], dx[8], dd[8], dg[8];
-            if (a.d) steps_of(a, row.s[n], step[n], row_gate, gate, f);
+            if (a.d) steps_of(row.s[n], step[n], row_gate, gate, f);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 dx[i] = a.gy ? row.gy[n][i] : 0.0f;
@@ -325,7 +332,7 @@ __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, floa
             }
             if (a.dx) store_eight(a.dx + r * a.dx_stride, c, a.channels, dx);
             if (a.dd) store_eight(a.dd + r * a.dd_stride, c, a.channels, dd);
-            if (a.dgate && a.gate_kind == SMX_GATE_FULL) store_eight(a.dgate + r * a.dgate_stride, c, a.channels, dg);
+            if (FULL && a.dgate) store_eight(a.dgate + r * a.dgate_stride, c, a.channels, dg);
         }
         if (a.dgate && a.gate_kind == SMX_GATE_ROW && lane == 0)
             a.dgate[r * a.dgate_stride] = static_cast<T>(tu * (1.0f - row_gate));
@@ -508,8 +515,8 @@ int32_t smx_residual_norm(const SmxResidualNormArgs* args, void* stream) {
                 constexpr int G = decltype(g)::value, N = decltype(times)::value;
                 constexpr int threads = threads_of(G), groups = threads / G;
                 const i64 want = (a.rows + groups - 1) / groups, full = kUnits * (2048 / threads);
-                k_residual_norm<T, G, N><<<static_cast<unsigned>(want < full ? want : full), threads, 0,
-                                           static_cast<hipStream_t>(stream)>>>(n);
+                (n.gate_kind == SMX_GATE_FULL ? k_residual_norm<T, true, G, N> : k_residual_norm<T, false, G, N>)<<<
+                    static_cast<unsigned>(want < full ? want : full), threads, 0, static_cast<hipStream_t>(stream)>>>(n);
             });
             SMX_LAUNCH_CHECK("k_residual_norm");
         });
@@ -567,8 +574,8 @@ int32_t smx_residual_norm_gradient(const SmxResidualNormGradientArgs* args, void
             if (a.rows > 0) {
                 with_gradient_shape(n.channels, [&](auto lanes, auto times) {
                     constexpr int G = decltype(lanes)::value, N = decltype(times)::value;
-                    k_norm_gradient<T, G, N><<<static_cast<unsigned>(count), threads_of(G), 0,
-                                               static_cast<hipStream_t>(stream)>>>(n, parts);
+                    (n.gate_kind == SMX_GATE_FULL ? k_norm_gradient<T, true, G, N> : k_norm_gradient<T, false, G, N>)<<<
+                        static_cast<unsigned>(count), threads_of(G), 0, static_cast<hipStream_t>(stream)>>>(n, parts);
                 });
                 SMX_LAUNCH_CHECK("k_norm_gradient");
             }
