@@ -504,13 +504,14 @@ void with_index(int32_t wide, F&& f) {
         f(std::int32_t{});
 }
 
-void check_embed(const void* types, i64 tokens, i64 num_types, i64 channels, int dtype) {
+void check_embed(const void* types, int32_t wide, i64 tokens, i64 num_types, i64 channels, int dtype) {
     constexpr i64 most = (1LL << 31) - 65536;  // indexes of a tile past the end stay in 31 bits
     require(tokens >= 0 && tokens <= most, "tokens must be in [0, 2^31 - 65536]");
     require(num_types >= 0 && num_types <= most, "num_types must be in [0, 2^31 - 65536]");
     require(channels >= 0 && channels <= 65535 * 512, "channels must be in [0, 65535 * 512]");
     require(dtype >= SMX_DTYPE_F32 && dtype <= SMX_DTYPE_F16, "unknown dtype code");
     require(tokens == 0 || types, "types is NULL");
+    require(aligned(types, wide ? 8 : 4), "types is not aligned to its values");
 }
 
 }  // namespace
@@ -526,7 +527,7 @@ int32_t smx_embed(const void* types, int32_t types_are_64bit, int64_t tokens, co
                   int64_t num_types, int64_t channels, int32_t dtype, float scale, void* out, int64_t out_stride,
                   void* stream) {
     return guarded([&] {
-        check_embed(types, tokens, num_types, channels, dtype);
+        check_embed(types, types_are_64bit, tokens, num_types, channels, dtype);
         check_rows(table, table_stride, num_types, channels, dtype, "table");
         check_rows(out, out_stride, tokens, channels, dtype, "out");
         if (tokens == 0 || channels == 0) return;
@@ -555,7 +556,7 @@ int32_t smx_embed_gradient(const void* types, int32_t types_are_64bit, int64_t t
                            int64_t grad_stride, int64_t num_types, int64_t channels, int32_t dtype, float scale,
                            void* out, int64_t out_stride, void* workspace, int64_t workspace_bytes, void* stream) {
     return guarded([&] {
-        check_embed(types, tokens, num_types, channels, dtype);
+        check_embed(types, types_are_64bit, tokens, num_types, channels, dtype);
         check_rows(grad, grad_stride, tokens, channels, dtype, "grad");
         check_rows(out, out_stride, num_types, channels, dtype, "out");
         check_workspace(workspace, workspace_bytes, smx_embed_gradient_workspace(tokens, num_types, channels));

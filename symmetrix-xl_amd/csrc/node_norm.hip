@@ -371,7 +371,7 @@ template <class T>
 __global__ void __launch_bounds__(1024) k_norm_gradient_join(Norm<T> a, const float* __restrict__ parts, int count) {
     __shared__ float room[16][64];
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = blockIdx.x * 64 + lane, k = blockIdx.y;
-    if (k == 0 ? !a.d && a.rows > 0 : !a.dnext) return;
+    if (k == 0 ? !a.d : !a.dnext) return;
     float sum = 0.0f;
     if (c < a.channels)
 #pragma unroll 8
@@ -392,6 +392,16 @@ __global__ void __launch_bounds__(1024) k_norm_gradient_join(Norm<T> a, const fl
     }
     if (a.dpost) a.dpost[c] = sum * scale * gate;
     if (a.dscale) a.dscale[c] = sum * a.post[c] * gate;
+}
+
+// The channel vectors' gradients of no rows.
+template <class T>
+__global__ void __launch_bounds__(256) k_norm_gradient_none(Norm<T> a) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= a.channels) return;
+    if (a.dgate_channel) a.dgate_channel[c] = static_cast<T>(0.0f);
+    for (float* const out : {a.dpost, a.dscale, a.dnext})
+        if (out) out[c] = 0.0f;
 }
 
 // f(lanes a row, times eight values a lane) for the forward kernel: up to 16 values
@@ -466,7 +476,7 @@ Norm<T> device_args(const SmxResidualNormArgs& a) {
     Norm<T> n{};
     n.rows = a.rows;
     n.channels = static_cast<int>(a.channels);
-    n.gate_kind = a.d || a.rows == 0 ? a.gate_kind : SMX_GATE_NONE;
+    n.gate_kind = a.d ? a.gate_kind : SMX_GATE_NONE;
     n.eps = a.eps;
     n.x = static_cast<const T*>(a.x);
     n.d = static_cast<const T*>(a.d);
@@ -543,7 +553,7 @@ int32_t smx_residual_norm_gradient(const SmxResidualNormGradientArgs* args, void
         if (g.grad_h) check_rows(g.grad_h, g.grad_h_stride, a.rows, a.channels, a.dtype, "grad_h");
         if (g.dx) check_rows(g.dx, g.dx_stride, a.rows, a.channels, a.dtype, "dx");
         require(a.d || a.rows == 0 || (!g.dd && !g.dgate && !g.dpost && !g.dscale), "gradients of d, gate, post or scale without d");
-        require(!g.dgate || a.gate_kind != SMX_GATE_NONE, "dgate without a gate");
+        require(!g.dgate || (a.gate_kind >= SMX_GATE_FULL && a.gate_kind <= SMX_GATE_ROW), "dgate without a gate");
         require(!g.dscale || a.scale, "dscale without scale");
         require(!g.dnext || a.next, "dnext without next");
         if (g.dd) check_rows(g.dd, g.dd_stride, a.rows, a.channels, a.dtype, "dd");
@@ -572,16 +582,20 @@ int32_t smx_residual_norm_gradient(const SmxResidualNormGradientArgs* args, void
             n.dscale = g.dscale;
             n.dnext = g.dnext;
             const bool sums = n.dgate_channel || n.dpost || n.dscale || n.dnext;
-            float* const parts = sums ? static_cast<float*>(g.workspace) : nullptr;
-            const i64 count = a.rows > 0 ? gradient_groups(a.rows, a.channels) : 0;
-            if (a.rows > 0) {
-                with_gradient_shape(n.channels, [&](auto lanes, auto times) {
-                    constexpr int G = decltype(lanes)::value, N = decltype(times)::value;
-                    (n.gate_kind == SMX_GATE_FULL ? k_norm_gradient<T, true, G, N> : k_norm_gradient<T, false, G, N>)<<<
-                        static_cast<unsigned>(count), threads_of(G), 0, static_cast<hipStream_t>(stream)>>>(n, parts);
-                });
-                SMX_LAUNCH_CHECK("k_norm_gradient");
+            if (a.rows == 0) {
+                if (!sums) return;
+                k_norm_gradient_none<T><<<blocks_for(a.channels, 256), 256, 0, static_cast<hipStream_t>(stream)>>>(n);
+                SMX_LAUNCH_CHECK("k_norm_gradient_none");
+                return;
             }
+            float* const parts = sums ? static_cast<float*>(g.workspace) : nullptr;
+            const i64 count = gradient_groups(a.rows, a.channels);
+            with_gradient_shape(n.channels, [&](auto lanes, auto times) {
+                constexpr int G = decltype(lanes)::value, N = decltype(times)::value;
+                (n.gate_kind == SMX_GATE_FULL ? k_norm_gradient<T, true, G, N> : k_norm_gradient<T, false, G, N>)<<<
+                    static_cast<unsigned>(count), threads_of(G), 0, static_cast<hipStream_t>(stream)>>>(n, parts);
+            });
+            SMX_LAUNCH_CHECK("k_norm_gradient");
             if (sums) {
                 k_norm_gradient_join<T><<<dim3(blocks_for(a.channels, 64), kSums), 1024, 0,
                                           static_cast<hipStream_t>(stream)>>>(n, parts, static_cast<int>(count));

@@ -54,7 +54,14 @@ class BlockValues:
     __slots__ = ("shape", "_room", "_at")
 
     def __init__(self, values, scales, shape):
-        self.shape, self._room = tuple(shape), (values, scales)
+        rows, cols = shape
+        pitch, scale_pitch = _pitches(cols)
+        for t, name, width in ((values, "values", pitch), (scales, "scales", scale_pitch)):
+            if t.element_size() != 1 or tuple(t.shape) != (rows, width) or not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError("%s must be contiguous bytes [%d][%d], 16-byte aligned" % (name, rows, width))
+        if values.device != scales.device:
+            raise ValueError("values and scales must be on one device")
+        self.shape, self._room = (rows, cols), (values, scales)
         self._at = values.data_ptr(), scales.data_ptr()
 
     @classmethod

@@ -24,6 +24,7 @@ def test_embed_refuses():
     def call(types=FAKE, tokens=4, table=FAKE, stride=8, v=3, c=8, dtype=0, out=FAKE, out_stride=8):
         return lib.smx_embed(types, 0, tokens, table, stride, v, c, dtype, 1.0, out, out_stride, None)
     _refused(call(types=None), "types is NULL")
+    _refused(call(types=FAKE + 2), "types is not aligned")
     _refused(call(tokens=-1), "tokens")
     _refused(call(tokens=1 << 31), "tokens")
     _refused(call(v=-1), "num_types")
@@ -42,6 +43,7 @@ def test_embed_gradient_refuses():
         size = lib.smx_embed_gradient_workspace(tokens, v, c) if size is None else size
         return lib.smx_embed_gradient(types, 1, tokens, grad, stride, v, c, 1, 1.0, out, 8, room, size, None)
     _refused(call(types=None), "types is NULL")
+    _refused(call(types=FAKE + 4), "types is not aligned")  # int64 here
     _refused(call(grad=None), "grad is NULL")
     _refused(call(stride=4), "grad: the row stride")
     _refused(call(out=None), "out is NULL")
@@ -198,13 +200,21 @@ def test_python_refusals():
         node_ops.quantize(x, rows=False)
     with pytest.raises(ValueError, match="BlockValues"):
         node_ops.block_linear(x, x)
-    blocks = node_ops.BlockValues(torch.zeros(3, 128), torch.zeros(3, 4), (3, 9))
+    def bytes_of(*shape):
+        return torch.zeros(*shape, dtype=torch.uint8)
+    blocks = node_ops.BlockValues(bytes_of(3, 128), bytes_of(3, 4), (3, 9))
     with pytest.raises(ValueError, match="as many columns"):
         node_ops.block_linear(x, blocks)
     with pytest.raises(ValueError, match="as many columns"):
-        node_ops.block_product(node_ops.BlockValues(torch.zeros(3, 128), torch.zeros(3, 4), (3, 8)), blocks)
+        node_ops.block_product(node_ops.BlockValues(bytes_of(3, 128), bytes_of(3, 4), (3, 8)), blocks)
     with pytest.raises(ValueError, match="products are"):
         node_ops.block_product(blocks, blocks, torch.float64)
+    for values, scales, shape in ((bytes_of(3, 127), bytes_of(3, 4), (3, 9)), (bytes_of(3, 128), bytes_of(3, 1), (3, 9)),
+                                  (bytes_of(3, 128), bytes_of(3, 4), (3, 129)), (bytes_of(2, 128), bytes_of(3, 4), (3, 9)),
+                                  (torch.zeros(3, 128), bytes_of(3, 4), (3, 9)),
+                                  (bytes_of(128, 3).T, bytes_of(3, 4), (3, 9))):
+        with pytest.raises(ValueError, match="contiguous bytes"):
+            node_ops.BlockValues(values, scales, shape)
 
 
 # ---- the reference itself ----
