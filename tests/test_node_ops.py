@@ -47,10 +47,11 @@ def test_embed_gradient_refuses():
     _refused(call(grad=None), "grad is NULL")
     _refused(call(stride=4), "grad: the row stride")
     _refused(call(out=None), "out is NULL")
-    if lib.smx_embed_gradient_workspace(100, 3, 8):
-        _refused(call(size=0), "workspace")
-        _refused(call(room=None), "workspace")
-        _refused(call(room=FAKE + 8), "aligned")
+    assert lib.smx_embed_gradient_workspace(256, 3, 8) == 0  # few atoms need none
+    assert lib.smx_embed_gradient_workspace(5000, 3, 8) > 0
+    _refused(call(tokens=5000, size=0), "workspace")
+    _refused(call(tokens=5000, room=None), "workspace")
+    _refused(call(tokens=5000, room=FAKE + 8), "aligned")
     assert call(v=0, out=None) == 0
 
 

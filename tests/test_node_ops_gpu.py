@@ -55,7 +55,9 @@ def _types(gen, tokens, v, kind, dtype):
 EMBED = [(0, 5, 8, "any"), (1, 1, 1, "any"), (1, 89, 128, "any"), (63, 2, 3, "any"), (65, 7, 100, "outside"),
          (300, 89, 32, "none"), (1000, 3, 257, "one"), (1000, 256, 64, "any"), (1000, 257, 33, "outside"),
          (5000, 89, 128, "outside"), (5001, 2, 96, "any"), (4097, 70001, 40, "outside"), (40000, 300, 24, "any"),
-         (9000, 66000, 16, "any"), (30, 40, 2050, "any")]
+         (9000, 66000, 16, "any"), (30, 40, 2050, "any"), (256, 5, 600, "any"), (257, 5, 600, "any"),
+         (255, 20000, 96, "outside"), (200, 2, 20, "any"), (1024, 1024, 70, "outside"), (1025, 3, 40, "any"),
+         (900, 1025, 48, "outside")]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
