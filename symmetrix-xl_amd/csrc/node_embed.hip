@@ -336,7 +336,7 @@ constexpr int kRuns[3] = {64, 16, 8};
 // 256 / lanes groups a workgroup, each `length` sorted atoms of 8 lanes' channels.  A type whose atoms lie
 // within a group is done there; the first and last runs of the groups are joined in LDS, in order; what crosses
 // the workgroup's ends leaves as a part: [0] of a run that goes on from the workgroup before, [1] of one that starts here
-// and goes on in the next.  Bound by the gathered rows: 131,071 of 2 KB in 79 us (3.4 TB/s, and 0.6 of stores), eight
+// and goes on in the next.  Bound by the gathered rows: 131,071 of 2 KB in 76 us (3.5 TB/s, and 0.7 of stores), eight
 // of them under way a group and the next eight's places read meanwhile.
 template <class T>
 __global__ void __launch_bounds__(256) k_embed_runs(const int* __restrict__ keys, const int* __restrict__ order, i64 tokens,
@@ -385,6 +385,10 @@ __global__ void __launch_bounds__(256) k_embed_runs(const int* __restrict__ keys
     for (int b = 0; b < length; b += 8) {
         int here[8];
         Eight<T> row[8];
+        // all eight places are waited for here: a wait between the rows' loads would be for the rows before as well
+        // (131,071 rows of 2 KB: 84 -> 76 us)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(key[j]), "+v"(atom[j]));
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             here[j] = key[j];
