@@ -120,8 +120,7 @@ __global__ void __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) k_embed_gradient
 // The sort is a stable radix sort of (type, atom), eight bits a pass, least first; types outside the
 // table sort last as num_types.  Up to kSmall atoms one workgroup sorts in LDS; above, tiles of
 // kTile atoms (times up to 512 tiles) are counted, and each pass places a tile's atoms by the counts of all tiles
-// before it and counts the next pass's digits where they land.  The sort is latency, not bytes: 5 us in one
-// workgroup (135 atoms), 3.8 + 6.8 for 30,000 atoms, 4.9 + 2 x 13 for 131,071 and types of 16 bits.
+// before it.  The sort is latency, not bytes: 5 us a pass in one workgroup, 3.8 + 6.8 for 30,000 atoms.
 
 constexpr int kUnits = 256;  // compute units
 constexpr int kDigits = 256, kTile = 1024, kMostTiles = 512, kSmall = 4096;
@@ -250,30 +249,32 @@ __global__ void __launch_bounds__(1024) k_sort_small(const I* __restrict__ types
         if (in[k]) keys[wave * 64 * N + 64 * k + lane] = key[k], order[wave * 64 * N + 64 * k + lane] = atom[k];
 }
 
-// Counts the lowest digits of a tile's types; clears the later passes' counts and `seen`.
+// Counts a pass's digits of each tile, of the types or of the pass before's keys, into counts [tiles][256]; clears
+// `seen` where it is given.  (Counted by each pass for the next as it places its atoms, with atomics across the card, the
+// sort of 300,000 atoms took 44 us more.)
 template <class I>
 __global__ void __launch_bounds__(256) k_sort_count(const I* __restrict__ types, i64 tokens, i64 num_types, int tile,
-                                                    int* __restrict__ counts, i64 later, std::uint8_t* __restrict__ seen) {
+                                                    int shift, int* __restrict__ counts, std::uint8_t* __restrict__ seen) {
     __shared__ int count[kDigits];
     count[threadIdx.x] = 0;
     __syncthreads();
     const i64 first = static_cast<i64>(blockIdx.x) * tile, last = first + tile < tokens ? first + tile : tokens;
     for (i64 t = first + threadIdx.x; t < last; t += 256)
-        atomicAdd(&count[sort_key(types, t, num_types) & (kDigits - 1)], 1);
+        atomicAdd(&count[sort_key(types, t, num_types) >> shift & (kDigits - 1)], 1);
     __syncthreads();
     const i64 hop = static_cast<i64>(gridDim.x) * 256, me = static_cast<i64>(blockIdx.x) * 256 + threadIdx.x;
     counts[me] = count[threadIdx.x];
-    for (i64 i = hop + me; i < hop + later; i += hop) counts[i] = 0;
+    if (!seen) return;
     for (i64 v = me; v < num_types; v += hop) seen[v] = 0;
 }
 
 // One pass: a tile's atoms to their places, sixteen waves a workgroup (a pass is latency: its reads of the
-// counts, its scan and its scattered stores).  counts: this pass's [tiles][256]; next: the following
-// pass's, or NULL.  The first pass (types given) reads the types themselves.
+// counts, its scan and its scattered stores).  counts: this pass's [tiles][256].  The first pass (types
+// given) reads the types themselves.
 template <class I>
 __global__ void __launch_bounds__(1024) k_sort_place(const I* __restrict__ types, const int* __restrict__ keys_in,
                                                      const int* __restrict__ order_in, i64 tokens, i64 num_types, int tile,
-                                                     int shift, const int* __restrict__ counts, int* __restrict__ next,
+                                                     int shift, const int* __restrict__ counts,
                                                      int* __restrict__ keys, int* __restrict__ order) {
     constexpr int kWaves = 16, N = kTile / 1024;
     __shared__ RankRoom<kWaves> room;
@@ -322,8 +323,6 @@ __global__ void __launch_bounds__(1024) k_sort_place(const I* __restrict__ types
                 const int to = room.count[wave][digit[k]] + rank[k];
                 keys[to] = key[k];
                 order[to] = atom[k];
-                // (a sum of ones: its order does not matter)
-                if (next) atomicAdd(&next[to / tile * kDigits + (key[k] >> (shift + 8) & (kDigits - 1))], 1);
             }
         __syncthreads();
     }
@@ -571,7 +570,7 @@ Workspace plan_gradient(i64 tokens, i64 num_types, i64 channels) {
     if (!small) {
         w.keys[1] = take(4 * tokens);
         w.order[1] = take(4 * tokens);
-        w.counts = take(4LL * kDigits * w.tiles * w.passes);
+        w.counts = take(4LL * kDigits * w.tiles);
     }
     w.seen = take(num_types);
     w.parts = take(8LL * w.chunks * channels);
@@ -678,16 +677,17 @@ int32_t smx_embed_gradient(const void* types, int32_t types_are_64bit, int64_t t
                 SMX_LAUNCH_CHECK("k_sort_small");
                 return;
             }
-            const i64 pass = static_cast<i64>(w.tiles) * kDigits;
-            k_sort_count<I><<<w.tiles, 256, 0, queue>>>(z, tokens, num_types, w.tile, ints(w.counts), (w.passes - 1) * pass,
-                                                        seen);
-            SMX_LAUNCH_CHECK("k_sort_count");
             for (int p = 0; p < w.passes; ++p, at ^= 1) {
-                int* const counts = ints(w.counts) + p * pass;
+                int* const counts = ints(w.counts);
+                if (p == 0)
+                    k_sort_count<I><<<w.tiles, 256, 0, queue>>>(z, tokens, num_types, w.tile, 0, counts, seen);
+                else
+                    k_sort_count<int><<<w.tiles, 256, 0, queue>>>(ints(w.keys[at ^ 1]), tokens, num_types, w.tile, 8 * p, counts,
+                                                                  nullptr);
+                SMX_LAUNCH_CHECK("k_sort_count");
                 k_sort_place<I><<<w.tiles, 1024, 0, queue>>>(p ? nullptr : z, ints(w.keys[at ^ 1]), ints(w.order[at ^ 1]), tokens,
-                                                            num_types, w.tile, 8 * p, counts,
-                                                            p + 1 < w.passes ? counts + pass : nullptr, ints(w.keys[at]),
-                                                            ints(w.order[at]));
+                                                             num_types, w.tile, 8 * p, counts, ints(w.keys[at]),
+                                                             ints(w.order[at]));
                 SMX_LAUNCH_CHECK("k_sort_place");
             }
             at ^= 1;
