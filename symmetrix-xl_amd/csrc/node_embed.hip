@@ -21,25 +21,39 @@ inline int lanes_of(i64 channels) {
     return g;
 }
 
-// A group of lanes a row: its type, then sixteen bytes a lane of the table's row and of out's.  Bound by the stores
-// (131,071 rows of 2 KB in 99 us, 2.7 TB/s of stores; a fill reaches 3.4), below some ten thousand rows by latency (5,000
-// of 512 B: 3.0 us).  Several rows a group at once were slower (112 us at four).
-template <class T, class I>
+// A group of lanes a row: its type, then sixteen bytes a lane of the table's row and of out's.  Where out is more than the
+// last cache holds (256 MB, the rows read included) a group has four rows, whose types are waited for together (a wait
+// between the rows' loads would be for the rows before as well): 300,000 rows of 2 KB in 177 us, 212 at a row a group;
+// 131,071 in 78 to 82, 82 to 98.  Below it one row: 65,536 rows of 1 KB in 20.8 us, 21.4 at four; 5,000 of 512 B, where
+// latency counts, in 3.0 and 3.8.
+constexpr i64 kManyBytes = i64{192} << 20;
+
+template <class T, class I, int ROWS>
 __global__ void __launch_bounds__(256) k_embed(const I* __restrict__ types, i64 tokens, const T* __restrict__ table,
                                                i64 table_stride, i64 num_types, int channels, float scale,
                                                T* __restrict__ out, i64 out_stride, int lanes) {
     const int groups = 256 / lanes;
     const int c = 8 * (blockIdx.y * lanes + threadIdx.x % lanes);
     if (c >= channels) return;
-    for (i64 t = static_cast<i64>(blockIdx.x) * groups + threadIdx.x / lanes; t < tokens;
-         t += static_cast<i64>(gridDim.x) * groups) {
-        const int z = type_of(types, t, num_types);
-        Eight<T> row;
-        if (z >= 0) row = load_pack(table + z * table_stride, c, channels);
-        float v[8];
+    for (i64 t0 = (static_cast<i64>(blockIdx.x) * groups + threadIdx.x / lanes) * ROWS; t0 < tokens;
+         t0 += static_cast<i64>(gridDim.x) * groups * ROWS) {
+        int z[ROWS];
+        Eight<T> row[ROWS];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = z < 0 ? 0.0f : scale * row[i];
-        store_eight(out + t * out_stride, c, channels, v);
+        for (int k = 0; k < ROWS; ++k) z[k] = type_of(types, t0 + k < tokens ? t0 + k : tokens - 1, num_types);
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) asm volatile("" : "+v"(z[k]));
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k)
+            if (z[k] >= 0) row[k] = load_pack(table + z[k] * table_stride, c, channels);
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+            if (t0 + k >= tokens) break;
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = z[k] < 0 ? 0.0f : scale * row[k][i];
+            store_eight(out + (t0 + k) * out_stride, c, channels, v);
+        }
     }
 }
 
@@ -616,12 +630,14 @@ int32_t smx_embed(const void* types, int32_t types_are_64bit, int64_t tokens, co
             using T = decltype(t);
             with_index(types_are_64bit, [&](auto i) {
                 using I = decltype(i);
-                const int lanes = lanes_of(channels), groups = 256 / lanes;
-                const i64 want = (tokens + groups - 1) / groups;
-                k_embed<T, I><<<dim3(static_cast<unsigned>(want < (1 << 20) ? want : 1 << 20), blocks_for(channels, 8 * lanes)), 256,
-                                0, static_cast<hipStream_t>(stream)>>>(
-                    static_cast<const I*>(types), tokens, static_cast<const T*>(table), table_stride, num_types,
-                    static_cast<int>(channels), scale, static_cast<T*>(out), out_stride, lanes);
+                const bool many = tokens * channels * static_cast<i64>(sizeof(T)) >= kManyBytes;
+                const int lanes = lanes_of(channels), rows = 256 / lanes * (many ? 4 : 1);
+                const i64 want = (tokens + rows - 1) / rows;
+                (many ? k_embed<T, I, 4> : k_embed<T, I, 1>)<<<
+                    dim3(static_cast<unsigned>(want < (1 << 20) ? want : 1 << 20), blocks_for(channels, 8 * lanes)), 256, 0,
+                    static_cast<hipStream_t>(stream)>>>(static_cast<const I*>(types), tokens, static_cast<const T*>(table),
+                                                        table_stride, num_types, static_cast<int>(channels), scale,
+                                                        static_cast<T*>(out), out_stride, lanes);
                 SMX_LAUNCH_CHECK("k_embed");
             });
         });

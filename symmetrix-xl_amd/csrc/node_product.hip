@@ -195,6 +195,30 @@ __device__ __forceinline__ void store_four(const Product<O>& p, int i, int j, ac
     }
 }
 
+// Sixteen bytes of neighbouring outputs of row i from column j on.
+template <class O>
+__device__ __forceinline__ void store_sixteen(const Product<O>& p, int i, int j, i32x4 v) {
+    constexpr int kValues = 16 / sizeof(O);
+    struct __attribute__((packed, aligned(sizeof(O)))) Words {
+        i32x4 w;
+    };
+    if (i >= p.m) return;
+    O* const at = p.out + i * p.out_stride + j;
+    if (j + kValues <= p.n) {
+        reinterpret_cast<Words*>(at)->w = v;
+        return;
+    }
+    union {
+        i32x4 w;
+        O o[kValues];
+    } parts;
+    asm volatile("" : "+v"(v));  // (apart from the whole store)
+    parts.w = v;
+#pragma unroll
+    for (int q = 0; q < kValues; ++q)
+        if (j + q < p.n) at[q] = parts.o[q];
+}
+
 // 1 KB of LDS at byte `lds` (the wave's own, uniform) from 64 lanes' 16 bytes at their offsets `at`
 // into the buffer: memory to LDS without registers.  The compiler does not count it: dma_wait.
 __device__ __forceinline__ void dma(__amdgpu_buffer_rsrc_t from, unsigned lds, int at, int also) {
@@ -222,7 +246,7 @@ __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" :
 // four values lie side by side in a row of the output.  With KG == 1 a workgroup goes through every gridDim.x-th
 // tile, and the next one's first blocks arrive while this one's last are multiplied and stored.  With KG > 1, for
 // few tiles, KG groups of waves take every KG-th block each, so that their waits overlap, and their sums are joined in LDS.
-// Large products: 16384 x 8192 x 8192 in 861 us, 2,555 TFLOP/s (a library's product of 8-bit values with one scale
+// Large products: 16384 x 8192 x 8192 in 855 us, 2,570 TFLOP/s (a library's product of 8-bit values with one scale
 // reached 2,880): the matrix pipes are 57% busy at the 1.8 GHz that the clock falls to, LDS has no bank conflicts; a tile's
 // 192 KB of fragment reads and 64 KB of arriving blocks a step are as long as its products at LDS's 128 B a clock.
 // To FP32 8192 cubed takes 767 us, 1,433 TFLOP/s (a library's bf16 product 1,406).
@@ -383,10 +407,39 @@ k_product_tile(Product<O> p) {
             store_four(p, i_now + wm + 16 * f + lane % 16, j_now + wn + 16 * g + 4 * (lane / 16), v, blockIdx.y);
         };
         if constexpr (KG == 1) {
+            if (sizeof(O) == 4 || p.partial) {
 #pragma unroll
-            for (int f = 0; f < MF; ++f)
+                for (int f = 0; f < MF; ++f)
 #pragma unroll
-                for (int g = 0; g < NF; ++g) put(f, g, acc[f][g]);
+                    for (int g = 0; g < NF; ++g) put(f, g, acc[f][g]);
+                continue;
+            }
+            // Values of two bytes go through LDS (the last blocks' place, once all have read them), 16 rows at a time,
+            // so that a store is of sixteen bytes a lane and whole lines: 20000 x 1024 x 512 in 17.9 us, 20.9 without.
+            constexpr int kRow = 16 * NF * sizeof(O) + 16, kLanes = NF * sizeof(O);
+            static_assert(sizeof(O) == 4 || WAVES * 16 * kRow <= kStage);
+            std::uint8_t* const room = lds + (slot ^ 1) * kStage + wave * 16 * kRow;
+            __syncthreads();
+#pragma unroll
+            for (int f = 0; f < MF; ++f) {
+#pragma unroll
+                for (int g = 0; g < NF; ++g) {
+                    Pack<O, 4> o;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) o.v[q] = static_cast<O>(acc[f][g][q]);
+                    __builtin_memcpy(__builtin_assume_aligned(
+                                         room + lane % 16 * kRow + (16 * g + 4 * (lane / 16)) * sizeof(O), 4 * sizeof(O)),
+                                     &o, sizeof(o));
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+                for (int q = 0; q < kLanes / 4; ++q) {
+                    const int r = lane / kLanes + 64 / kLanes * q, c = lane % kLanes;
+                    store_sixteen(p, i_now + wm + 16 * f + r, j_now + wn + c * static_cast<int>(16 / sizeof(O)),
+                                  *reinterpret_cast<const i32x4*>(room + r * kRow + 16 * c));
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            }
         } else {
             // fragment q of every group is added up, in the groups' order, by group q % KG
             acc4* const room = reinterpret_cast<acc4*>(lds);
@@ -477,7 +530,7 @@ __global__ void __launch_bounds__(64 * KS) k_product_rows(Product<O> p, const T*
             }
         }
         if constexpr (RAW) {
-            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
             for (int q = 0; q < kAhead; ++q) {
 #pragma unroll
@@ -485,7 +538,7 @@ __global__ void __launch_bounds__(64 * KS) k_product_rows(Product<O> p, const T*
                     wa[q][h] = *reinterpret_cast<const i32x4*>(&brought[wave][q][row % kRawRows * kBlock + at + 64 * h]);
                 sa[q] = brought_scale[wave][q][row % kRawRows];
             }
-            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
 #pragma unroll
         for (int q = 0; q < kAhead; ++q) {

@@ -83,6 +83,17 @@ def test_embed_both_ways(gen, tokens, v, c, kind, index, dtype):
     assert torch.equal(got, ops.embed_gradient(z, grad, v, scale))  # the same bits again
 
 
+@pytest.mark.parametrize("dtype, c, more", [(F32, 1023, 1), (BF16, 2050, 0), (F16, 2048, 8)], ids=IDS)
+@pytest.mark.parametrize("index", [torch.int32, torch.int64], ids=["i32", "i64"])
+def test_embed_of_many_rows(gen, dtype, c, more, index):
+    """Outputs of over 200 MB, against the same rows in parts of a fiftieth."""
+    z = _types(gen, 51_203, 301, "outside", index)
+    table = _normal(gen, 301, c, dtype=dtype)
+    out = ops.embed(z, _view(table, 0, more), 1.7)
+    for i in range(0, z.numel(), 1000):
+        assert torch.equal(out[i:i + 1000], ops.embed(z[i:i + 1000].contiguous(), table, 1.7)), i
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("offset, more", [(0, 8), (1, 0), (3, 5)])
 def test_embed_strides(gen, offset, more, dtype):
@@ -361,6 +372,20 @@ def test_linear_sizes(gen, m, n, k, dtype):
     assert_within(y32, want, bound)
     if m:
         assert torch.equal(d(xt.float()), quantized(x.T)[0])
+
+
+# products of more tiles than the card holds at once, and of each tile's size, with edges in both directions
+MANY_TILES = [(2500, 2501, 200), (2500, 2499, 300), (4090, 4085, 140), (4090, 4085, 300), (4100, 4098, 260),
+              (8190, 4091, 130), (8190, 4091, 260), (100_000, 60, 130), (100_001, 61, 390)]
+
+
+@pytest.mark.parametrize("m, n, k", MANY_TILES)
+def test_product_of_many_tiles(gen, m, n, k):
+    x, w = ops.quantize(_normal(gen, m, k, dtype=BF16)), ops.quantize(_normal(gen, n, k) / math.sqrt(k))
+    a, b = d(x.float()), d(w.float())
+    want, bound = product(a, b)
+    for dtype in TYPES:
+        assert_within(ops.block_product(x, w, dtype), want, bound)
 
 
 def test_linear_without_inputs(gen):
