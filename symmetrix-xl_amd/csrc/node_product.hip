@@ -599,20 +599,24 @@ struct Plan {
 constexpr int kUnits = 256;  // compute units
 
 // The tile is the one whose rounds over the card take least: a unit holds one tile of 256 at a
-// time, two of 128 or four of 64, whose rates on large products are as 1 : 1/1.12 : 1/1.86 (2,607, 2,322 and
-// 1,401 TFLOP/s at 8192 x 8192 x 8192).  20000 x 1024 x 512: 38.9 us in 316 tiles of 256, two rounds, 28.5 in 1,256 of
-// 128; 4096 x 2048 x 8192 to FP32: 176 and 118 us.
+// time, two of 128 or four of 64, whose rates on large products are as 1 : 1/1.12 : 1/1.86 (2,600, 2,320 and
+// 1,400 TFLOP/s at 8192 x 8192 x 8192), but one round of four tiles of 64 on every unit is slower than one of 128
+// (2048 cubed 16.4 and 14.2 us).  20000 x 1024 x 512: 21.8 us in 316 tiles of 256, two rounds, 18.5 in 1,256 of 128.
+// Four groups of waves share the blocks of a tile of 64 where that leaves no unit two of them and the sum is long enough
+// for it: 1024 x 1024 x 2048 in 7.4 us (7.8 without), x 8192 in 20.9 (34.0), but x 512 in 5.0 (3.9).  Parts of the sum pay
+// from 24 blocks on: 100 x 1000 x 4096 in 8.4 us in four parts (9.0), 512 x 1024 x 2048 in 9.8 us in two (6.8).
 Plan plan_product(i64 m, i64 n, i64 k) {
     const auto tiles = [&](i64 t) { return (m + t - 1) / t * ((n + t - 1) / t); };
     const auto rounds = [&](i64 t, i64 held) { return (tiles(t) + held * kUnits - 1) / (held * kUnits); };
     const i64 blocks = (k + kBlock - 1) / kBlock;
-    const double t256 = 1.0 * rounds(256, 1), t128 = 1.12 / 2 * rounds(128, 2), t64 = 1.86 / 4 * rounds(64, 4);
+    const bool full = tiles(64) > 3 * kUnits && tiles(64) <= 4 * kUnits;
+    const double t256 = 1.0 * rounds(256, 1), t128 = 1.12 / 2 * rounds(128, 2), t64 = (full ? 2.4 : 1.86) / 4 * rounds(64, 4);
     Plan p{t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64, 1, 1, blocks};
     const i64 count = tiles(p.tile);
-    if (p.tile == 64 && count <= 2 * kUnits && blocks >= 4) {
+    if (p.tile == 64 && count <= kUnits && blocks >= 12) {
         p.groups = 4;
-        // parts of at least eight blocks, up to a tile for each unit
-        const i64 want = kUnits / count, most = blocks / 8, parts = want < most ? want : most;
+        // parts of at least eight blocks, up to a tile for each unit; a second launch joins them
+        const i64 want = kUnits / count, most = blocks < 24 ? 1 : blocks / 8, parts = want < most ? want : most;
         if (parts > 1) {
             p.split_blocks = ((blocks + parts - 1) / parts + 3) / 4 * 4;  // scales are read four blocks at a time
             p.splits = static_cast<int>((blocks + p.split_blocks - 1) / p.split_blocks);

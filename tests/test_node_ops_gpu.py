@@ -355,7 +355,7 @@ def test_quantize_strides(gen, offset, more, dtype):
 LINEAR = [(0, 8, 8), (1, 1, 1), (1, 16, 128), (1, 1000, 513), (2, 64, 300), (7, 33, 4096), (15, 128, 128),
           (16, 255, 129), (17, 16, 1000), (31, 512, 2048), (33, 100, 64), (64, 64, 64), (65, 4097, 130), (100, 1, 100),
           (128, 128, 512), (129, 300, 260), (200, 1030, 1), (257, 512, 640), (300, 257, 2050), (513, 300, 127),
-          (1000, 520, 1024), (30, 5000, 700), (520, 20, 9000)]
+          (1000, 520, 1024), (30, 5000, 700), (520, 20, 9000), (70, 1001, 5000), (700, 1300, 1500)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
