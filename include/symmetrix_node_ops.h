@@ -48,8 +48,8 @@ SMX_API int32_t smx_embed(const void* types, int32_t types_are_64bit, int64_t to
                           int64_t table_stride, int64_t num_types, int64_t channels, int32_t dtype, float scale,
                           void* out, int64_t out_stride, void* stream);
 /* out[v][c] = scale * sum over the t with types[t] == v of grad[t][c], every row
- * of out written (zeros for a type without atoms).  The atoms are sorted by type
- * (stably) and each type's rows summed in a fixed order. */
+ * of out written (zeros for a type without atoms).  Each type's rows are summed
+ * in FP32 and a fixed order: the same call gives the same bits. */
 SMX_API int64_t smx_embed_gradient_workspace(int64_t tokens, int64_t num_types, int64_t channels);
 SMX_API int32_t smx_embed_gradient(const void* types, int32_t types_are_64bit, int64_t tokens, const void* grad,
                                    int64_t grad_stride, int64_t num_types, int64_t channels, int32_t dtype,

@@ -15,9 +15,9 @@ __device__ __forceinline__ int type_of(const I* types, i64 t, i64 num_types) {
 
 // Lanes that share a row, eight channels each: a power of two up to a wave, which takes wider rows
 // in slabs of 512.
-inline int lanes_of(i64 channels) {
+inline int lanes_of(i64 channels, int most = 64) {
     int g = 8;
-    while (g < 64 && 8 * g < channels) g *= 2;
+    while (g < most && 8 * g < channels) g *= 2;
     return g;
 }
 
@@ -49,6 +49,7 @@ __global__ void __launch_bounds__(256) k_embed(const I* __restrict__ types, i64 
 #pragma unroll
         for (int k = 0; k < ROWS; ++k) {
             if (t0 + k >= tokens) break;
+            settle(row[k], c, channels);
             float v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = z[k] < 0 ? 0.0f : scale * row[k][i];
@@ -101,9 +102,11 @@ __global__ void __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) k_embed_gradient
                 }
 #pragma unroll
                 for (int j = 0; j < kAhead; ++j)
-                    if (atom[j] >= 0 && c < channels)
+                    if (atom[j] >= 0 && c < channels) {
+                        settle(row[j], c, channels);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) sum[i] += row[j][i];
+                    }
             }
         }
         for (int o = lanes; o < 64; o *= 2)
@@ -127,6 +130,92 @@ __global__ void __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) k_embed_gradient
             store_eight(out + v * out_stride, c, channels, sum);
         }
     }
+}
+
+// ---- the gradient of few species: no sort ----
+
+// The rows of the table in registers, V of them: a group of lanes, which hold a row, reads eight rows of the gradient
+// at once (every groups-th of the workgroup's), and adds each to its type's; WAVE: a group is whole waves, whose
+// rows' types are scalars (300,000 of 3 x 448 bf16: 77 us, 86 without).  The groups are joined in LDS, the workgroups' parts
+// [blocks][num_types][channels] by k_embed_species_join, both in order.  One reading and two launches: 300,000 atoms of 3
+// species x 448 FP32 in 106 us (5.1 TB/s; sorted 150), three waves a SIMD with eight rows under way each; 30,000 of 2 x
+// 256 in 13.0 (23.5 sorted), where a round of rows is all there is.
+template <class T, class I, int V, bool WAVE>
+__global__ void __launch_bounds__(256, 3) k_embed_species(const I* __restrict__ types, i64 tokens, const T* __restrict__ grad,
+                                                       i64 grad_stride, int num_types, int channels,
+                                                       float* __restrict__ parts, int lanes, i64 chunk) {
+    constexpr int kAhead = 8;
+    __shared__ float room[256 * 8];
+    const int groups = 256 / lanes, width = 8 * lanes, group = threadIdx.x / lanes, lane = threadIdx.x % lanes;
+    const int c = 8 * lane;
+    const i64 start = blockIdx.x * chunk, end = start + chunk < tokens ? start + chunk : tokens;
+    float acc[V][8];
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[v][i] = 0.0f;
+    int next[kAhead];
+    const auto read = [&](i64 t0) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const i64 t = t0 + j * groups;
+            next[j] = t < end ? type_of(types, t, num_types) : -1;
+        }
+    };
+    read(start + group);
+    for (i64 t0 = start + group; t0 < end; t0 += kAhead * groups) {
+        int z[kAhead];
+        Eight<T> row[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) asm volatile("" : "+v"(next[j]));  // waited for together, before the rows' loads
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            z[j] = WAVE ? __builtin_amdgcn_readfirstlane(next[j]) : next[j];
+            if (z[j] >= 0 && c < channels) row[j] = load_pack(grad + (t0 + j * groups) * grad_stride, c, channels);
+        }
+        read(t0 + kAhead * groups);
+        settle(row, c, channels);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+                if (z[j] == v)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) acc[v][i] += row[j][i];
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        if (v >= num_types) break;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) room[group * width + 8 * lane + i] = acc[v][i];
+        __syncthreads();
+        for (int w = threadIdx.x; w < channels; w += 256) {
+            float sum = room[w];
+            for (int g = 1; g < groups; ++g) sum += room[g * width + w];
+            parts[(static_cast<i64>(blockIdx.x) * num_types + v) * channels + w] = sum;
+        }
+        __syncthreads();
+    }
+}
+
+// 64 values of the table a workgroup, its sixteen waves every sixteenth part.
+template <class T>
+__global__ void __launch_bounds__(1024) k_embed_species_join(const float* __restrict__ parts, int count, int num_types,
+                                                             int channels, float scale, T* __restrict__ out, i64 out_stride) {
+    __shared__ float room[16][64];
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const i64 size = static_cast<i64>(num_types) * channels, at = static_cast<i64>(blockIdx.x) * 64 + lane;
+    float sum = 0.0f;
+    if (at < size)
+#pragma unroll 8
+        for (int p = wave; p < count; p += 16) sum += parts[p * size + at];
+    room[wave][lane] = sum;
+    __syncthreads();
+    if (wave || at >= size) return;
+#pragma unroll
+    for (int w = 1; w < 16; ++w) sum += room[w][lane];
+    out[at / channels * out_stride + at % channels] = static_cast<T>(scale * sum);
 }
 
 // ---- the gradient: atoms sorted by type, then runs of one type added up ----
@@ -350,8 +439,9 @@ constexpr int kRuns[3] = {64, 16, 8};
 // within a group is done there; the first and last runs of the groups are joined in LDS, in order; what crosses
 // the workgroup's ends leaves as a part: [0] of a run that goes on from the workgroup before, [1] of one that starts here
 // and goes on in the next.  Bound by the gathered rows: 131,071 of 2 KB in 76 us (3.5 TB/s, and 0.7 of stores), eight
-// of them under way a group and the next eight's places read meanwhile.
-template <class T>
+// of them under way a group and the next eight's places read meanwhile.  WHOLE: rows of whole eights of channels, whose
+// loads have no ends to settle (300,000 of 448 FP32 153 us, 173 with them; of 447 176).
+template <class T, bool WHOLE>
 __global__ void __launch_bounds__(256) k_embed_runs(const int* __restrict__ keys, const int* __restrict__ order, i64 tokens,
                                                     const T* __restrict__ grad, i64 grad_stride, int num_types,
                                                     int channels, float scale, T* __restrict__ out, i64 out_stride,
@@ -405,9 +495,11 @@ __global__ void __launch_bounds__(256) k_embed_runs(const int* __restrict__ keys
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             here[j] = key[j];
-            if (here[j] < num_types && c < channels) row[j] = load_pack(grad + static_cast<i64>(atom[j]) * grad_stride, c, channels);
+            if (here[j] < num_types && c < channels)
+                row[j] = load_pack(grad + static_cast<i64>(atom[j]) * grad_stride, c, WHOLE ? c + 8 : channels);
         }
         if (b + 8 < length) read(b + 8);
+        if constexpr (!WHOLE) settle(row, c, channels);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             if (here[j] >= num_types) continue;  // past the end, or no species: these sort last
@@ -550,6 +642,26 @@ bool few_atoms(i64 tokens, i64 num_types, i64 channels) {
     return tokens <= (num_types <= kFewRows && channels <= 256 ? kFewWide : kFew);
 }
 
+// Up to four species, whose rows the registers hold (eight take two waves a SIMD: 300,000 atoms x 448 bf16 101 us, 80
+// sorted), in rows of up to a workgroup's channels (100,000 atoms x 4,096 bf16 in two slabs 266 us, 218 sorted), where a type
+// has enough atoms for it: 1,000 atoms x 128 of one species 6.8 us, 12.7 in one launch; of three 9.5 and 6.3.
+constexpr i64 kSpecies = 4;
+constexpr int kSpeciesLanes = 256;
+
+bool few_species(i64 tokens, i64 num_types, i64 channels) {
+    return num_types <= kSpecies && channels <= 8 * kSpeciesLanes &&
+           tokens > (few_atoms(tokens, num_types, channels) ? 2 * kFew * num_types : kFew);
+}
+
+// The three workgroups that a unit holds, or as many as take whole rounds of rows (30,000 atoms of 4 x 1,024 FP32:
+// 38.7 us, 31.6 in whole rounds), and parts of at most an eighth of the rows.
+i64 species_blocks(i64 tokens, i64 num_types, i64 channels) {
+    const int lanes = lanes_of(channels, kSpeciesLanes);
+    const i64 round = 8 * (256 / lanes), rounds = (tokens + round - 1) / round, most = tokens / (8 * num_types);
+    const i64 each = (rounds + 3 * kUnits - 1) / (3 * kUnits), blocks = (rounds + each - 1) / each;
+    return blocks < most ? blocks : most;
+}
+
 // The parts of a gradient call's workspace, in bytes from its start.
 struct Workspace {
     i64 keys[2], order[2], counts, seen, parts, size;
@@ -645,7 +757,9 @@ int32_t smx_embed(const void* types, int32_t types_are_64bit, int64_t tokens, co
 }
 
 int64_t smx_embed_gradient_workspace(int64_t tokens, int64_t num_types, int64_t channels) {
-    if (num_types <= 0 || channels <= 0 || few_atoms(tokens, num_types, channels)) return 0;
+    if (num_types <= 0 || channels <= 0) return 0;
+    if (few_species(tokens, num_types, channels)) return 4 * species_blocks(tokens, num_types, channels) * num_types * channels;
+    if (few_atoms(tokens, num_types, channels)) return 0;
     return plan_gradient(tokens, num_types, channels).size;
 }
 
@@ -659,6 +773,28 @@ int32_t smx_embed_gradient(const void* types, int32_t types_are_64bit, int64_t t
         check_workspace(workspace, workspace_bytes, smx_embed_gradient_workspace(tokens, num_types, channels));
         if (num_types == 0 || channels == 0) return;
         const auto queue = static_cast<hipStream_t>(stream);
+        if (few_species(tokens, num_types, channels)) {
+            const int lanes = lanes_of(channels, kSpeciesLanes), v = static_cast<int>(num_types), c = static_cast<int>(channels);
+            const i64 blocks = species_blocks(tokens, num_types, channels), chunk = (tokens + blocks - 1) / blocks;
+            auto* const parts = static_cast<float*>(workspace);
+            with_dtype(dtype, [&](auto t) {
+                using T = decltype(t);
+                with_index(types_are_64bit, [&](auto i) {
+                    using I = decltype(i);
+                    (lanes >= 64 ? v <= 2 ? k_embed_species<T, I, 2, true> : k_embed_species<T, I, kSpecies, true>
+                     : v <= 2    ? k_embed_species<T, I, 2, false>
+                                 : k_embed_species<T, I, kSpecies, false>)<<<
+                        static_cast<unsigned>(blocks), 256, 0, queue>>>(
+                        static_cast<const I*>(types), tokens, static_cast<const T*>(grad), grad_stride, v, c, parts, lanes,
+                        chunk);
+                });
+                SMX_LAUNCH_CHECK("k_embed_species");
+                k_embed_species_join<T><<<blocks_for(num_types * channels, 64), 1024, 0, queue>>>(
+                    parts, static_cast<int>(blocks), v, c, scale, static_cast<T*>(out), out_stride);
+                SMX_LAUNCH_CHECK("k_embed_species_join");
+            });
+            return;
+        }
         if (few_atoms(tokens, num_types, channels)) {
             const int lanes = lanes_of(channels), waves = num_types > kFewRows ? 1 : tokens <= kFew ? kFew / 64 : kFewWide / 64;
             const unsigned rows = waves > 1 ? static_cast<unsigned>(num_types) : blocks_for(num_types, 4);
@@ -712,7 +848,7 @@ int32_t smx_embed_gradient(const void* types, int32_t types_are_64bit, int64_t t
             using T = decltype(t);
             auto* const parts = reinterpret_cast<float*>(base + w.parts);
             if (tokens > 0) {
-                k_embed_runs<T><<<dim3(static_cast<unsigned>(w.chunks), blocks_for(channels, 8 * w.lanes)), 256, 0, queue>>>(
+                (channels % 8 == 0 ? k_embed_runs<T, true> : k_embed_runs<T, false>)<<<dim3(static_cast<unsigned>(w.chunks), blocks_for(channels, 8 * w.lanes)), 256, 0, queue>>>(
                     ints(w.keys[at]), ints(w.order[at]), tokens, static_cast<const T*>(grad), grad_stride,
                     static_cast<int>(num_types), static_cast<int>(channels), scale, static_cast<T*>(out), out_stride, parts,
                     seen, w.lanes, w.length);

@@ -111,6 +111,14 @@ __device__ __forceinline__ void load_share(const Norm<T>& a, i64 r, int c, Share
     if constexpr (FULL) s.g = load_pack(a.gate + r * a.gate_stride, c, a.channels);
 }
 
+template <class T, bool FULL>
+__device__ __forceinline__ void settle_share(const Norm<T>& a, int c, Share<T, FULL>& s) {
+    settle(s.x, c, a.channels);
+    if (!a.d) return;
+    settle(s.d, c, a.channels);
+    if constexpr (FULL) settle(s.g, c, a.channels);
+}
+
 template <class T>
 __device__ __forceinline__ T row_gate_of(const Norm<T>& a, i64 r) {
     return a.gate_kind == SMX_GATE_ROW ? a.gate[r * a.gate_stride] : static_cast<T>(0.0f);
@@ -142,7 +150,7 @@ __device__ __forceinline__ float square_sum(const Eight<T>& d) {
 // a row is read once and its two sums stay between lanes; a lane keeps its channels'
 // weights for all its rows.  A group of 128 channels is 16 lanes, which is where an 8-bit block's
 // scale is found.  Bound by memory: five values of 16 bits a channel at 4.9 TB/s (32768 x 2048, 137 us) to 6.1 (60000 x 256,
-// 25 us); rows that do not start on 16 bytes lose a fifth (6791 x 999 FP32 32 us, x 1024 25).
+// 25 us); rows that end within eight channels lose a tenth (6791 x 999 FP32 24.9 us, x 1000 22.7).
 template <class T, bool FULL, int G, int N>
 __global__ void __launch_bounds__(threads_of(G)) k_residual_norm(Norm<T> a) {
     constexpr int kThreads = threads_of(G), kGroups = kThreads / G;
@@ -158,8 +166,10 @@ __global__ void __launch_bounds__(threads_of(G)) k_residual_norm(Norm<T> a) {
         Share<T, FULL> s[N];
         float sum[1] = {0.0f};
 #pragma unroll
+        for (int n = 0; n < N; ++n) load_share(a, r, 8 * (lane + G * n), s[n]);
+#pragma unroll
         for (int n = 0; n < N; ++n) {
-            load_share(a, r, 8 * (lane + G * n), s[n]);
+            settle_share(a, 8 * (lane + G * n), s[n]);
             if (a.d) sum[0] += square_sum(s[n].d);
         }
         float r1 = 0.0f, row_gate = 1.0f;
@@ -220,7 +230,7 @@ constexpr int kSums = 2;
 // with f = a post s and dx = G + r2 q - r2^2 m y, m = r2 mean(q y), those of y^2, q y and the three parts of
 //   sum t u = sum G f u + r2 sum q f u - r2^2 m sum y f u,
 // which is also a row gate's gradient over 1 - s.  The next row is read while
-// one is worked on (6791 x 999 FP32: 47.5 us, 54.9 without).  Bound by memory with two waves a SIMD:
+// one is worked on (6791 x 999 FP32: 47.5 us, 54.9 without; 45.1 since rows' ends are loaded like the rest).  Bound by memory with two waves a SIMD:
 // eight values a channel at 4.7 TB/s (32768 x 2048 bf16, 228 us; 8192 x 8192 FP32 441 us at 4.9); above 8,192 channels the
 // registers do not hold a lane's share and spill (4000 x 16384 bf16: 719 us, 1.5 TB/s).  The sums over rows stay in registers over all rows of a group, are joined in LDS for the
 // workgroup's groups, and leave as one part [kSums][channels] a workgroup.
@@ -269,6 +279,13 @@ __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, floa
             read(r, row);
         else if (r + hop < a.rows)
             read(r + hop, ahead);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int c = 8 * (lane + G * n);
+            settle_share(a, c, row.s[n]);
+            if (a.gy) settle(row.gy[n], c, a.channels);
+            if (a.gh) settle(row.gh[n], c, a.channels);
+        }
         float r1 = 0.0f;
         const float row_gate = a.gate_kind == SMX_GATE_ROW ? sigmoid(static_cast<float>(row.gate)) : 1.0f;
         if (a.d) {

@@ -65,17 +65,26 @@ __device__ __forceinline__ std::uint32_t bits_of(T v) {
         return __builtin_bit_cast(std::uint16_t, v);
 }
 
-// Eight values from column c on, zeros past the end.
+// Eight values from column c on (a multiple of eight), zeros past the end, in two steps, so that loads of several rows
+// can be on their way together: a lane whose eight pass the row's end loads the row's last eight, like the others in
+// one load without a branch of its own, and settle moves them to their places before they are used.  (With values
+// loaded one by one in a branch, each row's loads waited for those of the row before: the embedding's gradient of 300,000
+// rows of 447 FP32 took 254 us, of 448 137.)
 template <class T>
 __device__ __forceinline__ Eight<T> load_pack(const T* row, int c, int cols) {
     struct __attribute__((packed, aligned(sizeof(T)))) Words {
         std::uint32_t w[Eight<T>::kWords];
     };
     Eight<T> e;
-    if (c + 8 <= cols) {
-        const Words p = *reinterpret_cast<const Words*>(row + c);
+    if (cols >= 8) {
+        if (c < cols) {
+            const Words p = *reinterpret_cast<const Words*>(row + (c + 8 <= cols ? c : cols - 8));
 #pragma unroll
-        for (int i = 0; i < Eight<T>::kWords; ++i) e.w[i] = p.w[i];
+            for (int i = 0; i < Eight<T>::kWords; ++i) e.w[i] = p.w[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < Eight<T>::kWords; ++i) e.w[i] = 0;
+        }
         return e;
     }
     constexpr int kPer = 4 / sizeof(T);
@@ -87,9 +96,38 @@ __device__ __forceinline__ Eight<T> load_pack(const T* row, int c, int cols) {
     return e;
 }
 
+template <class T, int N>
+__device__ __forceinline__ void settle(Eight<T> (&e)[N], int c, int cols) {
+    if (cols < 8 || c >= cols || c + 8 <= cols) return;
+    constexpr int kWords = Eight<T>::kWords, kPer = 4 / sizeof(T);
+    const int by = -cols & 7;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        std::uint32_t(&w)[kWords] = e[n].w;
+        if (by & 4)
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) w[i] = i + 4 / kPer < kWords ? w[(i + 4 / kPer) % kWords] : 0u;
+        if (by & 2)
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) w[i] = i + 2 / kPer < kWords ? w[(i + 2 / kPer) % kWords] : 0u;
+        if (by & 1)
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                const std::uint32_t next = i + 1 < kWords ? w[(i + 1) % kWords] : 0u;
+                w[i] = kPer == 1 ? next : w[i] >> 16 | next << 16;
+            }
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void settle(Eight<T>& e, int c, int cols) {
+    settle(reinterpret_cast<Eight<T>(&)[1]>(e), c, cols);
+}
+
 template <class T>
 __device__ __forceinline__ void load_eight(const T* row, int c, int cols, float (&v)[8]) {
-    const Eight<T> p = load_pack(row, c, cols);
+    Eight<T> p = load_pack(row, c, cols);
+    settle(p, c, cols);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = p[i];
 }

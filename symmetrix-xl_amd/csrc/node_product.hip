@@ -67,14 +67,22 @@ __global__ void __launch_bounds__(256) k_quantize_tile(const T* __restrict__ x, 
     const i64 blocks_c = (cols + kBlock - 1) / kBlock;
     const i64 tr = blockIdx.x / blocks_c, tc = blockIdx.x % blocks_c;
     const i64 r0 = tr * kBlock + 8 * ty, c0 = tc * kBlock + 8 * tx;
+    Eight<T> in[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (r0 + i < rows) {
+            in[i] = load_pack(x + (r0 + i) * x_stride, static_cast<int>(c0), static_cast<int>(cols));
+        } else {
+#pragma unroll
+            for (int j = 0; j < Eight<T>::kWords; ++j) in[i].w[j] = 0;
+        }
+    }
     float v[8][8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        if (r0 + i < rows)
-            load_eight(x + (r0 + i) * x_stride, static_cast<int>(c0), static_cast<int>(cols), v[i]);
-        else
+        settle(in[i], static_cast<int>(c0), static_cast<int>(cols));
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+        for (int j = 0; j < 8; ++j) v[i][j] = in[i][j];
     }
     if constexpr (ROWS) {
         const int k = static_cast<int>(tc);
@@ -521,6 +529,8 @@ __global__ void __launch_bounds__(64 * KS) k_product_rows(Product<O> p, const T*
 #pragma unroll
         for (int q = 0; q < kAhead; ++q) {
             if constexpr (RAW) {
+                const int kb = kb0 + q * KS < p.blocks ? kb0 + q * KS : kb0;
+                settle(v[q], kb * kBlock + 8 * row, k);
                 float f[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) f[i] = v[q][i];

@@ -57,7 +57,9 @@ EMBED = [(0, 5, 8, "any"), (1, 1, 1, "any"), (1, 89, 128, "any"), (63, 2, 3, "an
          (5000, 89, 128, "outside"), (5001, 2, 96, "any"), (4097, 70001, 40, "outside"), (40000, 300, 24, "any"),
          (9000, 66000, 16, "any"), (30, 40, 2050, "any"), (256, 5, 600, "any"), (257, 5, 600, "any"),
          (255, 20000, 96, "outside"), (200, 2, 20, "any"), (1024, 1024, 70, "outside"), (1025, 3, 40, "any"),
-         (900, 1025, 48, "outside")]
+         (900, 1025, 48, "outside"), (257, 1, 700, "any"), (600, 1, 1, "any"), (700, 4, 2041, "outside"),
+         (2000, 3, 9, "outside"), (3001, 4, 2048, "any"), (2500, 2, 511, "outside"), (20011, 1, 130, "any"),
+         (30000, 4, 65, "outside"), (90001, 3, 31, "any"), (1500, 4, 2049, "any"), (700, 4, 300, "none")]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
