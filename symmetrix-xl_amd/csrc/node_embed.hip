@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(WAVES > 1 ? 64 * WAVES : 256) k_embed_gradient
 // rows' types are scalars (300,000 of 3 x 448 bf16: 77 us, 86 without).  The groups are joined in LDS, the workgroups' parts
 // [blocks][num_types][channels] by k_embed_species_join, both in order.  One reading and two launches: 300,000 atoms of 3
 // species x 448 FP32 in 106 us (5.1 TB/s; sorted 150), three waves a SIMD with eight rows under way each; 30,000 of 2 x
-// 256 in 13.0 (23.5 sorted), where a round of rows is all there is.
+// 256 in 12.1 (23.9 sorted), where a round of rows is all there is.
 template <class T, class I, int V, bool WAVE>
 __global__ void __launch_bounds__(256, 3) k_embed_species(const I* __restrict__ types, i64 tokens, const T* __restrict__ grad,
                                                        i64 grad_stride, int num_types, int channels,
@@ -199,22 +199,13 @@ __global__ void __launch_bounds__(256, 3) k_embed_species(const I* __restrict__ 
     }
 }
 
-// 64 values of the table a workgroup, its sixteen waves every sixteenth part.
 template <class T>
 __global__ void __launch_bounds__(1024) k_embed_species_join(const float* __restrict__ parts, int count, int num_types,
                                                              int channels, float scale, T* __restrict__ out, i64 out_stride) {
-    __shared__ float room[16][64];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    const i64 size = static_cast<i64>(num_types) * channels, at = static_cast<i64>(blockIdx.x) * 64 + lane;
-    float sum = 0.0f;
-    if (at < size)
-#pragma unroll 8
-        for (int p = wave; p < count; p += 16) sum += parts[p * size + at];
-    room[wave][lane] = sum;
-    __syncthreads();
-    if (wave || at >= size) return;
-#pragma unroll
-    for (int w = 1; w < 16; ++w) sum += room[w][lane];
+    const i64 size = static_cast<i64>(num_types) * channels;
+    const i64 at = static_cast<i64>(blockIdx.x) * kJoined + threadIdx.x % kJoined;
+    const float sum = sum_of_parts(parts + at, size, count, at < size);
+    if (threadIdx.x >= kJoined || at >= size) return;
     out[at / channels * out_stride + at % channels] = static_cast<T>(scale * sum);
 }
 
@@ -789,7 +780,7 @@ int32_t smx_embed_gradient(const void* types, int32_t types_are_64bit, int64_t t
                         chunk);
                 });
                 SMX_LAUNCH_CHECK("k_embed_species");
-                k_embed_species_join<T><<<blocks_for(num_types * channels, 64), 1024, 0, queue>>>(
+                k_embed_species_join<T><<<blocks_for(num_types * channels, kJoined), 1024, 0, queue>>>(
                     parts, static_cast<int>(blocks), v, c, scale, static_cast<T*>(out), out_stride);
                 SMX_LAUNCH_CHECK("k_embed_species_join");
             });

@@ -230,7 +230,7 @@ constexpr int kSums = 2;
 // with f = a post s and dx = G + r2 q - r2^2 m y, m = r2 mean(q y), those of y^2, q y and the three parts of
 //   sum t u = sum G f u + r2 sum q f u - r2^2 m sum y f u,
 // which is also a row gate's gradient over 1 - s.  The next row is read while
-// one is worked on (6791 x 999 FP32: 47.5 us, 54.9 without; 45.1 since rows' ends are loaded like the rest).  Bound by memory with two waves a SIMD:
+// one is worked on (6791 x 999 FP32: 47.5 us, 54.9 without; 43.8 since rows' ends are loaded like the rest).  Bound by memory with two waves a SIMD:
 // eight values a channel at 4.7 TB/s (32768 x 2048 bf16, 228 us; 8192 x 8192 FP32 441 us at 4.9); above 8,192 channels the
 // registers do not hold a lane's share and spill (4000 x 16384 bf16: 719 us, 1.5 TB/s).  The sums over rows stay in registers over all rows of a group, are joined in LDS for the
 // workgroup's groups, and leave as one part [kSums][channels] a workgroup.
@@ -382,21 +382,14 @@ __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, floa
     }
 }
 
-// Adds the workgroups' parts up: 64 channels of one sum a workgroup, its sixteen
-// waves every sixteenth part.
+// Adds the workgroups' parts up.
 template <class T>
 __global__ void __launch_bounds__(1024) k_norm_gradient_join(Norm<T> a, const float* __restrict__ parts, int count) {
-    __shared__ float room[16][64];
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, c = blockIdx.x * 64 + lane, k = blockIdx.y;
+    const int c = blockIdx.x * kJoined + threadIdx.x % kJoined, k = blockIdx.y;
     if (k == 0 ? !a.d : !a.dnext) return;
-    float sum = 0.0f;
-    if (c < a.channels)
-#pragma unroll 8
-        for (int p = wave; p < count; p += 16) sum += parts[(static_cast<i64>(p) * kSums + k) * a.channels + c];
-    room[wave][lane] = sum;
-    __syncthreads();
-    if (wave || c >= a.channels) return;
-    for (int w = 1; w < 16; ++w) sum += room[w][lane];
+    const float sum = sum_of_parts(parts + static_cast<i64>(k) * a.channels + c, static_cast<i64>(kSums) * a.channels, count,
+                                   c < a.channels);
+    if (threadIdx.x >= kJoined || c >= a.channels) return;
     if (k == 1) {
         a.dnext[c] = sum;
         return;
@@ -614,7 +607,7 @@ int32_t smx_residual_norm_gradient(const SmxResidualNormGradientArgs* args, void
             });
             SMX_LAUNCH_CHECK("k_norm_gradient");
             if (sums) {
-                k_norm_gradient_join<T><<<dim3(blocks_for(a.channels, 64), kSums), 1024, 0,
+                k_norm_gradient_join<T><<<dim3(blocks_for(a.channels, kJoined), kSums), 1024, 0,
                                           static_cast<hipStream_t>(stream)>>>(n, parts, static_cast<int>(count));
                 SMX_LAUNCH_CHECK("k_norm_gradient_join");
             }
