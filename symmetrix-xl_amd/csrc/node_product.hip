@@ -11,8 +11,8 @@
 //     2^-126 count as zero there.)
 // FP32 outputs take the bf16 form, so that their sums are FP32 sums.  16-bit outputs, which are rounded
 // to 2^-9 or 2^-12 anyway, take the 8-bit form, but for short sums (up to 256), where what the adder drops is as much as FP32
-// sums may be off, (k + 8) 2^-23 of the terms' magnitudes, or more (1.3 times that at 128 terms, 0.36 at 256): 20000 x 512 x 256
-// 17.0 us in the bf16 form, 14.2 in the 8-bit one; 20000 x 1024 x 512 28.9 and 22.9.
+// sums may be off, (k + 8) 2^-23 of the terms' magnitudes, or more (1.3 times that at 128 terms, 0.36 at 256): 20000 x 1024 x
+// 256 16.4 us in the bf16 form, 13.3 in the 8-bit one; x 512 25.0 and 18.3.
 #include "node_ops.hpp"
 
 namespace smx {
