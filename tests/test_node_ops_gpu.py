@@ -127,6 +127,23 @@ def test_embed_infinities_stay_in_their_rows(gen):
     assert torch.isfinite(out).all()
 
 
+@pytest.mark.parametrize("c", [3, 41, 200, 700])
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_embed_gradient_of_few_species(gen, dtype, c):
+    """Views of any alignment, and infinities that stay with their type and out of the masked rows."""
+    z = _types(gen, 3000, 3, "outside", torch.int64)
+    z[1], z[2] = 1, -1
+    grad = _normal(gen, 3000, c, dtype=dtype)
+    want = ops.embed_gradient(z, grad, 3)
+    for offset, more in ((0, 8), (1, 0), (3, 5)):
+        assert torch.equal(ops.embed_gradient(z, _view(grad, offset, more), 3), want)
+    grad[1, c - 1], grad[2, 0] = math.inf, math.nan
+    out = ops.embed_gradient(z, grad, 3)
+    assert out[1, c - 1] == math.inf
+    out[1, c - 1] = want[1, c - 1]
+    assert torch.equal(out, want)
+
+
 # ---- residual norm ----
 
 
@@ -477,6 +494,7 @@ def _calls(gen):
         y, xt = ops.block_linear(x, w, keep=True)
         return (y,) + ops.block_linear_gradient(gw, wt, xt)
     return [lambda: (ops.embed(z, table, 2.0),), lambda: (ops.embed_gradient(z, grad, 300, 2.0),),
+            lambda: (ops.embed_gradient(z, grad, 4, 2.0),),
             lambda: ops.residual_norm(x, dd, post, g, scale, nxt),
             lambda: ops.residual_norm_gradient(x, dd, post, g, scale, nxt, gy, gh), train,
             lambda: (ops.block_linear(x[:3], w),),
