@@ -11,6 +11,8 @@
 
 #include "node_ops.hpp"
 
+#include "group_sum.hpp"
+
 namespace smx {
 namespace node {
 namespace {
@@ -42,35 +44,6 @@ __device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf
 // Threads of a workgroup with G lanes a row: several rows' lanes up to a wave each, one row's above
 // (whose sums wait at barriers, so no other row may share the workgroup).
 constexpr int threads_of(int g) { return g > 64 ? g : 256; }
-
-// The sums of K values over G lanes, in all of them; G a power of two from 16 on, lanes side by
-// side, above a wave the whole workgroup (one barrier: consecutive calls take
-// the two halves of `room` in turn).
-template <int G, int K>
-struct GroupSum {
-    static constexpr int kWaves = G > 64 ? G / 64 : 1;
-    struct Room {
-        float v[2][K][kWaves];
-    };
-    __device__ __forceinline__ static void sum(float (&v)[K], Room& room, int& turn) {
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            v[k] = row_total(v[k]);
-            if constexpr (G >= 32) v[k] += __shfl_xor(v[k], 16);
-            if constexpr (G >= 64) v[k] += __shfl_xor(v[k], 32);
-        }
-        if constexpr (G > 64) {
-            turn ^= 1;
-            if (threadIdx.x % 64 == 0)
-#pragma unroll
-                for (int k = 0; k < K; ++k) room.v[turn][k][threadIdx.x / 64] = v[k];
-            __syncthreads();
-            const int w = threadIdx.x % 16;
-#pragma unroll
-            for (int k = 0; k < K; ++k) v[k] = row_total(w < kWaves ? room.v[turn][k][w] : 0.0f);
-        }
-    }
-};
 
 // What a lane keeps of the channels it holds, for all its rows: scale * post (times the gate, where
 // it is the channel's) and next.
@@ -238,7 +211,7 @@ template <class T, bool FULL, int G, int N>
 __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, float* __restrict__ parts) {
     constexpr int kThreads = threads_of(G), kGroups = kThreads / G;
     __shared__ union {
-        typename GroupSum<G, 5>::Room room;
+        typename GradientSums<G>::Room room;
         float join[kGroups > 1 ? kGroups : 1][kGroups > 1 ? G * 8 * N : 1];
     } lds;
     struct Row {
@@ -270,7 +243,7 @@ __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, floa
     // (a workgroup of 16 waves has half the registers a lane: other waves' work covers its reading)
     constexpr bool kAhead = threads_of(G) <= 512;
     const i64 hop = static_cast<i64>(gridDim.x) * kGroups;
-    int turn = 0;
+    GradientSums<G> sums{lds.room};
     i64 r = static_cast<i64>(blockIdx.x) * kGroups + threadIdx.x / G;
     Row row, ahead;
     if (kAhead && r < a.rows) read(r, row);
@@ -292,7 +265,7 @@ __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, floa
             float sum[1] = {0.0f};
 #pragma unroll
             for (int n = 0; n < N; ++n) sum[0] += square_sum(row.s[n].d);
-            GroupSum<G, 1>::sum(sum, *reinterpret_cast<typename GroupSum<G, 1>::Room*>(&lds.room), turn);
+            sums.sum(sum);
             r1 = rsqrtf(sum[0] * inv + a.eps);
         }
         float y[N][8], sum[5] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
@@ -316,7 +289,7 @@ __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, floa
                 sum[1] += q * y[n][i];
             }
         }
-        GroupSum<G, 5>::sum(sum, lds.room, turn);
+        sums.sum(sum);
         const float r2 = a.gh ? rsqrtf(sum[0] * inv + a.eps) : 0.0f;
         if constexpr (!kAhead) {
             // work gate and step out again below: sixteen registers less over the sums' barrier
