@@ -49,18 +49,23 @@ _one_runtime()
 
 class BlockValues:
     """A matrix in 8-bit blocks along its rows: E4M3 ``values`` [rows][columns rounded up to
-    128] and E8M0 ``scales`` (a byte for each block, four-aligned)."""
+    128] and E8M0 ``scales`` (a byte for each block, four-aligned).  Either may be given as uint8;
+    ``values`` is float8_e4m3fn and ``scales`` uint8 however they were."""
 
     __slots__ = ("shape", "_room", "_at")
 
     def __init__(self, values, scales, shape):
         rows, cols = shape
         pitch, scale_pitch = _pitches(cols)
-        for t, name, width in ((values, "values", pitch), (scales, "scales", scale_pitch)):
-            if t.element_size() != 1 or tuple(t.shape) != (rows, width) or not t.is_contiguous() or t.data_ptr() % 16:
-                raise ValueError("%s must be contiguous bytes [%d][%d], 16-byte aligned" % (name, rows, width))
+        for t, name, width, kind in ((values, "values", pitch, torch.float8_e4m3fn),
+                                     (scales, "scales", scale_pitch, torch.float8_e8m0fnu)):
+            if t.dtype not in (torch.uint8, kind) or tuple(t.shape) != (rows, width) or not t.is_contiguous() \
+                    or t.data_ptr() % 16:
+                raise ValueError("%s must be contiguous bytes (uint8 or %s) [%d][%d], 16-byte aligned"
+                                 % (name, str(kind).replace("torch.", ""), rows, width))
         if values.device != scales.device:
             raise ValueError("values and scales must be on one device")
+        values, scales = values.view(torch.float8_e4m3fn), scales.view(torch.uint8)
         self.shape, self._room = (rows, cols), (values, scales)
         self._at = values.data_ptr(), scales.data_ptr()
 
