@@ -50,9 +50,10 @@ _one_runtime()
 class BlockValues:
     """A matrix in 8-bit blocks along its rows: E4M3 ``values`` [rows][columns rounded up to
     128] and E8M0 ``scales`` (a byte for each block, four-aligned).  Either may be given as uint8;
-    ``values`` is float8_e4m3fn and ``scales`` uint8 however they were."""
+    ``values`` is float8_e4m3fn and ``scales`` uint8 however they were.  Copies (``copy``, ``pickle``,
+    ``torch.save`` and ``torch.load``) are made of these tensors and checked like new ones."""
 
-    __slots__ = ("shape", "_room", "_at")
+    __slots__ = ("shape", "_room")
 
     def __init__(self, values, scales, shape):
         rows, cols = shape
@@ -67,7 +68,6 @@ class BlockValues:
             raise ValueError("values and scales must be on one device")
         values, scales = values.view(torch.float8_e4m3fn), scales.view(torch.uint8)
         self.shape, self._room = (rows, cols), (values, scales)
-        self._at = values.data_ptr(), scales.data_ptr()
 
     @classmethod
     def _empty(cls, rows, cols, like):
@@ -76,9 +76,19 @@ class BlockValues:
         pitch, scale_pitch = _pitches(cols)
         room = torch.empty(rows * (pitch + scale_pitch), dtype=torch.uint8, device=like.device)
         self.shape, self._room = (rows, cols), room
-        at = room.data_ptr()
-        self._at = at, at + rows * pitch
         return self
+
+    @property
+    def _at(self):
+        """The addresses of values and scales, of the tensors as they are at each call."""
+        if isinstance(self._room, tuple):
+            return self._room[0].data_ptr(), self._room[1].data_ptr()
+        at = self._room.data_ptr()
+        return at, at + self.shape[0] * _pitches(self.shape[1])[0]
+
+    def __reduce__(self):
+        # (as uint8, which every way of saving a tensor takes)
+        return BlockValues, (self.values.view(torch.uint8), self.scales, self.shape)
 
     def _split(self):
         if not isinstance(self._room, tuple):
@@ -112,6 +122,9 @@ def _pitches(cols):
     blocks = -(-cols // _BLOCK)
     return blocks * _BLOCK, -(-blocks // 4) * 4
 
+
+# so that torch.load, which by default makes only what it knows to be safe, makes them too
+torch.serialization.add_safe_globals([BlockValues])
 
 # the current stream's handle without the Stream object around it, which costs more than some of the calls here
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \

@@ -1,4 +1,8 @@
-"""CPU tests of BlockValues (symmetrix.node_ops): what its bytes stand for however they are given."""
+"""CPU tests of BlockValues (symmetrix.node_ops): what its bytes stand for however they are given, and copies."""
+
+import copy
+import io
+import pickle
 
 import pytest
 import torch
@@ -36,3 +40,45 @@ def test_other_bytes_are_refused(kind):
         node_ops.BlockValues(values.view(kind), scales, want.shape)
     with pytest.raises(ValueError, match="scales must be contiguous bytes"):
         node_ops.BlockValues(values, scales.view(kind), want.shape)
+
+
+def _saved(b):
+    f = io.BytesIO()
+    torch.save({"weights": [b]}, f)
+    f.seek(0)
+    return torch.load(f)["weights"][0]
+
+
+COPIES = {"copy": copy.copy, "deepcopy": copy.deepcopy, "pickle": lambda b: pickle.loads(pickle.dumps(b)), "save": _saved}
+
+
+@pytest.mark.parametrize("way", list(COPIES))
+@pytest.mark.parametrize("together", [False, True])
+def test_copies_have_their_own_addresses(way, together):
+    values, scales, want = _bytes()
+    if together:  # as the operators make them: one allocation
+        b = node_ops.BlockValues._empty(*want.shape, want)
+        b.values.copy_(values.view(E4M3))
+        b.scales.copy_(scales)
+    else:
+        b = node_ops.BlockValues(values, scales, want.shape)
+    c = COPIES[way](b)
+    assert type(c) is node_ops.BlockValues and c.shape == b.shape
+    assert c._at == (c.values.data_ptr(), c.scales.data_ptr())
+    assert torch.equal(c.float(), want)
+    if way == "copy":  # shares the tensors, as torch's own do
+        assert c._at == b._at
+        return
+    room = [range(t.data_ptr(), t.data_ptr() + t.numel()) for t in (b.values, b.scales)]
+    assert not any(at in r for at in c._at for r in room)
+    b.values.view(torch.uint8).zero_()
+    assert torch.equal(c.float(), want)
+
+
+def test_addresses_are_those_of_the_call():
+    """Memory that was put in another place under the same tensor is read where it is."""
+    values, scales, want = _bytes()
+    b = node_ops.BlockValues(values, scales, want.shape)
+    other = b.values.clone()
+    b.values.set_(other)
+    assert b._at[0] == other.data_ptr()
