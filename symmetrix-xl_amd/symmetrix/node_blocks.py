@@ -5,6 +5,7 @@ and a linear of the descriptors start each atom's row, residual blocks update it
 product that gives the update and its gate side by side, and the gated residual with the
 next norm), and a vector reads the energy out.  It trains like any torch module; ``serve()`` keeps
 the weights in 8-bit blocks and runs a block in two launches, the norm handing its 8-bit rows to the product.
+First derivatives only: a gradient formed with ``create_graph`` raises ``RuntimeError`` when it is differentiated.
 
     python -m symmetrix.node_blocks --steps 300
 
@@ -15,12 +16,38 @@ weights of the tiny shape) and reports the error on a cell that it has not seen,
 from __future__ import annotations
 
 import argparse
+import functools
 import math
 import time
 
 import torch
 
 from . import node_ops as ops
+
+
+class _Undifferentiated(torch.autograd.Function):
+    """Gradients as they are, whose own derivatives are an error instead of missing."""
+
+    @staticmethod
+    def forward(ctx, anchor, *grads):
+        return tuple(g if g is None else g.view_as(g) for g in grads)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("symmetrix.node_blocks has first derivatives only: its gradients cannot be differentiated")
+
+
+def _once(backward):
+    """For a backward that records nothing: what it returns under ``create_graph`` raises when it is differentiated,
+    whether or not the gradients that came in ask for a graph (the result depends on saved inputs as well)."""
+    @functools.wraps(backward)
+    def wrapped(ctx, *grads):
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return out
+        return _Undifferentiated.apply(torch.zeros((), requires_grad=True), *out)
+    return wrapped
 
 
 class _Embed(torch.autograd.Function):
@@ -31,6 +58,7 @@ class _Embed(torch.autograd.Function):
         return ops.embed(types, table, scale)
 
     @staticmethod
+    @_once
     def backward(ctx, grad):
         types, = ctx.saved_tensors
         return ops.embed_gradient(types, grad.contiguous(), ctx.num_types, ctx.scale), None, None
@@ -44,6 +72,7 @@ class _Norm(torch.autograd.Function):
         return ops.norm(x, weight, eps)
 
     @staticmethod
+    @_once
     def backward(ctx, grad):
         x, weight = ctx.saved_tensors
         dx, *_, dw = ops.residual_norm_gradient(x, None, None, None, None, weight, None, grad.contiguous(), ctx.eps)
@@ -61,6 +90,7 @@ class _GatedResidual(torch.autograd.Function):
         return ops.residual_norm(x, both[:, :c], post, both[:, c:], scale, next_weight, eps)
 
     @staticmethod
+    @_once
     def backward(ctx, grad_y, grad_h):
         x, both, post, scale, next_weight = ctx.saved_tensors
         c = x.shape[1]
@@ -81,6 +111,7 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
+    @_once
     def backward(ctx, grad):
         need_x, need_w = ctx.needs_input_grad
         dx, dw = ops.block_linear_gradient(grad.contiguous(), ctx.w_columns if need_x else None,
