@@ -119,9 +119,21 @@ class _Linear(torch.autograd.Function):
         return dx, dw
 
 
+def _masked(types, descriptors, num_types):
+    """(which atoms have a type of the table, the descriptors with zeros for the others): a masked atom's row is
+    then zero all through, and shares no scale of 8-bit blocks with its neighbours."""
+    there = (types >= 0) & (types < num_types)
+    return there, torch.where(there[:, None], descriptors, 0)
+
+
+def _energies(h, readout, shift, types, there):
+    return torch.where(there, h.float() @ readout + shift[torch.where(there, types, 0).long()], 0)
+
+
 class NodeBlocks(torch.nn.Module):
     """Per-atom energies of ``types`` [atoms] and ``descriptors`` [atoms][descriptors].  Rows are
-    ``dtype``; parameters are float32."""
+    ``dtype``; parameters are float32.  An atom whose type is outside [0, num_types) is masked, as in
+    ``node_ops.embed``: its energy is zero, its descriptors are not looked at and nothing is learned from it."""
 
     def __init__(self, num_types, num_descriptors, channels=128, blocks=2, dtype=torch.float32, eps=1e-6):
         super().__init__()
@@ -143,17 +155,15 @@ class NodeBlocks(torch.nn.Module):
         self.readout = normal(channels, scale=0.1 / math.sqrt(channels))
         self.shift = torch.nn.Parameter(torch.zeros(num_types))
 
-    def _energies(self, h, types):
-        return h.float() @ self.readout + self.shift[types.long()]
-
     def forward(self, types, descriptors):
         t = self.dtype
+        there, descriptors = _masked(types, descriptors, self.table.shape[0])
         x = _Embed.apply(self.table.to(t), types, math.sqrt(self.channels))
         x = x + _Linear.apply(descriptors.to(t), self.lift.to(t))
         h = _Norm.apply(x, self.before, self.eps)
         for w, post, scale, nxt in zip(self.weights, self.post, self.scale, self.next):
             x, h = _GatedResidual.apply(x, _Linear.apply(h, w.to(t)), post, scale, nxt, self.eps)
-        return self._energies(h, types)
+        return _energies(h, self.readout, self.shift, types, there)
 
     def serve(self):
         """A function of (types, descriptors) with the present weights in 8-bit blocks."""
@@ -167,6 +177,7 @@ class NodeBlocks(torch.nn.Module):
 
         @torch.no_grad()
         def energies(types, descriptors):
+            there, descriptors = _masked(types, descriptors, table.shape[0])
             x = ops.embed(types, table, math.sqrt(c))
             x += ops.block_linear(descriptors.to(t), lift)
             h = ops.norm(x, before, eps, quantized=True)
@@ -174,7 +185,7 @@ class NodeBlocks(torch.nn.Module):
                 both = ops.block_product(h, w, t)
                 x, h = ops.residual_norm(x, both[:, :c], post, both[:, c:], scale, nxt, eps,
                                          quantized=k + 1 < len(weights))
-            return (h.float() @ readout if weights else ops.norm(x, before, eps).float() @ readout) + shift[types.long()]
+            return _energies(h if weights else ops.norm(x, before, eps), readout, shift, types, there)
         return energies
 
 

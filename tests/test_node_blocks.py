@@ -71,3 +71,49 @@ def test_slopes_alone_are_formed():
         change = (model(types, desc + h * way) - model(types, desc - h * way)).sum() / (2 * h)
     # O(h^2) of the third derivative, and FP32 roundings of 30 energies of size 1 (2^-20) over 2h
     assert abs(change - (slope * way).sum()) < 5e-3 * (1 + abs(change))
+
+
+# ---- masked atoms ----
+
+
+def _with_masked(n=30):
+    """Atoms with masked ones among them, whose descriptors are anything; which ones are real."""
+    types, desc = _inputs(n)
+    types[3], types[10], types[11], types[29] = -1, 5, 1 << 40, -(1 << 40)
+    there = (types >= 0) & (types < 5)
+    desc[3], desc[10, 2], desc[11] = float("nan"), float("inf"), 1e30
+    return types, desc, there
+
+
+def test_masked_atoms_have_no_energy_and_teach_nothing():
+    model = _head()
+    torch.nn.init.normal_(model.shift)
+    types, desc, there = _with_masked()
+    desc.requires_grad_()
+    w = torch.randn(30)
+    e = model(types, desc)
+    assert (e[~there] == 0).all()
+    (e * w).sum().backward()
+    got = {k: v.grad.clone() for k, v in model.named_parameters()}
+    slopes = desc.grad.clone()
+    assert (slopes[~there] == 0).all()
+    model.zero_grad()
+    desc2 = desc.detach()[there].requires_grad_()
+    e2 = model(types[there], desc2)
+    (e2 * w[there]).sum().backward()
+    # the same sums over the atoms with zeros among them: FP32 roundings
+    torch.testing.assert_close(e[there], e2, rtol=1e-5, atol=1e-6)
+    torch.testing.assert_close(slopes[there], desc2.grad, rtol=1e-5, atol=1e-6)
+    for k, v in model.named_parameters():
+        torch.testing.assert_close(got[k], v.grad, rtol=1e-5, atol=1e-5, msg=k)
+
+
+@pytest.mark.parametrize("blocks", [0, 2])
+def test_masked_atoms_served(blocks):
+    model = node_blocks.NodeBlocks(5, 12, 16, blocks)
+    torch.nn.init.normal_(model.shift)
+    types, desc, there = _with_masked()
+    e = model.serve()(types, desc)
+    assert (e[~there] == 0).all()
+    torch.testing.assert_close(e[there], model.serve()(types[there], desc[there]), rtol=1e-5, atol=1e-6)
+    torch.testing.assert_close(e, model(types, desc), rtol=1e-5, atol=1e-6)
