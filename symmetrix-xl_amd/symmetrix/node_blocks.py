@@ -51,6 +51,8 @@ def _once(backward):
 
 
 class _Embed(torch.autograd.Function):
+    """Rows in the table's type, and the table's gradient summed in FP32 and rounded to it once."""
+
     @staticmethod
     def forward(ctx, table, types, scale):
         ctx.save_for_backward(types)
@@ -100,12 +102,12 @@ class _GatedResidual(torch.autograd.Function):
 
 
 class _Linear(torch.autograd.Function):
-    """x @ weight.T in 8-bit blocks, its gradients likewise; the weights are brought to blocks along both
-    axes in one reading of them."""
+    """x @ weight.T in 8-bit blocks, its gradients likewise; the weights are brought to x's type and then to blocks along
+    both axes in one reading of them.  The weights' gradient is in their own type, whatever the rows' is."""
 
     @staticmethod
     def forward(ctx, x, weight):
-        rows, ctx.w_columns = ops.quantize(weight, columns=True)
+        rows, ctx.w_columns = ops.quantize(weight.to(x.dtype), columns=True)
         y, ctx.x_columns = ops.block_linear(x, rows, keep=True)
         ctx.weight_dtype = weight.dtype
         return y
@@ -159,10 +161,10 @@ class NodeBlocks(torch.nn.Module):
         t = self.dtype
         there, descriptors = _masked(types, descriptors, self.table.shape[0])
         x = _Embed.apply(self.table.to(t), types, math.sqrt(self.channels))
-        x = x + _Linear.apply(descriptors.to(t), self.lift.to(t))
+        x = x + _Linear.apply(descriptors.to(t), self.lift)
         h = _Norm.apply(x, self.before, self.eps)
         for w, post, scale, nxt in zip(self.weights, self.post, self.scale, self.next):
-            x, h = _GatedResidual.apply(x, _Linear.apply(h, w.to(t)), post, scale, nxt, self.eps)
+            x, h = _GatedResidual.apply(x, _Linear.apply(h, w), post, scale, nxt, self.eps)
         return _energies(h, self.readout, self.shift, types, there)
 
     def serve(self):

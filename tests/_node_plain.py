@@ -20,12 +20,13 @@ def _unit(x, eps):
 
 
 def norm(x, weight, eps=1e-6, quantized=False):
-    return weight * _unit(x, eps)
+    return (weight * _unit(x.float(), eps)).to(x.dtype)
 
 
 def residual_norm(x, d, post, gate=None, scale=None, next_weight=None, eps=1e-6, quantized=False):
-    y = x + (1 if scale is None else scale) * (1 if gate is None else torch.sigmoid(gate)) * post * _unit(d, eps)
-    return y, None if next_weight is None else next_weight * _unit(y, eps)
+    gate = 1 if gate is None else torch.sigmoid(gate.float())
+    y = x.float() + (1 if scale is None else scale) * gate * post * _unit(d.float(), eps)
+    return y.to(x.dtype), None if next_weight is None else norm(y, next_weight, eps).to(x.dtype)
 
 
 def residual_norm_gradient(x, d, post, gate, scale, next_weight, grad_y, grad_h, eps=1e-6):
@@ -45,7 +46,7 @@ def quantize(x, rows=True, columns=False):
 
 
 def block_product(a, b, dtype=torch.float32):
-    return (a @ b.T).to(dtype)
+    return (a.float() @ b.float().T).to(dtype)
 
 
 def block_linear(x, w, dtype=None, keep=False):

@@ -117,3 +117,16 @@ def test_masked_atoms_served(blocks):
     assert (e[~there] == 0).all()
     torch.testing.assert_close(e[there], model.serve()(types[there], desc[there]), rtol=1e-5, atol=1e-6)
     torch.testing.assert_close(e, model(types, desc), rtol=1e-5, atol=1e-6)
+
+
+# ---- types ----
+
+
+def test_weights_of_a_16_bit_head_get_gradients_of_their_own_type():
+    model = _head(dtype=torch.bfloat16)
+    types, desc = _inputs()
+    model(types, desc).square().sum().backward()
+    for w in (model.lift, *model.weights):
+        # of FP32 sums, of which bf16 holds one in 2^16
+        assert w.grad.dtype is torch.float32
+        assert (w.grad.bfloat16().float() == w.grad).float().mean() < 0.1
