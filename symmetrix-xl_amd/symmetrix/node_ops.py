@@ -12,7 +12,8 @@ Row tensors are float32, bfloat16 or float16 on the current HIP device, two-dime
 unit stride along the channels and any row stride.  Calls enqueue on torch's
 current stream and return without waiting; a tensor made on another stream
 is the caller's to order, as with torch's own operations.  Refused arguments raise
-``ValueError`` before anything is launched.  The functions take and return plain values and record
+``ValueError`` before anything is launched, and sizes that an operator has no kernel for
+``SymmetrixUnsupportedError`` before it launches.  The functions take and return plain values and record
 nothing for autograd (``symmetrix.node_blocks`` wraps them).
 
 torch brings a HIP runtime of its own, which this library shares when torch is
@@ -212,9 +213,11 @@ def embed_gradient(types, grad, num_types, scale=1.0):
     """The table's gradient [num_types][channels]: for each type, ``scale`` times the sum of
     its atoms' rows of ``grad``, in a fixed order."""
     code, t, c, stride = _rows(grad, "grad")
+    wide = _types(types, grad)
     if types.shape[0] != t:
         raise ValueError("grad has the wrong shape")
-    wide = _types(types, grad)
+    if num_types < 0:
+        raise ValueError("num_types must not be negative")
     stream = _stream(grad.get_device())
     out = grad.new_empty((num_types, c))
     size = lib.smx_embed_gradient_workspace(t, num_types, c)
@@ -401,10 +404,10 @@ def block_linear(x, w, dtype=None, keep=False):
     code, m, k, stride = _rows(x, "x")
     device = x.get_device()
     _check_blocks(w, "w", k, device)
+    out_code = code if dtype is None else _product_dtype(dtype)
     if keep:
         rows, columns = quantize(x, columns=True)
         return block_product(rows, w, x.dtype if dtype is None else dtype), columns
-    out_code = code if dtype is None else _product_dtype(dtype)
     current = _stream(device)
     n = w.shape[0]
     out = x.new_empty((m, n)) if dtype is None else x.new_empty((m, n), dtype=dtype)
@@ -421,12 +424,18 @@ def block_linear_gradient(grad, w_columns, x_columns, dtype=None):
 
     ``w_columns``: the weights' column blocks (``quantize(w, columns=True)[1]``), ``x_columns``
     those that ``block_linear(..., keep=True)`` gave; None leaves that gradient out."""
+    _, m, n, _ = _rows(grad, "grad")
+    for blocks, name, k in ((w_columns, "w_columns", n), (x_columns, "x_columns", m)):
+        if blocks is not None:
+            _check_blocks(blocks, name, k, grad.get_device())
+    dw_dtype = torch.float32 if dtype is None else dtype
+    _product_dtype(dw_dtype)
     if w_columns is None and x_columns is None:
         return None, None
     both = quantize(grad, rows=w_columns is not None, columns=x_columns is not None)
     rows, columns = both if isinstance(both, tuple) else (both, both)
     dx = None if w_columns is None else block_product(rows, w_columns, grad.dtype)
-    dw = None if x_columns is None else block_product(columns, x_columns, dtype or torch.float32)
+    dw = None if x_columns is None else block_product(columns, x_columns, dw_dtype)
     return dx, dw
 
 
