@@ -302,7 +302,9 @@ __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, floa
                     asm volatile("" : "+v"(row.gh[n].w[i]));
                 }
         }
-        const float ry = r2 * r2 * (r2 * (sum[1] * inv)), tu = sum[2] + r2 * sum[3] - ry * sum[4], m1 = tu * inv;
+        // (without h's gradient, sums that take y are not looked at: they may be infinite)
+        const float ry = a.gh ? r2 * r2 * (r2 * (sum[1] * inv)) : 0.0f;
+        const float tu = a.gh ? sum[2] + r2 * sum[3] - ry * sum[4] : sum[2], m1 = tu * inv;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int c = 8 * (lane + G * n);
