@@ -70,7 +70,9 @@ enum { SMX_GATE_NONE = 0, SMX_GATE_FULL = 1, SMX_GATE_CHANNEL = 2, SMX_GATE_ROW 
  * scale are not read.  scale NULL: ones.  y NULL: not written.  next NULL: no h.
  * y may be x.  With h_scales, h is written as 8-bit blocks (below) instead of
  * `dtype`: h the values [rows][smx_block_stride(channels)] and h_scales
- * [rows][smx_block_scale_stride(channels)].  channels <= 16384. */
+ * [rows][smx_block_scale_stride(channels)].  channels <= 16384.  The sigmoid, and one minus it in the gradients, come
+ * from the hardware exponential of a logit's magnitude: within 2^-20 of themselves in FP32 rows, whatever the
+ * logit (below FP32's normal numbers, from magnitudes of 87 on, zero), and |logit| 2^-24 more in 16-bit rows. */
 typedef struct SmxResidualNormArgs {
     uint32_t struct_size;
     int32_t dtype;

@@ -38,8 +38,29 @@ struct Norm {
     float *dpost, *dscale, *dnext;
 };
 
-// 1 / (1 + e^-g) on the hardware exponential and reciprocal, about 2^-22 of it
-__device__ __forceinline__ float sigmoid(float g) { return __builtin_amdgcn_rcpf(1.0f + __expf(-g)); }
+// e^-a for a >= 0 (an infinity gives 0).  The hardware exponential of a log2(e), whose rounding alone is a 2^-24 of the
+// result: 16-bit rows take it as it is (at a logit of 80, 2^-18).  For FP32 rows what the rounding left out, and what log2(e)
+// has beyond FP32, is added to first order: 2^-22 for every a.
+template <class T>
+__device__ __forceinline__ float exp_minus(float a) {
+    const float hi = a * -1.44269504f, e = __builtin_amdgcn_exp2f(hi);
+    if constexpr (sizeof(T) == 4) {
+        const float lo = __builtin_fmaf(a, -1.92596303e-8f, __builtin_fmaf(a, -1.44269504f, -hi));
+        return a < 128.0f ? __builtin_fmaf(e * 0.693147181f, lo, e) : e;
+    }
+    return e;
+}
+
+// s = 1 / (1 + e^-g), and 1 - s as a quotient of its own: as a difference it has no digit left from g = 17 on.
+struct Gate {
+    float s, rest;
+};
+
+template <class T>
+__device__ __forceinline__ Gate gate_of(float g) {
+    const float t = exp_minus<T>(__builtin_fabsf(g)), near = __builtin_amdgcn_rcpf(1.0f + t), far = t * near;
+    return g < 0.0f ? Gate{far, near} : Gate{near, far};
+}
 
 // Threads of a workgroup with G lanes a row: several rows' lanes up to a wave each, one row's above
 // (whose sums wait at barriers, so no other row may share the workgroup).
@@ -62,7 +83,7 @@ __device__ __forceinline__ void load_channels(const Norm<T>& a, int c, float (&s
         if (a.gate_kind == SMX_GATE_CHANNEL) {
             load_eight(a.gate, c, a.channels, v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) step[i] *= sigmoid(v[i]);
+            for (int i = 0; i < 8; ++i) step[i] *= gate_of<T>(v[i]).s;
         }
     }
     if (a.next) load_eight(a.next, c, a.channels, next);
@@ -97,18 +118,13 @@ __device__ __forceinline__ T row_gate_of(const Norm<T>& a, i64 r) {
     return a.gate_kind == SMX_GATE_ROW ? a.gate[r * a.gate_stride] : static_cast<T>(0.0f);
 }
 
-// scale * post * gate of eight channels; zeros past the end.
+// The gate of channel i of a lane's eight, where it is not in the channel's step.
 template <class T, bool FULL>
-__device__ __forceinline__ void steps_of(const Share<T, FULL>& s, const float (&step)[8], float row_gate, float (&gate)[8],
-                                         float (&f)[8]) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if constexpr (FULL)
-            gate[i] = sigmoid(s.g[i]);
-        else
-            gate[i] = row_gate;
-        f[i] = step[i] * gate[i];
-    }
+__device__ __forceinline__ Gate gate_at(const Share<T, FULL>& s, int i, const Gate& row_gate) {
+    if constexpr (FULL)
+        return gate_of<T>(s.g[i]);
+    else
+        return row_gate;
 }
 
 template <class T>
@@ -145,9 +161,10 @@ __global__ void __launch_bounds__(threads_of(G)) k_residual_norm(Norm<T> a) {
             settle_share(a, 8 * (lane + G * n), s[n]);
             if (a.d) sum[0] += square_sum(s[n].d);
         }
-        float r1 = 0.0f, row_gate = 1.0f;
+        float r1 = 0.0f;
+        Gate row_gate{1.0f, 0.0f};
         if (a.d) {
-            if (a.gate_kind == SMX_GATE_ROW) row_gate = sigmoid(static_cast<float>(row_gate_of(a, r)));
+            if (a.gate_kind == SMX_GATE_ROW) row_gate = gate_of<T>(static_cast<float>(row_gate_of(a, r)));
             GroupSum<G, 1>::sum(sum, room, turn);
             r1 = rsqrtf(sum[0] * inv + a.eps);
         }
@@ -159,10 +176,8 @@ __global__ void __launch_bounds__(threads_of(G)) k_residual_norm(Norm<T> a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[n][i] = s[n].x[i];
             if (a.d) {
-                float gate[8], f[8];
-                steps_of(s[n], step[n], row_gate, gate, f);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[n][i] += f[i] * (s[n].d[i] * r1);
+                for (int i = 0; i < 8; ++i) y[n][i] += step[n][i] * gate_at(s[n], i, row_gate).s * (s[n].d[i] * r1);
             }
             if (a.y) store_eight(a.y + r * a.y_stride, c, a.channels, y[n]);
 #pragma unroll
@@ -260,7 +275,7 @@ __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, floa
             if (a.gh) settle(row.gh[n], c, a.channels);
         }
         float r1 = 0.0f;
-        const float row_gate = a.gate_kind == SMX_GATE_ROW ? sigmoid(static_cast<float>(row.gate)) : 1.0f;
+        const Gate row_gate = a.gate_kind == SMX_GATE_ROW ? gate_of<T>(static_cast<float>(row.gate)) : Gate{1.0f, 0.0f};
         if (a.d) {
             float sum[1] = {0.0f};
 #pragma unroll
@@ -269,17 +284,17 @@ __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, floa
             r1 = rsqrtf(sum[0] * inv + a.eps);
         }
         float y[N][8], sum[5] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        Gate kept[N][8];  // (where a lane has the registers; else the gates are formed again in the second round)
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int c = 8 * (lane + G * n);
-            float gate[8], f[8];
-            if (a.d) steps_of(row.s[n], step[n], row_gate, gate, f);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 y[n][i] = row.s[n].x[i];
                 const float q = a.gh ? row.gh[n][i] * next[n][i] : 0.0f;
                 if (a.d) {
-                    const float fu = f[i] * (row.s[n].d[i] * r1);
+                    kept[n][i] = gate_at(row.s[n], i, row_gate);
+                    const float fu = step[n][i] * kept[n][i].s * (row.s[n].d[i] * r1);
                     y[n][i] += fu;
                     sum[2] += a.gy ? row.gy[n][i] * fu : 0.0f;
                     sum[3] += q * fu;
@@ -308,8 +323,7 @@ __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, floa
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int c = 8 * (lane + G * n);
-            float gate[8], f[8], dx[8], dd[8], dg[8];
-            if (a.d) steps_of(row.s[n], step[n], row_gate, gate, f);
+            float dx[8], dd[8], dg[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 dx[i] = a.gy ? row.gy[n][i] : 0.0f;
@@ -319,10 +333,11 @@ __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, floa
                     acc[1][n][i] += g * (y[n][i] * r2);
                 }
                 if (a.d) {
-                    const float u = row.s[n].d[i] * r1, t = dx[i] * f[i];
-                    acc[0][n][i] += dx[i] * (gate[i] * u);
+                    const Gate gate = kAhead ? kept[n][i] : gate_at(row.s[n], i, row_gate);
+                    const float u = row.s[n].d[i] * r1, t = dx[i] * (step[n][i] * gate.s);
+                    acc[0][n][i] += dx[i] * (gate.s * u);
                     dd[i] = r1 * (t - u * m1);
-                    dg[i] = t * u * (1.0f - gate[i]);
+                    dg[i] = t * u * gate.rest;
                 }
             }
             if (a.dx) store_eight(a.dx + r * a.dx_stride, c, a.channels, dx);
@@ -330,7 +345,7 @@ __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, floa
             if (FULL && a.dgate) store_eight(a.dgate + r * a.dgate_stride, c, a.channels, dg);
         }
         if (a.dgate && a.gate_kind == SMX_GATE_ROW && lane == 0)
-            a.dgate[r * a.dgate_stride] = static_cast<T>(tu * (1.0f - row_gate));
+            a.dgate[r * a.dgate_stride] = static_cast<T>(tu * row_gate.rest);
         if constexpr (kAhead) row = ahead;
     }
     if (!parts) return;
@@ -370,13 +385,13 @@ __global__ void __launch_bounds__(1024) k_norm_gradient_join(Norm<T> a, const fl
         return;
     }
     const float scale = a.scale ? a.scale[c] : 1.0f;
-    float gate = 1.0f;
+    Gate gate{1.0f, 0.0f};
     if (a.gate_kind == SMX_GATE_CHANNEL) {  // S was summed without the channel's gate
-        gate = sigmoid(static_cast<float>(a.gate[c]));
-        if (a.dgate_channel) a.dgate_channel[c] = static_cast<T>(sum * a.post[c] * scale * gate * (1.0f - gate));
+        gate = gate_of<T>(static_cast<float>(a.gate[c]));
+        if (a.dgate_channel) a.dgate_channel[c] = static_cast<T>(sum * a.post[c] * scale * gate.s * gate.rest);
     }
-    if (a.dpost) a.dpost[c] = sum * scale * gate;
-    if (a.dscale) a.dscale[c] = sum * a.post[c] * gate;
+    if (a.dpost) a.dpost[c] = sum * scale * gate.s;
+    if (a.dscale) a.dscale[c] = sum * a.post[c] * gate.s;
 }
 
 // The channel vectors' gradients of no rows.
