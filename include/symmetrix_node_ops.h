@@ -141,10 +141,15 @@ SMX_API int32_t smx_block_quantize(const void* x, int64_t x_stride, int32_t dtyp
                                    uint8_t* values, uint8_t* scales, uint8_t* values_t, uint8_t* scales_t,
                                    void* stream);
 /* out[i][j] = sum over k of a[i][k] b[j][k], a [m][k] and b [n][k] in 8-bit blocks, k < 2^23 - 127.
- * FP32 outputs are FP32 sums.  16-bit outputs of more than 256 terms come from the 8-bit matrix
- * instruction, which aligns eight products to the largest of them and drops what lies 2^-13 below it:
- * about 2^-16 of an output's norm, below the outputs' own rounding (2^-9 or 2^-12).  An infinity or
- * NaN in a row of an operand makes that row of products NaN, and no other. */
+ * FP32 outputs, and 16-bit ones of up to 256 terms, are FP32 sums of the operands' values as bf16 numbers,
+ * which hold them exactly from 2^-126 on, round them to multiples of 2^-133 below, and have infinity for the one value
+ * that is beyond FP32 (2^128, to which the largest FP32 numbers round).  16-bit outputs of more than
+ * 256 terms come from the 8-bit matrix instruction, which takes every value as it is but aligns eight products to the
+ * largest of them and drops what lies 2^-13 below it: up to 7 x 2^-13 of the largest of each eight.  In sums of many
+ * terms of one size that is about 2^-16 of an output's norm, below the outputs' own rounding (2^-9 or 2^-12); where
+ * single products stand far above the others it may be up to 2^-10 of those, which float16 is finer than and which stays
+ * when they cancel: FP32 outputs have neither.  An infinity or NaN in a row of an operand makes that row of products NaN,
+ * and no other. */
 SMX_API int64_t smx_block_product_workspace(int64_t m, int64_t n, int64_t k);
 SMX_API int32_t smx_block_product(const uint8_t* a_values, const uint8_t* a_scales, const uint8_t* b_values,
                                   const uint8_t* b_scales, int64_t m, int64_t n, int64_t k, int32_t dtype, void* out,

@@ -5,10 +5,11 @@
 //   - 8-bit: v_mfma_scale_f32_16x16x128_f8f6f4 sums one block of 128 and applies both operands'
 //     scales, powers of two, by itself.  Its adder aligns eight products to the largest of them
 //     and drops what lies below 2^-13 of that one (measured: 2^16 + 127 products of 2^2 comes out
-//     28 short, those of 2^4 exact): 2^-16 of an output's norm in rows of normal values, however long.
+//     28 short, those of 2^4 exact): 2^-16 of an output's norm in rows of normal values, however long, and at most
+//     7 x 2^-13 of the largest of each eight.
 //   - bf16: an E4M3 value times its scale is a bf16 value exactly (v_cvt_scalef32_pk_bf16_fp8), and
 //     v_mfma_f32_16x16x32_bf16 sums as FP32 does, 2^-24 to 2^-27 of the norm there, at half the rate.  (Values below
-//     2^-126 count as zero there.)
+//     2^-126 are bf16's subnormal numbers, multiples of 2^-133; the instructions keep these.)
 // FP32 outputs take the bf16 form, so that their sums are FP32 sums.  16-bit outputs, which are rounded
 // to 2^-9 or 2^-12 anyway, take the 8-bit form, but for short sums (up to 256), where what the adder drops is as much as FP32
 // sums may be off, (k + 8) 2^-23 of the terms' magnitudes, or more (1.3 times that at 128 terms, 0.36 at 256): 20000 x 1024 x
@@ -255,8 +256,9 @@ __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" :
 // tile, and the next one's first blocks arrive while this one's last are multiplied and stored.  With KG > 1, for
 // few tiles, KG groups of waves take every KG-th block each, so that their waits overlap, and their sums are joined in LDS.
 // Large products: 16384 x 8192 x 8192 in 855 us, 2,570 TFLOP/s (a library's product of 8-bit values with one scale
-// reached 2,880): the matrix pipes are 57% busy at the 1.8 GHz that the clock falls to, LDS has no bank conflicts; a tile's
-// 192 KB of fragment reads and 64 KB of arriving blocks a step are as long as its products at LDS's 128 B a clock.
+// reached 2,880): the matrix pipes are busy 57% of the cycles at the 1.8 GHz that the clock falls to, LDS instructions 23%,
+// without bank conflicts (counted).  Neither is full; what is left, by exclusion, are the waits at each step's barrier, which
+// one workgroup a unit has no other work to cover with.
 // To FP32 8192 cubed takes 767 us, 1,433 TFLOP/s (a library's bf16 product 1,406).
 template <class O, bool WIDE, int BM, int BN, int WM, int WN, int KG>
 __global__ void __launch_bounds__(64 * WM * WN * KG, (BM + BN) * kBlock * KG * 2 > 81920 ? 1 : 2)
@@ -368,13 +370,13 @@ k_product_tile(Product<O> p) {
                 i32x8 vb[NF];
 #pragma unroll
                 for (int g = 0; g < NF; ++g) vb[g] = fragment(BM + wn + 16 * g);
-            if (kb + KG < last) {
-                stage(kb + KG, slot);
-            } else if (KG == 1 && turn + static_cast<int>(gridDim.x) < tiles) {
-                turn_to(turn + gridDim.x);
-                stage_scales(first / 4, scale_slot);
-                stage(first, slot);
-            }
+                if (kb + KG < last) {
+                    stage(kb + KG, slot);
+                } else if (KG == 1 && turn + static_cast<int>(gridDim.x) < tiles) {
+                    turn_to(turn + gridDim.x);
+                    stage_scales(first / 4, scale_slot);
+                    stage(first, slot);
+                }
                 if constexpr (!WIDE) {
 #pragma unroll
                     for (int f = 0; f < MF; ++f) {
