@@ -138,8 +138,8 @@ __device__ __forceinline__ float square_sum(const Eight<T>& d) {
 // G lanes a row, each N times eight neighbouring values in registers, so that
 // a row is read once and its two sums stay between lanes; a lane keeps its channels'
 // weights for all its rows.  A group of 128 channels is 16 lanes, which is where an 8-bit block's
-// scale is found.  Bound by memory: five values of 16 bits a channel at 4.9 TB/s (32768 x 2048, 137 us) to 6.1 (60000 x 256,
-// 25 us); rows that end within eight channels lose a tenth (6791 x 999 FP32 24.9 us, x 1000 22.7).
+// scale is found.  Bound by memory: five values of 16 bits a channel at 5.0 TB/s (32768 x 2048, 133 us) to 5.9 (60000 x 256,
+// 26 us); rows that end within eight channels lose a tenth (6791 x 999 FP32 24.9 us, x 1000 22.7).
 template <class T, bool FULL, int G, int N>
 __global__ void __launch_bounds__(threads_of(G)) k_residual_norm(Norm<T> a) {
     constexpr int kThreads = threads_of(G), kGroups = kThreads / G;
@@ -218,10 +218,11 @@ constexpr int kSums = 2;
 // with f = a post s and dx = G + r2 q - r2^2 m y, m = r2 mean(q y), those of y^2, q y and the three parts of
 //   sum t u = sum G f u + r2 sum q f u - r2^2 m sum y f u,
 // which is also a row gate's gradient over 1 - s.  The next row is read while
-// one is worked on (6791 x 999 FP32: 47.5 us, 54.9 without; 43.8 since rows' ends are loaded like the rest).  Bound by memory with two waves a SIMD:
-// eight values a channel at 4.7 TB/s (32768 x 2048 bf16, 228 us; 8192 x 8192 FP32 441 us at 4.9); above 8,192 channels the
-// registers do not hold a lane's share and spill (4000 x 16384 bf16: 719 us, 1.5 TB/s).  The sums over rows stay in registers over all rows of a group, are joined in LDS for the
-// workgroup's groups, and leave as one part [kSums][channels] a workgroup.
+// one is worked on (6791 x 999 FP32: 47.5 us, 54.9 without; 43.8 since rows' ends are loaded like the rest).  Bound by memory
+// with two or three waves a SIMD: eight values a channel at 4.7 TB/s (32768 x 2048 bf16, 228 us; 8192 x 8192 FP32 443 us at
+// 4.8); above 8,192 channels a lane has sixteen values of each array in 128 registers and spills (4000 x 16384 bf16: 684 us,
+// 1.5 TB/s).  The sums over rows stay in registers over all rows of a group, are joined in LDS for the workgroup's groups, and
+// leave as one part [kSums][channels] a workgroup.
 template <class T, bool FULL, int G, int N>
 __global__ void __launch_bounds__(threads_of(G)) k_norm_gradient(Norm<T> a, float* __restrict__ parts) {
     constexpr int kThreads = threads_of(G), kGroups = kThreads / G;
@@ -441,8 +442,8 @@ void with_gradient_shape(int channels, F&& f) {
 
 constexpr i64 kUnits = 256;  // compute units
 
-// Workgroups of a gradient call, each of which leaves a part: as many as the card holds at once (two
-// waves a SIMD), and at least two rows a group.
+// Workgroups of a gradient call, each of which leaves a part: as many as the card holds at once at two
+// waves a SIMD, and at least two rows a group.
 i64 gradient_groups(i64 rows, i64 channels) {
     i64 groups = 1, threads = 256;
     with_gradient_shape(static_cast<int>(channels), [&](auto g, auto) {

@@ -82,7 +82,8 @@ class _Norm(torch.autograd.Function):
 
 
 class _GatedResidual(torch.autograd.Function):
-    """(y, h) from x and a block's output rows [update | gate logits]."""
+    """(y, h) from x and a block's output rows [update | gate logits].  These come in the rows' type: rounded to 16 bits in a
+    16-bit head, which halves the largest array that a block writes and reads, at the size of the rounding of y itself."""
 
     @staticmethod
     def forward(ctx, x, both, post, scale, next_weight, eps):
