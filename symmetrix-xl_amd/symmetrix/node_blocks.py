@@ -30,7 +30,7 @@ class _Undifferentiated(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, anchor, *grads):
-        return tuple(g if g is None else g.view_as(g) for g in grads)
+        return tuple(g if g is None else g.clone() for g in grads)
 
     @staticmethod
     def backward(ctx, *grads):

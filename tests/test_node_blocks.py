@@ -130,3 +130,14 @@ def test_weights_of_a_16_bit_head_get_gradients_of_their_own_type():
         # of FP32 sums, of which bf16 holds one in 2^16
         assert w.grad.dtype is torch.float32
         assert (w.grad.bfloat16().float() == w.grad).float().mean() < 0.1
+
+
+@pytest.mark.parametrize("name", ["embed", "norm", "residual", "linear"])
+def test_gradients_of_a_graph_are_changed_in_place(name):
+    """As any gradient may be whose own derivatives nobody asks for."""
+    call, leaf = _calls()[name]
+    y = call()
+    want, = torch.autograd.grad(y, leaf, torch.ones_like(y), retain_graph=True)
+    got, = torch.autograd.grad(y, leaf, torch.ones_like(y), create_graph=True)
+    got.mul_(2.0)
+    assert torch.equal(got, 2 * want)
