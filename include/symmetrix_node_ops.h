@@ -162,6 +162,76 @@ SMX_API int32_t smx_block_linear(const void* x, int64_t x_stride, int32_t dtype,
                                  void* out, int64_t out_stride, void* workspace, int64_t workspace_bytes,
                                  void* stream);
 
+/* ---- rows by kind ---- */
+
+/* A plan of `rows` rows by their kind, types[t] in [0, num_types) (int32, or int64 when types_are_64bit); a row of another
+ * type is masked.  The plan is device memory (16-byte aligned, smx_group_plan_bytes of it), an input of the products below for
+ * the same rows and num_types.  As int32 it holds from byte 16 on the offsets, num_types + 1 of them (of the sorted rows of
+ * type z the first is offsets[z] and the one past the last offsets[z + 1]), and from byte smx_group_plan_order on the rows
+ * in order: by type, of one type as they come, the masked ones last.  Up to 2^30 rows and 4,096 types. */
+SMX_API int64_t smx_group_plan_bytes(int64_t rows, int64_t num_types);
+SMX_API int64_t smx_group_plan_order(int64_t num_types);
+SMX_API int64_t smx_group_rows_workspace(int64_t rows, int64_t num_types);
+SMX_API int32_t smx_group_rows(const void* types, int32_t types_are_64bit, int64_t rows, int64_t num_types, void* plan,
+                               int64_t plan_bytes, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* out[t] = w[z] x[t] with z the type of row t and w [num_types][outputs][inputs] (w_stride between rows, w_type_stride
+ * between types, in values); the rows of masked t are zeros.  Values are `dtype`, out is out_dtype: that or FP32.  Products of FP32
+ * values are formed of three bf16 parts of each, to FP32's precision (2^-24 of a product; a value below 2^-110 is off by up to
+ * 2^-134).  An infinity or NaN makes the outputs infinite or NaN that it is a term of, and no others.  inputs, outputs
+ * <= 2^24. */
+SMX_API int32_t smx_grouped_linear(const void* x, int64_t x_stride, int32_t dtype, const void* w, int64_t w_stride,
+                                   int64_t w_type_stride, const void* plan, int64_t rows, int64_t num_types, int64_t inputs,
+                                   int64_t outputs, int32_t out_dtype, void* out, int64_t out_stride, void* stream);
+/* Its gradients from that of out, grad [rows][outputs]: dx[t] = w[z]^T grad[t], zeros for masked t, */
+SMX_API int32_t smx_grouped_linear_by_rows(const void* grad, int64_t grad_stride, int32_t dtype, const void* w, int64_t w_stride,
+                                           int64_t w_type_stride, const void* plan, int64_t rows, int64_t num_types,
+                                           int64_t inputs, int64_t outputs, int32_t out_dtype, void* dx, int64_t dx_stride,
+                                           void* stream);
+/* and dw[z] = the sum over rows of type z of grad[t] x[t]^T, every matrix of dw written (zeros for a type without rows), summed
+ * in a fixed order. */
+SMX_API int64_t smx_grouped_linear_by_weights_workspace(int64_t rows, int64_t num_types, int64_t inputs, int64_t outputs);
+SMX_API int32_t smx_grouped_linear_by_weights(const void* grad, int64_t grad_stride, const void* x, int64_t x_stride, int32_t dtype,
+                                              const void* plan, int64_t rows, int64_t num_types, int64_t inputs,
+                                              int64_t outputs, int32_t out_dtype, void* dw, int64_t dw_stride,
+                                              int64_t dw_type_stride, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- gradients' norm and clipping ---- */
+
+/* norm = scale * sqrt(sum of the squares of all values) of num_tensors tensors of counts[i] values of type dtypes[i], packed.
+ * tensors, counts and dtypes are host arrays, read within the call; tensors' values, norm and the workspace are on the device.
+ * Squares and sums are FP64 and have a fixed order, so no FP32 value is too large for its square, and norm is rounded once.
+ * scale (of gradients whose loss was scaled, 1 / the loss's) is positive and finite.  Up to 98,304 tensors. */
+SMX_API int64_t smx_gradient_norm_workspace(void);
+SMX_API int32_t smx_gradient_norm(const void* const* tensors, const int64_t* counts, const int32_t* dtypes, int64_t num_tensors,
+                                  float scale, float* norm, void* workspace, int64_t workspace_bytes, void* stream);
+/* The same, and out[i] = tensors[i] * scale * min(1, max_norm / norm) in out_dtypes[i]: out[i] may be tensors[i] where its type
+ * is the same; outputs overlap nothing else.  The factor is FP32, from the norm in FP64.  A norm that is infinite
+ * makes every finite value zero and the others NaN, one that is NaN makes all NaN: look at norm.  With a factor of one, values in place
+ * are left as they are. */
+SMX_API int32_t smx_clip_gradients(const void* const* tensors, const int64_t* counts, const int32_t* dtypes, int64_t num_tensors,
+                                   float max_norm, float scale, void* const* out, const int32_t* out_dtypes, float* norm,
+                                   void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- products in 8-bit integers ---- */
+
+/* A matrix [rows][cols] in 8-bit integers: values [rows][smx_integer_stride(cols)] (cols rounded up to 128, the rest zeros; 16-byte
+ * aligned) and an FP32 scale for each row.  A row's scale is the FP32 quotient of its largest magnitude and 127, at least
+ * 2^-126, and a value the whole number nearest to the exact quotient by the scale, ties to even.  A row with an
+ * infinity or NaN has the scale NaN and zeros. */
+SMX_API int64_t smx_integer_stride(int64_t cols);
+SMX_API int32_t smx_integer_quantize(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int64_t cols, int8_t* values,
+                                     float* scales, void* stream);
+/* out[i][j] = a_scales[i] b_scales[j] sum over k of a[i][k] b[j][k], a [m][k] and b [n][k] as above, k <= 2^17: the sum is exact and
+ * is rounded when it becomes FP32, at either scale, and to `dtype`. */
+SMX_API int32_t smx_integer_product(const int8_t* a_values, const float* a_scales, const int8_t* b_values, const float* b_scales,
+                                    int64_t m, int64_t n, int64_t k, int32_t dtype, void* out, int64_t out_stride, void* stream);
+/* The same with a = x [m][k] of `dtype`, brought to integers within the call; out is out_dtype. */
+SMX_API int64_t smx_integer_linear_workspace(int64_t m, int64_t n, int64_t k);
+SMX_API int32_t smx_integer_linear(const void* x, int64_t x_stride, int32_t dtype, const int8_t* w_values, const float* w_scales,
+                                   int64_t m, int64_t n, int64_t k, int32_t out_dtype, void* out, int64_t out_stride,
+                                   void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

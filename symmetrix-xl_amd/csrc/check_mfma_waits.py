@@ -3,7 +3,7 @@
 
 An instruction other than an MFMA that reads or overwrites a register written
 by v_mfma_f32_16x16x4_f32 (8 passes) must issue at least ten wait states after
-it, on every path, and after v_mfma_f32_16x16x32_bf16 (4 passes) at least eight,
+it, on every path, and after v_mfma_f32_16x16x32_bf16, v_mfma_f32_16x16x32_f16 and v_mfma_i32_16x16x64_i8 (4 passes) at least eight,
 and after v_mfma_scale_f32_16x16x128_f8f6f4 (8 passes) at least eleven; the hardware does not interlock.  The compiler inserts the waits, but in kernels
 whose MFMA chains sat in runtime-conditional blocks it padded only the
 fall-through path into a join, and a read on the taken branch came one
@@ -11,7 +11,7 @@ instruction after its MFMA (a stale accumulator element, silently wrong).
 This walks each kernel's control-flow graph backwards from every instruction
 that touches a register (VALU operands, memory addresses and data) and reports
 those with fewer than MIN wait states since an MFMA that writes the register,
-over any path (a bf16 MFMA counts two more, a scaled one one less); an s_nop N counts N + 1, other
+over any path (one of 4 passes counts two more, a scaled one one less); an s_nop N counts N + 1, other
 instructions one.  A scaled MFMA whose result overlaps an operand, which it would overwrite while it still reads
 it, is reported with no wait states: the compiler allocates that where accumulator and result are different values.
 
@@ -33,6 +33,8 @@ _SINGLE = re.compile(r"([av])(\d+)$")
 
 # wait states an MFMA asks for less than the default (16x16x4 FP32, 8 passes)
 _SLACK = {"v_mfma_f32_16x16x32_bf16": 2,  # 4 passes
+          "v_mfma_f32_16x16x32_f16": 2,  # 4 passes
+          "v_mfma_i32_16x16x64_i8": 2,  # 4 passes
           "v_mfma_scale_f32_16x16x128_f8f6f4": -1}
 _MORE = 1  # wait states that some ask for above the default
 

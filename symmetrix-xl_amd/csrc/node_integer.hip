@@ -1,0 +1,404 @@
+// Products in 8-bit integers with an FP32 scale for each row of both operands (a token of x, a channel of the weights), and the
+// kernel that brings rows to that form.
+//
+//   scale = max(max |x| / 127, 2^-126)     q = the whole number nearest to x / scale, ties to even
+//   out[i][j] = scale_a[i] scale_b[j] sum over k of q_a[i][k] q_b[j][k]
+//
+// Sums are of 32-bit integers (v_mfma_i32_16x16x64_i8) and exact up to 2^17 terms (2^17 * 127^2 < 2^31); a product is rounded
+// when its sum becomes FP32 and at each scale, by 2^-24 each, and to the output's type.
+#include <cmath>
+
+#include "node_tiles.hpp"
+
+namespace smx {
+namespace node {
+namespace {
+
+constexpr i64 kMostTerms = 1 << 17;
+
+// Quotients are the nearest whole numbers to the exact x / scale: the one from the rounded reciprocal is corrected by the sign
+// of what it leaves, r = x - q scale, which is exact in FP32 (a multiple of half the scale's last place, less than the scale).
+__device__ __forceinline__ int nearest(float x, float scale, float inverse) {
+    float q = rintf(x * inverse);
+    const float r = fmaf(-q, scale, x), twice = 2.0f * __builtin_fabsf(r);
+    if (twice > scale || (twice == scale && (static_cast<int>(q) & 1))) q += r > 0.0f ? 1.0f : -1.0f;
+    return static_cast<int>(q);
+}
+
+__device__ __forceinline__ unsigned four(const float* v, float scale, float inverse) {
+    unsigned w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w |= static_cast<unsigned>(nearest(v[i], scale, inverse) & 0xff) << (8 * i);
+    return w;
+}
+
+// A row's scale from the largest of its magnitudes' bits (infinities and NaN above all): NaN where the row has one of these.
+__device__ __forceinline__ float scale_of_bits(unsigned top) {
+    if (top >= 0x7f800000u) return __builtin_nanf("");
+    const float scale = __uint_as_float(top) / 127.0f;
+    return scale > 0x1p-126f ? scale : 0x1p-126f;
+}
+
+// Lanes a row, eight values each at a time; rows of up to 8 LANES PACKS values stay in registers between the largest magnitude and
+// the quotients, longer ones (PACKS 0) are read again.
+template <class T, int LANES, int PACKS>
+__global__ void __launch_bounds__(256) k_quantize_integers(const T* __restrict__ x, i64 x_stride, i64 rows, int cols,
+                                                           std::int8_t* __restrict__ values, i64 pitch,
+                                                           float* __restrict__ scales) {
+    __shared__ unsigned room[2][4];
+    const int lane = threadIdx.x % LANES;
+    int turn = 0;
+    for (i64 r = blockIdx.x * (256 / LANES) + threadIdx.x / LANES; r < rows; r += static_cast<i64>(gridDim.x) * (256 / LANES)) {
+        const T* const row = x + r * x_stride;
+        Eight<T> held[PACKS ? PACKS : 1];
+        unsigned top = 0;
+        const auto look = [&](const Eight<T>& e) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const unsigned b = __float_as_uint(e[i]) & 0x7fffffffu;
+                top = b > top ? b : top;
+            }
+        };
+        if constexpr (PACKS > 0) {
+#pragma unroll
+            for (int q = 0; q < PACKS; ++q) held[q] = load_pack(row, 8 * (q * LANES + lane), cols);
+#pragma unroll
+            for (int q = 0; q < PACKS; ++q) {
+                settle(held[q], 8 * (q * LANES + lane), cols);
+                look(held[q]);
+            }
+        } else {
+            for (int c = 8 * lane; c < cols; c += 8 * LANES) {
+                Eight<T> e = load_pack(row, c, cols);
+                settle(e, c, cols);
+                look(e);
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < (LANES < 64 ? LANES : 64); o *= 2) {
+            const unsigned other = __shfl_xor(top, o);
+            top = other > top ? other : top;
+        }
+        if constexpr (LANES > 64) {
+            // (the two halves of the room in turn: a wave past the barrier may be in its next row while another still reads)
+            turn ^= 1;
+            if (threadIdx.x % 64 == 0) room[turn][threadIdx.x / 64] = top;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < 4; ++w) top = room[turn][w] > top ? room[turn][w] : top;
+        }
+        const float scale = scale_of_bits(top);
+        if (lane == 0) scales[r] = scale;
+        const bool fine = top < 0x7f800000u;
+        const float inverse = 1.0f / scale;
+        const auto put = [&](const Eight<T>& e, int c) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = fine ? e[i] : 0.0f;
+            *reinterpret_cast<uint2*>(values + r * pitch + c) =
+                fine ? make_uint2(four(v, scale, inverse), four(v + 4, scale, inverse)) : make_uint2(0, 0);
+        };
+        if constexpr (PACKS > 0) {
+#pragma unroll
+            for (int q = 0; q < PACKS; ++q) {
+                const int c = 8 * (q * LANES + lane);
+                if (c < pitch) put(held[q], c);
+            }
+        } else {
+            for (int c = 8 * lane; c < pitch; c += 8 * LANES) {
+                Eight<T> e = load_pack(row, c, cols);
+                settle(e, c, cols);
+                put(e, c);
+            }
+        }
+    }
+}
+
+template <class O>
+struct Integers {
+    const std::int8_t *a, *b;
+    const float *as, *bs;
+    int m, n, k;
+    i64 pitch;
+    O* out;
+    i64 out_stride;
+    int tiles_m, tiles_n;
+};
+
+template <class O>
+__device__ __forceinline__ void store_scaled(const Integers<O>& p, int i, int j, i32x4 v) {
+    if (i >= p.m) return;
+    O* const at = p.out + i * p.out_stride + j;
+    const float a = p.as[i];
+    float o[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) o[q] = static_cast<float>(v[q]) * a * (j + q < p.n ? p.bs[j + q] : 0.0f);
+    if (j + 4 <= p.n) {
+        Pack<O, 4> w;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) w.v[q] = static_cast<O>(o[q]);
+        *reinterpret_cast<Pack<O, 4>*>(at) = w;
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (j + q < p.n) at[q] = static_cast<O>(apart(o[q]));
+    }
+}
+
+template <class O, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : 2) k_integer_tiles(Integers<O> p) {
+    using T = std::int8_t;
+    using A = Step<T, Lie::Rows, BM>;
+    using B = Step<T, Lie::Rows, BN>;
+    constexpr int WAVES = WM * WN, NA = A::kPieces / 64 / WAVES, NB = B::kPieces / 64 / WAVES, MF = BM / WM / 16,
+                  NF = BN / WN / 16;
+    constexpr unsigned kStage = (BM + BN) * kStepBytes;
+    __shared__ __attribute__((aligned(1024))) std::uint8_t lds[2 * kStage];
+    const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<std::uintptr_t>((__attribute__((address_space(3))) std::uint8_t*)lds));
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+    const int tiles = p.tiles_m * p.tiles_n, steps = static_cast<int>(p.pitch / kStepBytes);
+    int i0, j0;
+    const T *at_a[NA], *at_b[NB];
+    const auto turn_to = [&](int turn) {
+        const int id = xcd_remap(turn, tiles);
+        const int band = id / (4 * p.tiles_n), in = id % (4 * p.tiles_n);
+        const int high = p.tiles_m - 4 * band < 4 ? p.tiles_m - 4 * band : 4;
+        i0 = (4 * band + in % high) * BM, j0 = in / high * BN;
+#pragma unroll
+        for (int q = 0; q < NA; ++q) {
+            const int e = (wave + WAVES * q) * 64 + lane, r = i0 + A::row_at(e);
+            at_a[q] = p.a + (r < p.m ? r : p.m - 1) * p.pitch + A::piece_at(e) * 16;
+        }
+#pragma unroll
+        for (int q = 0; q < NB; ++q) {
+            const int e = (wave + WAVES * q) * 64 + lane, r = j0 + B::row_at(e);
+            at_b[q] = p.b + (r < p.n ? r : p.n - 1) * p.pitch + B::piece_at(e) * 16;
+        }
+    };
+    const auto stage = [&](int s, int slot) {
+        const unsigned to = __builtin_amdgcn_readfirstlane(lds0 + slot * kStage);
+#pragma unroll
+        for (int q = 0; q < NA; ++q) fetch(at_a[q] + s * kStepBytes, to + (wave + WAVES * q) * 1024);
+#pragma unroll
+        for (int q = 0; q < NB; ++q) fetch(at_b[q] + s * kStepBytes, to + BM * kStepBytes + (wave + WAVES * q) * 1024);
+    };
+    int slot = 0;
+    turn_to(blockIdx.x);
+    stage(0, 0);
+    for (int turn = blockIdx.x; turn < tiles; turn += gridDim.x) {
+        const int i_now = i0, j_now = j0;
+        i32x4 acc[MF][NF];
+#pragma unroll
+        for (int f = 0; f < MF; ++f)
+#pragma unroll
+            for (int g = 0; g < NF; ++g) acc[f][g] = i32x4{0, 0, 0, 0};
+        for (int s = 0; s < steps; ++s) {
+            arrived();
+            __syncthreads();
+            const std::uint8_t* const tile = lds + slot * kStage;
+            slot ^= 1;
+            Fragment<T> vb[NF];
+#pragma unroll
+            for (int g = 0; g < NF; ++g) vb[g] = B::read(tile + BM * kStepBytes, wn + 16 * g, lane);
+            if (s + 1 < steps) {
+                stage(s + 1, slot);
+            } else if (turn + static_cast<int>(gridDim.x) < tiles) {
+                turn_to(turn + gridDim.x);
+                stage(0, slot);
+            }
+#pragma unroll
+            for (int f = 0; f < MF; ++f) {
+                const Fragment<T> va = A::read(tile, wm + 16 * f, lane);
+#pragma unroll
+                for (int g = 0; g < NF; ++g) acc[f][g] = Fragment<T>::multiply(vb[g], va, acc[f][g]);
+            }
+        }
+        settle_products();
+#pragma unroll
+        for (int f = 0; f < MF; ++f)
+#pragma unroll
+            for (int g = 0; g < NF; ++g)
+                store_scaled(p, i_now + wm + 16 * f + lane % 16, j_now + wn + 16 * g + 4 * (lane / 16), acc[f][g]);
+    }
+}
+
+constexpr i64 kFewRows = 16;
+
+template <class O, int NF, int KS>
+__global__ void __launch_bounds__(64 * KS) k_integer_rows(Integers<O> p) {
+    using T = std::int8_t;
+    __shared__ FewRoom<T, NF, KS> room;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), row = lane % 16;
+    const int j0 = xcd_remap(blockIdx.x, gridDim.x) * 16 * NF;
+    const T* b[NF];
+#pragma unroll
+    for (int g = 0; g < NF; ++g) {
+        const int j = j0 + 16 * g + row;
+        b[g] = p.b + (j < p.n ? j : p.n - 1) * p.pitch;
+    }
+    const i32x4 sum = few_rows<T, true, NF, KS>(p.a + (row < p.m ? row : p.m - 1) * p.pitch, b, static_cast<int>(p.pitch), room);
+    if (wave >= NF) return;
+    store_scaled(p, row, j0 + 16 * wave + 4 * (lane / 16), sum);
+}
+
+template <class O>
+__global__ void __launch_bounds__(256) k_integer_zero(O* __restrict__ out, i64 out_stride, i64 m, i64 n) {
+    for (i64 e = static_cast<i64>(blockIdx.x) * 256 + threadIdx.x; e < m * n; e += static_cast<i64>(gridDim.x) * 256)
+        out[e / n * out_stride + e % n] = static_cast<O>(0.0f);
+}
+
+void check_sizes(i64 m, i64 n, i64 k) {
+    constexpr i64 most = (1LL << 31) - 512;
+    require(m >= 0 && m <= most && n >= 0 && n <= most && k >= 0 && k <= most, "sizes must be in [0, 2^31 - 512]");
+    if (k > kMostTerms) throw std::domain_error("integer products sum over up to 2^17 values");
+}
+
+void check_integers(const void* values, const void* scales, i64 rows, i64 cols, const char* name) {
+    if (rows == 0) return;
+    if ((cols > 0 && !values) || !scales) throw std::invalid_argument(std::string(name) + " is NULL");
+    if (!aligned(values, 16) || !aligned(scales, 4))
+        throw std::invalid_argument(std::string(name) + ": integers must be 16-byte aligned, their scales 4-byte");
+}
+
+i64 pitch_of(i64 cols) { return (cols + kStepBytes - 1) / kStepBytes * kStepBytes; }
+
+template <class T>
+void launch_quantize(const T* x, i64 x_stride, i64 rows, i64 cols, std::int8_t* values, float* scales, hipStream_t stream) {
+    const i64 pitch = pitch_of(cols);
+    const auto go = [&](auto lanes, auto packs) {
+        constexpr int L = decltype(lanes)::value, P = decltype(packs)::value;
+        const i64 groups = (rows + 256 / L - 1) / (256 / L);
+        k_quantize_integers<T, L, P><<<static_cast<unsigned>(groups < 16384 ? groups : 16384), 256, 0, stream>>>(
+            x, x_stride, rows, static_cast<int>(cols), values, pitch, scales);
+        SMX_LAUNCH_CHECK("k_quantize_integers");
+    };
+    using std::integral_constant;
+    const auto l = [&](auto lanes) { return lanes; };
+    if (pitch <= 128) go(l(integral_constant<int, 16>{}), integral_constant<int, 1>{});
+    else if (pitch <= 512) go(l(integral_constant<int, 64>{}), integral_constant<int, 1>{});
+    else if (pitch <= 1024) go(l(integral_constant<int, 64>{}), integral_constant<int, 2>{});
+    else if (pitch <= 2048) go(l(integral_constant<int, 256>{}), integral_constant<int, 1>{});
+    else if (pitch <= 4096) go(l(integral_constant<int, 256>{}), integral_constant<int, 2>{});
+    else if (pitch <= 8192) go(l(integral_constant<int, 256>{}), integral_constant<int, 4>{});
+    else go(l(integral_constant<int, 256>{}), integral_constant<int, 0>{});
+}
+
+void quantize(const void* x, i64 x_stride, int dtype, i64 rows, i64 cols, std::int8_t* values, float* scales, hipStream_t stream) {
+    if (rows == 0) return;
+    with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        launch_quantize(static_cast<const T*>(x), x_stride, rows, cols, values, scales, stream);
+    });
+}
+
+int tile_for(i64 m, i64 n) {
+    const auto rounds = [&](i64 t, i64 held) {
+        return ((m + t - 1) / t * ((n + t - 1) / t) + held * kComputeUnits - 1) / (held * kComputeUnits);
+    };
+    const double t256 = 1.0 * rounds(256, 1), t128 = 1.12 / 2 * rounds(128, 2), t64 = 1.86 / 4 * rounds(64, 4);
+    return t256 <= t128 && t256 <= t64 ? 256 : t128 <= t64 ? 128 : 64;
+}
+
+template <class O>
+void launch_product(const std::int8_t* a, const float* as, const std::int8_t* b, const float* bs, i64 m, i64 n, i64 k, O* out,
+                    i64 out_stride, hipStream_t stream) {
+    if (k == 0) {
+        k_integer_zero<O><<<static_cast<unsigned>(m * n < 256 * 4096 ? (m * n + 255) / 256 : 4096), 256, 0, stream>>>(
+            out, out_stride, m, n);
+        SMX_LAUNCH_CHECK("k_integer_zero");
+        return;
+    }
+    Integers<O> p{};
+    p.a = a, p.as = as, p.b = b, p.bs = bs;
+    p.m = static_cast<int>(m), p.n = static_cast<int>(n), p.k = static_cast<int>(k);
+    p.pitch = pitch_of(k);
+    p.out = out, p.out_stride = out_stride;
+    if (m <= kFewRows) {
+        k_integer_rows<O, 1, 8><<<blocks_for(n, 16), 512, 0, stream>>>(p);
+        SMX_LAUNCH_CHECK("k_integer_rows");
+        return;
+    }
+    const i64 t = tile_for(m, n), tiles_m = (m + t - 1) / t, tiles_n = (n + t - 1) / t;
+    require(tiles_m * tiles_n < (1LL << 31) && 8 * tiles_n < (1LL << 31), "the product has too many tiles");
+    p.tiles_m = static_cast<int>(tiles_m), p.tiles_n = static_cast<int>(tiles_n);
+    const auto grid = [&](i64 held) {
+        const i64 most = held * kComputeUnits;
+        return static_cast<unsigned>(tiles_m * tiles_n < most ? tiles_m * tiles_n : most);
+    };
+    switch (t) {
+        case 256: k_integer_tiles<O, 256, 256, 2, 4><<<grid(1), 512, 0, stream>>>(p); break;
+        case 128: k_integer_tiles<O, 128, 128, 2, 2><<<grid(2), 256, 0, stream>>>(p); break;
+        default: k_integer_tiles<O, 64, 64, 2, 2><<<grid(4), 256, 0, stream>>>(p);
+    }
+    SMX_LAUNCH_CHECK("k_integer_tiles");
+}
+
+}  // namespace
+}  // namespace node
+}  // namespace smx
+
+using namespace smx;
+using namespace smx::node;
+
+extern "C" {
+
+int64_t smx_integer_stride(int64_t cols) { return cols > 0 ? pitch_of(cols) : 0; }
+
+int32_t smx_integer_quantize(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int64_t cols, int8_t* values,
+                             float* scales, void* stream) {
+    return guarded([&] {
+        check_sizes(rows, 0, 0);
+        require(cols >= 0 && cols < (1LL << 31) - 512, "sizes must be in [0, 2^31 - 512)");
+        require(dtype >= SMX_DTYPE_F32 && dtype <= SMX_DTYPE_F16, "unknown dtype code");
+        check_rows(x, x_stride, rows, cols, dtype, "x");
+        check_integers(values, scales, rows, cols, "values");
+        quantize(x, x_stride, dtype, rows, cols, values, scales, static_cast<hipStream_t>(stream));
+    });
+}
+
+int32_t smx_integer_product(const int8_t* a_values, const float* a_scales, const int8_t* b_values, const float* b_scales, int64_t m,
+                            int64_t n, int64_t k, int32_t dtype, void* out, int64_t out_stride, void* stream) {
+    return guarded([&] {
+        check_sizes(m, n, k);
+        require(dtype >= SMX_DTYPE_F32 && dtype <= SMX_DTYPE_F16, "unknown dtype code");
+        check_integers(a_values, a_scales, m, k, "a");
+        check_integers(b_values, b_scales, n, k, "b");
+        check_rows(out, out_stride, m, n, dtype, "out");
+        if (m == 0 || n == 0) return;
+        with_dtype(dtype, [&](auto o) {
+            using O = decltype(o);
+            launch_product<O>(a_values, a_scales, b_values, b_scales, m, n, k, static_cast<O*>(out), out_stride,
+                              static_cast<hipStream_t>(stream));
+        });
+    });
+}
+
+int64_t smx_integer_linear_workspace(int64_t m, int64_t n, int64_t k) {
+    return m > 0 && n > 0 && k > 0 ? m * pitch_of(k) + 4 * m : 0;
+}
+
+int32_t smx_integer_linear(const void* x, int64_t x_stride, int32_t dtype, const int8_t* w_values, const float* w_scales, int64_t m,
+                           int64_t n, int64_t k, int32_t out_dtype, void* out, int64_t out_stride, void* workspace,
+                           int64_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        check_sizes(m, n, k);
+        require(dtype >= SMX_DTYPE_F32 && dtype <= SMX_DTYPE_F16, "unknown dtype code");
+        require(out_dtype >= SMX_DTYPE_F32 && out_dtype <= SMX_DTYPE_F16, "unknown dtype code");
+        check_rows(x, x_stride, m, k, dtype, "x");
+        check_integers(w_values, w_scales, n, k, "w");
+        check_rows(out, out_stride, m, n, out_dtype, "out");
+        check_workspace(workspace, workspace_bytes, smx_integer_linear_workspace(m, n, k));
+        if (m == 0 || n == 0) return;
+        auto* const values = static_cast<std::int8_t*>(workspace);
+        auto* const scales = k > 0 ? reinterpret_cast<float*>(values + m * pitch_of(k)) : nullptr;
+        if (k > 0) quantize(x, x_stride, dtype, m, k, values, scales, static_cast<hipStream_t>(stream));
+        with_dtype(out_dtype, [&](auto o) {
+            using O = decltype(o);
+            launch_product<O>(values, scales, w_values, w_scales, m, n, k, static_cast<O*>(out), out_stride,
+                              static_cast<hipStream_t>(stream));
+        });
+    });
+}
+
+}  // extern "C"

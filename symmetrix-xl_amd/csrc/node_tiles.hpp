@@ -1,0 +1,281 @@
+// Products in tiles, shared by the products by kind of row and the products in 8-bit integers: operands go to LDS in steps of
+// 128 bytes of the summed axis, and matrix instructions take them from there.
+//
+// An operand lies in one of two ways: its summed axis along the rows (Rows: x and the weights of a forward product) or
+// across them (Columns: the weights of a gradient by x, both operands of one by the weights).  A step of an operand of
+// B outer indices is B * 128 bytes of LDS either way, in pieces of 16 bytes:
+//   Rows     [B][8 pieces], a row's pieces permuted by half the row's number, so that the 16 rows that a fragment
+//            read meets at once lie in different banks;
+//   Columns  [128 / size][B * size / 16 pieces], 16 columns together, these permuted by the row, so that the rows that a
+//            transposing read (ds_read_b64_tr_b16: four rows of 16 columns for 16 lanes) meets at once do.
+// Pieces go from memory to LDS without registers where rows are aligned to 16 bytes and as long as whole pieces; a piece that
+// is not there (past the summed axis' end) is read from a place of zeros, so both operands are zero there and infinities
+// outside a sum stay outside.  Other rows go through registers (DIRECT false).
+//
+// The order of the summed axis inside a step is the operands' own affair, as long as it is one: of 16-bit values,
+// piece p holds 8 p .. 8 p + 7, instruction q takes pieces 4 q .. 4 q + 3, lane group l / 16 the piece 4 q + l / 16.
+#pragma once
+
+#include "node_ops.hpp"
+
+namespace smx {
+namespace node {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+enum class Lie { Rows, Columns };
+
+constexpr int kStepBytes = 128;
+constexpr int kComputeUnits = 256;
+
+// where pieces that are not there are read from
+static __device__ const uint4 kNothing[1] = {};
+
+// 1 KB of LDS at byte `lds` (the wave's own, uniform) from 64 lanes' 16 bytes: memory to LDS without registers.  The compiler
+// does not count it: arrived().
+__device__ __forceinline__ void fetch(const void* at, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(at) : "memory");
+}
+__device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// The accumulators of a chain of MFMAs are read by other instructions right after it; eighteen wait states on every path
+// into what follows, with the scheduler fenced on both sides.
+__device__ __forceinline__ void settle_products() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 8\n\ts_nop 8");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// Sixteen bytes of a row from value c on (c a multiple of what they hold), zeros past its end, at any alignment: a piece that
+// passes the end loads the row's last sixteen bytes, and settle_piece moves them to their places.
+template <class T>
+__device__ __forceinline__ i32x4 load_piece(const T* row, i64 c, i64 cols) {
+    constexpr int kPer = 16 / sizeof(T);
+    struct __attribute__((packed, aligned(sizeof(T)))) Words {
+        i32x4 w;
+    };
+    if (cols >= kPer) {
+        if (c >= cols) return i32x4{0, 0, 0, 0};
+        return reinterpret_cast<const Words*>(row + (c + kPer <= cols ? c : cols - kPer))->w;
+    }
+    i32x4 w{0, 0, 0, 0};
+    constexpr int kHalf = 4 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+        if (c + i < cols) w[i / kHalf] |= static_cast<int>(bits_of(row[c + i]) << (i % kHalf * 8 * sizeof(T)));
+    return w;
+}
+
+template <class T>
+__device__ __forceinline__ i32x4 settle_piece(i32x4 w, i64 c, i64 cols) {
+    constexpr int kPer = 16 / sizeof(T);
+    if (cols < kPer || c >= cols || c + kPer <= cols) return w;
+    const int by = static_cast<int>(c + kPer - cols) * static_cast<int>(sizeof(T));  // bytes to move down
+    if (by & 8) w = i32x4{w[2], w[3], 0, 0};
+    if (by & 4) w = i32x4{w[1], w[2], w[3], 0};
+    if constexpr (sizeof(T) == 2) {
+        if (by & 2) {
+            const auto half = [](int lo, int hi) {
+                return static_cast<int>(static_cast<unsigned>(lo) >> 16 | static_cast<unsigned>(hi) << 16);
+            };
+            w = i32x4{half(w[0], w[1]), half(w[1], w[2]), half(w[2], w[3]), half(w[3], 0)};
+        }
+    }
+    return w;
+}
+
+// ---- the arithmetic of a step by type ----
+
+// 128 bytes of the summed axis of 16 outer indices, as the matrix instructions take them: lane l has outer index l % 16.
+template <class T>
+struct Fragment;
+
+template <>
+struct Fragment<bf16> {
+    using Sum = acc4;
+    i32x4 v[2];
+    __device__ __forceinline__ void set(i32x4 a, i32x4 b) { v[0] = a, v[1] = b; }
+    __device__ __forceinline__ static acc4 multiply(const Fragment& b, const Fragment& a, acc4 acc) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b.v[q]), __builtin_bit_cast(bf16x8, a.v[q]),
+                                                          acc, 0, 0, 0);
+        return acc;
+    }
+};
+
+template <>
+struct Fragment<f16> {
+    using Sum = acc4;
+    i32x4 v[2];
+    __device__ __forceinline__ void set(i32x4 a, i32x4 b) { v[0] = a, v[1] = b; }
+    __device__ __forceinline__ static acc4 multiply(const Fragment& b, const Fragment& a, acc4 acc) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, b.v[q]), __builtin_bit_cast(f16x8, a.v[q]),
+                                                         acc, 0, 0, 0);
+        return acc;
+    }
+};
+
+// FP32 values as three bf16 parts each, six products (device_common.hpp): FP32's precision at a rate of 1/6 of bf16's, where
+// the FP32 matrix instructions have 1/16.
+template <>
+struct Fragment<float> {
+    using Sum = acc4;
+    SplitOperand parts;
+    __device__ __forceinline__ void set(i32x4 a, i32x4 b) {
+        typedef int i32x8 __attribute__((ext_vector_type(8)));
+        const i32x8 both = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        parts = split_operand(__builtin_bit_cast(f32x8, both));
+    }
+    __device__ __forceinline__ static acc4 multiply(const Fragment& b, const Fragment& a, acc4 acc) {
+        return split_product(b.parts, a.parts, acc);
+    }
+};
+
+template <>
+struct Fragment<std::int8_t> {
+    using Sum = i32x4;
+    i32x4 v[2];
+    __device__ __forceinline__ void set(i32x4 a, i32x4 b) { v[0] = a, v[1] = b; }
+    __device__ __forceinline__ static i32x4 multiply(const Fragment& b, const Fragment& a, i32x4 acc) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(b.v[q], a.v[q], acc, 0, 0, 0);
+        return acc;
+    }
+};
+
+// ---- an operand's step in LDS ----
+
+template <class T, Lie L, int B>
+struct Step {
+    static constexpr int kValues = kStepBytes / static_cast<int>(sizeof(T));  // of the summed axis
+    static constexpr int kPieces = B * 8;
+    static constexpr int kRowPieces = L == Lie::Rows ? 8 : B * static_cast<int>(sizeof(T)) / 16;
+    static constexpr int kGroup = static_cast<int>(sizeof(T));  // pieces of 16 columns
+
+    __device__ __forceinline__ static int turned(int row) {
+        if constexpr (L == Lie::Rows) return row / 2 % 8;
+        if constexpr (sizeof(T) == 2) return (row / 8 * 4 + row % 4) & (B / 16 - 1);
+        return row / 4 % 4;
+    }
+    // the row and the piece of it that lie at piece e of the step
+    __device__ __forceinline__ static int row_at(int e) { return e / kRowPieces; }
+    __device__ __forceinline__ static int piece_at(int e) {
+        const int p = e % kRowPieces, t = turned(e / kRowPieces);
+        if constexpr (L == Lie::Rows) return p ^ t;
+        return ((p / kGroup) ^ t) * kGroup + p % kGroup;
+    }
+    // 16 outer indices from `outer` (a multiple of 16) on
+    __device__ __forceinline__ static Fragment<T> read(const std::uint8_t* tile, int outer, int lane) {
+        Fragment<T> f;
+        if constexpr (L == Lie::Rows) {
+            const int at = (lane % 16) * kStepBytes + ((lane / 16) ^ (lane % 16 / 2)) * 16;
+            f.set(*reinterpret_cast<const i32x4*>(tile + outer * kStepBytes + at),
+                  *reinterpret_cast<const i32x4*>(tile + outer * kStepBytes + (at ^ 64)));
+        } else if constexpr (sizeof(T) == 2) {
+            using At = __attribute__((address_space(3))) s16x4*;
+            constexpr int kPitch = B * 2;
+            const std::uint8_t* const at = tile + (8 * (lane / 16) + lane % 16 / 4) * kPitch +
+                                           ((outer / 16) ^ (lane / 4 & (B / 16 - 1))) * 32 + lane % 4 * 8;
+            i32x4 v[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                typedef int i32x2 __attribute__((ext_vector_type(2)));
+                i32x2 h[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    h[k] = __builtin_bit_cast(i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                         (At)(at + (32 * q + 4 * k) * kPitch)));
+                v[q] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3);
+            }
+            f.set(v[0], v[1]);
+        } else {
+            constexpr int kPitch = B * 4;
+            const std::uint8_t* const at = tile + 4 * (lane / 16) * kPitch + ((outer / 16) ^ (lane / 16)) * 64 + lane % 16 * 4;
+            i32x4 v[2];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i / 4][i % 4] = *reinterpret_cast<const int*>(at + (i % 4 + 16 * (i / 4)) * kPitch);
+            f.set(v[0], v[1]);
+        }
+        return f;
+    }
+};
+
+// ---- up to sixteen rows ----
+
+// Where the waves of few_rows meet.
+template <class T, int NF, int KS>
+struct FewRoom {
+    typename Fragment<T>::Sum v[KS][NF][64];
+};
+
+// Sixteen rows of a times 16 NF rows of b by KS waves, every KS-th step each, joined in LDS: where the bytes of b are all of it, they
+// go straight to registers, kAhead steps of them under way at once.  `a` and `b`: the rows of the lane (l % 16).  Fragment g's sums
+// are wave g's (lane l: column l % 16, four rows of b from 4 (l / 16) on).
+template <class T, bool DIRECT, int NF, int KS>
+__device__ __forceinline__ typename Fragment<T>::Sum few_rows(const T* a, const T* const (&b)[NF], int k, FewRoom<T, NF, KS>& room) {
+    using Sum = typename Fragment<T>::Sum;
+    constexpr int kAhead = 4, kValues = kStepBytes / static_cast<int>(sizeof(T)), kPer = 16 / static_cast<int>(sizeof(T));
+    // (a wave's branches have to be the whole wave's to the compiler too: matrix instructions run for all lanes)
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int steps = (k + kValues - 1) / kValues;
+    const auto load = [&](const T* row, int c) {
+        if constexpr (DIRECT)
+            return *reinterpret_cast<const i32x4*>(c < k ? static_cast<const void*>(row + c) : kNothing);
+        else
+            return load_piece(row, c, k);
+    };
+    Sum acc[NF];
+#pragma unroll
+    for (int g = 0; g < NF; ++g) acc[g] = Sum{0, 0, 0, 0};
+    for (int s0 = wave; s0 < steps; s0 += KS * kAhead) {
+        i32x4 wb[kAhead][NF][2], wa[kAhead][2];
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {
+            const int s = s0 + q * KS < steps ? s0 + q * KS : s0;  // (a step read twice is used once)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int c = s * kValues + (lane / 16 + 4 * h) * kPer;
+                wa[q][h] = load(a, c);
+#pragma unroll
+                for (int g = 0; g < NF; ++g) wb[q][g][h] = load(b[g], c);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {
+            if (s0 + q * KS >= steps) break;
+            if constexpr (!DIRECT)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int c = (s0 + q * KS) * kValues + (lane / 16 + 4 * h) * kPer;
+                    wa[q][h] = settle_piece<T>(wa[q][h], c, k);
+#pragma unroll
+                    for (int g = 0; g < NF; ++g) wb[q][g][h] = settle_piece<T>(wb[q][g][h], c, k);
+                }
+            Fragment<T> va, vb;
+            va.set(wa[q][0], wa[q][1]);
+#pragma unroll
+            for (int g = 0; g < NF; ++g) {
+                vb.set(wb[q][g][0], wb[q][g][1]);
+                acc[g] = Fragment<T>::multiply(vb, va, acc[g]);
+            }
+            settle_products();  // (the next step is conditional)
+        }
+    }
+    settle_products();
+#pragma unroll
+    for (int g = 0; g < NF; ++g) room.v[wave][g][lane] = acc[g];
+    __syncthreads();
+    const int mine = wave < NF ? wave : 0;
+    Sum sum = room.v[0][mine][lane];
+#pragma unroll
+    for (int w = 1; w < KS; ++w) sum += room.v[w][mine][lane];
+    return sum;
+}
+
+}  // namespace node
+}  // namespace smx

@@ -219,6 +219,24 @@ SIGNATURES = [
     ("smx_block_product", _i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp]),
     ("smx_block_linear_workspace", _i64, [_i64, _i64, _i64]),
     ("smx_block_linear", _i32, [_vp, _i64, _i32, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp]),
+    ("smx_group_plan_bytes", _i64, [_i64, _i64]),
+    ("smx_group_plan_order", _i64, [_i64]),
+    ("smx_group_rows_workspace", _i64, [_i64, _i64]),
+    ("smx_group_rows", _i32, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _vp]),
+    ("smx_grouped_linear", _i32, [_vp, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _i64, _vp]),
+    ("smx_grouped_linear_by_rows", _i32, [_vp, _i64, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _i64,
+                                          _vp]),
+    ("smx_grouped_linear_by_weights_workspace", _i64, [_i64, _i64, _i64, _i64]),
+    ("smx_grouped_linear_by_weights", _i32, [_vp, _i64, _vp, _i64, _i32, _vp, _i64, _i64, _i64, _i64, _i32, _vp, _i64, _i64,
+                                             _vp, _i64, _vp]),
+    ("smx_gradient_norm_workspace", _i64, []),
+    ("smx_gradient_norm", _i32, [_vp, _vp, _vp, _i64, _f32, _vp, _vp, _i64, _vp]),
+    ("smx_clip_gradients", _i32, [_vp, _vp, _vp, _i64, _f32, _f32, _vp, _vp, _vp, _vp, _i64, _vp]),
+    ("smx_integer_stride", _i64, [_i64]),
+    ("smx_integer_quantize", _i32, [_vp, _i64, _i32, _i64, _i64, _vp, _vp, _vp]),
+    ("smx_integer_product", _i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp]),
+    ("smx_integer_linear_workspace", _i64, [_i64, _i64, _i64]),
+    ("smx_integer_linear", _i32, [_vp, _i64, _i32, _vp, _vp, _i64, _i64, _i64, _i32, _vp, _i64, _vp, _i64, _vp]),
 ]
 
 

@@ -6,7 +6,13 @@ of (include/symmetrix_node_ops.h).
 * ``norm``, ``residual_norm`` / ``residual_norm_gradient``: the norms before and
   after a block with its gate and residual scale;
 * ``quantize``, ``block_product``, ``block_linear`` / ``block_linear_gradient``:
-  products of E4M3 values with a power-of-two scale for each block of 128.
+  products of E4M3 values with a power-of-two scale for each block of 128;
+* ``group_rows``, ``grouped_linear`` / ``grouped_linear_gradient``: rows by their
+  type, products with a weight matrix for each type, and their gradients;
+* ``gradient_norm``, ``clip_gradients``: the norm of many gradients together, and
+  their clipping;
+* ``quantize_integers``, ``integer_product``, ``integer_linear``: products of 8-bit
+  integers with a scale for each row of both operands.
 
 Row tensors are float32, bfloat16 or float16 on the current HIP device, two-dimensional, with
 unit stride along the channels and any row stride.  Calls enqueue on torch's
@@ -28,7 +34,7 @@ import ctypes
 import torch
 
 from . import _native
-from ._native import check, lib
+from ._native import SymmetrixUnsupportedError, check, lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _BLOCK = 128
@@ -439,5 +445,297 @@ def block_linear_gradient(grad, w_columns, x_columns, dtype=None):
     return dx, dw
 
 
+# ---- rows by type ----
+
+
+class RowGroups:
+    """Rows in the order of their types (``group_rows``): ``order`` int32 [rows], by type, of one type as they come, masked
+    ones last; ``offsets`` int32 [num_types + 1], where each type's rows begin in it.  Both lie on the device."""
+
+    __slots__ = ("rows", "num_types", "_room")
+
+    def __init__(self, rows, num_types, room):
+        self.rows, self.num_types, self._room = rows, num_types, room
+
+    @property
+    def offsets(self):
+        return self._room[4:5 + self.num_types]
+
+    @property
+    def order(self):
+        return self._room[lib.smx_group_plan_order(self.num_types) // 4:]
+
+    def __reduce__(self):
+        raise TypeError("RowGroups are not copied: make them of the types again (symmetrix.node_ops.group_rows)")
+
+
+def group_rows(types, num_types):
+    """``RowGroups`` of ``types`` (a contiguous int32 or int64 vector); a type outside [0, num_types) masks its row."""
+    wide = _types(types, types)
+    if num_types < 1:
+        raise ValueError("num_types must be positive")
+    if num_types > 4096:
+        raise SymmetrixUnsupportedError("rows are grouped by up to 4096 types")
+    stream = _stream(types.get_device())
+    t = types.shape[0]
+    size = lib.smx_group_plan_bytes(t, num_types)
+    plan = torch.empty(size // 4, dtype=torch.int32, device=types.device)
+    work = lib.smx_group_rows_workspace(t, num_types)
+    room = _workspace(work, types)
+    check(lib.smx_group_rows(types.data_ptr(), wide, t, num_types, plan.data_ptr(), size, _at(room), work, stream))
+    return RowGroups(t, num_types, plan)
+
+
+def _grouped(t, name, groups):
+    """Checks rows of groups; (type code, channels, row stride)."""
+    if not isinstance(groups, RowGroups):
+        raise ValueError("groups must be RowGroups (symmetrix.node_ops.group_rows)")
+    code, r, c, stride = _rows(t, name)
+    if r != groups.rows or groups._room.get_device() != t.get_device():
+        raise ValueError("%s must have the rows that were grouped, on their device" % name)
+    return code, c, stride
+
+
+def _type_weights(w, like, num_types, outputs, inputs):
+    """Checks weights [num_types][outputs][inputs]; (row stride, type stride)."""
+    if w.dtype is not like.dtype or w.get_device() != like.get_device():
+        raise ValueError("w must have the type and device of the rows")
+    if w.dim() != 3 or w.shape[0] != num_types or (outputs is not None and w.shape[1] != outputs) \
+            or (inputs is not None and w.shape[2] != inputs):
+        raise ValueError("w must be [types][outputs][inputs] of the grouped types and the rows' channels")
+    v, n, k = w.shape
+    by_type, by_row, unit = w.stride()
+    if (unit != 1 and k > 1) or (by_row < k and n > 1):
+        raise ValueError("w must have unit stride along its inputs and rows that do not overlap")
+    if n <= 1:
+        by_row = k
+    if v > 1 and by_type < (n - 1) * by_row + k and n and k:
+        raise ValueError("the types' matrices in w must not overlap")
+    return by_row, by_type if v > 1 else n * by_row
+
+
+def _out_dtype(dtype, like):
+    if dtype is None or dtype is like.dtype:
+        return like.dtype
+    if dtype is not torch.float32:
+        raise ValueError("products by type are of the rows' type or float32")
+    return dtype
+
+
+def grouped_linear(x, w, groups, dtype=None):
+    """Each row of ``x`` [rows][inputs] through its type's matrix of ``w`` [num_types][outputs][inputs]; a masked row gives
+    zeros.  Sums are FP32; in x's type unless ``dtype`` is float32."""
+    code, k, xs = _grouped(x, "x", groups)
+    ws, wt = _type_weights(w, x, groups.num_types, None, k)
+    dtype = _out_dtype(dtype, x)
+    stream = _stream(x.get_device())
+    n = w.shape[1]
+    out = torch.empty((groups.rows, n), dtype=dtype, device=x.device)
+    rc = lib.smx_grouped_linear(x.data_ptr(), xs, code, w.data_ptr(), ws, wt, groups._room.data_ptr(), groups.rows,
+                                groups.num_types, k, n, _DTYPES[dtype], out.data_ptr(), n, stream)
+    if rc:
+        check(rc)
+    return out
+
+
+def grouped_linear_gradient(grad, x, w, groups, dtype=None):
+    """``(dx, dw)`` of ``grouped_linear`` from the gradient [rows][outputs] of its result: dx in grad's type (None where ``w`` is
+    None) and dw [num_types][outputs][inputs] in float32, or ``dtype`` (None where ``x`` is None).  A type without rows
+    has a gradient of zeros."""
+    code, n, gs = _grouped(grad, "grad", groups)
+    v, rows, plan = groups.num_types, groups.rows, groups._room.data_ptr()
+    if x is not None:
+        if x.dtype is not grad.dtype:
+            raise ValueError("x must have the type and device of grad")
+        _, k, xs = _grouped(x, "x", groups)
+    if w is not None:
+        ws, wt = _type_weights(w, grad, v, n, None if x is None else k)
+    dw_dtype = _out_dtype(torch.float32 if dtype is None else dtype, grad)
+    stream = _stream(grad.get_device())
+    dx = dw = None
+    if w is not None:
+        dx = grad.new_empty((rows, w.shape[2]))
+        check(lib.smx_grouped_linear_by_rows(grad.data_ptr(), gs, code, w.data_ptr(), ws, wt, plan, rows, v, w.shape[2], n,
+                                             code, dx.data_ptr(), w.shape[2], stream))
+    if x is not None:
+        dw = torch.empty((v, n, k), dtype=dw_dtype, device=grad.device)
+        size = lib.smx_grouped_linear_by_weights_workspace(rows, v, k, n)
+        room = _workspace(size, grad)
+        check(lib.smx_grouped_linear_by_weights(grad.data_ptr(), gs, x.data_ptr(), xs, code, plan, rows, v, k, n,
+                                                _DTYPES[dw_dtype], dw.data_ptr(), k, n * k, _at(room), size, stream))
+    return dx, dw
+
+
+# ---- gradients' norm and clipping ----
+
+
+def _packed(t):
+    """Whether t's values fill one piece of memory, in whatever order of its axes."""
+    if t.is_contiguous():
+        return True
+    at = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if stride != at:
+            return False
+        at *= size
+    return True
+
+
+class _Tensors:
+    """The addresses, counts and types of tensors, for the length of a call."""
+
+    def __init__(self, tensors, name):
+        n = len(tensors)
+        self.tensors = n
+        self.at, self.counts, self.codes = (ctypes.c_void_p * n)(), (ctypes.c_int64 * n)(), (ctypes.c_int32 * n)()
+        device = tensors[0].get_device()
+        for i, t in enumerate(tensors):
+            code = _DTYPES.get(t.dtype)
+            if code is None or t.layout is not torch.strided:
+                raise ValueError("%s must be dense float32, bfloat16 or float16 tensors" % name)
+            if t.get_device() != device:
+                raise ValueError("%s must be on one device" % name)
+            if not _packed(t):
+                raise ValueError("%s must fill their memory without gaps or overlaps" % name)
+            self.at[i], self.counts[i], self.codes[i] = t.data_ptr(), t.numel(), code
+        self.device = device
+
+
+def _norm_room(like):
+    size = lib.smx_gradient_norm_workspace()
+    return torch.empty((), dtype=torch.float32, device=like.device), _workspace(size, like), size
+
+
+def _listed(tensors, name):
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if not tensors:
+        raise ValueError("%s are none" % name)
+    return tensors
+
+
+def gradient_norm(tensors, scale=1.0):
+    """``scale`` times the 2-norm of all values of ``tensors`` together, a float32 scalar on their device.  The tensors are
+    float32, bfloat16 or float16, in any mix, and fill their memory without gaps."""
+    tensors = _listed(tensors, "tensors")
+    t = _Tensors(tensors, "tensors")
+    stream = _stream(t.device)
+    norm, room, size = _norm_room(tensors[0])
+    check(lib.smx_gradient_norm(t.at, t.counts, t.codes, t.tensors, scale, norm.data_ptr(), room.data_ptr(), size, stream))
+    return norm
+
+
+def clip_gradients(tensors, max_norm, scale=1.0, out=None):
+    """Brings ``tensors`` to a norm of ``max_norm`` at most: each becomes ``tensor * scale * min(1, max_norm / norm)``, in place or
+    in ``out`` (tensors of their shapes, of any of the types).  The norm before it, ``scale`` times the 2-norm of all values
+    (``scale`` of gradients whose loss was scaled, 1 / the loss's), is returned as a float32 scalar on
+    their device; nothing waits for it."""
+    tensors = _listed(tensors, "tensors")
+    t = _Tensors(tensors, "tensors")
+    o = t
+    if out is not None:
+        out = _listed(out, "out")
+        if len(out) != len(tensors):
+            raise ValueError("out must be as many tensors")
+        o = _Tensors(out, "out")
+        if o.device != t.device:
+            raise ValueError("out must be on the tensors' device")
+        for a, b in zip(tensors, out):
+            if a.shape != b.shape or (a.stride() != b.stride() and not (a.is_contiguous() and b.is_contiguous())):
+                raise ValueError("out must have the tensors' shapes and strides")
+    stream = _stream(t.device)
+    norm, room, size = _norm_room(tensors[0])
+    check(lib.smx_clip_gradients(t.at, t.counts, t.codes, t.tensors, max_norm, scale, o.at, o.codes, norm.data_ptr(),
+                                 room.data_ptr(), size, stream))
+    return norm
+
+
+# ---- products in 8-bit integers ----
+
+
+class IntegerValues:
+    """A matrix in 8-bit integers: int8 ``values`` [rows][columns rounded up to 128, the rest zeros] and a float32 scale for each row,
+    ``scales`` [rows].  Copies (``copy``, ``pickle``, ``torch.save`` and ``torch.load``) are made of these tensors and
+    checked like new ones."""
+
+    __slots__ = ("shape", "values", "scales")
+
+    def __init__(self, values, scales, shape):
+        rows, cols = shape
+        pitch = -(-cols // 128) * 128
+        if values.dtype is not torch.int8 or tuple(values.shape) != (rows, pitch) or not values.is_contiguous() \
+                or values.data_ptr() % 16:
+            raise ValueError("values must be contiguous int8 [%d][%d], 16-byte aligned" % (rows, pitch))
+        if scales.dtype is not torch.float32 or tuple(scales.shape) != (rows,) or not scales.is_contiguous():
+            raise ValueError("scales must be contiguous float32 [%d]" % rows)
+        if values.device != scales.device:
+            raise ValueError("values and scales must be on one device")
+        self.shape, self.values, self.scales = (rows, cols), values, scales
+
+    def __reduce__(self):
+        return IntegerValues, (self.values, self.scales, self.shape)
+
+    def float(self):
+        """The values that the integers stand for, in float32."""
+        return self.values[:, :self.shape[1]].to(torch.float32) * self.scales[:, None]
+
+
+torch.serialization.add_safe_globals([IntegerValues])
+
+
+def quantize_integers(x):
+    """``x`` in 8-bit integers: for each row the whole numbers nearest to its values' quotients by a scale, a 127th of
+    the largest magnitude."""
+    code, r, c, stride = _rows(x, "x")
+    stream = _stream(x.get_device())
+    out = IntegerValues.__new__(IntegerValues)
+    out.shape = (r, c)
+    out.values = torch.empty((r, -(-c // 128) * 128), dtype=torch.int8, device=x.device)
+    out.scales = torch.empty(r, dtype=torch.float32, device=x.device)
+    check(lib.smx_integer_quantize(x.data_ptr(), stride, code, r, c, out.values.data_ptr(), out.scales.data_ptr(), stream))
+    return out
+
+
+def _check_integers(b, name, k, device):
+    if not isinstance(b, IntegerValues):
+        raise ValueError("%s must be IntegerValues (symmetrix.node_ops.quantize_integers)" % name)
+    if b.shape[1] != k or b.values.get_device() != device:
+        raise ValueError("%s must have as many columns as the other operand, on its device" % name)
+
+
+def integer_product(a, b, dtype=torch.float32):
+    """``a @ b.T`` of two ``IntegerValues``, [m][k] and [n][k]; the sums are exact."""
+    if not isinstance(a, IntegerValues):
+        raise ValueError("a must be IntegerValues (symmetrix.node_ops.quantize_integers)")
+    m, k = a.shape
+    device = a.values.get_device()
+    _check_integers(b, "b", k, device)
+    n = b.shape[0]
+    code = _product_dtype(dtype)
+    stream = _stream(device)
+    out = torch.empty((m, n), dtype=dtype, device=a.values.device)
+    check(lib.smx_integer_product(a.values.data_ptr(), a.scales.data_ptr(), b.values.data_ptr(), b.scales.data_ptr(), m, n, k,
+                                  code, out.data_ptr(), n, stream))
+    return out
+
+
+def integer_linear(x, w, dtype=None):
+    """``x @ w.T`` with x [m][k] brought to 8-bit integers within the call and ``w`` the weights' ``IntegerValues`` [n][k]; in
+    x's type unless ``dtype`` is given."""
+    code, m, k, stride = _rows(x, "x")
+    device = x.get_device()
+    _check_integers(w, "w", k, device)
+    out_code = code if dtype is None else _product_dtype(dtype)
+    current = _stream(device)
+    n = w.shape[0]
+    out = x.new_empty((m, n)) if dtype is None else x.new_empty((m, n), dtype=dtype)
+    size = lib.smx_integer_linear_workspace(m, n, k)
+    room = _workspace(size, x)
+    check(lib.smx_integer_linear(x.data_ptr(), stride, code, w.values.data_ptr(), w.scales.data_ptr(), m, n, k, out_code,
+                                 out.data_ptr(), n, _at(room), size, current))
+    return out
+
+
 __all__ = ["BlockValues", "embed", "embed_gradient", "norm", "residual_norm", "residual_norm_gradient", "quantize",
-           "block_product", "block_linear", "block_linear_gradient"]
+           "block_product", "block_linear", "block_linear_gradient", "RowGroups", "group_rows", "grouped_linear",
+           "grouped_linear_gradient", "gradient_norm", "clip_gradients", "IntegerValues", "quantize_integers",
+           "integer_product", "integer_linear"]
