@@ -216,8 +216,8 @@ SMX_API int32_t smx_clip_gradients(const void* const* tensors, const int64_t* co
 /* ---- products in 8-bit integers ---- */
 
 /* A matrix [rows][cols] in 8-bit integers: values [rows][smx_integer_stride(cols)] (cols rounded up to 128, the rest zeros; 16-byte
- * aligned) and an FP32 scale for each row.  A row's scale is the FP32 quotient of its largest magnitude and 127, at least
- * 2^-126, and a value the whole number nearest to the exact quotient by the scale, ties to even.  A row with an
+ * aligned) and an FP32 scale for each row.  A row's scale is the FP32 product of its largest magnitude and the
+ * FP32 number next to 1/127 (0x1.020408p-7), at least 2^-126, and a value the whole number nearest to the exact quotient by the scale, ties to even.  A row with an
  * infinity or NaN has the scale NaN and zeros. */
 SMX_API int64_t smx_integer_stride(int64_t cols);
 SMX_API int32_t smx_integer_quantize(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int64_t cols, int8_t* values,

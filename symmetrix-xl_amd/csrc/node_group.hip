@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kThreads) k_group_place(const I* __restrict__ 
         __syncthreads();
         // the round's counts, and in the first round where each kind begins
         int total[(kDigits + kThreads - 1) / kThreads];
-        unsigned long long carry = 0;
+        unsigned long long carry = 0, carry_small = 0, carry_large = 0;
 #pragma unroll
         for (int c = 0; c < (kDigits + kThreads - 1) / kThreads; ++c) {
             if (c * kThreads > kinds) break;
@@ -126,13 +126,23 @@ __global__ void __launch_bounds__(kThreads) k_group_place(const I* __restrict__ 
                 sum_before(static_cast<unsigned long long>(all > 0) << 32 | static_cast<unsigned>(all), room, whole) + carry;
             carry += whole;
             const int start = static_cast<int>(seen & 0xffffffffu), index = static_cast<int>(seen >> 32);
-            if (d > kinds) continue;
-            base[d] = start + before;
+            if (d <= kinds) base[d] = start + before;
             if (blockIdx.x > 0) continue;
+            // tiles of 64 and 128 rows, and of 256
+            const auto tiles = [&](int size) { return static_cast<unsigned>((all + size - 1) / size); };
+            unsigned long long small_whole, large_whole;
+            const unsigned long long small =
+                sum_before(static_cast<unsigned long long>(tiles(64)) << 32 | tiles(128), room, small_whole) + carry_small;
+            const unsigned long long large = sum_before(tiles(256), room, large_whole) + carry_large;
+            carry_small += small_whole, carry_large += large_whole;
+            if (d > kinds) continue;
             plan[plan_offsets() + d] = start;
             if (all > 0) {
                 plan[plan_present(kinds) + index] = d;
                 plan[plan_start(kinds) + index] = start;
+                plan[plan_tiles(kinds, 0) + index] = static_cast<int>(small >> 32);
+                plan[plan_tiles(kinds, 1) + index] = static_cast<int>(small & 0xffffffffu);
+                plan[plan_tiles(kinds, 2) + index] = static_cast<int>(large);
             }
         }
         if (at == first && blockIdx.x == 0 && threadIdx.x == 0) {
@@ -140,6 +150,9 @@ __global__ void __launch_bounds__(kThreads) k_group_place(const I* __restrict__ 
             plan[0] = present;
             plan[1] = static_cast<int>(rows), plan[2] = kinds, plan[3] = 0;
             plan[plan_start(kinds) + present] = static_cast<int>(rows);
+            plan[plan_tiles(kinds, 0) + present] = static_cast<int>(carry_small >> 32);
+            plan[plan_tiles(kinds, 1) + present] = static_cast<int>(carry_small & 0xffffffffu);
+            plan[plan_tiles(kinds, 2) + present] = static_cast<int>(carry_large);
             plan[plan_offsets() + kinds + 1] = static_cast<int>(rows);
         }
         __syncthreads();

@@ -22,18 +22,17 @@ void with_types(int dtype, int out_dtype, F&& f) {
     });
 }
 
-// The tile whose rounds over the card take least, for rows spread evenly over the kinds: a unit holds one tile of 256, two of
-// 128 or four of 64.
-int tile_for(i64 kinds, i64 rows, i64 tiles_of_rows_at_least, i64 n) {
+// The tile whose rounds over the card take least, for `units` of rows of a tile: a unit holds one tile of 256, two of 128 or four of
+// 64.  Tiles through registers are of 128 or 64.
+template <class F>
+int tile_for(F&& units, i64 n, bool direct) {
     const auto cost = [&](i64 t, i64 held, double work) {
-        const i64 k = kinds < rows ? kinds : rows, each = (rows + k - 1) / k;
-        i64 units = k * ((each + t - 1) / t);
-        if (units < tiles_of_rows_at_least) units = tiles_of_rows_at_least;
-        const i64 count = units * ((n + t - 1) / t);
+        const i64 count = units(t) * ((n + t - 1) / t);
         return work / static_cast<double>(held) * static_cast<double>((count + held * kComputeUnits - 1) / (held * kComputeUnits));
     };
-    const double c256 = cost(256, 1, 1.0), c128 = cost(128, 2, 1.12 / 2), c64 = cost(64, 4, 1.86 / 4);
-    return c256 <= c128 && c256 <= c64 ? 256 : c128 <= c64 ? 128 : 64;
+    const double c256 = cost(256, 1, 1.0), c128 = cost(128, 2, 1.12), c64 = cost(64, 4, 1.86);
+    if (direct && c256 <= c128 && c256 <= c64) return 256;
+    return c128 <= c64 ? 128 : 64;
 }
 
 // Rows of a kind up to which k_grouped_rows reads its weights straight to registers.
@@ -49,7 +48,8 @@ Cut cut_rows(Way way, i64 rows, i64 kinds, i64 n, bool direct) {
             return c;
         }
     }
-    if (direct) c.tile = tile_for(kinds, rows, 0, n);
+    // (rows spread evenly over the kinds: their numbers are known to the device alone)
+    c.tile = tile_for([&](i64 t) { return k * (((rows + k - 1) / k + t - 1) / t); }, n, direct);
     return c;
 }
 
@@ -58,7 +58,7 @@ i64 run_for(i64 rows, i64 m, i64 n) {
     const i64 tiles = (m + 127) / 128 * ((n + 127) / 128);
     i64 run = (rows * tiles / (2 * kComputeUnits) + 255) / 256 * 256;
     if (run < 512) run = 512;
-    return run < rows ? run : rows > 0 ? rows : 1;
+    return run < rows ? run : rows + 1;  // (not cut)
 }
 
 i64 cuts_of(i64 rows, i64 run) { return rows > 0 ? (rows - 1) / run : 0; }
@@ -101,9 +101,11 @@ void product(Way way, const void* a, i64 a_stride, const void* w, i64 w_stride, 
     p.tokens = static_cast<int>(rows), p.kinds = static_cast<int>(kinds);
     p.n = static_cast<int>(n), p.k = static_cast<int>(k);
     const i64 w_cols = way == Way::Forward ? k : n;
-    const bool direct = wide(a, a_stride, k, sizeof(T)) && wide(w, w_stride, w_cols, sizeof(T)) &&
-                        (kinds == 1 || w_kind * static_cast<i64>(sizeof(T)) % 16 == 0);
-    const Cut cut = cut_rows(way, rows, kinds, n, direct);
+    const bool aligned_rows = wide(a, a_stride, k, sizeof(T)) && wide(w, w_stride, w_cols, sizeof(T)) &&
+                              (kinds == 1 || w_kind * static_cast<i64>(sizeof(T)) % 16 == 0);
+    const bool direct = sizeof(T) == 2 && aligned_rows;
+    Cut cut = cut_rows(way, rows, kinds, n, direct);
+    if (cut.tile == 16) cut.direct = aligned_rows;
     p.tiles_m = 1, p.tiles_n = static_cast<int>((n + cut.tile - 1) / cut.tile);
     require((kinds + 1 + rows / cut.tile) * p.tiles_n < (1LL << 31), "the product has too many tiles");
     launch_grouped<T, O>(p, way, cut, stream);
@@ -119,10 +121,10 @@ void weights_gradient(const void* grad, i64 grad_stride, const void* x, i64 x_st
     p.plan = static_cast<const int*>(plan);
     p.tokens = static_cast<int>(rows), p.kinds = static_cast<int>(kinds);
     p.m = static_cast<int>(m), p.n = static_cast<int>(n);
-    const bool direct = wide(grad, grad_stride, m, sizeof(T)) && wide(x, x_stride, n, sizeof(T));
+    const bool direct = sizeof(T) == 2 && wide(grad, grad_stride, m, sizeof(T)) && wide(x, x_stride, n, sizeof(T));
     const i64 run = run_for(rows, m, n), cuts = cuts_of(rows, run);
     p.run = static_cast<int>(run), p.units = static_cast<int>(kinds + rows / run);
-    Cut cut{128, direct, 0};
+    Cut cut{tile_for([&](i64 t) { return (kinds < rows ? kinds : rows) * ((m + t - 1) / t) + cuts; }, n, direct), direct, 0};
     p.tiles_m = static_cast<int>((m + cut.tile - 1) / cut.tile), p.tiles_n = static_cast<int>((n + cut.tile - 1) / cut.tile);
     require(p.units * static_cast<i64>(p.tiles_m) * p.tiles_n < (1LL << 31), "the product has too many tiles");
     p.partial = static_cast<float*>(workspace);

@@ -5,20 +5,20 @@
 //   by x      dx_t = W_z(t)^T g_t          the same with the weights read across their rows
 //   by W      dW_z = sum over t of g_t x_t^T    a tile: BM x BN of one kind's weights, a run of its rows summed
 //
-// Sizes of the kinds are known to the device alone, so a launch has as many workgroups as the card holds, which walk the
-// tiles that the plan gives.  Tile u of the rows: with the kinds that have rows in order, p the p-th and s(p) its first sorted row, kind
-// p's tiles are numbered from p + s(p) / BM on.  It has at most 1 + s(p + 1) / BM - s(p) / BM of them, so numbers do not
-// meet, and at most one a kind is not used.  Likewise the runs of a kind's rows in the weights' gradient, cut at multiples of
-// `run` sorted rows: kind z's are numbered from z + offset(z) / run on.
+// Sizes of the kinds are known to the device alone, so a launch has as many workgroups as the card holds, which walk the tiles that
+// the plan gives.  The runs of a kind's rows in the weights' gradient are cut at multiples of `run` sorted rows: kind z's are
+// numbered from z + offset(z) / run on, of which it has at most 1 + offset(z + 1) / run - offset(z) / run.
 #pragma once
+
+#include <type_traits>
 
 #include "node_tiles.hpp"
 
 namespace smx {
 namespace node {
 
-// ---- the plan (node_group.hip), in ints: the number of kinds that have rows; offsets; these kinds and their first
-// sorted rows; the order.  Rows of no kind are kind `kinds`. ----
+// ---- the plan (node_group.hip), in ints: the number of kinds that have rows; offsets; these kinds, their first sorted rows
+// and first tiles of 64, 128 and 256 rows; the order.  Rows of no kind are kind `kinds`. ----
 
 constexpr i64 kMostKinds = 4096;
 constexpr i64 kMostRows = (1LL << 31) - 65536;
@@ -27,7 +27,9 @@ inline __host__ __device__ i64 plan_room(i64 kinds) { return (kinds + 5) / 4 * 4
 inline __host__ __device__ i64 plan_offsets() { return 4; }
 inline __host__ __device__ i64 plan_present(i64 kinds) { return 4 + plan_room(kinds); }
 inline __host__ __device__ i64 plan_start(i64 kinds) { return 4 + 2 * plan_room(kinds); }
-inline __host__ __device__ i64 plan_order(i64 kinds) { return 4 + 3 * plan_room(kinds); }
+// the first tile of each of these kinds, and the number of tiles, where tiles have 64 << size rows
+inline __host__ __device__ i64 plan_tiles(i64 kinds, int size) { return 4 + (3 + size) * plan_room(kinds); }
+inline __host__ __device__ i64 plan_order(i64 kinds) { return 4 + 6 * plan_room(kinds); }
 
 enum class Way { Forward, ByRows, ByWeights };
 
@@ -79,214 +81,503 @@ __device__ __forceinline__ void store_outputs(O* row, int j, int n, acc4 v) {
     }
 }
 
-template <class T, class O, Way WAY, bool DIRECT, int BM, int BN, int WM, int WN>
+// Eight neighbouring outputs of two bytes from column j on.
+template <class O>
+__device__ __forceinline__ void store_piece(O* row, int j, int n, i32x4 v) {
+    struct __attribute__((packed, aligned(2))) Words {
+        i32x4 w;
+    };
+    if (j + 8 <= n) {
+        reinterpret_cast<Words*>(row + j)->w = v;
+        return;
+    }
+    asm volatile("" : "+v"(v));  // (apart from the whole store)
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+        if (j + q < n) row[j + q] = __builtin_bit_cast(O, static_cast<std::uint16_t>(static_cast<unsigned>(v[q / 2]) >> (16 * (q % 2))));
+}
+
+// Where a workgroup is: the tile that comes next, found while the one before is multiplied.  Up to 64 kinds are kept in
+// the lanes of each wave, so that a tile is found without a read; more are looked up.
+template <class T, class O, Way WAY, int BM, int BN>
+struct Walk {
+    const Grouped<T, O>& p;
+    const int* order;
+    int count, units, tiles, turn;
+    int base_of, first_of, end_of, kind_of;  // of the lane's kind
+    int row0, rows, i0, j0, kind, slot;  // of the tile: sorted rows; columns of out (by W: rows too); the partial sums' place, or -1
+
+    __device__ __forceinline__ Walk(const Grouped<T, O>& p) : p(p), order(p.plan + plan_order(p.kinds)), turn(blockIdx.x) {
+        const int lane = threadIdx.x % 64;
+        count = WAY == Way::ByWeights ? p.kinds : p.plan[0];
+        const int at = lane < count ? lane : count - 1;
+        base_of = base(at), first_of = starts()[at], end_of = starts()[at + 1];
+        kind_of = WAY == Way::ByWeights ? at : p.plan[plan_present(p.kinds) + at];
+        units = WAY == Way::ByWeights ? p.units : base(count);
+        tiles = units * p.tiles_m * p.tiles_n;
+    }
+    __device__ __forceinline__ const int* starts() const {
+        return p.plan + (WAY == Way::ByWeights ? plan_offsets() : plan_start(p.kinds));
+    }
+    // the first unit of the q-th kind
+    __device__ __forceinline__ int base(int q) const {
+        if constexpr (WAY == Way::ByWeights) return q + starts()[q] / p.run;
+        return p.plan[plan_tiles(p.kinds, BM == 64 ? 0 : BM == 128 ? 1 : 2) + q];
+    }
+    // the kind of unit u: its index, first unit, first and last sorted row and number
+    __device__ __forceinline__ void find(int u, int& at, int& first, int& begin, int& end) {
+        if (count <= 64) {
+            const int lane = threadIdx.x % 64;
+            at = __popcll(__ballot(lane < count && base_of <= u)) - 1;
+            first = __builtin_amdgcn_readlane(base_of, at), kind = __builtin_amdgcn_readlane(kind_of, at);
+            begin = __builtin_amdgcn_readlane(first_of, at), end = __builtin_amdgcn_readlane(end_of, at);
+        } else {
+            at = last_up_to(u, count, [&](int q) { return base(q); });
+            first = base(at), begin = starts()[at], end = starts()[at + 1];
+            kind = WAY == Way::ByWeights ? at : p.plan[plan_present(p.kinds) + at];
+        }
+    }
+    // 0: no tile; 1: one to be summed; 2: one of zeros
+    __device__ __forceinline__ int look() {
+        int at, first, begin, end;
+        if constexpr (WAY == Way::ByWeights) {
+            // the card is on one run of rows at a time, as runs differ in length; each XCD has a part of its tiles, in bands of four
+            const int per = p.tiles_m * p.tiles_n, u = turn / per, id = xcd_remap(turn % per, per);
+            find(u, at, first, begin, end);
+            const int band = id / (4 * p.tiles_n), in = id % (4 * p.tiles_n);
+            const int high = p.tiles_m - 4 * band < 4 ? p.tiles_m - 4 * band : 4;
+            i0 = (4 * band + in % high) * BM, j0 = in / high * BN;
+            const int run = u - at;
+            slot = -1, rows = 0, row0 = begin;
+            if (begin == end) return run == begin / p.run ? 2 : 0;
+            if (run > (end - 1) / p.run) return 0;
+            const int from = run * p.run, to = from + p.run;
+            if (begin < from) slot = 2 * run;
+            else if (end > to) slot = 2 * run + 1;
+            row0 = begin > from ? begin : from;
+            rows = (end < to ? end : to) - row0;
+            return 1;
+        } else {
+            // bands of four units, each column by column: neighbours share rows and weights in an XCD's L2
+            const int id = xcd_remap(turn, tiles);
+            const int band = id / (4 * p.tiles_n), in = id % (4 * p.tiles_n);
+            const int high = units - 4 * band < 4 ? units - 4 * band : 4, u = 4 * band + in % high;
+            find(u, at, first, begin, end);
+            // the kind's rows in as many tiles as it takes, of one height: a tile costs what its rows' products do, and reading the
+            // weights again for a few rows would cost nearly as much as for all (64 kinds of about 512 rows: HEIGHTS)
+            const int tiles_of = (end - begin + BM - 1) / BM, each = ((end - begin + tiles_of - 1) / tiles_of + 15) / 16 * 16;
+            row0 = begin + (u - first) * each;
+            rows = end - row0 < each ? end - row0 : each;
+            j0 = in / high * BN, i0 = 0, slot = -1;
+            return kind == p.kinds || p.k == 0 ? 2 : 1;
+        }
+    }
+    // the outputs' row i of the tile
+    __device__ __forceinline__ O* out_row(int i) const {
+        if constexpr (WAY == Way::ByWeights)
+            return p.out + kind * p.out_kind + (i0 + i) * p.out_stride;
+        else
+            return p.out + order[row0 + i] * p.out_stride;
+    }
+    __device__ __forceinline__ int out_rows() const {
+        if constexpr (WAY == Way::ByWeights) return p.m - i0 < BM ? p.m - i0 : BM;
+        return rows;
+    }
+    // goes on from `turn` to the next tile to be summed; the zeros on the way are written
+    __device__ __forceinline__ bool next() {
+        for (; turn < tiles; turn += gridDim.x) {
+            const int what = look();
+            if (what == 1) return true;
+            if (what == 0) continue;
+            const int high = out_rows();
+            for (int e = threadIdx.x; e < high * (BN / 4); e += blockDim.x)
+                if (const int j = j0 + e % (BN / 4) * 4; j < p.n)
+                    store_outputs(out_row(e / (BN / 4)), j, p.n, acc4{0.0f, 0.0f, 0.0f, 0.0f});
+        }
+        return false;
+    }
+};
+
+// The sums of a workgroup's waves to their rows; `room`: LDS that no one reads any more, for outputs of two bytes.
+template <class T, class O, Way WAY, int BM, int BN, int MF, int NF, class W>
+__device__ __forceinline__ void put_tile(const W& w, const acc4 (&acc)[MF][NF], int wm, int wn, int lane, std::uint8_t* room) {
+    const Grouped<T, O>& p = w.p;
+    const int high = w.out_rows();
+    if constexpr (WAY == Way::ByWeights) {
+        if (w.slot >= 0) {
+#pragma unroll
+            for (int f = 0; f < MF; ++f) {
+                const int i = wm + 16 * f + lane % 16;
+                if (i >= high) continue;
+                float* const row = p.partial + (static_cast<i64>(w.slot) * p.m + w.i0 + i) * p.n;
+#pragma unroll
+                for (int g = 0; g < NF; ++g) store_outputs(row, w.j0 + wn + 16 * g + 4 * (lane / 16), p.n, acc[f][g]);
+            }
+            return;
+        }
+    }
+    if constexpr (sizeof(O) == 4) {
+#pragma unroll
+        for (int f = 0; f < MF; ++f) {
+            const int i = wm + 16 * f + lane % 16;
+            if (i >= high) continue;
+            O* const row = w.out_row(i);
+#pragma unroll
+            for (int g = 0; g < NF; ++g) store_outputs(row, w.j0 + wn + 16 * g + 4 * (lane / 16), p.n, acc[f][g]);
+        }
+    } else {
+        // Values of two bytes are put together in LDS, 16 rows at a time, so that a store is of sixteen bytes a lane and whole lines.
+        constexpr int kRow = 16 * NF * 2 + 16, kLanes = NF * 2;
+        room += threadIdx.x / 64 * 16 * kRow;
+#pragma unroll
+        for (int f = 0; f < MF; ++f) {
+#pragma unroll
+            for (int g = 0; g < NF; ++g) {
+                Pack<O, 4> o;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) o.v[q] = static_cast<O>(acc[f][g][q]);
+                __builtin_memcpy(__builtin_assume_aligned(room + lane % 16 * kRow + (16 * g + 4 * (lane / 16)) * 2, 8), &o, 8);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int q = 0; q < kLanes / 4; ++q) {
+                const int r = lane / kLanes + 64 / kLanes * q, c = lane % kLanes, i = wm + 16 * f + r, j = w.j0 + wn + c * 8;
+                const i32x4 v = *reinterpret_cast<const i32x4*>(room + r * kRow + 16 * c);
+                if (i < high && j < p.n) store_piece(w.out_row(i), j, p.n, v);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+    }
+}
+
+// Rows of 16-bit values that go to LDS by themselves: BM x BN outputs a workgroup, a step of 64 values of the summed axis multiplied
+// while the next one arrives, and the next tile's first while this one's last is multiplied and stored.
+template <class T, class O, Way WAY, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : 2) k_grouped_tiles(Grouped<T, O> p) {
+    static_assert(sizeof(T) == 2);
     constexpr Lie LA = WAY == Way::ByWeights ? Lie::Columns : Lie::Rows, LB = WAY == Way::Forward ? Lie::Rows : Lie::Columns;
-    using A = Step<T, LA, BM>;
-    using B = Step<T, LB, BN>;
-    constexpr int WAVES = WM * WN, NA = A::kPieces / 64 / WAVES, NB = B::kPieces / 64 / WAVES, MF = BM / WM / 16,
-                  NF = BN / WN / 16, kPer = 16 / static_cast<int>(sizeof(T));
-    constexpr unsigned kStage = (BM + BN) * kStepBytes;
-    static_assert(A::kPieces % (64 * WAVES) == 0 && B::kPieces % (64 * WAVES) == 0);
-    static_assert(WAY != Way::ByWeights || BM == BN);
+    constexpr int kValues = 64;
+    using A = Step<LA, BM, kValues>;
+    using B = Step<LB, BN, kValues>;
+    constexpr int WAVES = WM * WN, NA = A::kPieces / 64 / WAVES, NB = B::kPieces / 64 / WAVES, MF = BM / WM / 16, NF = BN / WN / 16;
+    constexpr unsigned kStage = A::kBytes + B::kBytes;
+    static_assert(WAVES * 16 * (16 * NF * 2 + 16) <= kStage && (WAY != Way::ByWeights || BM == BN));
     __shared__ __attribute__((aligned(1024))) std::uint8_t lds[2 * kStage];
     const unsigned lds0 = static_cast<unsigned>(reinterpret_cast<std::uintptr_t>((__attribute__((address_space(3))) std::uint8_t*)lds));
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
-    const int* const order = p.plan + plan_order(p.kinds);
-    const int present = WAY == Way::ByWeights ? 0 : p.plan[0];
-    const int units = WAY == Way::ByWeights ? p.units : present + p.tokens / BM;
-    const int tiles = units * p.tiles_m * p.tiles_n;
+    using Walker = Walk<T, O, WAY, BM, BN>;
+    Walker walk(p);
 
-    // the tile whose steps are being read
-    struct Tile {
-        int row0, rows;  // sorted rows: of the tile, or of the run
-        int i0, j0;
-        int kind, steps, slot;  // slot: of the partial sums, or -1
-    } next;
-    const T* at_a[NA];  // Rows: where the lane's pieces of the first step are
-    const T* at_b[NB];
-    int id_a[NA];  // Columns of gathered rows: the rows of the step to come (a's and b's are the same)
-    const auto steps_of = [](int k) { return (k + A::kValues - 1) / A::kValues; };
-    const auto rows_of_step = [&](int s) {  // by W: asks for the ids of a step's rows, -1 past the end
+    // (the lane's number anew where it is used once a tile: addresses formed of it are not kept across the steps)
+    const auto piece = [&](int q) {
+        int l = lane;
+        asm volatile("" : "+v"(l));
+        return (wave + WAVES * q) * 64 + l;
+    };
+    const T *at_a[NA], *at_b[NB];  // the lane's pieces of the step to come; gathered Columns: the pieces' columns
+    int id[NA];  // the rows of a's pieces, asked for a step ahead: gathered Rows of the next tile, gathered Columns of the next step
+    int values = 0, ids_at = 0;  // of the summed axis, left; by W: the row that the next step's ids begin at
+    int absent = 0;  // rows of the tile: from here on none are multiplied, nor read
+    const auto ask = [&](int from) {
 #pragma unroll
         for (int q = 0; q < NA; ++q) {
-            const int r = s * A::kValues + A::row_at((wave + WAVES * q) * 64 + lane);
-            id_a[q] = r < next.rows ? order[next.row0 + r] : -1;
+            const int r = from + A::row_at(piece(q));
+            id[q] = walk.order[walk.row0 + (r < walk.rows ? r : walk.rows - 1)];
         }
     };
-    const auto turn_to = [&](int turn) {
-        const int id = xcd_remap(turn, tiles);
+    // to the first step of the walk's tile, whose ids are there
+    const auto begin = [&] {
         if constexpr (WAY == Way::ByWeights) {
-            const int per = p.tiles_m * p.tiles_n, u = id / per, in = id % per;
-            const int* const offsets = p.plan + plan_offsets();
-            next.kind = last_up_to(u, p.kinds, [&](int z) { return z + offsets[z] / p.run; });
-            next.i0 = in % p.tiles_m * BM, next.j0 = in / p.tiles_m * BN;
-            const int begin = offsets[next.kind], end = offsets[next.kind + 1], run = u - next.kind;
-            next.slot = -1, next.rows = 0, next.steps = 0, next.row0 = begin;
-            if (begin == end) return run == begin / p.run;
-            if (run > (end - 1) / p.run) return false;
-            const int first = run * p.run, last = first + p.run;
-            if (begin < first) next.slot = 2 * run;
-            else if (end > last) next.slot = 2 * run + 1;
-            next.row0 = begin > first ? begin : first;
-            next.rows = (end < last ? end : last) - next.row0;
-            next.steps = steps_of(next.rows);
-            rows_of_step(0);
-        } else {
-            // bands of four units, each column by column: neighbours share rows and weights in an XCD's L2
-            const int band = id / (4 * p.tiles_n), in = id % (4 * p.tiles_n);
-            const int high = units - 4 * band < 4 ? units - 4 * band : 4, u = 4 * band + in % high;
-            const int* const start = p.plan + plan_start(p.kinds);
-            const int at = last_up_to(u, present, [&](int q) { return q + start[q] / BM; });
-            next.row0 = start[at] + (u - at - start[at] / BM) * BM;
-            next.rows = start[at + 1] - next.row0 < BM ? start[at + 1] - next.row0 : BM;
-            next.kind = p.plan[plan_present(p.kinds) + at];
-            next.j0 = in / high * BN, next.i0 = 0;
-            next.steps = next.kind == p.kinds ? 0 : steps_of(p.k);
-            if (next.rows <= 0) return false;
-            if (next.steps == 0) return true;
+            values = walk.rows, ids_at = 0;
+            // (columns past the row's end are no one's: any place of the row does)
 #pragma unroll
             for (int q = 0; q < NA; ++q) {
-                const int e = (wave + WAVES * q) * 64 + lane, r = A::row_at(e);
-                at_a[q] = p.a + order[next.row0 + (r < next.rows ? r : next.rows - 1)] * p.a_stride;
+                const int c = walk.i0 + A::piece_at(piece(q)) * 8;
+                at_a[q] = p.a + (c < p.m ? c : 0);
             }
-            const T* const w = p.b + next.kind * p.b_kind;
 #pragma unroll
             for (int q = 0; q < NB; ++q) {
-                const int r = B::row_at((wave + WAVES * q) * 64 + lane);
+                const int c = walk.j0 + B::piece_at(piece(q)) * 8;
+                at_b[q] = p.b + (c < p.n ? c : 0);
+            }
+        } else {
+            values = p.k, absent = __builtin_amdgcn_readfirstlane((walk.rows + 15) / 16 * 16);
+#pragma unroll
+            for (int q = 0; q < NA; ++q) at_a[q] = p.a + id[q] * p.a_stride + A::piece_at(piece(q)) * 8;
+            const T* const w = p.b + walk.kind * p.b_kind;
+#pragma unroll
+            for (int q = 0; q < NB; ++q) {
+                const int r = B::row_at(piece(q)), c = B::piece_at(piece(q)) * 8;
                 if constexpr (LB == Lie::Rows)
-                    at_b[q] = w + (next.j0 + r < p.n ? next.j0 + r : p.n - 1) * p.b_stride;
+                    at_b[q] = w + (walk.j0 + r < p.n ? walk.j0 + r : p.n - 1) * p.b_stride + c;
                 else
-                    at_b[q] = w + r * p.b_stride;
+                    at_b[q] = w + r * p.b_stride + (walk.j0 + c < p.n ? walk.j0 + c : 0);
             }
         }
-        return true;
     };
-    // (row and column of a's and b's pieces in memory; rows of no one are NULL)
-    const auto piece_a = [&](int q, int s, const T*& row, i64& c, i64& cols) {
-        const int piece = A::piece_at((wave + WAVES * q) * 64 + lane);
-        if constexpr (LA == Lie::Rows) {
-            row = at_a[q], c = static_cast<i64>(s) * A::kValues + piece * kPer, cols = p.k;
-        } else {
-            row = id_a[q] < 0 ? nullptr : p.a + id_a[q] * p.a_stride;
-            c = next.i0 + piece * kPer, cols = p.m;
-        }
-    };
-    const auto piece_b = [&](int q, int s, const T*& row, i64& c, i64& cols) {
-        const int e = (wave + WAVES * q) * 64 + lane, piece = B::piece_at(e);
-        if constexpr (LB == Lie::Rows) {
-            row = at_b[q], c = static_cast<i64>(s) * B::kValues + piece * kPer, cols = p.k;
-        } else if constexpr (WAY == Way::ByRows) {
-            const int r = s * B::kValues + B::row_at(e);
-            row = r < p.k ? at_b[q] + static_cast<i64>(s) * B::kValues * p.b_stride : nullptr;
-            c = next.j0 + piece * kPer, cols = p.n;
-        } else {
-            row = id_a[q] < 0 ? nullptr : p.b + id_a[q] * p.b_stride;
-            c = next.j0 + piece * kPer, cols = p.n;
-        }
-    };
-    i32x4 held_a[DIRECT ? 1 : NA], held_b[DIRECT ? 1 : NB];
-    // asks for step s of the tile `next`; DIRECT: into the slot, else into registers, which keep() brings there
-    const auto stage = [&](int s, int slot) {
+    // asks for the step to come, and goes on
+    const auto stage = [&](int slot) {
         const unsigned to = __builtin_amdgcn_readfirstlane(lds0 + slot * kStage);
-        const T* row;
-        i64 c, cols;
+        const auto all = [&](auto whole) {
+            constexpr bool WHOLE = decltype(whole)::value;
 #pragma unroll
-        for (int q = 0; q < NA; ++q) {
-            piece_a(q, s, row, c, cols);
-            if constexpr (DIRECT)
-                fetch(row && c < cols ? static_cast<const void*>(row + c) : kNothing, to + (wave + WAVES * q) * 1024);
-            else
-                held_a[q] = row ? settle_piece<T>(load_piece(row, c, cols), c, cols) : i32x4{0, 0, 0, 0};
-        }
+            for (int q = 0; q < NA; ++q) {
+                if (LA == Lie::Rows && 8 * (wave + WAVES * q) >= absent) continue;
+                const T* at = WAY == Way::ByWeights ? at_a[q] + id[q] * p.a_stride : at_a[q];
+                if (!WHOLE) {
+                    const int v = LA == Lie::Rows ? A::piece_at(piece(q)) * 8 : A::row_at(piece(q));
+                    at = v < values ? at : reinterpret_cast<const T*>(kNothing);
+                }
+                fetch(at, to + (wave + WAVES * q) * 1024);
+            }
 #pragma unroll
-        for (int q = 0; q < NB; ++q) {
-            piece_b(q, s, row, c, cols);
-            if constexpr (DIRECT)
-                fetch(row && c < cols ? static_cast<const void*>(row + c) : kNothing,
-                      to + BM * kStepBytes + (wave + WAVES * q) * 1024);
-            else
-                held_b[q] = row ? settle_piece<T>(load_piece(row, c, cols), c, cols) : i32x4{0, 0, 0, 0};
-        }
-        if constexpr (WAY == Way::ByWeights)
-            if (s + 1 < next.steps) rows_of_step(s + 1);
-    };
-    const auto keep = [&](int slot) {
-        if constexpr (!DIRECT) {
-            std::uint8_t* const to = lds + slot * kStage + lane * 16;
+            for (int q = 0; q < NB; ++q) {
+                const T* at = WAY == Way::ByWeights ? at_b[q] + id[q] * p.b_stride : at_b[q];
+                if (!WHOLE) {
+                    const int v = LB == Lie::Rows ? B::piece_at(piece(q)) * 8 : B::row_at(piece(q));
+                    at = v < values ? at : reinterpret_cast<const T*>(kNothing);
+                }
+                fetch(at, to + A::kBytes + (wave + WAVES * q) * 1024);
+            }
+        };
+        if (values >= kValues) all(std::true_type{});
+        else all(std::false_type{});
+        values -= kValues;
+        if constexpr (WAY == Way::ByWeights) {
+            ids_at += kValues;
+            if (values > 0) ask(ids_at);
+        } else {
 #pragma unroll
-            for (int q = 0; q < NA; ++q) *reinterpret_cast<i32x4*>(to + (wave + WAVES * q) * 1024) = held_a[q];
+            for (int q = 0; q < NA; ++q) at_a[q] += kValues;
 #pragma unroll
-            for (int q = 0; q < NB; ++q)
-                *reinterpret_cast<i32x4*>(to + BM * kStepBytes + (wave + WAVES * q) * 1024) = held_b[q];
+            for (int q = 0; q < NB; ++q) at_b[q] += LB == Lie::Rows ? static_cast<i64>(kValues) : kValues * p.b_stride;
         }
     };
 
-    int slot = 0, turn = blockIdx.x;
-    const auto advance = [&](int to) {  // to the next tile that is one, its first step into slot `to`
-        while (turn < tiles && !turn_to(turn)) turn += gridDim.x;
-        if (turn < tiles && next.steps > 0) stage(0, to);
-    };
-    advance(0);
-    if (turn < tiles && next.steps > 0) keep(0);
-    while (turn < tiles) {
-        const Tile now = next;
+    if (!walk.next()) return;
+    ask(0);
+    begin();
+    stage(0);
+    int slot = 0;
+    for (bool more = true; more;) {
+        const Walker now = walk;
+        const int steps = ((WAY == Way::ByWeights ? now.rows : p.k) + kValues - 1) / kValues, high = __builtin_amdgcn_readfirstlane(now.out_rows());
         acc4 acc[MF][NF];
 #pragma unroll
         for (int f = 0; f < MF; ++f)
 #pragma unroll
             for (int g = 0; g < NF; ++g) acc[f][g] = acc4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s = 0; s < now.steps; ++s) {
-            if constexpr (DIRECT) arrived();
+        for (int s = 0; s < steps; ++s) {
+            arrived();
             __syncthreads();  // the step is there, and all have read the one before
             const std::uint8_t* const tile = lds + slot * kStage;
             slot ^= 1;
-            Fragment<T> vb[NF];
+            i32x4 vb[NF];
 #pragma unroll
-            for (int g = 0; g < NF; ++g) vb[g] = B::read(tile + BM * kStepBytes, wn + 16 * g, lane);
-            if (s + 1 < now.steps) {
-                stage(s + 1, slot);
-            } else {
-                turn += gridDim.x;
-                advance(slot);
+            for (int g = 0; g < NF; ++g) vb[g] = B::read(tile + A::kBytes, wn + 16 * g, 0, lane);
+            if (s + 1 < steps) {
+                stage(slot);
+            } else if (more && steps > 1) {
+                begin();
+                stage(slot);
+            }
+            if (s == (steps > 1 ? steps - 2 : 0)) {
+                // the next tile, a step before its first is asked for
+                walk.turn += gridDim.x;
+                more = walk.next();
+                if (more) ask(0);
+                if (more && steps == 1) {
+                    begin();
+                    stage(slot);
+                }
             }
 #pragma unroll
-            for (int f = 0; f < MF; ++f) {
-                const Fragment<T> va = A::read(tile, wm + 16 * f, lane);
+            for (int q = 0; q < 2; ++q) {
+                if (q > 0)
 #pragma unroll
-                for (int g = 0; g < NF; ++g) acc[f][g] = Fragment<T>::multiply(vb[g], va, acc[f][g]);
+                    for (int g = 0; g < NF; ++g) vb[g] = B::read(tile + A::kBytes, wn + 16 * g, q, lane);
+#pragma unroll
+                for (int f = 0; f < MF; ++f) {
+                    if (wm + 16 * f >= high) break;  // no rows of the tile
+                    const i32x4 va = A::read(tile, wm + 16 * f, q, lane);
+#pragma unroll
+                    for (int g = 0; g < NF; ++g) acc[f][g] = Multiply<T>::add(vb[g], va, acc[f][g]);
+                }
             }
-            if (s + 1 < now.steps || (turn < tiles && next.steps > 0)) keep(slot);
-        }
-        if (now.steps == 0) {  // zeros: nothing was read
-            turn += gridDim.x;
-            advance(slot);
-            if (turn < tiles && next.steps > 0) keep(slot);
         }
         settle_products();
-        const int j0 = now.j0 + wn;
+        if constexpr (sizeof(O) == 2) __syncthreads();  // all have read the last step, whose place is used
+        put_tile<T, O, WAY, BM, BN, MF, NF>(now, acc, wm, wn, lane, lds + (slot ^ 1) * kStage);
+    }
+}
+
+// Rows at any alignment, and FP32 ones, which become three bf16 parts on the way: through registers, where a step waits while the one
+// before is multiplied.  Steps are of 64 16-bit or 32 FP32 values; one place in LDS, so that several workgroups share a unit and
+// one brings a step to LDS while another multiplies.
+template <class T, class O, Way WAY, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN, 2) k_grouped_held(Grouped<T, O> p) {
+    constexpr Lie LA = WAY == Way::ByWeights ? Lie::Columns : Lie::Rows, LB = WAY == Way::Forward ? Lie::Rows : Lie::Columns;
+    constexpr bool SPLIT = sizeof(T) == 4;
+    constexpr int kValues = SPLIT ? 32 : 64, PARTS = SPLIT ? 3 : 1, kPer = 16 / static_cast<int>(sizeof(T));
+    using A = Step<LA, BM, kValues>;
+    using B = Step<LB, BN, kValues>;
+    constexpr int THREADS = 64 * WM * WN, NA = BM * kValues / kPer / THREADS, NB = BN * kValues / kPer / THREADS, MF = BM / WM / 16,
+                  NF = BN / WN / 16;
+    static_assert(sizeof(O) == 4 || WM * WN * 16 * (16 * NF * 2 + 16) <= (A::kBytes + B::kBytes) * PARTS);
+    static_assert(WAY != Way::ByWeights || BM == BN);
+    __shared__ __attribute__((aligned(1024))) std::uint8_t lds[(A::kBytes + B::kBytes) * PARTS];
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
+    using Walker = Walk<T, O, WAY, BM, BN>;
+    Walker walk(p);
+
+    // piece q of the lane: sixteen bytes of the memory's rows, side by side for neighbouring lanes
+    const auto row_of = [&](int q, auto rows, int width) {  // width: outer indices
+        return (q * THREADS + static_cast<int>(threadIdx.x)) / (decltype(rows)::value ? kValues / kPer : width / kPer);
+    };
+    const auto column_of = [&](int q, auto rows, int width) {
+        return (q * THREADS + static_cast<int>(threadIdx.x)) % (decltype(rows)::value ? kValues / kPer : width / kPer) * kPer;
+    };
+    constexpr std::bool_constant<LA == Lie::Rows> rows_a{};
+    constexpr std::bool_constant<LB == Lie::Rows> rows_b{};
+    const T *at_a[NA], *at_b[NB];
+    int values = 0, done = 0;  // of the summed axis: left, behind
+    const auto begin = [&] {
+        values = WAY == Way::ByWeights ? walk.rows : p.k, done = 0;
+        if constexpr (WAY != Way::ByWeights) {
 #pragma unroll
-        for (int f = 0; f < MF; ++f) {
-            const int i = wm + 16 * f + lane % 16;
-            if constexpr (WAY == Way::ByWeights) {
-                if (now.i0 + i >= p.m) continue;
-                if (now.slot >= 0) {
-                    float* const row = p.partial + (static_cast<i64>(now.slot) * p.m + now.i0 + i) * p.n;
+            for (int q = 0; q < NA; ++q) {
+                const int r = row_of(q, rows_a, BM);
+                at_a[q] = p.a + walk.order[walk.row0 + (r < walk.rows ? r : walk.rows - 1)] * p.a_stride;
+            }
+            const T* const w = p.b + walk.kind * p.b_kind;
 #pragma unroll
-                    for (int g = 0; g < NF; ++g) store_outputs(row, j0 + 16 * g + 4 * (lane / 16), p.n, acc[f][g]);
-                } else {
-                    O* const row = p.out + now.kind * p.out_kind + (now.i0 + i) * p.out_stride;
-#pragma unroll
-                    for (int g = 0; g < NF; ++g) store_outputs(row, j0 + 16 * g + 4 * (lane / 16), p.n, acc[f][g]);
-                }
-            } else {
-                if (i >= now.rows) continue;
-                O* const row = p.out + order[now.row0 + i] * p.out_stride;
-#pragma unroll
-                for (int g = 0; g < NF; ++g) store_outputs(row, j0 + 16 * g + 4 * (lane / 16), p.n, acc[f][g]);
+            for (int q = 0; q < NB; ++q) {
+                const int r = row_of(q, rows_b, BN);
+                if constexpr (LB == Lie::Rows)
+                    at_b[q] = w + (walk.j0 + r < p.n ? walk.j0 + r : p.n - 1) * p.b_stride;
+                else
+                    at_b[q] = w + r * p.b_stride;
             }
         }
+    };
+    i32x4 held_a[NA], held_b[NB];
+    int id[NA];  // gathered Columns: the rows of the step to come
+    const auto ask = [&] {
+        if constexpr (WAY == Way::ByWeights)
+#pragma unroll
+            for (int q = 0; q < NA; ++q) {
+                const int r = row_of(q, rows_a, BM);
+                id[q] = walk.order[walk.row0 + done + (r < values ? r : values - 1)];
+            }
+    };
+    // column and row's end of a's and b's pieces of the step `at` values on
+    const auto columns_a = [&](int q, int at) {
+        return LA == Lie::Rows ? at + column_of(q, rows_a, BM) : walk.i0 + column_of(q, rows_a, BM);
+    };
+    const auto columns_b = [&](int q, int at) {
+        return LB == Lie::Rows ? at + column_of(q, rows_b, BN) : walk.j0 + column_of(q, rows_b, BN);
+    };
+    const int end_a = WAY == Way::ByWeights ? p.m : p.k, end_b = WAY == Way::Forward ? p.k : p.n;
+    // asks for the step to come, and goes on; pieces that pass a row's end are settled when they are used
+    const auto load = [&] {
+#pragma unroll
+        for (int q = 0; q < NA; ++q) {
+            const T* row;
+            if constexpr (LA == Lie::Rows) row = at_a[q];
+            else row = row_of(q, rows_a, BM) < values ? p.a + id[q] * p.a_stride : nullptr;
+            held_a[q] = row ? load_piece(row, columns_a(q, done), end_a) : i32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int q = 0; q < NB; ++q) {
+            const T* row;
+            if constexpr (LB == Lie::Rows) row = at_b[q];
+            else if constexpr (WAY == Way::ByRows) row = row_of(q, rows_b, BN) < values ? at_b[q] + done * p.b_stride : nullptr;
+            else row = row_of(q, rows_b, BN) < values ? p.b + id[q] * p.b_stride : nullptr;
+            held_b[q] = row ? load_piece(row, columns_b(q, done), end_b) : i32x4{0, 0, 0, 0};
+        }
+        values -= kValues, done += kValues;
+        if (values > 0) ask();
+    };
+    const auto put = [&](auto step, std::uint8_t* to, int row, int column, i32x4 w) {
+        using S = decltype(step);
+        if constexpr (SPLIT) {
+            const FourParts f = split_four(w);
+#pragma unroll
+            for (int k = 0; k < 3; ++k)
+                *reinterpret_cast<uint2*>(to + k * S::kBytes + S::place(row, column / 8, column / 4 % 2)) = f.part[k];
+        } else {
+            *reinterpret_cast<i32x4*>(to + S::place(row, column / 8, 0)) = w;
+        }
+    };
+
+    bool more = walk.next();
+    if (!more) return;
+    begin();
+    ask();
+    load();
+    while (more) {
+        const Walker now = walk;
+        const int steps = ((WAY == Way::ByWeights ? now.rows : p.k) + kValues - 1) / kValues, high = __builtin_amdgcn_readfirstlane(now.out_rows());
+        acc4 acc[MF][NF];
+#pragma unroll
+        for (int f = 0; f < MF; ++f)
+#pragma unroll
+            for (int g = 0; g < NF; ++g) acc[f][g] = acc4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s = 0; s < steps; ++s) {
+            __syncthreads();  // all have read the step before
+#pragma unroll
+            for (int q = 0; q < NA; ++q)
+                put(A{}, lds, row_of(q, rows_a, BM), column_of(q, rows_a, BM),
+                    settle_piece<T>(held_a[q], columns_a(q, done - kValues), end_a));
+#pragma unroll
+            for (int q = 0; q < NB; ++q)
+                put(B{}, lds + A::kBytes * PARTS, row_of(q, rows_b, BN), column_of(q, rows_b, BN),
+                    settle_piece<T>(held_b[q], columns_b(q, done - kValues), end_b));
+            __syncthreads();
+            if (s + 1 == steps) {
+                walk.turn += gridDim.x;
+                more = walk.next();
+                if (more) begin(), ask();
+            }
+            if (more) load();
+            if constexpr (SPLIT) {
+                Parts vb[NF];
+#pragma unroll
+                for (int g = 0; g < NF; ++g)
+#pragma unroll
+                    for (int k = 0; k < 3; ++k)
+                        vb[g].part[k] = B::read(lds + A::kBytes * PARTS + k * B::kBytes, wn + 16 * g, 0, lane);
+#pragma unroll
+                for (int f = 0; f < MF; ++f) {
+                    if (wm + 16 * f >= high) break;
+                    Parts va;
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) va.part[k] = A::read(lds + k * A::kBytes, wm + 16 * f, 0, lane);
+#pragma unroll
+                    for (int g = 0; g < NF; ++g) acc[f][g] = add_parts(vb[g], va, acc[f][g]);
+                }
+            } else {
+                i32x4 vb[NF][2];
+#pragma unroll
+                for (int g = 0; g < NF; ++g)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) vb[g][q] = B::read(lds + A::kBytes, wn + 16 * g, q, lane);
+#pragma unroll
+                for (int f = 0; f < MF; ++f)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        if (wm + 16 * f >= high) break;
+                        const i32x4 va = A::read(lds, wm + 16 * f, q, lane);
+#pragma unroll
+                        for (int g = 0; g < NF; ++g) acc[f][g] = Multiply<T>::add(vb[g][q], va, acc[f][g]);
+                    }
+            }
+        }
+        settle_products();
+        if constexpr (sizeof(O) == 2) __syncthreads();  // all have read the last step, whose place is used
+        put_tile<T, O, WAY, BM, BN, MF, NF>(now, acc, wm, wn, lane, lds);
     }
 }
 
@@ -349,16 +640,22 @@ template <class T, class O>
 void launch_grouped(const Grouped<T, O>& p, Way way, const Cut& cut, hipStream_t stream) {
     const auto tiles = [&](auto w) {
         constexpr Way W = decltype(w)::value;
-        if (!cut.direct) {
-            k_grouped_tiles<T, O, W, false, 128, 128, 2, 2><<<2 * kComputeUnits, 256, 0, stream>>>(p);
-        } else if (cut.tile == 256) {
-            k_grouped_tiles<T, O, W, true, 256, 256, 2, 4><<<kComputeUnits, 512, 0, stream>>>(p);
-        } else if (cut.tile == 128) {
-            k_grouped_tiles<T, O, W, true, 128, 128, 2, 2><<<2 * kComputeUnits, 256, 0, stream>>>(p);
-        } else {
-            k_grouped_tiles<T, O, W, true, 64, 64, 2, 2><<<4 * kComputeUnits, 256, 0, stream>>>(p);
+        if constexpr (sizeof(T) == 2) {
+            if (cut.direct) {
+                switch (cut.tile) {
+                    case 256: k_grouped_tiles<T, O, W, 256, 256, 2, 4><<<kComputeUnits, 512, 0, stream>>>(p); break;
+                    case 128: k_grouped_tiles<T, O, W, 128, 128, 2, 2><<<2 * kComputeUnits, 256, 0, stream>>>(p); break;
+                    default: k_grouped_tiles<T, O, W, 64, 64, 2, 2><<<4 * kComputeUnits, 256, 0, stream>>>(p);
+                }
+                SMX_LAUNCH_CHECK("k_grouped_tiles");
+                return;
+            }
         }
-        SMX_LAUNCH_CHECK("k_grouped_tiles");
+        if (cut.tile == 128)
+            k_grouped_held<T, O, W, 128, 128, 2, 2><<<2 * kComputeUnits, 256, 0, stream>>>(p);
+        else
+            k_grouped_held<T, O, W, 64, 64, 2, 2><<<4 * kComputeUnits, 256, 0, stream>>>(p);
+        SMX_LAUNCH_CHECK("k_grouped_held");
     };
     using std::integral_constant;
     if (way == Way::ByRows) return tiles(integral_constant<Way, Way::ByRows>{});

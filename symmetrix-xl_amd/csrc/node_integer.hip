@@ -1,8 +1,11 @@
 // Products in 8-bit integers with an FP32 scale for each row of both operands (a token of x, a channel of the weights), and the
 // kernel that brings rows to that form.
 //
-//   scale = max(max |x| / 127, 2^-126)     q = the whole number nearest to x / scale, ties to even
+//   scale = max(max |x| * (1 / 127), 2^-126)     q = the whole number nearest to x / scale, ties to even
 //   out[i][j] = scale_a[i] scale_b[j] sum over k of q_a[i][k] q_b[j][k]
+//
+// The scale is one product in FP32 by the FP32 number next to 1/127, which is what torch's x.abs().amax(1) / 127 gives on the card as
+// well: a scale of its own last place would move quotients that lie next to ties.
 //
 // Sums are of 32-bit integers (v_mfma_i32_16x16x64_i8) and exact up to 2^17 terms (2^17 * 127^2 < 2^31); a product is rounded
 // when its sum becomes FP32 and at each scale, by 2^-24 each, and to the output's type.
@@ -35,7 +38,7 @@ __device__ __forceinline__ unsigned four(const float* v, float scale, float inve
 // A row's scale from the largest of its magnitudes' bits (infinities and NaN above all): NaN where the row has one of these.
 __device__ __forceinline__ float scale_of_bits(unsigned top) {
     if (top >= 0x7f800000u) return __builtin_nanf("");
-    const float scale = __uint_as_float(top) / 127.0f;
+    const float scale = __uint_as_float(top) * (1.0f / 127.0f);
     return scale > 0x1p-126f ? scale : 0x1p-126f;
 }
 
@@ -148,8 +151,8 @@ __device__ __forceinline__ void store_scaled(const Integers<O>& p, int i, int j,
 template <class O, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : 2) k_integer_tiles(Integers<O> p) {
     using T = std::int8_t;
-    using A = Step<T, Lie::Rows, BM>;
-    using B = Step<T, Lie::Rows, BN>;
+    using A = Step<Lie::Rows, BM, kStepBytes / 2>;
+    using B = Step<Lie::Rows, BN, kStepBytes / 2>;
     constexpr int WAVES = WM * WN, NA = A::kPieces / 64 / WAVES, NB = B::kPieces / 64 / WAVES, MF = BM / WM / 16,
                   NF = BN / WN / 16;
     constexpr unsigned kStage = (BM + BN) * kStepBytes;
@@ -198,9 +201,11 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : 2) k_integer
             __syncthreads();
             const std::uint8_t* const tile = lds + slot * kStage;
             slot ^= 1;
-            Fragment<T> vb[NF];
+            i32x4 vb[NF][2];
 #pragma unroll
-            for (int g = 0; g < NF; ++g) vb[g] = B::read(tile + BM * kStepBytes, wn + 16 * g, lane);
+            for (int g = 0; g < NF; ++g)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) vb[g][q] = B::read(tile + BM * kStepBytes, wn + 16 * g, q, lane);
             if (s + 1 < steps) {
                 stage(s + 1, slot);
             } else if (turn + static_cast<int>(gridDim.x) < tiles) {
@@ -209,9 +214,13 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : 2) k_integer
             }
 #pragma unroll
             for (int f = 0; f < MF; ++f) {
-                const Fragment<T> va = A::read(tile, wm + 16 * f, lane);
+                i32x4 va[2];
 #pragma unroll
-                for (int g = 0; g < NF; ++g) acc[f][g] = Fragment<T>::multiply(vb[g], va, acc[f][g]);
+                for (int q = 0; q < 2; ++q) va[q] = A::read(tile, wm + 16 * f, q, lane);
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int g = 0; g < NF; ++g) acc[f][g] = Multiply<T>::add(vb[g][q], va[q], acc[f][g]);
             }
         }
         settle_products();

@@ -13,6 +13,7 @@ from symmetrix._native import lib
 
 pytestmark = pytest.mark.gpu
 
+UNIT_127 = float.fromhex("0x1.020408p-7")  # the FP32 number next to 1/127
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 TYPES = [F32, BF16, F16]
 IDS = ["f32", "bf16", "f16"]
@@ -32,7 +33,7 @@ def _by_hand(x):
     """(integers, FP32 scales) of finite x, in float64 on the CPU."""
     x = d(x)
     top = x.abs().amax(1) if x.shape[1] else torch.zeros(len(x)).double()
-    scale = (top / 127).float().clamp(min=2.0 ** -126)
+    scale = (top * UNIT_127).float().clamp(min=2.0 ** -126)  # (a product of two FP32 numbers is exact in float64)
     return torch.round(x / scale.double()[:, None]), scale
 
 
@@ -62,7 +63,7 @@ def test_quantize(gen, r, c, dtype):
 
 def test_ties_zeros_and_small_rows():
     x = torch.zeros(6, 40, device="cuda")
-    x[1] = torch.arange(40) / 2 - 10  # scale 1: halves are ties
+    x[1] = torch.arange(40) / 2 - 10
     x[1, 0], x[2, 3], x[3, 5] = 127.0, 2.0 ** -149, 3.4e38
     x[4] = 2.0 ** -120 * (torch.arange(40) - 20.0)
     x[5] = torch.linspace(-1, 1, 40)
@@ -76,7 +77,7 @@ def test_ties_zeros_and_small_rows():
 def test_quotients_next_to_ties(gen):
     """x at (q + 1/2) scale, and the values beside it: the quotient's own rounding may not move them over the border."""
     top = 1 + torch.rand(200, generator=gen, device="cuda")
-    scale = (top.double() / 127).float()
+    scale = (top.double() * UNIT_127).float()
     tie = (torch.arange(126, device="cuda").double() + 0.5)[None] * scale.double()[:, None]
     tie = tie.float()
     up, down = torch.nextafter(tie, tie + 1), torch.nextafter(tie, tie - 1)
