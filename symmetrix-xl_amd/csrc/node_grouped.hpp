@@ -186,7 +186,10 @@ struct Walk {
     // goes on from `turn` to the next tile to be summed; the zeros on the way are written
     __device__ __forceinline__ bool next() {
         for (; turn < tiles; turn += gridDim.x) {
-            const int what = look();
+            const int what = __builtin_amdgcn_readfirstlane(look());
+            // (looked up or not, all lanes have the same: addresses formed of it are scalar)
+            row0 = __builtin_amdgcn_readfirstlane(row0), rows = __builtin_amdgcn_readfirstlane(rows);
+            kind = __builtin_amdgcn_readfirstlane(kind), slot = __builtin_amdgcn_readfirstlane(slot);
             if (what == 1) return true;
             if (what == 0) continue;
             const int high = out_rows();
@@ -276,14 +279,46 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : 2) k_grouped
         return (wave + WAVES * q) * 64 + l;
     };
     const T *at_a[NA], *at_b[NB];  // the lane's pieces of the step to come; gathered Columns: the pieces' columns
-    int id[NA];  // the rows of a's pieces, asked for a step ahead: gathered Rows of the next tile, gathered Columns of the next step
+    // The rows of a's pieces, asked for a step ahead: gathered Rows of the next tile, and gathered Columns of the next step.  The rows of
+    // these are a few for each fetch of a wave, so they are read as scalars, and picked by the lanes when the step's
+    // products are on their way: a lane's own reads would be waited for with the step's (8192 cubed: 1,409 us, 1,055 so).
+    constexpr int kIds = WAY == Way::ByWeights ? 64 / A::kRowPieces : 1;
+    using Scalars = const __attribute__((address_space(4))) int*;
+    const Scalars scalars = (Scalars)(reinterpret_cast<std::uintptr_t>(walk.order));
+    int id[NA];
+    struct Asked {
+        int v[NA][kIds];
+    };
     int values = 0, ids_at = 0;  // of the summed axis, left; by W: the row that the next step's ids begin at
     int absent = 0;  // rows of the tile: from here on none are multiplied, nor read
     const auto ask = [&](int from) {
+        Asked to;
+#pragma unroll
+        for (int q = 0; q < NA; ++q)
+#pragma unroll
+            for (int i = 0; i < kIds; ++i) {
+                const int r = from + (wave + WAVES * q) * kIds + i;
+                to.v[q][i] = scalars[walk.row0 + (r < walk.rows ? r : walk.rows - 1)];
+            }
+        return to;
+    };
+    const auto pick = [&](const Asked& of) {
 #pragma unroll
         for (int q = 0; q < NA; ++q) {
-            const int r = from + A::row_at(piece(q));
-            id[q] = walk.order[walk.row0 + (r < walk.rows ? r : walk.rows - 1)];
+            id[q] = of.v[q][0];
+#pragma unroll
+            for (int i = 1; i < kIds; ++i) id[q] = lane / A::kRowPieces == i ? of.v[q][i] : id[q];
+        }
+    };
+    const auto ask_first = [&] {
+        if constexpr (WAY == Way::ByWeights) {
+            pick(ask(0));
+        } else {
+#pragma unroll
+            for (int q = 0; q < NA; ++q) {
+                const int r = A::row_at(piece(q));
+                id[q] = walk.order[walk.row0 + (r < walk.rows ? r : walk.rows - 1)];
+            }
         }
     };
     // to the first step of the walk's tile, whose ids are there
@@ -346,7 +381,6 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : 2) k_grouped
         values -= kValues;
         if constexpr (WAY == Way::ByWeights) {
             ids_at += kValues;
-            if (values > 0) ask(ids_at);
         } else {
 #pragma unroll
             for (int q = 0; q < NA; ++q) at_a[q] += kValues;
@@ -356,9 +390,11 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : 2) k_grouped
     };
 
     if (!walk.next()) return;
-    ask(0);
+    ask_first();
     begin();
     stage(0);
+    if constexpr (WAY == Way::ByWeights)
+        if (values > 0) pick(ask(ids_at));
     int slot = 0;
     for (bool more = true; more;) {
         const Walker now = walk;
@@ -373,9 +409,11 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : 2) k_grouped
             __syncthreads();  // the step is there, and all have read the one before
             const std::uint8_t* const tile = lds + slot * kStage;
             slot ^= 1;
-            i32x4 vb[NF];
+            const auto read_a = [&](int f, int q) { return A::read(tile, wm + 16 * f, q, lane); };
+            const auto read_b = [&](int g, int q) { return B::read(tile + A::kBytes, wn + 16 * g, q, lane); };
+            i32x4 vb[NF], va = read_a(0, 0);
 #pragma unroll
-            for (int g = 0; g < NF; ++g) vb[g] = B::read(tile + A::kBytes, wn + 16 * g, 0, lane);
+            for (int g = 0; g < NF; ++g) vb[g] = read_b(g, 0);
             if (s + 1 < steps) {
                 stage(slot);
             } else if (more && steps > 1) {
@@ -386,25 +424,34 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : 2) k_grouped
                 // the next tile, a step before its first is asked for
                 walk.turn += gridDim.x;
                 more = walk.next();
-                if (more) ask(0);
+                if (more) ask_first();
                 if (more && steps == 1) {
                     begin();
                     stage(slot);
                 }
             }
+            Asked asked;
+            // each fragment is read while the one before is multiplied; those without rows of the tile are left out
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                if (q > 0)
+                if (q > 0) {
+                    if constexpr (WAY == Way::ByWeights)
+                        if (values > 0) asked = ask(ids_at);
+                    va = read_a(0, q);
 #pragma unroll
-                    for (int g = 0; g < NF; ++g) vb[g] = B::read(tile + A::kBytes, wn + 16 * g, q, lane);
+                    for (int g = 0; g < NF; ++g) vb[g] = read_b(g, q);
+                }
 #pragma unroll
                 for (int f = 0; f < MF; ++f) {
-                    if (wm + 16 * f >= high) break;  // no rows of the tile
-                    const i32x4 va = A::read(tile, wm + 16 * f, q, lane);
+                    if (wm + 16 * f >= high) break;
+                    const i32x4 now_a = va;
+                    if (f + 1 < MF) va = read_a(f + 1, q);
 #pragma unroll
-                    for (int g = 0; g < NF; ++g) acc[f][g] = Multiply<T>::add(vb[g], va, acc[f][g]);
+                    for (int g = 0; g < NF; ++g) acc[f][g] = Multiply<T>::add(vb[g], now_a, acc[f][g]);
                 }
             }
+            if constexpr (WAY == Way::ByWeights)
+                if (values > 0) pick(asked);
         }
         settle_products();
         if constexpr (sizeof(O) == 2) __syncthreads();  // all have read the last step, whose place is used
