@@ -61,6 +61,8 @@ __global__ void __launch_bounds__(kThreads) k_group_place(const I* __restrict__ 
     __shared__ __attribute__((aligned(16))) std::uint16_t count[kWaves][kDigits];  // of a round: of each wave, then of the waves before
     __shared__ int base[kDigits];
     __shared__ unsigned long long room[kWaves];
+    __shared__ int most;  // rows of a kind
+    if (threadIdx.x == 0) most = 0;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     int* const order = plan + plan_order(kinds);
     const i64 first = blockIdx.x * tile, last = first + tile < rows ? first + tile : rows;
@@ -137,6 +139,7 @@ __global__ void __launch_bounds__(kThreads) k_group_place(const I* __restrict__ 
             carry_small += small_whole, carry_large += large_whole;
             if (d > kinds) continue;
             plan[plan_offsets() + d] = start;
+            if (d < kinds) atomicMax(&most, all);
             if (all > 0) {
                 plan[plan_present(kinds) + index] = d;
                 plan[plan_start(kinds) + index] = start;
@@ -145,17 +148,17 @@ __global__ void __launch_bounds__(kThreads) k_group_place(const I* __restrict__ 
                 plan[plan_tiles(kinds, 2) + index] = static_cast<int>(large);
             }
         }
+        __syncthreads();
         if (at == first && blockIdx.x == 0 && threadIdx.x == 0) {
             const int present = static_cast<int>(carry >> 32);
             plan[0] = present;
-            plan[1] = static_cast<int>(rows), plan[2] = kinds, plan[3] = 0;
+            plan[1] = static_cast<int>(rows), plan[2] = kinds, plan[3] = most;
             plan[plan_start(kinds) + present] = static_cast<int>(rows);
             plan[plan_tiles(kinds, 0) + present] = static_cast<int>(carry_small >> 32);
             plan[plan_tiles(kinds, 1) + present] = static_cast<int>(carry_small & 0xffffffffu);
             plan[plan_tiles(kinds, 2) + present] = static_cast<int>(carry_large);
             plan[plan_offsets() + kinds + 1] = static_cast<int>(rows);
         }
-        __syncthreads();
 #pragma unroll
         for (int k = 0; k < kPerLane; ++k)
             if (in[k])

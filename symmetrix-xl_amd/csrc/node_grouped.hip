@@ -22,23 +22,39 @@ void with_types(int dtype, int out_dtype, F&& f) {
     });
 }
 
-// The tile whose rounds over the card take least, for `units` of rows of a tile: a unit holds one tile of 256, two of 128 or four of
-// 64.  Tiles through registers are of 128 or 64.
+// What tiles of 256, 128 and 64 cost, in us: a step of 64 values of the summed axis with `filled` tiles on a unit, which holds one,
+// two or four of them, and what a tile takes beside its steps (measured: 8192 cubed, and 2,048 rows of 2,048 values).
+constexpr int kSizes[3] = {256, 128, 64};
+int held(int tile) { return 65536 / (tile * tile) < 1 ? 1 : tile == 128 ? 2 : 4; }
+double step_time(int tile, i64 filled) {
+    if (tile == 256) return 1.9;
+    if (tile == 128) return 1.15;
+    return 0.5 + 0.19 * static_cast<double>(filled < 4 ? filled : 4);
+}
+double tile_time(int tile, i64 steps, i64 filled) {
+    return static_cast<double>(steps) * step_time(tile, filled) + (tile == 256 ? 4.0 : tile == 128 ? 2.5 : 2.0);
+}
+
+i64 ceil_of(i64 a, i64 b) { return (a + b - 1) / b; }
+
+// The tile that takes least by these for `units(tile)` of rows and n columns; tiles through registers are of 128 or 64.
 template <class F>
-int tile_for(F&& units, i64 n, bool direct) {
-    const auto cost = [&](i64 t, i64 held, double work) {
-        const i64 count = units(t) * ((n + t - 1) / t);
-        return work / static_cast<double>(held) * static_cast<double>((count + held * kComputeUnits - 1) / (held * kComputeUnits));
-    };
-    const double c256 = cost(256, 1, 1.0), c128 = cost(128, 2, 1.12), c64 = cost(64, 4, 1.86);
-    if (direct && c256 <= c128 && c256 <= c64) return 256;
-    return c128 <= c64 ? 128 : 64;
+int tile_for(F&& units, i64 n, i64 k, bool largest) {
+    int best = 64;
+    double least = 1e300;
+    for (const int t : kSizes) {
+        if (t == 256 && !largest) continue;
+        const i64 count = units(t) * ceil_of(n, t), card = held(t) * kComputeUnits;
+        const double cost = static_cast<double>(ceil_of(count, card)) * tile_time(t, ceil_of(k, 64), ceil_of(count, kComputeUnits));
+        if (cost < least) least = cost, best = t;
+    }
+    return best;
 }
 
 // Rows of a kind up to which k_grouped_rows reads its weights straight to registers.
 constexpr i64 kFewRows = 16;
 
-Cut cut_rows(Way way, i64 rows, i64 kinds, i64 n, bool direct) {
+Cut cut_rows(Way way, i64 rows, i64 kinds, i64 n, i64 inner, bool direct, bool split) {
     Cut c{128, direct, 0};
     const i64 k = kinds < rows ? kinds : rows;
     if (way == Way::Forward && rows <= k * kFewRows) {
@@ -49,19 +65,42 @@ Cut cut_rows(Way way, i64 rows, i64 kinds, i64 n, bool direct) {
         }
     }
     // (rows spread evenly over the kinds: their numbers are known to the device alone)
-    c.tile = tile_for([&](i64 t) { return k * (((rows + k - 1) / k + t - 1) / t); }, n, direct);
+    c.tile = tile_for([&](i64 t) { return k * ceil_of(ceil_of(rows, k), t); }, n, inner, direct && !split);
     return c;
 }
 
-// Rows summed together in the weights' gradient: as many as leave two tiles of 128 to each unit if one kind had them all.
-i64 run_for(i64 rows, i64 m, i64 n) {
-    const i64 tiles = (m + 127) / 128 * ((n + 127) / 128);
-    i64 run = (rows * tiles / (2 * kComputeUnits) + 255) / 256 * 256;
-    if (run < 512) run = 512;
-    return run < rows ? run : rows + 1;  // (not cut)
-}
+// The weights' gradient of m x n a kind: the tile, the units of rows that the card holds at once, and the least run, so that no more
+// than two rounds are cut (run_of): 0 where that is all rows.
+struct Runs {
+    int tile;
+    i64 round, least, slots;
+};
 
-i64 cuts_of(i64 rows, i64 run) { return rows > 0 ? (rows - 1) / run : 0; }
+Runs runs_for(i64 rows, i64 kinds, i64 m, i64 n, bool largest) {
+    Runs best{};
+    double least = 1e300;
+    const i64 k = kinds < rows ? kinds : rows < 1 ? 1 : rows, each = ceil_of(rows < 1 ? 1 : rows, k);
+    for (const int t : kSizes) {
+        if (t == 256 && !largest) continue;
+        const i64 per = ceil_of(m, t) * ceil_of(n, t), card = held(t) * kComputeUnits, round = per < card ? card / per : 1;
+        i64 run = ceil_of(rows, 2 * round);
+        run = run < 512 ? 512 : ceil_of(run, 64) * 64;
+        // (rows spread evenly: cut into two rounds at most, or not)
+        const auto cost_of = [&](i64 rounds, i64 r) {
+            return static_cast<double>(rounds) * tile_time(t, ceil_of(r, 64), ceil_of(k * per, kComputeUnits));
+        };
+        double cost = cost_of(ceil_of(k * per, card), each);
+        if (round > k) {
+            const i64 cut = ceil_of(rows, round - k) < run ? run : ceil_of(rows, round - k);
+            if (const double c = cost_of(1, cut) + 10; cut < each && c < cost) cost = c;
+        }
+        if (cost < least) {
+            least = cost;
+            best = {t, round, run < rows ? run : 0, run < rows ? 2 * (rows / run + 1) : 0};
+        }
+    }
+    return best;
+}
 
 bool wide(const void* p, i64 stride, i64 cols, int size) {
     return aligned(p, 16) && stride * size % 16 == 0 && cols * size % 16 == 0;
@@ -72,6 +111,8 @@ void check_kinds(i64 rows, i64 kinds) {
     require(kinds >= 1, "there must be a kind at least");
     if (kinds > kMostKinds) throw std::domain_error("products by kind take up to 4096 kinds");
 }
+
+bool widths_ok(i64 a, i64 b) { return a <= (1 << 24) && b <= (1 << 24); }
 
 void check_width(i64 v, const char* what) {
     if (v < 0 || v > (1 << 24)) throw std::invalid_argument(std::string(what) + " must be in [0, 2^24]");
@@ -101,11 +142,9 @@ void product(Way way, const void* a, i64 a_stride, const void* w, i64 w_stride, 
     p.tokens = static_cast<int>(rows), p.kinds = static_cast<int>(kinds);
     p.n = static_cast<int>(n), p.k = static_cast<int>(k);
     const i64 w_cols = way == Way::Forward ? k : n;
-    const bool aligned_rows = wide(a, a_stride, k, sizeof(T)) && wide(w, w_stride, w_cols, sizeof(T)) &&
-                              (kinds == 1 || w_kind * static_cast<i64>(sizeof(T)) % 16 == 0);
-    const bool direct = sizeof(T) == 2 && aligned_rows;
-    Cut cut = cut_rows(way, rows, kinds, n, direct);
-    if (cut.tile == 16) cut.direct = aligned_rows;
+    const bool direct = wide(a, a_stride, k, sizeof(T)) && wide(w, w_stride, w_cols, sizeof(T)) &&
+                        (kinds == 1 || w_kind * static_cast<i64>(sizeof(T)) % 16 == 0);
+    const Cut cut = cut_rows(way, rows, kinds, n, k, direct, sizeof(T) == 4);
     p.tiles_m = 1, p.tiles_n = static_cast<int>((n + cut.tile - 1) / cut.tile);
     require((kinds + 1 + rows / cut.tile) * p.tiles_n < (1LL << 31), "the product has too many tiles");
     launch_grouped<T, O>(p, way, cut, stream);
@@ -121,18 +160,22 @@ void weights_gradient(const void* grad, i64 grad_stride, const void* x, i64 x_st
     p.plan = static_cast<const int*>(plan);
     p.tokens = static_cast<int>(rows), p.kinds = static_cast<int>(kinds);
     p.m = static_cast<int>(m), p.n = static_cast<int>(n);
-    const bool direct = sizeof(T) == 2 && wide(grad, grad_stride, m, sizeof(T)) && wide(x, x_stride, n, sizeof(T));
-    const i64 run = run_for(rows, m, n), cuts = cuts_of(rows, run);
-    p.run = static_cast<int>(run), p.units = static_cast<int>(kinds + rows / run);
-    Cut cut{tile_for([&](i64 t) { return (kinds < rows ? kinds : rows) * ((m + t - 1) / t) + cuts; }, n, direct), direct, 0};
+    const bool direct = wide(grad, grad_stride, m, sizeof(T)) && wide(x, x_stride, n, sizeof(T));
+    const Runs runs = runs_for(rows, kinds, m, n, direct && sizeof(T) == 2);
+    p.round = static_cast<int>(runs.round), p.least = static_cast<int>(runs.least);
+    const Cut cut{runs.tile, direct, 0};
     p.tiles_m = static_cast<int>((m + cut.tile - 1) / cut.tile), p.tiles_n = static_cast<int>((n + cut.tile - 1) / cut.tile);
-    require(p.units * static_cast<i64>(p.tiles_m) * p.tiles_n < (1LL << 31), "the product has too many tiles");
+    require((kinds + (runs.least ? rows / runs.least : 0)) * p.tiles_m * p.tiles_n < (1LL << 31), "the product has too many tiles");
     p.partial = static_cast<float*>(workspace);
     launch_grouped<T, O>(p, Way::ByWeights, cut, stream);
-    if (cuts > 0) {
-        const i64 blocks = (m * n + 1023) / 1024;
-        k_grouped_join<O><<<dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096), static_cast<unsigned>(cuts)), 256, 0, stream>>>(
-            p.partial, p.plan, p.kinds, p.run, p.m, p.n, p.out, out_stride, out_kind);
+    if (runs.least > 0) {
+        Grouped<O, O> j{};
+        j.out = p.out, j.out_stride = out_stride, j.out_kind = out_kind;
+        j.plan = p.plan, j.tokens = p.tokens, j.kinds = p.kinds, j.m = p.m, j.n = p.n;
+        j.round = p.round, j.least = p.least, j.partial = p.partial;
+        const i64 blocks = ceil_of(m * n, 1024), cuts = (rows - 1) / runs.least;
+        k_grouped_join<O><<<dim3(static_cast<unsigned>(blocks < 1024 ? blocks : 1024), static_cast<unsigned>(cuts < 64 ? cuts : 64)),
+                            256, 0, stream>>>(j);
         SMX_LAUNCH_CHECK("k_grouped_join");
     }
 }
@@ -186,8 +229,10 @@ int32_t smx_grouped_linear_by_rows(const void* grad, int64_t grad_stride, int32_
 
 int64_t smx_grouped_linear_by_weights_workspace(int64_t rows, int64_t num_types, int64_t inputs, int64_t outputs) {
     if (rows <= 0 || num_types <= 0 || inputs <= 0 || outputs <= 0) return 0;
-    const i64 cuts = cuts_of(rows, run_for(rows, outputs, inputs));
-    return cuts > 0 ? 4 * 2 * (cuts + 1) * outputs * inputs : 0;
+    if (!widths_ok(inputs, outputs)) return 0;
+    // (for rows at any alignment)
+    const i64 a = runs_for(rows, num_types, outputs, inputs, true).slots, b = runs_for(rows, num_types, outputs, inputs, false).slots;
+    return 4 * (a > b ? a : b) * outputs * inputs;
 }
 
 int32_t smx_grouped_linear_by_weights(const void* grad, int64_t grad_stride, const void* x, int64_t x_stride, int32_t dtype,

@@ -17,7 +17,8 @@
 namespace smx {
 namespace node {
 
-// ---- the plan (node_group.hip), in ints: the number of kinds that have rows; offsets; these kinds, their first sorted rows
+// ---- the plan (node_group.hip), in ints: the number of kinds that have rows, that of all rows, of
+// kinds and of the rows of the largest; offsets; these kinds, their first sorted rows
 // and first tiles of 64, 128 and 256 rows; the order.  Rows of no kind are kind `kinds`. ----
 
 constexpr i64 kMostKinds = 4096;
@@ -47,9 +48,28 @@ struct Grouped {
     int n;  // columns of out
     int k;  // summed (by W: the rows are)
     int tiles_m, tiles_n;
-    int run, units;   // by W
+    int round, least;  // by W: units that the card holds at once, and the least run (0: kinds are not cut)
     float* partial;  // by W, [2 per run][m][n], where kinds may be cut
 };
+
+// Rows summed together in the weights' gradient, from the kinds' sizes, which the device has: a kind in one run where that takes no
+// longer than a round or two of runs that fill the card, whose parts have to be joined (about 500 rows' time).  20,000 rows of 10 kinds
+// are not cut, 30,000 of 2 in 59 runs.
+__device__ __forceinline__ int run_of(const int* plan, int tokens, int round, int least) {
+    const int count = plan[0], most = plan[3], whole = tokens + 1;
+    if (least == 0) return whole;
+    int run = whole;
+    i64 best = static_cast<i64>((count + round - 1) / round) * most;
+    for (int r = 1; r <= 2; ++r) {
+        const int units = r * round - count;
+        if (units <= 0) continue;
+        int each = ((tokens + units - 1) / units + 63) / 64 * 64;
+        each = each < least ? least : each;
+        const i64 cost = static_cast<i64>(r) * each + 512;
+        if (each < most && cost < best) best = cost, run = each;
+    }
+    return run;
+}
 
 // the last of the `count` ascending keys (key(0) <= u) that is <= u; by a whole wave
 template <class F>
@@ -103,17 +123,18 @@ template <class T, class O, Way WAY, int BM, int BN>
 struct Walk {
     const Grouped<T, O>& p;
     const int* order;
-    int count, units, tiles, turn;
+    int count, units, tiles, turn, run;
     int base_of, first_of, end_of, kind_of;  // of the lane's kind
     int row0, rows, i0, j0, kind, slot;  // of the tile: sorted rows; columns of out (by W: rows too); the partial sums' place, or -1
 
     __device__ __forceinline__ Walk(const Grouped<T, O>& p) : p(p), order(p.plan + plan_order(p.kinds)), turn(blockIdx.x) {
         const int lane = threadIdx.x % 64;
         count = WAY == Way::ByWeights ? p.kinds : p.plan[0];
+        run = WAY == Way::ByWeights ? __builtin_amdgcn_readfirstlane(run_of(p.plan, p.tokens, p.round, p.least)) : 0;
         const int at = lane < count ? lane : count - 1;
         base_of = base(at), first_of = starts()[at], end_of = starts()[at + 1];
         kind_of = WAY == Way::ByWeights ? at : p.plan[plan_present(p.kinds) + at];
-        units = WAY == Way::ByWeights ? p.units : base(count);
+        units = WAY == Way::ByWeights ? p.kinds + p.tokens / run : base(count);
         tiles = units * p.tiles_m * p.tiles_n;
     }
     __device__ __forceinline__ const int* starts() const {
@@ -121,7 +142,7 @@ struct Walk {
     }
     // the first unit of the q-th kind
     __device__ __forceinline__ int base(int q) const {
-        if constexpr (WAY == Way::ByWeights) return q + starts()[q] / p.run;
+        if constexpr (WAY == Way::ByWeights) return q + starts()[q] / run;
         return p.plan[plan_tiles(p.kinds, BM == 64 ? 0 : BM == 128 ? 1 : 2) + q];
     }
     // the kind of unit u: its index, first unit, first and last sorted row and number
@@ -147,13 +168,13 @@ struct Walk {
             const int band = id / (4 * p.tiles_n), in = id % (4 * p.tiles_n);
             const int high = p.tiles_m - 4 * band < 4 ? p.tiles_m - 4 * band : 4;
             i0 = (4 * band + in % high) * BM, j0 = in / high * BN;
-            const int run = u - at;
+            const int nth = u - at;
             slot = -1, rows = 0, row0 = begin;
-            if (begin == end) return run == begin / p.run ? 2 : 0;
-            if (run > (end - 1) / p.run) return 0;
-            const int from = run * p.run, to = from + p.run;
-            if (begin < from) slot = 2 * run;
-            else if (end > to) slot = 2 * run + 1;
+            if (begin == end) return nth == begin / run ? 2 : 0;
+            if (nth > (end - 1) / run) return 0;
+            const int from = nth * run, to = from + run;
+            if (begin < from) slot = 2 * nth;
+            else if (end > to) slot = 2 * nth + 1;
             row0 = begin > from ? begin : from;
             rows = (end < to ? end : to) - row0;
             return 1;
@@ -462,8 +483,8 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : 2) k_grouped
 // Rows at any alignment, and FP32 ones, which become three bf16 parts on the way: through registers, where a step waits while the one
 // before is multiplied.  Steps are of 64 16-bit or 32 FP32 values; one place in LDS, so that several workgroups share a unit and
 // one brings a step to LDS while another multiplies.
-template <class T, class O, Way WAY, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN, 2) k_grouped_held(Grouped<T, O> p) {
+template <class T, class O, Way WAY, bool ALIGNED, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN, BM == 128 ? 2 : 4) k_grouped_held(Grouped<T, O> p) {
     constexpr Lie LA = WAY == Way::ByWeights ? Lie::Columns : Lie::Rows, LB = WAY == Way::Forward ? Lie::Rows : Lie::Columns;
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int kValues = SPLIT ? 32 : 64, PARTS = SPLIT ? 3 : 1, kPer = 16 / static_cast<int>(sizeof(T));
@@ -488,7 +509,7 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) k_grouped_held(Grouped<T, O> 
     };
     constexpr std::bool_constant<LA == Lie::Rows> rows_a{};
     constexpr std::bool_constant<LB == Lie::Rows> rows_b{};
-    const T *at_a[NA], *at_b[NB];
+    const T *at_a[NA], *at_b[NB];  // the rows of the lane's pieces; ALIGNED: the pieces of the step to come
     int values = 0, done = 0;  // of the summed axis: left, behind
     const auto begin = [&] {
         values = WAY == Way::ByWeights ? walk.rows : p.k, done = 0;
@@ -497,15 +518,19 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) k_grouped_held(Grouped<T, O> 
             for (int q = 0; q < NA; ++q) {
                 const int r = row_of(q, rows_a, BM);
                 at_a[q] = p.a + walk.order[walk.row0 + (r < walk.rows ? r : walk.rows - 1)] * p.a_stride;
+                if constexpr (ALIGNED) at_a[q] += column_of(q, rows_a, BM);
             }
             const T* const w = p.b + walk.kind * p.b_kind;
 #pragma unroll
             for (int q = 0; q < NB; ++q) {
-                const int r = row_of(q, rows_b, BN);
-                if constexpr (LB == Lie::Rows)
+                const int r = row_of(q, rows_b, BN), c = column_of(q, rows_b, BN);
+                if constexpr (LB == Lie::Rows) {
                     at_b[q] = w + (walk.j0 + r < p.n ? walk.j0 + r : p.n - 1) * p.b_stride;
-                else
+                    if constexpr (ALIGNED) at_b[q] += c;
+                } else {
                     at_b[q] = w + r * p.b_stride;
+                    if constexpr (ALIGNED) at_b[q] += walk.j0 + c < p.n ? walk.j0 + c : 0;
+                }
             }
         }
     };
@@ -529,23 +554,57 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) k_grouped_held(Grouped<T, O> 
     const int end_a = WAY == Way::ByWeights ? p.m : p.k, end_b = WAY == Way::Forward ? p.k : p.n;
     // asks for the step to come, and goes on; pieces that pass a row's end are settled when they are used
     const auto load = [&] {
+        if constexpr (ALIGNED) {
+            const auto all = [&](auto whole) {
+                constexpr bool WHOLE = decltype(whole)::value;
+                const auto from = [&](const T* at, int v) {
+                    return load_sixteen(WHOLE || v < values ? static_cast<const void*>(at) : kNothing);
+                };
 #pragma unroll
-        for (int q = 0; q < NA; ++q) {
-            const T* row;
-            if constexpr (LA == Lie::Rows) row = at_a[q];
-            else row = row_of(q, rows_a, BM) < values ? p.a + id[q] * p.a_stride : nullptr;
-            held_a[q] = row ? load_piece(row, columns_a(q, done), end_a) : i32x4{0, 0, 0, 0};
-        }
+                for (int q = 0; q < NA; ++q) {
+                    const int r = row_of(q, rows_a, BM), c = column_of(q, rows_a, BM);
+                    if constexpr (LA == Lie::Rows) held_a[q] = from(at_a[q], c);
+                    else held_a[q] = from(p.a + id[q] * p.a_stride + (walk.i0 + c < p.m ? walk.i0 + c : 0), r);
+                }
 #pragma unroll
-        for (int q = 0; q < NB; ++q) {
-            const T* row;
-            if constexpr (LB == Lie::Rows) row = at_b[q];
-            else if constexpr (WAY == Way::ByRows) row = row_of(q, rows_b, BN) < values ? at_b[q] + done * p.b_stride : nullptr;
-            else row = row_of(q, rows_b, BN) < values ? p.b + id[q] * p.b_stride : nullptr;
-            held_b[q] = row ? load_piece(row, columns_b(q, done), end_b) : i32x4{0, 0, 0, 0};
+                for (int q = 0; q < NB; ++q) {
+                    const int r = row_of(q, rows_b, BN), c = column_of(q, rows_b, BN);
+                    if constexpr (LB == Lie::Rows) held_b[q] = from(at_b[q], c);
+                    else if constexpr (WAY == Way::ByRows) held_b[q] = from(at_b[q], r);
+                    else held_b[q] = from(p.b + id[q] * p.b_stride + (walk.j0 + c < p.n ? walk.j0 + c : 0), r);
+                }
+            };
+            if (values >= kValues) all(std::true_type{});
+            else all(std::false_type{});
+            if constexpr (WAY != Way::ByWeights) {
+#pragma unroll
+                for (int q = 0; q < NA; ++q) at_a[q] += kValues;
+#pragma unroll
+                for (int q = 0; q < NB; ++q) at_b[q] += LB == Lie::Rows ? static_cast<i64>(kValues) : kValues * p.b_stride;
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < NA; ++q) {
+                const T* row;
+                if constexpr (LA == Lie::Rows) row = at_a[q];
+                else row = row_of(q, rows_a, BM) < values ? p.a + id[q] * p.a_stride : nullptr;
+                held_a[q] = row ? load_piece(row, columns_a(q, done), end_a) : i32x4{0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int q = 0; q < NB; ++q) {
+                const T* row;
+                if constexpr (LB == Lie::Rows) row = at_b[q];
+                else if constexpr (WAY == Way::ByRows) row = row_of(q, rows_b, BN) < values ? at_b[q] + done * p.b_stride : nullptr;
+                else row = row_of(q, rows_b, BN) < values ? p.b + id[q] * p.b_stride : nullptr;
+                held_b[q] = row ? load_piece(row, columns_b(q, done), end_b) : i32x4{0, 0, 0, 0};
+            }
         }
         values -= kValues, done += kValues;
         if (values > 0) ask();
+    };
+    const auto settled = [&](i32x4 w, int c, int end) {
+        if constexpr (ALIGNED) return w;
+        else return settle_piece<T>(w, c, end);
     };
     const auto put = [&](auto step, std::uint8_t* to, int row, int column, i32x4 w) {
         using S = decltype(step);
@@ -577,11 +636,11 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) k_grouped_held(Grouped<T, O> 
 #pragma unroll
             for (int q = 0; q < NA; ++q)
                 put(A{}, lds, row_of(q, rows_a, BM), column_of(q, rows_a, BM),
-                    settle_piece<T>(held_a[q], columns_a(q, done - kValues), end_a));
+                    settled(held_a[q], columns_a(q, done - kValues), end_a));
 #pragma unroll
             for (int q = 0; q < NB; ++q)
                 put(B{}, lds + A::kBytes * PARTS, row_of(q, rows_b, BN), column_of(q, rows_b, BN),
-                    settle_piece<T>(held_b[q], columns_b(q, done - kValues), end_b));
+                    settled(held_b[q], columns_b(q, done - kValues), end_b));
             __syncthreads();
             if (s + 1 == steps) {
                 walk.turn += gridDim.x;
@@ -590,20 +649,29 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) k_grouped_held(Grouped<T, O> 
             }
             if (more) load();
             if constexpr (SPLIT) {
-                Parts vb[NF];
+                // two columns of fragments at a time, so that the registers are those of three workgroups a unit
+                constexpr int kAtOnce = NF < 2 ? NF : 2;
 #pragma unroll
-                for (int g = 0; g < NF; ++g)
+                for (int g0 = 0; g0 < NF; g0 += kAtOnce) {
+                    Parts vb[kAtOnce];
 #pragma unroll
-                    for (int k = 0; k < 3; ++k)
-                        vb[g].part[k] = B::read(lds + A::kBytes * PARTS + k * B::kBytes, wn + 16 * g, 0, lane);
+                    for (int g = 0; g < kAtOnce; ++g)
 #pragma unroll
-                for (int f = 0; f < MF; ++f) {
-                    if (wm + 16 * f >= high) break;
+                        for (int k = 0; k < 3; ++k)
+                            vb[g].part[k] = B::read(lds + A::kBytes * PARTS + k * B::kBytes, wn + 16 * (g0 + g), 0, lane);
                     Parts va;
 #pragma unroll
-                    for (int k = 0; k < 3; ++k) va.part[k] = A::read(lds + k * A::kBytes, wm + 16 * f, 0, lane);
+                    for (int k = 0; k < 3; ++k) va.part[k] = A::read(lds + k * A::kBytes, wm, 0, lane);
 #pragma unroll
-                    for (int g = 0; g < NF; ++g) acc[f][g] = add_parts(vb[g], va, acc[f][g]);
+                    for (int f = 0; f < MF; ++f) {
+                        if (wm + 16 * f >= high) break;
+                        const Parts now_a = va;
+                        if (f + 1 < MF)
+#pragma unroll
+                            for (int k = 0; k < 3; ++k) va.part[k] = A::read(lds + k * A::kBytes, wm + 16 * (f + 1), 0, lane);
+#pragma unroll
+                        for (int g = 0; g < kAtOnce; ++g) acc[f][g0 + g] = add_parts(vb[g], now_a, acc[f][g0 + g]);
+                    }
                 }
             } else {
                 i32x4 vb[NF][2];
@@ -628,23 +696,40 @@ __global__ void __launch_bounds__(64 * WM * WN, 2) k_grouped_held(Grouped<T, O> 
     }
 }
 
-// The sums of kinds whose rows are cut: a workgroup row for each cut, which joins, in order, the runs of the kind that it
-// is the first cut of.
+// The sums of kinds whose rows are cut: workgroups in turn for each cut, which join, in order, the runs of the kind that it is the
+// first cut of, four neighbouring values a lane.
 template <class O>
-__global__ void __launch_bounds__(256) k_grouped_join(const float* __restrict__ partial, const int* __restrict__ plan, int kinds,
-                                                      int run, int m, int n, O* __restrict__ out, i64 out_stride, i64 out_kind) {
-    const int cut = blockIdx.y + 1;
-    const int* const offsets = plan + plan_offsets();
-    if (cut * run >= offsets[kinds]) return;
-    // (of kinds without rows at the cut itself, the last: it is the one whose rows follow)
-    const int kind = last_up_to(cut * run, kinds, [&](int z) { return offsets[z]; });
-    const int begin = offsets[kind], end = offsets[kind + 1], first = begin / run, last = (end - 1) / run;
-    if (begin >= cut * run || first + 1 != cut) return;
-    const i64 size = static_cast<i64>(m) * n;
-    for (i64 e = static_cast<i64>(blockIdx.x) * 256 + threadIdx.x; e < size; e += static_cast<i64>(gridDim.x) * 256) {
-        float sum = partial[(2 * first + 1) * size + e];
-        for (int r = cut; r <= last; ++r) sum += partial[2 * r * size + e];
-        out[kind * out_kind + e / n * out_stride + e % n] = static_cast<O>(sum);
+__global__ void __launch_bounds__(256) k_grouped_join(Grouped<O, O> p) {
+    const int run = run_of(p.plan, p.tokens, p.round, p.least), kinds = p.kinds;
+    const int* const offsets = p.plan + plan_offsets();
+    const i64 size = static_cast<i64>(p.m) * p.n;
+    for (int cut = blockIdx.y + 1; cut <= (p.tokens - 1) / run; cut += gridDim.y) {
+        if (cut * run >= offsets[kinds]) return;
+        // (of kinds without rows at the cut itself, the last: it is the one whose rows follow)
+        const int kind = last_up_to(cut * run, kinds, [&](int z) { return offsets[z]; });
+        const int begin = offsets[kind], first = begin / run, last = (offsets[kind + 1] - 1) / run;
+        if (begin >= cut * run || first + 1 != cut) continue;
+        for (i64 e = 4 * (static_cast<i64>(blockIdx.x) * 256 + threadIdx.x); e < size; e += 1024LL * gridDim.x) {
+            const auto part = [&](int slot) {
+                const float* const at = p.partial + slot * size + e;
+                if (e + 4 <= size) return *reinterpret_cast<const Pack<float, 4>*>(at);
+                Pack<float, 4> v;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) v.v[q] = e + q < size ? at[q] : 0.0f;
+                return v;
+            };
+            Pack<float, 4> sum = part(2 * first + 1);
+#pragma unroll 8
+            for (int r = cut; r <= last; ++r) {
+                const Pack<float, 4> v = part(2 * r);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) sum.v[q] += v.v[q];
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (e + q < size)
+                    p.out[kind * p.out_kind + (e + q) / p.n * p.out_stride + (e + q) % p.n] = static_cast<O>(sum.v[q]);
+        }
     }
 }
 
@@ -679,7 +764,7 @@ __global__ void __launch_bounds__(64 * KS) k_grouped_rows(Grouped<T, O> p) {
 // How a call is cut (node_grouped.hip).
 struct Cut {
     int tile;  // 256, 128, 64, or 16: k_grouped_rows
-    bool direct;
+    bool direct;  // rows are aligned to 16 bytes, and as long as whole ones
     int units;  // of 16 rows, at most
 };
 
@@ -698,10 +783,19 @@ void launch_grouped(const Grouped<T, O>& p, Way way, const Cut& cut, hipStream_t
                 return;
             }
         }
-        if (cut.tile == 128)
-            k_grouped_held<T, O, W, 128, 128, 2, 2><<<2 * kComputeUnits, 256, 0, stream>>>(p);
-        else
-            k_grouped_held<T, O, W, 64, 64, 2, 2><<<4 * kComputeUnits, 256, 0, stream>>>(p);
+        const auto held = [&](auto aligned_rows) {
+            constexpr bool ALIGNED = decltype(aligned_rows)::value;
+            if (cut.tile == 128)
+                k_grouped_held<T, O, W, ALIGNED, 128, 128, 2, 2><<<2 * kComputeUnits, 256, 0, stream>>>(p);
+            else
+                k_grouped_held<T, O, W, ALIGNED, 64, 64, 2, 2><<<4 * kComputeUnits, 256, 0, stream>>>(p);
+        };
+        if constexpr (sizeof(T) == 4) {
+            if (cut.direct) held(std::true_type{});
+            else held(std::false_type{});
+        } else {
+            held(std::false_type{});
+        }
         SMX_LAUNCH_CHECK("k_grouped_held");
     };
     using std::integral_constant;

@@ -33,6 +33,11 @@ constexpr int kComputeUnits = 256;
 // where pieces that are not there are read from
 static __device__ const uint4 kNothing[1] = {};
 
+// sixteen bytes of global memory (a choice of two places is one of any address space to the compiler)
+__device__ __forceinline__ i32x4 load_sixteen(const void* at) {
+    return *(const __attribute__((address_space(1))) i32x4*)(reinterpret_cast<std::uintptr_t>(at));
+}
+
 // 1 KB of LDS at byte `lds` (the wave's own, uniform) from 64 lanes' 16 bytes: memory to LDS without registers.  The compiler
 // does not count it: arrived().
 __device__ __forceinline__ void fetch(const void* at, unsigned lds) {
@@ -229,7 +234,7 @@ __device__ __forceinline__ SumOf<T> few_rows(const T* a, const T* const (&b)[NF]
     const int steps = (k + kValues - 1) / kValues;
     const auto load = [&](const T* row, int c) {
         if constexpr (DIRECT)
-            return *reinterpret_cast<const i32x4*>(c < k ? static_cast<const void*>(row + c) : kNothing);
+            return load_sixteen(c < k ? static_cast<const void*>(row + c) : kNothing);
         else
             return load_piece(row, c, k);
     };
