@@ -121,32 +121,35 @@ __device__ __forceinline__ void store_piece(O* row, int j, int n, i32x4 v) {
 // the lanes of each wave, so that a tile is found without a read; more are looked up.
 template <class T, class O, Way WAY, int BM, int BN>
 struct Walk {
-    const Grouped<T, O>& p;
+    const Grouped<T, O>* of;
     const int* order;
     int count, units, tiles, turn, run;
     int base_of, first_of, end_of, kind_of;  // of the lane's kind
     int row0, rows, i0, j0, kind, slot;  // of the tile: sorted rows; columns of out (by W: rows too); the partial sums' place, or -1
 
-    __device__ __forceinline__ Walk(const Grouped<T, O>& p) : p(p), order(p.plan + plan_order(p.kinds)), turn(blockIdx.x) {
+    __device__ __forceinline__ explicit Walk(const Grouped<T, O>& p) : of(&p), order(p.plan + plan_order(p.kinds)), turn(blockIdx.x) {
         const int lane = threadIdx.x % 64;
-        count = WAY == Way::ByWeights ? p.kinds : p.plan[0];
+        count = __builtin_amdgcn_readfirstlane(WAY == Way::ByWeights ? p.kinds : p.plan[0]);
         run = WAY == Way::ByWeights ? __builtin_amdgcn_readfirstlane(run_of(p.plan, p.tokens, p.round, p.least)) : 0;
         const int at = lane < count ? lane : count - 1;
         base_of = base(at), first_of = starts()[at], end_of = starts()[at + 1];
         kind_of = WAY == Way::ByWeights ? at : p.plan[plan_present(p.kinds) + at];
-        units = WAY == Way::ByWeights ? p.kinds + p.tokens / run : base(count);
+        units = __builtin_amdgcn_readfirstlane(WAY == Way::ByWeights ? p.kinds + p.tokens / run : base(count));
         tiles = units * p.tiles_m * p.tiles_n;
     }
     __device__ __forceinline__ const int* starts() const {
+        const Grouped<T, O>& p = *of;
         return p.plan + (WAY == Way::ByWeights ? plan_offsets() : plan_start(p.kinds));
     }
     // the first unit of the q-th kind
     __device__ __forceinline__ int base(int q) const {
+        const Grouped<T, O>& p = *of;
         if constexpr (WAY == Way::ByWeights) return q + starts()[q] / run;
         return p.plan[plan_tiles(p.kinds, BM == 64 ? 0 : BM == 128 ? 1 : 2) + q];
     }
     // the kind of unit u: its index, first unit, first and last sorted row and number
     __device__ __forceinline__ void find(int u, int& at, int& first, int& begin, int& end) {
+        const Grouped<T, O>& p = *of;
         if (count <= 64) {
             const int lane = threadIdx.x % 64;
             at = __popcll(__ballot(lane < count && base_of <= u)) - 1;
@@ -160,6 +163,7 @@ struct Walk {
     }
     // 0: no tile; 1: one to be summed; 2: one of zeros
     __device__ __forceinline__ int look() {
+        const Grouped<T, O>& p = *of;
         int at, first, begin, end;
         if constexpr (WAY == Way::ByWeights) {
             // the card is on one run of rows at a time, as runs differ in length; each XCD has a part of its tiles, in bands of four
@@ -195,17 +199,20 @@ struct Walk {
     }
     // the outputs' row i of the tile
     __device__ __forceinline__ O* out_row(int i) const {
+        const Grouped<T, O>& p = *of;
         if constexpr (WAY == Way::ByWeights)
             return p.out + kind * p.out_kind + (i0 + i) * p.out_stride;
         else
             return p.out + order[row0 + i] * p.out_stride;
     }
     __device__ __forceinline__ int out_rows() const {
+        const Grouped<T, O>& p = *of;
         if constexpr (WAY == Way::ByWeights) return p.m - i0 < BM ? p.m - i0 : BM;
         return rows;
     }
     // goes on from `turn` to the next tile to be summed; the zeros on the way are written
     __device__ __forceinline__ bool next() {
+        const Grouped<T, O>& p = *of;
         for (; turn < tiles; turn += gridDim.x) {
             const int what = __builtin_amdgcn_readfirstlane(look());
             // (looked up or not, all lanes have the same: addresses formed of it are scalar)
@@ -225,7 +232,7 @@ struct Walk {
 // The sums of a workgroup's waves to their rows; `room`: LDS that no one reads any more, for outputs of two bytes.
 template <class T, class O, Way WAY, int BM, int BN, int MF, int NF, class W>
 __device__ __forceinline__ void put_tile(const W& w, const acc4 (&acc)[MF][NF], int wm, int wn, int lane, std::uint8_t* room) {
-    const Grouped<T, O>& p = w.p;
+    const Grouped<T, O>& p = *w.of;
     const int high = w.out_rows();
     if constexpr (WAY == Way::ByWeights) {
         if (w.slot >= 0) {
@@ -274,16 +281,22 @@ __device__ __forceinline__ void put_tile(const W& w, const acc4 (&acc)[MF][NF], 
     }
 }
 
-// Rows of 16-bit values that go to LDS by themselves: BM x BN outputs a workgroup, a step of 64 values of the summed axis multiplied
-// while the next one arrives, and the next tile's first while this one's last is multiplied and stored.
+// Rows of 16-bit values that go to LDS by themselves: BM x BN outputs a workgroup, in steps of 64 values of the summed axis.  While one is
+// multiplied, the one after it arrives, over the tile's end into the next tile.
+//
+// 8192 cubed bf16 in 829 us, 1,327 TFLOP/s (a library's product 1,197): a tile of 256 has 2,050 cycles of matrix instructions a step and as
+// many of LDS (192 KB of fragments, 64 KB that arrive), which overlap as far as each fragment is read one ahead of its use.  Steps
+// of 32 with up to five places in LDS, asked for two to four ahead, were slower everywhere (2,048 x 2,048 x 2,048 of two types:
+// 39.4 and 33.9 us): it is not the memory's latency that is waited for.
 template <class T, class O, Way WAY, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : 2) k_grouped_tiles(Grouped<T, O> p) {
+__global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : BM + BN > 128 ? 2 : 4) k_grouped_tiles(Grouped<T, O> p) {
     static_assert(sizeof(T) == 2);
     constexpr Lie LA = WAY == Way::ByWeights ? Lie::Columns : Lie::Rows, LB = WAY == Way::Forward ? Lie::Rows : Lie::Columns;
-    constexpr int kValues = 64;
-    using A = Step<LA, BM, kValues>;
-    using B = Step<LB, BN, kValues>;
-    constexpr int WAVES = WM * WN, NA = A::kPieces / 64 / WAVES, NB = B::kPieces / 64 / WAVES, MF = BM / WM / 16, NF = BN / WN / 16;
+    constexpr int V = 64;
+    using A = Step<LA, BM, V>;
+    using B = Step<LB, BN, V>;
+    constexpr int WAVES = WM * WN, NA = A::kPieces / 64 / WAVES, NB = B::kPieces / 64 / WAVES, MF = BM / WM / 16, NF = BN / WN / 16,
+                  Q = V / 32;
     constexpr unsigned kStage = A::kBytes + B::kBytes;
     static_assert(WAVES * 16 * (16 * NF * 2 + 16) <= kStage && (WAY != Way::ByWeights || BM == BN));
     __shared__ __attribute__((aligned(1024))) std::uint8_t lds[2 * kStage];
@@ -291,28 +304,29 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : 2) k_grouped
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
     using Walker = Walk<T, O, WAY, BM, BN>;
-    Walker walk(p);
+    Walker walk(p);  // the tile that steps are asked for of
 
     // (the lane's number anew where it is used once a tile: addresses formed of it are not kept across the steps)
-    const auto piece = [&](int q) {
+    const auto piece = [&](int q) __attribute__((always_inline)) {
         int l = lane;
         asm volatile("" : "+v"(l));
         return (wave + WAVES * q) * 64 + l;
     };
-    const T *at_a[NA], *at_b[NB];  // the lane's pieces of the step to come; gathered Columns: the pieces' columns
-    // The rows of a's pieces, asked for a step ahead: gathered Rows of the next tile, and gathered Columns of the next step.  The rows of
-    // these are a few for each fetch of a wave, so they are read as scalars, and picked by the lanes when the step's
-    // products are on their way: a lane's own reads would be waited for with the step's (8192 cubed: 1,409 us, 1,055 so).
-    constexpr int kIds = WAY == Way::ByWeights ? 64 / A::kRowPieces : 1;
+    const T *at_a[NA], *at_b[NB];  // the lane's pieces of the step to come
+    int column_a[NA], column_b[NB];  // gathered Columns: the pieces' columns
+    // The rows of a's pieces: of gathered Rows of a tile, of gathered Columns of the next step.  They are a few for each fetch of a wave, so
+    // they are read as scalars, the latter a step ahead: a lane's own reads would be waited for with the steps' (8192 cubed by W:
+    // 1,409 us, 1,055 so).
+    constexpr int kIds = 64 / A::kRowPieces;
     using Scalars = const __attribute__((address_space(4))) int*;
     const Scalars scalars = (Scalars)(reinterpret_cast<std::uintptr_t>(walk.order));
     int id[NA];
     struct Asked {
         int v[NA][kIds];
     };
-    int values = 0, ids_at = 0;  // of the summed axis, left; by W: the row that the next step's ids begin at
+    int values = 0;  // of the summed axis, left
     int absent = 0;  // rows of the tile: from here on none are multiplied, nor read
-    const auto ask = [&](int from) {
+    const auto ask = [&](int from) __attribute__((always_inline)) {
         Asked to;
 #pragma unroll
         for (int q = 0; q < NA; ++q)
@@ -323,7 +337,7 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : 2) k_grouped
             }
         return to;
     };
-    const auto pick = [&](const Asked& of) {
+    const auto pick = [&](const Asked& of) __attribute__((always_inline)) {
 #pragma unroll
         for (int q = 0; q < NA; ++q) {
             id[q] = of.v[q][0];
@@ -331,31 +345,21 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : 2) k_grouped
             for (int i = 1; i < kIds; ++i) id[q] = lane / A::kRowPieces == i ? of.v[q][i] : id[q];
         }
     };
-    const auto ask_first = [&] {
+    // to the first step of the walk's tile
+    const auto begin = [&]() __attribute__((always_inline)) {
+        pick(ask(0));
         if constexpr (WAY == Way::ByWeights) {
-            pick(ask(0));
-        } else {
-#pragma unroll
-            for (int q = 0; q < NA; ++q) {
-                const int r = A::row_at(piece(q));
-                id[q] = walk.order[walk.row0 + (r < walk.rows ? r : walk.rows - 1)];
-            }
-        }
-    };
-    // to the first step of the walk's tile, whose ids are there
-    const auto begin = [&] {
-        if constexpr (WAY == Way::ByWeights) {
-            values = walk.rows, ids_at = 0;
+            values = walk.rows;
             // (columns past the row's end are no one's: any place of the row does)
 #pragma unroll
             for (int q = 0; q < NA; ++q) {
                 const int c = walk.i0 + A::piece_at(piece(q)) * 8;
-                at_a[q] = p.a + (c < p.m ? c : 0);
+                column_a[q] = c < p.m ? c : 0;
             }
 #pragma unroll
             for (int q = 0; q < NB; ++q) {
                 const int c = walk.j0 + B::piece_at(piece(q)) * 8;
-                at_b[q] = p.b + (c < p.n ? c : 0);
+                column_b[q] = c < p.n ? c : 0;
             }
         } else {
             values = p.k, absent = __builtin_amdgcn_readfirstlane((walk.rows + 15) / 16 * 16);
@@ -373,110 +377,132 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : 2) k_grouped
         }
     };
     // asks for the step to come, and goes on
-    const auto stage = [&](int slot) {
-        const unsigned to = __builtin_amdgcn_readfirstlane(lds0 + slot * kStage);
-        const auto all = [&](auto whole) {
+    const auto stage = [&](int slot) __attribute__((always_inline)) {
+        const unsigned to = __builtin_amdgcn_readfirstlane(lds0 + slot * kStage + wave * 1024);
+        const auto all = [&](auto whole) __attribute__((always_inline)) {
             constexpr bool WHOLE = decltype(whole)::value;
-#pragma unroll
-            for (int q = 0; q < NA; ++q) {
-                if (LA == Lie::Rows && 8 * (wave + WAVES * q) >= absent) continue;
-                const T* at = WAY == Way::ByWeights ? at_a[q] + id[q] * p.a_stride : at_a[q];
+            each_of<NA>([&](auto n) __attribute__((always_inline)) {
+                constexpr int q = decltype(n)::value;
+                const T* at = WAY == Way::ByWeights ? p.a + (id[q] * p.a_stride + column_a[q]) : at_a[q];
                 if (!WHOLE) {
                     const int v = LA == Lie::Rows ? A::piece_at(piece(q)) * 8 : A::row_at(piece(q));
                     at = v < values ? at : reinterpret_cast<const T*>(kNothing);
                 }
-                fetch(at, to + (wave + WAVES * q) * 1024);
-            }
-#pragma unroll
-            for (int q = 0; q < NB; ++q) {
-                const T* at = WAY == Way::ByWeights ? at_b[q] + id[q] * p.b_stride : at_b[q];
+                if (LA == Lie::Rows && (wave + WAVES * q) * kIds >= absent) at = reinterpret_cast<const T*>(kNothing);
+                fetch<WAVES * q * 1024>(at, to);
+            });
+            each_of<NB>([&](auto n) __attribute__((always_inline)) {
+                constexpr int q = decltype(n)::value;
+                const T* at = WAY == Way::ByWeights ? p.b + (id[q] * p.b_stride + column_b[q]) : at_b[q];
                 if (!WHOLE) {
                     const int v = LB == Lie::Rows ? B::piece_at(piece(q)) * 8 : B::row_at(piece(q));
                     at = v < values ? at : reinterpret_cast<const T*>(kNothing);
                 }
-                fetch(at, to + A::kBytes + (wave + WAVES * q) * 1024);
-            }
+                fetch<A::kBytes + WAVES * q * 1024>(at, to);
+            });
         };
-        if (values >= kValues) all(std::true_type{});
+        if (values >= V) all(std::true_type{});
         else all(std::false_type{});
-        values -= kValues;
-        if constexpr (WAY == Way::ByWeights) {
-            ids_at += kValues;
-        } else {
+        values -= V;
+        if constexpr (WAY != Way::ByWeights) {
 #pragma unroll
-            for (int q = 0; q < NA; ++q) at_a[q] += kValues;
+            for (int q = 0; q < NA; ++q) at_a[q] += V;
 #pragma unroll
-            for (int q = 0; q < NB; ++q) at_b[q] += LB == Lie::Rows ? static_cast<i64>(kValues) : kValues * p.b_stride;
+            for (int q = 0; q < NB; ++q) at_b[q] += LB == Lie::Rows ? static_cast<i64>(V) : V * p.b_stride;
         }
     };
 
+    int slot = 0;
+    bool other = false, more = true;  // the walk is a tile ahead of the products; it has not ended
+    // asks for one more step, of the walk's tile or the first of the one after
+    const auto ahead = [&](int to) __attribute__((always_inline)) {
+        if (values <= 0) {
+            if (!more) return;
+            walk.turn += gridDim.x;
+            more = walk.next();
+            if (!more) return;
+            other = true;
+            begin();
+        }
+        stage(to);
+    };
+    // by W: the rows of the step that is asked for next
+    const auto ask_next = [&]() __attribute__((always_inline)) { return ask(walk.rows - values); };
+
     if (!walk.next()) return;
-    ask_first();
+    Walker now = walk;  // the tile that is multiplied
     begin();
     stage(0);
     if constexpr (WAY == Way::ByWeights)
-        if (values > 0) pick(ask(ids_at));
-    int slot = 0;
-    for (bool more = true; more;) {
-        const Walker now = walk;
-        const int steps = ((WAY == Way::ByWeights ? now.rows : p.k) + kValues - 1) / kValues, high = __builtin_amdgcn_readfirstlane(now.out_rows());
+        if (values > 0) pick(ask_next());
+    for (;;) {
+        const int steps = ((WAY == Way::ByWeights ? now.rows : p.k) + V - 1) / V, high = __builtin_amdgcn_readfirstlane(now.out_rows());
         acc4 acc[MF][NF];
 #pragma unroll
         for (int f = 0; f < MF; ++f)
 #pragma unroll
             for (int g = 0; g < NF; ++g) acc[f][g] = acc4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s = 0; s < steps; ++s) {
-            arrived();
-            __syncthreads();  // the step is there, and all have read the one before
-            const std::uint8_t* const tile = lds + slot * kStage;
-            slot ^= 1;
-            const auto read_a = [&](int f, int q) { return A::read(tile, wm + 16 * f, q, lane); };
-            const auto read_b = [&](int g, int q) { return B::read(tile + A::kBytes, wn + 16 * g, q, lane); };
-            i32x4 vb[NF], va = read_a(0, 0);
+        const auto sum = [&](auto full) __attribute__((always_inline)) {
+            for (int s = 0; s < steps; ++s) {
+                arrived();
+                __syncthreads();  // the step is there, and all have read the one before
+                const std::uint8_t* const tile = lds + slot * kStage;
+                slot ^= 1;
+                const auto read_a = [&](int f, int q) __attribute__((always_inline)) { return A::read(tile, wm + 16 * f, q, lane); };
+                const auto read_b = [&](int g, int q) __attribute__((always_inline)) { return B::read(tile + A::kBytes, wn + 16 * g, q, lane); };
+                i32x4 vb[NF], va = read_a(0, 0);
 #pragma unroll
-            for (int g = 0; g < NF; ++g) vb[g] = read_b(g, 0);
-            if (s + 1 < steps) {
-                stage(slot);
-            } else if (more && steps > 1) {
-                begin();
-                stage(slot);
-            }
-            if (s == (steps > 1 ? steps - 2 : 0)) {
-                // the next tile, a step before its first is asked for
-                walk.turn += gridDim.x;
-                more = walk.next();
-                if (more) ask_first();
-                if (more && steps == 1) {
-                    begin();
-                    stage(slot);
-                }
-            }
-            Asked asked;
-            // each fragment is read while the one before is multiplied; those without rows of the tile are left out
+                for (int g = 0; g < NF; ++g) vb[g] = read_b(g, 0);
+                ahead(slot);
+                Asked asked;
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                if (q > 0) {
+                for (int q = 0; q < Q; ++q) {
                     if constexpr (WAY == Way::ByWeights)
-                        if (values > 0) asked = ask(ids_at);
-                    va = read_a(0, q);
+                        if (q + 1 == Q && values > 0) asked = ask_next();
+                    // each fragment is read while the one before is multiplied
+                    i32x4 next_b[NF];
 #pragma unroll
-                    for (int g = 0; g < NF; ++g) vb[g] = read_b(g, q);
+                    for (int f = 0; f < MF; ++f) {
+                        if (!decltype(full)::value && wm + 16 * f >= high) continue;  // no rows of the tile
+                        const i32x4 now_a = va;
+                        if (f + 1 < MF) va = read_a(f + 1, q);
+                        else if (q + 1 < Q) va = read_a(0, q + 1);
+                        if (f + 2 == MF && q + 1 < Q)
+#pragma unroll
+                            for (int g = 0; g < NF; ++g) next_b[g] = read_b(g, q + 1);
+#pragma unroll
+                        for (int g = 0; g < NF; ++g) acc[f][g] = Multiply<T>::add(vb[g], now_a, acc[f][g]);
+                        if (decltype(full)::value) {
+                            // (in this order: left to itself the compiler has each read waited for at once)
+                            constexpr int kReadsA = LA == Lie::Rows ? 1 : 2, kReadsB = LB == Lie::Rows ? 1 : 2;
+                            if (f + 1 < MF || q + 1 < Q) __builtin_amdgcn_sched_group_barrier(0x100, kReadsA, 0);
+                            if (f + 2 == MF && q + 1 < Q) __builtin_amdgcn_sched_group_barrier(0x100, kReadsB * NF, 0);
+                            __builtin_amdgcn_sched_group_barrier(0x008, NF, 0);
+                        }
+                    }
+                    if (q + 1 < Q) {
+                        if (!decltype(full)::value) {
+                            va = read_a(0, q + 1);
+#pragma unroll
+                            for (int g = 0; g < NF; ++g) next_b[g] = read_b(g, q + 1);
+                        }
+#pragma unroll
+                        for (int g = 0; g < NF; ++g) vb[g] = next_b[g];
+                    }
                 }
-#pragma unroll
-                for (int f = 0; f < MF; ++f) {
-                    if (wm + 16 * f >= high) break;
-                    const i32x4 now_a = va;
-                    if (f + 1 < MF) va = read_a(f + 1, q);
-#pragma unroll
-                    for (int g = 0; g < NF; ++g) acc[f][g] = Multiply<T>::add(vb[g], now_a, acc[f][g]);
-                }
+                if constexpr (WAY == Way::ByWeights)
+                    if (values > 0) pick(asked);
             }
-            if constexpr (WAY == Way::ByWeights)
-                if (values > 0) pick(asked);
-        }
+        };
+        // (a loop each for waves whose fragments all have rows and for others: between conditions the reads would not be ahead)
+        if (WAY == Way::ByWeights || wm + 16 * MF <= high) sum(std::true_type{});
+        else sum(std::false_type{});
         settle_products();
         if constexpr (sizeof(O) == 2) __syncthreads();  // all have read the last step, whose place is used
         put_tile<T, O, WAY, BM, BN, MF, NF>(now, acc, wm, wn, lane, lds + (slot ^ 1) * kStage);
+        if (!other) return;  // (a tile's last step has asked for one of the next, if there is one)
+        now = walk;
+        other = false;
     }
 }
 

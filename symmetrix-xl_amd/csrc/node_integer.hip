@@ -180,11 +180,9 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : 2) k_integer
         }
     };
     const auto stage = [&](int s, int slot) {
-        const unsigned to = __builtin_amdgcn_readfirstlane(lds0 + slot * kStage);
-#pragma unroll
-        for (int q = 0; q < NA; ++q) fetch(at_a[q] + s * kStepBytes, to + (wave + WAVES * q) * 1024);
-#pragma unroll
-        for (int q = 0; q < NB; ++q) fetch(at_b[q] + s * kStepBytes, to + BM * kStepBytes + (wave + WAVES * q) * 1024);
+        const unsigned to = __builtin_amdgcn_readfirstlane(lds0 + slot * kStage + wave * 1024);
+        each_of<NA>([&](auto q) { fetch<WAVES * q * 1024>(at_a[q] + s * kStepBytes, to); });
+        each_of<NB>([&](auto q) { fetch<BM * kStepBytes + WAVES * q * 1024>(at_b[q] + s * kStepBytes, to); });
     };
     int slot = 0;
     turn_to(blockIdx.x);
@@ -201,11 +199,11 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : 2) k_integer
             __syncthreads();
             const std::uint8_t* const tile = lds + slot * kStage;
             slot ^= 1;
-            i32x4 vb[NF][2];
+            const auto read_a = [&](int f, int q) { return A::read(tile, wm + 16 * f, q, lane); };
+            const auto read_b = [&](int g, int q) { return B::read(tile + BM * kStepBytes, wn + 16 * g, q, lane); };
+            i32x4 vb[NF], va = read_a(0, 0);
 #pragma unroll
-            for (int g = 0; g < NF; ++g)
-#pragma unroll
-                for (int q = 0; q < 2; ++q) vb[g][q] = B::read(tile + BM * kStepBytes, wn + 16 * g, q, lane);
+            for (int g = 0; g < NF; ++g) vb[g] = read_b(g, 0);
             if (s + 1 < steps) {
                 stage(s + 1, slot);
             } else if (turn + static_cast<int>(gridDim.x) < tiles) {
@@ -213,14 +211,26 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : 2) k_integer
                 stage(0, slot);
             }
 #pragma unroll
-            for (int f = 0; f < MF; ++f) {
-                i32x4 va[2];
+            for (int q = 0; q < 2; ++q) {
+                // each fragment is read while the one before is multiplied
+                i32x4 next_b[NF];
 #pragma unroll
-                for (int q = 0; q < 2; ++q) va[q] = A::read(tile, wm + 16 * f, q, lane);
+                for (int f = 0; f < MF; ++f) {
+                    const i32x4 now_a = va;
+                    if (f + 1 < MF || q == 0) va = read_a((f + 1) % MF, q + (f + 1) / MF);
+                    if (f + 2 == MF && q == 0)
 #pragma unroll
-                for (int q = 0; q < 2; ++q)
+                        for (int g = 0; g < NF; ++g) next_b[g] = read_b(g, 1);
 #pragma unroll
-                    for (int g = 0; g < NF; ++g) acc[f][g] = Multiply<T>::add(vb[g][q], va[q], acc[f][g]);
+                    for (int g = 0; g < NF; ++g) acc[f][g] = Multiply<T>::add(vb[g], now_a, acc[f][g]);
+                    // (in this order: left to itself the compiler has each read waited for at once)
+                    if (f + 1 < MF || q == 0) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    if (f + 2 == MF && q == 0) __builtin_amdgcn_sched_group_barrier(0x100, NF, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x008, NF, 0);
+                }
+                if (q == 0)
+#pragma unroll
+                    for (int g = 0; g < NF; ++g) vb[g] = next_b[g];
             }
         }
         settle_products();

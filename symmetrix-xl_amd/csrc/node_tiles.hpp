@@ -16,6 +16,9 @@
 // instruction q takes pieces 4 q .. 4 q + 3, lane group l / 16 the piece 4 q + l / 16.
 #pragma once
 
+#include <type_traits>
+#include <utility>
+
 #include "node_ops.hpp"
 
 namespace smx {
@@ -38,10 +41,16 @@ __device__ __forceinline__ i32x4 load_sixteen(const void* at) {
     return *(const __attribute__((address_space(1))) i32x4*)(reinterpret_cast<std::uintptr_t>(at));
 }
 
-// 1 KB of LDS at byte `lds` (the wave's own, uniform) from 64 lanes' 16 bytes: memory to LDS without registers.  The compiler
+// 1 KB of LDS at byte lds + OFFSET (the wave's own, uniform) from 64 lanes' 16 bytes: memory to LDS without registers.  The compiler
 // does not count it: arrived().
+template <int OFFSET>
 __device__ __forceinline__ void fetch(const void* at, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(at) : "memory");
+    asm volatile("s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(at), "n"(OFFSET) : "memory", "scc");
+}
+// f(0), ..., f(N - 1) with the number as a constant
+template <int N, class F>
+__device__ __forceinline__ void each_of(F&& f) {
+    [&]<int... I>(std::integer_sequence<int, I...>) __attribute__((always_inline)) { (f(std::integral_constant<int, I>{}), ...); }(std::make_integer_sequence<int, N>{});
 }
 __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
