@@ -25,7 +25,7 @@ void with_types(int dtype, int out_dtype, F&& f) {
 // What tiles of 256, 128 and 64 cost, in us: a step of 64 values of the summed axis with `filled` tiles on a unit, which holds one,
 // two or four of them, and what a tile takes beside its steps (measured: 8192 cubed, and 2,048 rows of 2,048 values).
 constexpr int kSizes[3] = {256, 128, 64};
-int held(int tile) { return 65536 / (tile * tile) < 1 ? 1 : tile == 128 ? 2 : 4; }
+int held(int tile) { return tile == 256 ? 1 : tile == 128 ? 2 : 4; }
 double step_time(int tile, i64 filled) {
     if (tile == 256) return 1.9;
     if (tile == 128) return 1.15;

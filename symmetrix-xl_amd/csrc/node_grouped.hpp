@@ -314,9 +314,9 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : BM + BN > 12
     };
     const T *at_a[NA], *at_b[NB];  // the lane's pieces of the step to come
     int column_a[NA], column_b[NB];  // gathered Columns: the pieces' columns
-    // The rows of a's pieces: of gathered Rows of a tile, of gathered Columns of the next step.  They are a few for each fetch of a wave, so
-    // they are read as scalars, the latter a step ahead: a lane's own reads would be waited for with the steps' (8192 cubed by W:
-    // 1,409 us, 1,055 so).
+    // The rows of a's pieces: of gathered Rows of a tile, of gathered Columns of the next step.  The latter are a few for each fetch of a wave,
+    // so they are read as scalars, a step ahead: a lane's own reads would be waited for with the step's (8192 cubed by W: 1,409 us, 1,055
+    // so).
     constexpr int kIds = 64 / A::kRowPieces;
     using Scalars = const __attribute__((address_space(4))) int*;
     const Scalars scalars = (Scalars)(reinterpret_cast<std::uintptr_t>(walk.order));
@@ -347,7 +347,15 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : BM + BN > 12
     };
     // to the first step of the walk's tile
     const auto begin = [&]() __attribute__((always_inline)) {
-        pick(ask(0));
+        if constexpr (WAY == Way::ByWeights) {
+            pick(ask(0));
+        } else {
+#pragma unroll
+            for (int q = 0; q < NA; ++q) {
+                const int r = A::row_at(piece(q));
+                id[q] = walk.order[walk.row0 + (r < walk.rows ? r : walk.rows - 1)];
+            }
+        }
         if constexpr (WAY == Way::ByWeights) {
             values = walk.rows;
             // (columns past the row's end are no one's: any place of the row does)
@@ -494,8 +502,10 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : BM + BN > 12
                     if (values > 0) pick(asked);
             }
         };
-        // (a loop each for waves whose fragments all have rows and for others: between conditions the reads would not be ahead)
-        if (WAY == Way::ByWeights || wm + 16 * MF <= high) sum(std::true_type{});
+        // (In tiles of 256 a loop each for waves whose fragments all have rows and for others: between conditions the reads would not be
+        // ahead.  In smaller ones, whose kernels are short, twice the instructions cost more than the products of no rows: 6,791 rows of
+        // 89 types, 224 x 1,000, CODE.)
+        if (WAY == Way::ByWeights || BM < 256 || wm + 16 * MF <= high) sum(std::true_type{});
         else sum(std::false_type{});
         settle_products();
         if constexpr (sizeof(O) == 2) __syncthreads();  // all have read the last step, whose place is used
