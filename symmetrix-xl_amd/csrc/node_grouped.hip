@@ -173,9 +173,10 @@ void weights_gradient(const void* grad, i64 grad_stride, const void* x, i64 x_st
         j.out = p.out, j.out_stride = out_stride, j.out_kind = out_kind;
         j.plan = p.plan, j.tokens = p.tokens, j.kinds = p.kinds, j.m = p.m, j.n = p.n;
         j.round = p.round, j.least = p.least, j.partial = p.partial;
-        const i64 blocks = ceil_of(m * n, 1024), cuts = (rows - 1) / runs.least;
-        k_grouped_join<O><<<dim3(static_cast<unsigned>(blocks < 1024 ? blocks : 1024), static_cast<unsigned>(cuts < 64 ? cuts : 64)),
-                            256, 0, stream>>>(j);
+        // (few workgroups: whether there is anything to join is known to the device alone)
+        const i64 blocks = ceil_of(m * n, 1024), cuts = (rows - 1) / runs.least, most = kinds < cuts ? kinds : cuts;
+        k_grouped_join<O><<<dim3(static_cast<unsigned>(blocks < 256 ? blocks : 256), static_cast<unsigned>(most < 4 ? most : 4)), 256, 0,
+                            stream>>>(j);
         SMX_LAUNCH_CHECK("k_grouped_join");
     }
 }

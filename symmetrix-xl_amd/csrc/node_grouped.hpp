@@ -124,6 +124,7 @@ struct Walk {
     const Grouped<T, O>* of;
     const int* order;
     int count, units, tiles, turn, run;
+    bool even;  // by W: runs are of about one length
     int base_of, first_of, end_of, kind_of;  // of the lane's kind
     int row0, rows, i0, j0, kind, slot;  // of the tile: sorted rows; columns of out (by W: rows too); the partial sums' place, or -1
 
@@ -131,6 +132,8 @@ struct Walk {
         const int lane = threadIdx.x % 64;
         count = __builtin_amdgcn_readfirstlane(WAY == Way::ByWeights ? p.kinds : p.plan[0]);
         run = WAY == Way::ByWeights ? __builtin_amdgcn_readfirstlane(run_of(p.plan, p.tokens, p.round, p.least)) : 0;
+        even = WAY == Way::ByWeights && p.tiles_m * p.tiles_n <= 64 &&
+               __builtin_amdgcn_readfirstlane(run <= p.tokens || static_cast<i64>(p.plan[3]) * p.plan[0] <= 3 * (static_cast<i64>(p.tokens) / 2));
         const int at = lane < count ? lane : count - 1;
         base_of = base(at), first_of = starts()[at], end_of = starts()[at + 1];
         kind_of = WAY == Way::ByWeights ? at : p.plan[plan_present(p.kinds) + at];
@@ -166,8 +169,10 @@ struct Walk {
         const Grouped<T, O>& p = *of;
         int at, first, begin, end;
         if constexpr (WAY == Way::ByWeights) {
-            // the card is on one run of rows at a time, as runs differ in length; each XCD has a part of its tiles, in bands of four
-            const int per = p.tiles_m * p.tiles_n, u = turn / per, id = xcd_remap(turn % per, per);
+            // Tiles in bands of four.  Runs of about one length and few tiles go to an XCD each, which then reads their rows once (20,000 x 512
+            // x 1,024 of ten types 68 us, 72 else; of 64 types with 128 tiles each 964 and 897); otherwise all XCDs are on one run at a time.
+            const int per = p.tiles_m * p.tiles_n, all = xcd_remap(turn, tiles);
+            const int u = even ? all / per : turn / per, id = even ? all % per : xcd_remap(turn % per, per);
             find(u, at, first, begin, end);
             const int band = id / (4 * p.tiles_n), in = id % (4 * p.tiles_n);
             const int high = p.tiles_m - 4 * band < 4 ? p.tiles_m - 4 * band : 4;
@@ -732,39 +737,43 @@ __global__ void __launch_bounds__(64 * WM * WN, BM == 128 ? 2 : 4) k_grouped_hel
     }
 }
 
-// The sums of kinds whose rows are cut: workgroups in turn for each cut, which join, in order, the runs of the kind that it is the
-// first cut of, four neighbouring values a lane.
+// The sums of kinds whose rows are cut: rows of workgroups take these kinds in turn and join their runs in order, four neighbouring
+// values a lane.
 template <class O>
 __global__ void __launch_bounds__(256) k_grouped_join(Grouped<O, O> p) {
-    const int run = run_of(p.plan, p.tokens, p.round, p.least), kinds = p.kinds;
+    const int run = run_of(p.plan, p.tokens, p.round, p.least), kinds = p.kinds, lane = threadIdx.x % 64;
+    if (run > p.tokens) return;
     const int* const offsets = p.plan + plan_offsets();
     const i64 size = static_cast<i64>(p.m) * p.n;
-    for (int cut = blockIdx.y + 1; cut <= (p.tokens - 1) / run; cut += gridDim.y) {
-        if (cut * run >= offsets[kinds]) return;
-        // (of kinds without rows at the cut itself, the last: it is the one whose rows follow)
-        const int kind = last_up_to(cut * run, kinds, [&](int z) { return offsets[z]; });
-        const int begin = offsets[kind], first = begin / run, last = (offsets[kind + 1] - 1) / run;
-        if (begin >= cut * run || first + 1 != cut) continue;
-        for (i64 e = 4 * (static_cast<i64>(blockIdx.x) * 256 + threadIdx.x); e < size; e += 1024LL * gridDim.x) {
-            const auto part = [&](int slot) {
-                const float* const at = p.partial + slot * size + e;
-                if (e + 4 <= size) return *reinterpret_cast<const Pack<float, 4>*>(at);
-                Pack<float, 4> v;
+    unsigned nth = 0;
+    for (int base = 0; base < kinds; base += 64) {
+        const int mine = base + lane < kinds ? base + lane : kinds - 1, from = offsets[mine], to = offsets[mine + 1];
+        unsigned long long cut = __ballot(base + lane < kinds && to > from && from / run != (to - 1) / run);
+        for (; cut; cut &= cut - 1) {
+            if (nth++ % gridDim.y != blockIdx.y) continue;
+            const int at = __builtin_ctzll(cut), kind = base + at;
+            const int first = __builtin_amdgcn_readlane(from, at) / run, last = (__builtin_amdgcn_readlane(to, at) - 1) / run;
+            for (i64 e = 4 * (static_cast<i64>(blockIdx.x) * 256 + threadIdx.x); e < size; e += 1024LL * gridDim.x) {
+                const auto part = [&](int slot) {
+                    const float* const at = p.partial + slot * size + e;
+                    if (e + 4 <= size) return *reinterpret_cast<const Pack<float, 4>*>(at);
+                    Pack<float, 4> v;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) v.v[q] = e + q < size ? at[q] : 0.0f;
-                return v;
-            };
-            Pack<float, 4> sum = part(2 * first + 1);
+                    for (int q = 0; q < 4; ++q) v.v[q] = e + q < size ? at[q] : 0.0f;
+                    return v;
+                };
+                Pack<float, 4> sum = part(2 * first + 1);
 #pragma unroll 8
-            for (int r = cut; r <= last; ++r) {
-                const Pack<float, 4> v = part(2 * r);
+                for (int r = first + 1; r <= last; ++r) {
+                    const Pack<float, 4> v = part(2 * r);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) sum.v[q] += v.v[q];
+                    for (int q = 0; q < 4; ++q) sum.v[q] += v.v[q];
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (e + q < size)
+                        p.out[kind * p.out_kind + (e + q) / p.n * p.out_stride + (e + q) % p.n] = static_cast<O>(sum.v[q]);
             }
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                if (e + q < size)
-                    p.out[kind * p.out_kind + (e + q) / p.n * p.out_stride + (e + q) % p.n] = static_cast<O>(sum.v[q]);
         }
     }
 }
