@@ -124,8 +124,11 @@ __global__ void __launch_bounds__(kThreads) k_clip(Tensors t, const double* __re
     int power;
     const float by = static_cast<float>(frexp(factor, &power));
     const float two = ldexpf(1.0f, power);
-    for (unsigned chunk = blockIdx.x; chunk < t.first[t.tensors]; chunk += gridDim.x) {
-        const int i = tensor_of(t, chunk);
+    // The tensors come the last first, and a tensor's last chunk too: what was read last is still in the last cache (256 MB).
+    const unsigned chunks = t.first[t.tensors];
+    for (unsigned nth = blockIdx.x; nth < chunks; nth += gridDim.x) {
+        const int i = tensor_of(t, nth);
+        const unsigned chunk = t.first[i] + t.first[i + 1] - 1 - nth;
         const i64 from = static_cast<i64>(chunk - t.first[i]) * kChunk;
         const i64 n = t.count[i] - from < kChunk ? t.count[i] - from : kChunk;
         const bool whole = factor == 1.0;
@@ -201,15 +204,16 @@ void check_outputs(const List& l) {
     }
 }
 
-// f(table, chunks) for each launch's tensors
+// f(table, chunks) for each launch's tensors, from the first tensor on or (`backwards`) from the last
 template <class F>
-void each_table(const List& l, F&& f) {
+void each_table(const List& l, F&& f, bool backwards = false) {
     Tensors t;
-    i64 i = 0;
-    while (i < l.tensors) {
+    i64 done = 0;
+    while (done < l.tensors) {
         t.tensors = 0;
         i64 chunks = 0;
-        for (; i < l.tensors && t.tensors < kTensors; ++i) {
+        for (; done < l.tensors && t.tensors < kTensors; ++done) {
+            const i64 i = backwards ? l.tensors - 1 - done : done;
             if (l.counts[i] == 0) continue;
             const i64 more = chunks_of(l.counts[i]);
             if (chunks + more > (1LL << 31)) {
@@ -295,7 +299,7 @@ int32_t smx_clip_gradients(const void* const* tensors, const int64_t* counts, co
             k_clip<<<grid, kThreads, 0, at>>>(t, parts, used, scale, max_norm, first);
             SMX_LAUNCH_CHECK("k_clip");
             first = nullptr;
-        });
+        }, true);
     });
 }
 

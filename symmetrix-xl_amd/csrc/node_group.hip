@@ -30,27 +30,39 @@ __global__ void __launch_bounds__(kThreads) k_group_count(const I* __restrict__ 
     for (int d = threadIdx.x; d <= kinds; d += kThreads) counts[blockIdx.x * (kinds + 1LL) + d] = count[d];
 }
 
-// Sums of the threads before, of two numbers in one: the workgroup's total in `all`.
-__device__ __forceinline__ unsigned long long sum_before(unsigned long long v, unsigned long long (&room)[kWaves],
-                                                         unsigned long long& all) {
+// Sums of the threads before, of two numbers in one each: the workgroup's totals in `all`.
+template <int N>
+struct Sums {
+    unsigned long long v[N];
+};
+
+template <int N>
+__device__ __forceinline__ Sums<N> sum_before(const Sums<N>& of, unsigned long long (&room)[3][kWaves], Sums<N>& all) {
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    unsigned long long sum = v;
+    Sums<N> sum = of;
 #pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        const unsigned long long below = __shfl_up(sum, o);
-        if (lane >= o) sum += below;
-    }
-    __syncthreads();
-    if (lane == 63) room[wave] = sum;
-    __syncthreads();
-    unsigned long long before = sum - v;
-    all = 0;
+    for (int o = 1; o < 64; o *= 2)
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        if (w < wave) before += room[w];
-        all += room[w];
+        for (int i = 0; i < N; ++i) {
+            const unsigned long long below = __shfl_up(sum.v[i], o);
+            if (lane >= o) sum.v[i] += below;
+        }
+    __syncthreads();
+    if (lane == 63)
+#pragma unroll
+        for (int i = 0; i < N; ++i) room[i][wave] = sum.v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        sum.v[i] -= of.v[i];
+        all.v[i] = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            if (w < wave) sum.v[i] += room[i][w];
+            all.v[i] += room[i][w];
+        }
     }
-    return before;
+    return sum;
 }
 
 // BITS: of a kind; the waves' counts of all kinds are in LDS (150 KB of it at 13 bits).  ONE: one workgroup, nothing was counted.
@@ -60,7 +72,7 @@ __global__ void __launch_bounds__(kThreads) k_group_place(const I* __restrict__ 
     constexpr int kDigits = BITS == 13 ? kMostKinds + 8 : 1 << BITS;
     __shared__ __attribute__((aligned(16))) std::uint16_t count[kWaves][kDigits];  // of a round: of each wave, then of the waves before
     __shared__ int base[kDigits];
-    __shared__ unsigned long long room[kWaves];
+    __shared__ unsigned long long room[3][kWaves];
     __shared__ int most;  // rows of a kind
     if (threadIdx.x == 0) most = 0;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
@@ -96,7 +108,7 @@ __global__ void __launch_bounds__(kThreads) k_group_place(const I* __restrict__ 
         __syncthreads();
         // the round's counts, and in the first round where each kind begins
         int total[(kDigits + kThreads - 1) / kThreads];
-        unsigned long long carry = 0, carry_small = 0, carry_large = 0;
+        Sums<3> carry{};
 #pragma unroll
         for (int c = 0; c < (kDigits + kThreads - 1) / kThreads; ++c) {
             if (c * kThreads > kinds) break;
@@ -116,47 +128,55 @@ __global__ void __launch_bounds__(kThreads) k_group_place(const I* __restrict__ 
             if constexpr (ONE) {
                 all = sum;
             } else if (d <= kinds) {
-#pragma unroll 8
+#pragma unroll 32
                 for (int b = 0; b < static_cast<int>(gridDim.x); ++b) {
                     const int n = counts[b * (kinds + 1LL) + d];
                     before += b < static_cast<int>(blockIdx.x) ? n : 0;
                     all += n;
                 }
             }
-            unsigned long long whole;
-            const unsigned long long seen =
-                sum_before(static_cast<unsigned long long>(all > 0) << 32 | static_cast<unsigned>(all), room, whole) + carry;
-            carry += whole;
-            const int start = static_cast<int>(seen & 0xffffffffu), index = static_cast<int>(seen >> 32);
-            if (d <= kinds) base[d] = start + before;
-            if (blockIdx.x > 0) continue;
+            const unsigned long long seen = static_cast<unsigned long long>(all > 0) << 32 | static_cast<unsigned>(all);
+            if (blockIdx.x > 0) {
+                Sums<1> whole;
+                const Sums<1> sums = sum_before(Sums<1>{seen}, room, whole);
+                if (d <= kinds) base[d] = static_cast<int>((sums.v[0] + carry.v[0]) & 0xffffffffu) + before;
+                carry.v[0] += whole.v[0];
+                continue;
+            }
             // tiles of 64 and 128 rows, and of 256
             const auto tiles = [&](int size) { return static_cast<unsigned>((all + size - 1) / size); };
-            unsigned long long small_whole, large_whole;
-            const unsigned long long small =
-                sum_before(static_cast<unsigned long long>(tiles(64)) << 32 | tiles(128), room, small_whole) + carry_small;
-            const unsigned long long large = sum_before(tiles(256), room, large_whole) + carry_large;
-            carry_small += small_whole, carry_large += large_whole;
+            Sums<3> whole;
+            Sums<3> sums = sum_before(Sums<3>{seen, static_cast<unsigned long long>(tiles(64)) << 32 | tiles(128), tiles(256)}, room, whole);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) sums.v[i] += carry.v[i], carry.v[i] += whole.v[i];
+            const int start = static_cast<int>(sums.v[0] & 0xffffffffu), index = static_cast<int>(sums.v[0] >> 32);
+            int largest = d < kinds ? all : 0;
+#pragma unroll
+            for (int o = 1; o < 64; o *= 2) {
+                const int other = __shfl_xor(largest, o);
+                largest = other > largest ? other : largest;
+            }
+            if (lane == 0) atomicMax(&most, largest);
             if (d > kinds) continue;
+            base[d] = start + before;
             plan[plan_offsets() + d] = start;
-            if (d < kinds) atomicMax(&most, all);
             if (all > 0) {
                 plan[plan_present(kinds) + index] = d;
                 plan[plan_start(kinds) + index] = start;
-                plan[plan_tiles(kinds, 0) + index] = static_cast<int>(small >> 32);
-                plan[plan_tiles(kinds, 1) + index] = static_cast<int>(small & 0xffffffffu);
-                plan[plan_tiles(kinds, 2) + index] = static_cast<int>(large);
+                plan[plan_tiles(kinds, 0) + index] = static_cast<int>(sums.v[1] >> 32);
+                plan[plan_tiles(kinds, 1) + index] = static_cast<int>(sums.v[1] & 0xffffffffu);
+                plan[plan_tiles(kinds, 2) + index] = static_cast<int>(sums.v[2]);
             }
         }
         __syncthreads();
         if (at == first && blockIdx.x == 0 && threadIdx.x == 0) {
-            const int present = static_cast<int>(carry >> 32);
+            const int present = static_cast<int>(carry.v[0] >> 32);
             plan[0] = present;
             plan[1] = static_cast<int>(rows), plan[2] = kinds, plan[3] = most;
             plan[plan_start(kinds) + present] = static_cast<int>(rows);
-            plan[plan_tiles(kinds, 0) + present] = static_cast<int>(carry_small >> 32);
-            plan[plan_tiles(kinds, 1) + present] = static_cast<int>(carry_small & 0xffffffffu);
-            plan[plan_tiles(kinds, 2) + present] = static_cast<int>(carry_large);
+            plan[plan_tiles(kinds, 0) + present] = static_cast<int>(carry.v[1] >> 32);
+            plan[plan_tiles(kinds, 1) + present] = static_cast<int>(carry.v[1] & 0xffffffffu);
+            plan[plan_tiles(kinds, 2) + present] = static_cast<int>(carry.v[2]);
             plan[plan_offsets() + kinds + 1] = static_cast<int>(rows);
         }
 #pragma unroll

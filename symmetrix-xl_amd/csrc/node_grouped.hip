@@ -55,12 +55,18 @@ int tile_for(F&& units, i64 n, i64 k, bool largest) {
 constexpr i64 kFewRows = 16;
 
 Cut cut_rows(Way way, i64 rows, i64 kinds, i64 n, i64 inner, bool direct, bool split) {
-    Cut c{128, direct, 0};
+    Cut c{128, direct, 0, 0, 0};
     const i64 k = kinds < rows ? kinds : rows;
     if (way == Way::Forward && rows <= k * kFewRows) {
         const i64 units = (kinds + 1 < rows ? kinds + 1 : rows) + rows / 16;
         if (units * ((n + 15) / 16) < (1LL << 31)) {
+            // Columns and waves of a workgroup: 64 where that still makes two a unit, and the waves such that each has eight steps or more, of
+            // which four are under way (147 rows of 32 types, 1,024 x 2,048: 22.4 us at 64 and 2, 25.7 at 64 and 4, 48.6 at 16 and
+            // 8; 64 of 8, 4,096 squared FP32: 162, 114 and 118; one row, 2,048 x 4,096: 10.4, 10.1 and 8.2, 7.7 at 16 and 4).
+            const i64 steps = ceil_of(inner * (split ? 4 : 2), kStepBytes);
             c.tile = 16, c.units = static_cast<int>(units);
+            c.columns = units * ceil_of(n, 64) >= 2 * kComputeUnits ? 64 : 16;
+            c.waves = (c.columns == 64 ? 2 : 4) * (steps >= 64 ? 2 : 1);
             return c;
         }
     }
@@ -145,7 +151,7 @@ void product(Way way, const void* a, i64 a_stride, const void* w, i64 w_stride, 
     const bool direct = wide(a, a_stride, k, sizeof(T)) && wide(w, w_stride, w_cols, sizeof(T)) &&
                         (kinds == 1 || w_kind * static_cast<i64>(sizeof(T)) % 16 == 0);
     const Cut cut = cut_rows(way, rows, kinds, n, k, direct, sizeof(T) == 4);
-    p.tiles_m = 1, p.tiles_n = static_cast<int>((n + cut.tile - 1) / cut.tile);
+    p.tiles_m = 1, p.tiles_n = static_cast<int>(ceil_of(n, cut.tile == 16 ? cut.columns : cut.tile));
     require((kinds + 1 + rows / cut.tile) * p.tiles_n < (1LL << 31), "the product has too many tiles");
     launch_grouped<T, O>(p, way, cut, stream);
 }
@@ -163,7 +169,7 @@ void weights_gradient(const void* grad, i64 grad_stride, const void* x, i64 x_st
     const bool direct = wide(grad, grad_stride, m, sizeof(T)) && wide(x, x_stride, n, sizeof(T));
     const Runs runs = runs_for(rows, kinds, m, n, direct && sizeof(T) == 2);
     p.round = static_cast<int>(runs.round), p.least = static_cast<int>(runs.least);
-    const Cut cut{runs.tile, direct, 0};
+    const Cut cut{runs.tile, direct, 0, 0, 0};
     p.tiles_m = static_cast<int>((m + cut.tile - 1) / cut.tile), p.tiles_n = static_cast<int>((n + cut.tile - 1) / cut.tile);
     require((kinds + (runs.least ? rows / runs.least : 0)) * p.tiles_m * p.tiles_n < (1LL << 31), "the product has too many tiles");
     p.partial = static_cast<float*>(workspace);

@@ -810,7 +810,8 @@ __global__ void __launch_bounds__(64 * KS) k_grouped_rows(Grouped<T, O> p) {
 struct Cut {
     int tile;  // 256, 128, 64, or 16: k_grouped_rows
     bool direct;  // rows are aligned to 16 bytes, and as long as whole ones
-    int units;  // of 16 rows, at most
+    int units;    // of 16 rows, at most
+    int columns, waves;  // of a workgroup of k_grouped_rows: 64 and 2 or 4, or 16 and 4 or 8
 };
 
 template <class T, class O>
@@ -847,11 +848,18 @@ void launch_grouped(const Grouped<T, O>& p, Way way, const Cut& cut, hipStream_t
     if (way == Way::ByRows) return tiles(integral_constant<Way, Way::ByRows>{});
     if (way == Way::ByWeights) return tiles(integral_constant<Way, Way::ByWeights>{});
     if (cut.tile != 16) return tiles(integral_constant<Way, Way::Forward>{});
-    const unsigned grid = static_cast<unsigned>(cut.units) * static_cast<unsigned>(p.tiles_n);
-    if (cut.direct)
-        k_grouped_rows<T, O, true, 1, 8><<<grid, 512, 0, stream>>>(p);
-    else
-        k_grouped_rows<T, O, false, 1, 8><<<grid, 512, 0, stream>>>(p);
+    const auto rows = [&](auto nf, auto ks) {
+        constexpr int NF = decltype(nf)::value, KS = decltype(ks)::value;
+        const unsigned grid = static_cast<unsigned>(cut.units) * static_cast<unsigned>(p.tiles_n);
+        if (cut.direct)
+            k_grouped_rows<T, O, true, NF, KS><<<grid, 64 * KS, 0, stream>>>(p);
+        else
+            k_grouped_rows<T, O, false, NF, KS><<<grid, 64 * KS, 0, stream>>>(p);
+    };
+    if (cut.columns == 64 && cut.waves == 2) rows(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+    else if (cut.columns == 64) rows(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+    else if (cut.waves == 4) rows(integral_constant<int, 1>{}, integral_constant<int, 4>{});
+    else rows(integral_constant<int, 1>{}, integral_constant<int, 8>{});
     SMX_LAUNCH_CHECK("k_grouped_rows");
 }
 

@@ -29,7 +29,9 @@ this module refuses to load then.
 
 from __future__ import annotations
 
+import array
 import ctypes
+import operator
 
 import torch
 
@@ -581,29 +583,37 @@ def _packed(t):
     return True
 
 
-class _Tensors:
-    """The addresses, counts and types of tensors, for the length of a call."""
+_dtypes_of = operator.attrgetter("dtype")
+_T = torch.Tensor
 
-    def __init__(self, tensors, name):
-        n = len(tensors)
-        self.tensors = n
-        self.at, self.counts, self.codes = (ctypes.c_void_p * n)(), (ctypes.c_int64 * n)(), (ctypes.c_int32 * n)()
-        device = tensors[0].get_device()
-        for i, t in enumerate(tensors):
-            code = _DTYPES.get(t.dtype)
-            if code is None or t.layout is not torch.strided:
-                raise ValueError("%s must be dense float32, bfloat16 or float16 tensors" % name)
-            if t.get_device() != device:
-                raise ValueError("%s must be on one device" % name)
-            if not _packed(t):
-                raise ValueError("%s must fill their memory without gaps or overlaps" % name)
-            self.at[i], self.counts[i], self.codes[i] = t.data_ptr(), t.numel(), code
-        self.device = device
+
+def _table(tensors, name):
+    """(addresses, counts, type codes, device, whether all are contiguous) of tensors, for the length of a call.  One pass of a built-in over all of
+    them for each: a loop over them in Python took longer than the kernels for a small head's."""
+    try:
+        codes = array.array("i", map(_DTYPES.__getitem__, map(_dtypes_of, tensors)))
+        packed = all(map(_T.is_contiguous, tensors))
+    except (KeyError, RuntimeError):
+        raise ValueError("%s must be dense float32, bfloat16 or float16 tensors" % name) from None
+    devices = set(map(_T.get_device, tensors))
+    if len(devices) != 1:
+        raise ValueError("%s must be on one device" % name)
+    if not packed and not all(map(_packed, tensors)):
+        raise ValueError("%s must fill their memory without gaps or overlaps" % name)
+    return array.array("Q", map(_T.data_ptr, tensors)), array.array("q", map(_T.numel, tensors)), codes, devices.pop(), \
+        packed
+
+
+def _of(a):
+    return a.buffer_info()[0]
+
+
+_NORM_ROOM = lib.smx_gradient_norm_workspace()
 
 
 def _norm_room(like):
-    size = lib.smx_gradient_norm_workspace()
-    return torch.empty((), dtype=torch.float32, device=like.device), _workspace(size, like), size
+    return (torch.empty((), dtype=torch.float32, device=like.device),
+            torch.empty(_NORM_ROOM, dtype=torch.uint8, device=like.device), _NORM_ROOM)
 
 
 def _listed(tensors, name):
@@ -617,35 +627,39 @@ def gradient_norm(tensors, scale=1.0):
     """``scale`` times the 2-norm of all values of ``tensors`` together, a float32 scalar on their device.  The tensors are
     float32, bfloat16 or float16, in any mix, and fill their memory without gaps."""
     tensors = _listed(tensors, "tensors")
-    t = _Tensors(tensors, "tensors")
-    stream = _stream(t.device)
+    at, counts, codes, device, _ = _table(tensors, "tensors")
+    stream = _stream(device)
     norm, room, size = _norm_room(tensors[0])
-    check(lib.smx_gradient_norm(t.at, t.counts, t.codes, t.tensors, scale, norm.data_ptr(), room.data_ptr(), size, stream))
+    check(lib.smx_gradient_norm(_of(at), _of(counts), _of(codes), len(tensors), scale, norm.data_ptr(), room.data_ptr(), size,
+                                stream))
     return norm
 
 
 def clip_gradients(tensors, max_norm, scale=1.0, out=None):
     """Brings ``tensors`` to a norm of ``max_norm`` at most: each becomes ``tensor * scale * min(1, max_norm / norm)``, in place or
-    in ``out`` (tensors of their shapes, of any of the types).  The norm before it, ``scale`` times the 2-norm of all values
+    in ``out`` (tensors of as many values each, in the same order, of any of the types).  The norm before it, ``scale`` times the 2-norm of all values
     (``scale`` of gradients whose loss was scaled, 1 / the loss's), is returned as a float32 scalar on
     their device; nothing waits for it."""
     tensors = _listed(tensors, "tensors")
-    t = _Tensors(tensors, "tensors")
-    o = t
+    at, counts, codes, device, packed = _table(tensors, "tensors")
+    to, to_codes = at, codes
     if out is not None:
         out = _listed(out, "out")
         if len(out) != len(tensors):
             raise ValueError("out must be as many tensors")
-        o = _Tensors(out, "out")
-        if o.device != t.device:
+        to, to_counts, to_codes, to_device, to_packed = _table(out, "out")
+        if to_device != device:
             raise ValueError("out must be on the tensors' device")
-        for a, b in zip(tensors, out):
-            if a.shape != b.shape or (a.stride() != b.stride() and not (a.is_contiguous() and b.is_contiguous())):
-                raise ValueError("out must have the tensors' shapes and strides")
-    stream = _stream(t.device)
+        if to_counts != counts:
+            raise ValueError("out must have the tensors' shapes")
+        # (contiguous ones of as many values hold them in one order)
+        if not (packed and to_packed) and any(a.shape != b.shape or a.stride() != b.stride() for a, b in zip(tensors, out)
+                                              if not (a.is_contiguous() and b.is_contiguous())):
+            raise ValueError("out must have the tensors' shapes and strides")
+    stream = _stream(device)
     norm, room, size = _norm_room(tensors[0])
-    check(lib.smx_clip_gradients(t.at, t.counts, t.codes, t.tensors, max_norm, scale, o.at, o.codes, norm.data_ptr(),
-                                 room.data_ptr(), size, stream))
+    check(lib.smx_clip_gradients(_of(at), _of(counts), _of(codes), len(tensors), max_norm, scale, _of(to), _of(to_codes),
+                                 norm.data_ptr(), room.data_ptr(), size, stream))
     return norm
 
 

@@ -252,10 +252,10 @@ def test_integers_at_the_boundary():
     _bad(product(k=(1 << 17) + 1), "2^17", SMX_ERR_UNSUPPORTED)
     assert product(m=0, a=None, sa=None, out=None) == 0
 
-    size = lib.smx_integer_linear_workspace(4, 6, 8)
-    assert size == 4 * 128 + 16 and lib.smx_integer_linear_workspace(0, 6, 8) == 0
+    size = lib.smx_integer_linear_workspace(40, 6, 8)
+    assert size == 40 * 128 + 160 and lib.smx_integer_linear_workspace(0, 6, 8) == 0
 
-    def linear(x=P, xs=8, dt=1, w=P, sw=P, m=4, n=6, k=8, odt=1, out=P, os=6, room=P, size=size):
+    def linear(x=P, xs=8, dt=1, w=P, sw=P, m=40, n=6, k=8, odt=1, out=P, os=6, room=P, size=size):
         return lib.smx_integer_linear(x, xs, dt, w, sw, m, n, k, odt, out, os, room, size, None)
     _bad(linear(x=None), "x is NULL")
     _bad(linear(w=None), "w is NULL")
