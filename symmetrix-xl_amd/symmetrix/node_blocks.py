@@ -3,11 +3,12 @@
 ``NodeBlocks`` gives per-atom energies from species and per-atom descriptors: the species embedding
 and a linear of the descriptors start each atom's row, residual blocks update it (a norm, an 8-bit
 product that gives the update and its gate side by side, and the gated residual with the
-next norm), and a vector reads the energy out.  It trains like any torch module; ``serve()`` keeps
-the weights in 8-bit blocks and runs a block in two launches, the norm handing its 8-bit rows to the product.
+next norm), and a vector reads the energy out.  With ``by_species`` each species has block weights of its own.  It trains
+like any torch module; ``serve()`` keeps the shared weights in 8-bit blocks, where a block is two launches, the norm handing its
+8-bit rows to the product, or in 8-bit integers, which are finer for a normed row's values.
 First derivatives only: a gradient formed with ``create_graph`` raises ``RuntimeError`` when it is differentiated.
 
-    python -m symmetrix.node_blocks --steps 300
+    python -m symmetrix.node_blocks --steps 300 --by-species --clip 1.0
 
 fits it to the per-atom energies of a MACE evaluator on displaced SrTiO3 cells (random-init
 weights of the tiny shape) and reports the error on a cell that it has not seen, trained and served.
@@ -122,6 +123,27 @@ class _Linear(torch.autograd.Function):
         return dx, dw
 
 
+class _SpeciesLinear(torch.autograd.Function):
+    """Each row through its species' matrix of weight [species][outputs][inputs], brought to x's type; FP32 sums, the weights'
+    gradient in their own type."""
+
+    @staticmethod
+    def forward(ctx, x, weight, groups):
+        w = weight.to(x.dtype)
+        ctx.save_for_backward(x, w)
+        ctx.groups, ctx.weight_dtype = groups, weight.dtype
+        return ops.grouped_linear(x, w, groups)
+
+    @staticmethod
+    @_once
+    def backward(ctx, grad):
+        x, w = ctx.saved_tensors
+        need_x, need_w, _ = ctx.needs_input_grad
+        same = ctx.weight_dtype if ctx.weight_dtype is x.dtype else torch.float32
+        dx, dw = ops.grouped_linear_gradient(grad.contiguous(), x if need_w else None, w if need_x else None, ctx.groups, same)
+        return dx, None if dw is None else dw.to(ctx.weight_dtype), None
+
+
 def _masked(types, descriptors, num_types):
     """(which atoms have a type of the table, the descriptors with zeros for the others): a masked atom's row is
     then zero all through, and shares no scale of 8-bit blocks with its neighbours."""
@@ -135,10 +157,10 @@ def _energies(h, readout, shift, types, there):
 
 class NodeBlocks(torch.nn.Module):
     """Per-atom energies of ``types`` [atoms] and ``descriptors`` [atoms][descriptors].  Rows are
-    ``dtype``; parameters are float32.  An atom whose type is outside [0, num_types) is masked, as in
+    ``dtype``; parameters are float32.  With ``by_species`` a block's weights are a matrix for each type (up to 4,096 types).  An atom whose type is outside [0, num_types) is masked, as in
     ``node_ops.embed``: its energy is zero, its descriptors are not looked at and nothing is learned from it."""
 
-    def __init__(self, num_types, num_descriptors, channels=128, blocks=2, dtype=torch.float32, eps=1e-6):
+    def __init__(self, num_types, num_descriptors, channels=128, blocks=2, dtype=torch.float32, eps=1e-6, by_species=False):
         super().__init__()
 
         def normal(*shape, scale=1.0):
@@ -146,12 +168,13 @@ class NodeBlocks(torch.nn.Module):
 
         def ones(value=1.0):
             return torch.nn.Parameter(torch.full((channels,), value))
-        self.dtype, self.eps, self.channels = dtype, eps, channels
+        self.dtype, self.eps, self.channels, self.by_species = dtype, eps, channels, by_species
+        own = (num_types,) if by_species else ()
         self.table = normal(num_types, channels, scale=1 / math.sqrt(channels))
         self.lift = normal(channels, num_descriptors, scale=1 / math.sqrt(num_descriptors))
         self.before = ones()
         self.weights = torch.nn.ParameterList(
-            [normal(2 * channels, channels, scale=1 / math.sqrt(channels)) for _ in range(blocks)])
+            [normal(*own, 2 * channels, channels, scale=1 / math.sqrt(channels)) for _ in range(blocks)])
         self.post = torch.nn.ParameterList([ones() for _ in range(blocks)])
         self.scale = torch.nn.ParameterList([ones(0.5) for _ in range(blocks)])
         self.next = torch.nn.ParameterList([ones() for _ in range(blocks)])
@@ -164,16 +187,23 @@ class NodeBlocks(torch.nn.Module):
         x = _Embed.apply(self.table.to(t), types, math.sqrt(self.channels))
         x = x + _Linear.apply(descriptors.to(t), self.lift)
         h = _Norm.apply(x, self.before, self.eps)
+        groups = ops.group_rows(types, self.table.shape[0]) if self.by_species else None
         for w, post, scale, nxt in zip(self.weights, self.post, self.scale, self.next):
-            x, h = _GatedResidual.apply(x, _Linear.apply(h, w), post, scale, nxt, self.eps)
+            both = _SpeciesLinear.apply(h, w, groups) if self.by_species else _Linear.apply(h, w)
+            x, h = _GatedResidual.apply(x, both, post, scale, nxt, self.eps)
         return _energies(h, self.readout, self.shift, types, there)
 
-    def serve(self):
-        """A function of (types, descriptors) with the present weights in 8-bit blocks."""
+    def serve(self, form="blocks"):
+        """A function of (types, descriptors) with the present weights in 8-bit ``form``: "blocks" (E4M3 with a scale for each
+        128) or "integers" (with a scale for each row).  Weights by species are kept in the rows' type."""
+        if form not in ("blocks", "integers"):
+            raise ValueError("weights are served in blocks or integers")
+        quantize, linear = (ops.quantize, ops.block_linear) if form == "blocks" else (ops.quantize_integers, ops.integer_linear)
+        by_species, handed = self.by_species, form == "blocks" and not self.by_species
         with torch.no_grad():
             t = self.dtype
-            table, lift = self.table.detach().to(t).clone(), ops.quantize(self.lift.detach().to(t))
-            weights = [ops.quantize(w.detach().to(t)) for w in self.weights]
+            table, lift = self.table.detach().to(t).clone(), quantize(self.lift.detach().to(t))
+            weights = [w.detach().to(t).clone() if by_species else quantize(w.detach().to(t)) for w in self.weights]
             before, readout, shift = (p.detach().clone() for p in (self.before, self.readout, self.shift))
             vectors = [tuple(p.detach().clone() for p in v) for v in zip(self.post, self.scale, self.next)]
         c, eps = self.channels, self.eps
@@ -182,12 +212,17 @@ class NodeBlocks(torch.nn.Module):
         def energies(types, descriptors):
             there, descriptors = _masked(types, descriptors, table.shape[0])
             x = ops.embed(types, table, math.sqrt(c))
-            x += ops.block_linear(descriptors.to(t), lift)
-            h = ops.norm(x, before, eps, quantized=True)
+            x += linear(descriptors.to(t), lift)
+            # (rows handed to a block product are in blocks already)
+            h = ops.norm(x, before, eps, quantized=handed)
+            groups = ops.group_rows(types, table.shape[0]) if by_species and weights else None
             for k, (w, (post, scale, nxt)) in enumerate(zip(weights, vectors)):
-                both = ops.block_product(h, w, t)
+                if by_species:
+                    both = ops.grouped_linear(h, w, groups)
+                else:
+                    both = ops.block_product(h, w, t) if handed else ops.integer_linear(h, w)
                 x, h = ops.residual_norm(x, both[:, :c], post, both[:, c:], scale, nxt, eps,
-                                         quantized=k + 1 < len(weights))
+                                         quantized=handed and k + 1 < len(weights))
             return _energies(h if weights else ops.norm(x, before, eps), readout, shift, types, there)
         return energies
 
@@ -211,9 +246,10 @@ def descriptors_of(system, type_of, cutoff=5.0, radial=8):
     return out.reshape(n, -1).astype(np.float32)
 
 
-def fit(steps=300, cells=3, channels=128, blocks=2, dtype=torch.float32, seed=0, report=print):
+def fit(steps=300, cells=3, channels=128, blocks=2, dtype=torch.float32, seed=0, report=print, by_species=False, clip=None,
+        form="blocks"):
     """Fits the head to an evaluator's per-atom energies; the errors (eV/atom, root mean square) on an unseen cell of
-    the trained head and of the served one, and that of the species' means."""
+    the trained head and of the served one, and that of the species' means.  ``clip``: the largest norm of a step's gradients."""
     import numpy as np
 
     from . import random_model, systems
@@ -238,13 +274,15 @@ def fit(steps=300, cells=3, channels=128, blocks=2, dtype=torch.float32, seed=0,
     target = energy - means[types.long()]
     unit = target[train].std()
     target = (target / unit).float()
-    model = NodeBlocks(len(type_of), desc.shape[1], channels, blocks, dtype).cuda()
+    model = NodeBlocks(len(type_of), desc.shape[1], channels, blocks, dtype, by_species=by_species).cuda()
     adam = torch.optim.Adam(model.parameters(), lr=2e-3)
     begin = time.perf_counter()
     for step in range(steps):
         adam.zero_grad(set_to_none=True)
         loss = (model(types[train], desc[train]) - target[train]).square().mean()
         loss.backward()
+        if clip is not None:
+            ops.clip_gradients([p.grad for p in model.parameters()], clip)
         adam.step()
         if report and (step % 100 == 0 or step + 1 == steps):
             report("step %d: loss %.4f" % (step, loss.item()))
@@ -253,7 +291,7 @@ def fit(steps=300, cells=3, channels=128, blocks=2, dtype=torch.float32, seed=0,
     def error(values):
         return float(((values - target[test]) * unit).square().mean().sqrt())
     with torch.no_grad():
-        trained, served = error(model(types[test], desc[test])), error(model.serve()(types[test], desc[test]))
+        trained, served = error(model(types[test], desc[test])), error(model.serve(form)(types[test], desc[test]))
     result = {"trained": trained, "served": served, "means": error(torch.zeros_like(target[test])),
               "ms_per_step": 1e3 * took / max(1, steps)}
     if report:
@@ -269,8 +307,12 @@ def main(argv=None):
     ap.add_argument("--channels", type=int, default=128)
     ap.add_argument("--blocks", type=int, default=2)
     ap.add_argument("--dtype", choices=("float32", "bfloat16", "float16"), default="float32")
+    ap.add_argument("--by-species", action="store_true", help="block weights for each species")
+    ap.add_argument("--clip", type=float, help="the largest norm of a step's gradients")
+    ap.add_argument("--form", choices=("blocks", "integers"), default="blocks", help="the served weights' 8-bit form")
     args = ap.parse_args(argv)
-    fit(args.steps, args.cells, args.channels, args.blocks, getattr(torch, args.dtype))
+    fit(args.steps, args.cells, args.channels, args.blocks, getattr(torch, args.dtype), by_species=args.by_species,
+        clip=args.clip, form=args.form)
 
 
 if __name__ == "__main__":

@@ -31,6 +31,7 @@ from __future__ import annotations
 
 import array
 import ctypes
+import functools
 import operator
 
 import torch
@@ -465,10 +466,15 @@ class RowGroups:
 
     @property
     def order(self):
-        return self._room[lib.smx_group_plan_order(self.num_types) // 4:]
+        return self._room[_plan_order(self.num_types) // 4:]
 
     def __reduce__(self):
         raise TypeError("RowGroups are not copied: make them of the types again (symmetrix.node_ops.group_rows)")
+
+
+@functools.lru_cache(maxsize=None)
+def _plan_order(num_types):
+    return lib.smx_group_plan_order(num_types)
 
 
 def group_rows(types, num_types):
@@ -480,7 +486,7 @@ def group_rows(types, num_types):
         raise SymmetrixUnsupportedError("rows are grouped by up to 4096 types")
     stream = _stream(types.get_device())
     t = types.shape[0]
-    size = lib.smx_group_plan_bytes(t, num_types)
+    size = _plan_order(num_types) + 4 * t
     plan = torch.empty(size // 4, dtype=torch.int32, device=types.device)
     work = lib.smx_group_rows_workspace(t, num_types)
     room = _workspace(work, types)
