@@ -792,7 +792,6 @@ __global__ void __launch_bounds__(64 * KS) k_grouped_rows(Grouped<T, O> p) {
     const int rows = start[at + 1] - row0 < 16 ? start[at + 1] - row0 : 16, row = lane % 16;
     if (rows <= 0) return;
     const int id = order[row0 + (row < rows ? row : rows - 1)];
-    acc4 sum{0.0f, 0.0f, 0.0f, 0.0f};
     if (kind < p.kinds) {
         const T* b[NF];
 #pragma unroll
@@ -800,10 +799,12 @@ __global__ void __launch_bounds__(64 * KS) k_grouped_rows(Grouped<T, O> p) {
             const int j = j0 + 16 * g + row;
             b[g] = p.b + kind * p.b_kind + (j < p.n ? j : p.n - 1) * p.b_stride;
         }
-        sum = few_rows<T, DIRECT, NF, KS>(p.a + id * p.a_stride, b, p.k, room);
+        few_rows<T, DIRECT, NF, KS>(p.a + id * p.a_stride, b, p.k, room);
     }
-    if (wave >= NF || row >= rows) return;
-    store_outputs(p.out + id * p.out_stride, j0 + 16 * wave + 4 * (lane / 16), p.n, sum);
+    if (row >= rows) return;
+    for (int g = wave; g < NF; g += KS)
+        store_outputs(p.out + id * p.out_stride, j0 + 16 * g + 4 * (lane / 16), p.n,
+                      kind < p.kinds ? joined(room, g) : acc4{0.0f, 0.0f, 0.0f, 0.0f});
 }
 
 // How a call is cut (node_grouped.hip).

@@ -260,9 +260,8 @@ __global__ void __launch_bounds__(64 * KS) k_integer_rows(Integers<O> p) {
         const int j = j0 + 16 * g + row;
         b[g] = p.b + (j < p.n ? j : p.n - 1) * p.pitch;
     }
-    const i32x4 sum = few_rows<T, true, NF, KS>(p.a + (row < p.m ? row : p.m - 1) * p.pitch, b, static_cast<int>(p.pitch), room);
-    if (wave >= NF) return;
-    store_scaled(p, row, j0 + 16 * wave + 4 * (lane / 16), sum);
+    few_rows<T, true, NF, KS>(p.a + (row < p.m ? row : p.m - 1) * p.pitch, b, static_cast<int>(p.pitch), room);
+    for (int g = wave; g < NF; g += KS) store_scaled(p, row, j0 + 16 * g + 4 * (lane / 16), joined(room, g));
 }
 
 // Up to kRawRows rows of x as they are given, of up to kRawTerms values: each workgroup brings them to integers itself, in LDS, while its
@@ -360,10 +359,7 @@ __global__ void __launch_bounds__(64 * KS) k_integer_raw(Integers<O> p, const T*
     room.v[wave][0][lane] = acc;
     __syncthreads();
     if (wave > 0) return;
-    i32x4 sum = room.v[0][0][lane];
-#pragma unroll
-    for (int w = 1; w < KS; ++w) sum += room.v[w][0][lane];
-    store_scaled(p, row, j0 + 4 * (lane / 16), sum, mine);
+    store_scaled(p, row, j0 + 4 * (lane / 16), joined(room, 0), mine);
 }
 
 template <class O>

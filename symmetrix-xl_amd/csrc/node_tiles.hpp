@@ -232,10 +232,10 @@ struct FewRoom {
 };
 
 // Sixteen rows of a times 16 NF rows of b by KS waves, every KS-th step each, joined in LDS: where the bytes of b are all of it, they
-// go straight to registers, kAhead steps of them under way at once.  `a` and `b`: the rows of the lane (l % 16).  Fragment g's sums
-// are wave g's (lane l: column l % 16, four rows of b from 4 (l / 16) on).
+// go straight to registers, kAhead steps of them under way at once.  `a` and `b`: the rows of the lane (l % 16).  The sums of the
+// waves are left in the room; joined() adds up fragment g's (lane l: column l % 16, four rows of b from 4 (l / 16) on).
 template <class T, bool DIRECT, int NF, int KS>
-__device__ __forceinline__ SumOf<T> few_rows(const T* a, const T* const (&b)[NF], int k, FewRoom<T, NF, KS>& room) {
+__device__ __forceinline__ void few_rows(const T* a, const T* const (&b)[NF], int k, FewRoom<T, NF, KS>& room) {
     using Sum = SumOf<T>;
     constexpr int kAhead = 4, kValues = kStepBytes / static_cast<int>(sizeof(T)), kPer = 16 / static_cast<int>(sizeof(T));
     // (a wave's branches have to be the whole wave's to the compiler too: matrix instructions run for all lanes)
@@ -296,10 +296,14 @@ __device__ __forceinline__ SumOf<T> few_rows(const T* a, const T* const (&b)[NF]
 #pragma unroll
     for (int g = 0; g < NF; ++g) room.v[wave][g][lane] = acc[g];
     __syncthreads();
-    const int mine = wave < NF ? wave : 0;
-    Sum sum = room.v[0][mine][lane];
+}
+
+template <class T, int NF, int KS>
+__device__ __forceinline__ SumOf<T> joined(const FewRoom<T, NF, KS>& room, int g) {
+    const int lane = threadIdx.x % 64;
+    SumOf<T> sum = room.v[0][g][lane];
 #pragma unroll
-    for (int w = 1; w < KS; ++w) sum += room.v[w][mine][lane];
+    for (int w = 1; w < KS; ++w) sum += room.v[w][g][lane];
     return sum;
 }
 
