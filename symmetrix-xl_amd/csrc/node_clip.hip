@@ -113,6 +113,29 @@ __global__ void __launch_bounds__(kThreads) k_norm_join(const double* __restrict
     if (threadIdx.x == 0) *norm = static_cast<float>(v);
 }
 
+// out = at * by * two: sixteen bytes of the outputs a lane, side by side for neighbouring lanes.
+template <class T, class O>
+__device__ __forceinline__ void scaled(const T* at, O* out, i64 n, float by, float two) {
+    constexpr int N = 16 / sizeof(O), kAhead = 4;
+    i64 c = N * static_cast<i64>(threadIdx.x);
+    for (; c + N * kThreads * (kAhead - 1) + N <= n; c += N * kThreads * kAhead) {
+        Pack<T, N> e[kAhead];
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) e[q] = *reinterpret_cast<const Pack<T, N>*>(at + c + N * kThreads * q);
+#pragma unroll
+        for (int q = 0; q < kAhead; ++q) {
+            Pack<O, N> o;
+#pragma unroll
+            for (int i = 0; i < N; ++i) o.v[i] = static_cast<O>(static_cast<float>(e[q].v[i]) * by * two);
+            *reinterpret_cast<Pack<O, N>*>(out + c + N * kThreads * q) = o;
+        }
+    }
+    for (; c < n; c += N * kThreads)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (c + i < n) out[c + i] = static_cast<O>(static_cast<float>(at[c + i]) * by * two);
+}
+
 __global__ void __launch_bounds__(kThreads) k_clip(Tensors t, const double* __restrict__ parts, int count, float scale,
                                                    float max_norm, float* __restrict__ norm) {
     __shared__ double room[kThreads / 64];
@@ -134,12 +157,7 @@ __global__ void __launch_bounds__(kThreads) k_clip(Tensors t, const double* __re
         const bool whole = factor == 1.0;
         const auto go = [&](auto* at, auto* out) {
             if (whole && static_cast<const void*>(at) == out) return;  // values as they are, in place
-            each_eight(at + from, n, [&](const auto& e, i64 c, int left) {
-                float v[8];
-#pragma unroll
-                for (int q = 0; q < 8; ++q) v[q] = e[q] * by * two;
-                store_eight(out + from + c, 0, left, v);
-            });
+            scaled(at + from, out + from, n, by, two);
         };
         const auto to = [&](auto* at) {
             if (t.out_kind[i] == SMX_DTYPE_F32) go(at, static_cast<float*>(t.out[i]));
