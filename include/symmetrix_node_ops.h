@@ -166,7 +166,7 @@ SMX_API int32_t smx_block_linear(const void* x, int64_t x_stride, int32_t dtype,
 
 /* A plan of `rows` rows by their kind, types[t] in [0, num_types) (int32, or int64 when types_are_64bit); a row of another
  * type is masked.  The plan is device memory (16-byte aligned, smx_group_plan_bytes of it), an input of the products below for
- * the same rows and num_types.  As int32 it holds from byte 16 on the offsets, num_types + 1 of them (of the sorted rows of
+ * the same rows and num_types (with a plan of others they write nothing).  As int32 it holds from byte 16 on the offsets, num_types + 1 of them (of the sorted rows of
  * type z the first is offsets[z] and the one past the last offsets[z + 1]), and from byte smx_group_plan_order on the rows
  * in order: by type, of one type as they come, the masked ones last.  Up to 2^30 rows and 4,096 types. */
 SMX_API int64_t smx_group_plan_bytes(int64_t rows, int64_t num_types);
@@ -177,8 +177,8 @@ SMX_API int32_t smx_group_rows(const void* types, int32_t types_are_64bit, int64
 
 /* out[t] = w[z] x[t] with z the type of row t and w [num_types][outputs][inputs] (w_stride between rows, w_type_stride
  * between types, in values); the rows of masked t are zeros.  Values are `dtype`, out is out_dtype: that or FP32.  Products of FP32
- * values are formed of three bf16 parts of each, to FP32's precision (2^-24 of a product; a value below 2^-110 is off by up to
- * 2^-134).  An infinity or NaN makes the outputs infinite or NaN that it is a term of, and no others.  inputs, outputs
+ * values are formed of three bf16 parts of each, to FP32's precision (2^-24 of a product; parts below 2^-126 count as zero, so a
+ * value below 2^-102 is off by up to 2^-126).  An infinity or NaN makes the outputs infinite or NaN that it is a term of, and no others.  inputs, outputs
  * <= 2^24. */
 SMX_API int32_t smx_grouped_linear(const void* x, int64_t x_stride, int32_t dtype, const void* w, int64_t w_stride,
                                    int64_t w_type_stride, const void* plan, int64_t rows, int64_t num_types, int64_t inputs,

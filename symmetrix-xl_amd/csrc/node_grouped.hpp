@@ -22,7 +22,6 @@ namespace node {
 // and first tiles of 64, 128 and 256 rows; the order.  Rows of no kind are kind `kinds`. ----
 
 constexpr i64 kMostKinds = 4096;
-constexpr i64 kMostRows = (1LL << 31) - 65536;
 
 inline __host__ __device__ i64 plan_room(i64 kinds) { return (kinds + 5) / 4 * 4; }
 inline __host__ __device__ i64 plan_offsets() { return 4; }
@@ -31,6 +30,9 @@ inline __host__ __device__ i64 plan_start(i64 kinds) { return 4 + 2 * plan_room(
 // the first tile of each of these kinds, and the number of tiles, where tiles have 64 << size rows
 inline __host__ __device__ i64 plan_tiles(i64 kinds, int size) { return 4 + (3 + size) * plan_room(kinds); }
 inline __host__ __device__ i64 plan_order(i64 kinds) { return 4 + 6 * plan_room(kinds); }
+
+// whether a plan is of so many rows and kinds: nothing is read or written by another
+__device__ __forceinline__ bool plan_fits(const int* plan, int rows, int kinds) { return plan[1] == rows && plan[2] == kinds; }
 
 enum class Way { Forward, ByRows, ByWeights };
 
@@ -130,10 +132,16 @@ struct Walk {
 
     __device__ __forceinline__ explicit Walk(const Grouped<T, O>& p) : of(&p), order(p.plan + plan_order(p.kinds)), turn(blockIdx.x) {
         const int lane = threadIdx.x % 64;
+        count = run = units = tiles = 0, even = false;
+        base_of = first_of = end_of = kind_of = 0;
+        if (!__builtin_amdgcn_readfirstlane(plan_fits(p.plan, p.tokens, p.kinds))) return;
         count = __builtin_amdgcn_readfirstlane(WAY == Way::ByWeights ? p.kinds : p.plan[0]);
-        run = WAY == Way::ByWeights ? __builtin_amdgcn_readfirstlane(run_of(p.plan, p.tokens, p.round, p.least)) : 0;
-        even = WAY == Way::ByWeights && p.tiles_m * p.tiles_n <= 64 &&
-               __builtin_amdgcn_readfirstlane(run <= p.tokens || static_cast<i64>(p.plan[3]) * p.plan[0] <= 3 * (static_cast<i64>(p.tokens) / 2));
+        if constexpr (WAY == Way::ByWeights) {
+            run = __builtin_amdgcn_readfirstlane(run_of(p.plan, p.tokens, p.round, p.least));
+            even = p.tiles_m * p.tiles_n <= 64 &&
+                   __builtin_amdgcn_readfirstlane(run <= p.tokens ||
+                                                  static_cast<i64>(p.plan[3]) * p.plan[0] <= 3 * (static_cast<i64>(p.tokens) / 2));
+        }
         const int at = lane < count ? lane : count - 1;
         base_of = base(at), first_of = starts()[at], end_of = starts()[at + 1];
         kind_of = WAY == Way::ByWeights ? at : p.plan[plan_present(p.kinds) + at];
@@ -742,7 +750,9 @@ __global__ void __launch_bounds__(64 * WM * WN, BM == 128 ? 2 : 4) k_grouped_hel
 // values a lane.
 template <class O>
 __global__ void __launch_bounds__(256) k_grouped_join(Grouped<O, O> p) {
-    const int run = run_of(p.plan, p.tokens, p.round, p.least), kinds = p.kinds, lane = threadIdx.x % 64;
+    const int kinds = p.kinds, lane = threadIdx.x % 64;
+    if (!plan_fits(p.plan, p.tokens, kinds)) return;
+    const int run = run_of(p.plan, p.tokens, p.round, p.least);
     if (run > p.tokens) return;
     const int* const offsets = p.plan + plan_offsets();
     const i64 size = static_cast<i64>(p.m) * p.n;
@@ -785,7 +795,7 @@ __global__ void __launch_bounds__(64 * KS) k_grouped_rows(Grouped<T, O> p) {
     __shared__ FewRoom<T, NF, KS> room;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int present = p.plan[0], u = blockIdx.x / p.tiles_n, j0 = blockIdx.x % p.tiles_n * 16 * NF;
-    if (u >= present + p.tokens / 16) return;
+    if (u >= present + p.tokens / 16 || !plan_fits(p.plan, p.tokens, p.kinds)) return;
     const int* const start = p.plan + plan_start(p.kinds);
     const int* const order = p.plan + plan_order(p.kinds);
     const int at = last_up_to(u, present, [&](int q) { return q + start[q] / 16; });

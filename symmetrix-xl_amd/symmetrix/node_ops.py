@@ -453,20 +453,24 @@ def block_linear_gradient(grad, w_columns, x_columns, dtype=None):
 
 class RowGroups:
     """Rows in the order of their types (``group_rows``): ``order`` int32 [rows], by type, of one type as they come, masked
-    ones last; ``offsets`` int32 [num_types + 1], where each type's rows begin in it.  Both lie on the device."""
+    ones last; ``offsets`` int32 [num_types + 1], where each type's rows begin in it.  Both lie on the device and are what the
+    products read: they are not to be written to."""
 
-    __slots__ = ("rows", "num_types", "_room")
+    __slots__ = ("_rows", "_num_types", "_room")
 
     def __init__(self, rows, num_types, room):
-        self.rows, self.num_types, self._room = rows, num_types, room
+        self._rows, self._num_types, self._room = rows, num_types, room
+
+    rows = property(lambda self: self._rows)
+    num_types = property(lambda self: self._num_types)
 
     @property
     def offsets(self):
-        return self._room[4:5 + self.num_types]
+        return self._room[4:5 + self._num_types]
 
     @property
     def order(self):
-        return self._room[_plan_order(self.num_types) // 4:]
+        return self._room[_plan_order(self._num_types) // 4:]
 
     def __reduce__(self):
         raise TypeError("RowGroups are not copied: make them of the types again (symmetrix.node_ops.group_rows)")
@@ -589,7 +593,7 @@ def _packed(t):
     return True
 
 
-_dtypes_of = operator.attrgetter("dtype")
+_dtypes_of, _needs_grad = operator.attrgetter("dtype"), operator.attrgetter("requires_grad")
 _T = torch.Tensor
 
 
@@ -645,7 +649,7 @@ def clip_gradients(tensors, max_norm, scale=1.0, out=None):
     """Brings ``tensors`` to a norm of ``max_norm`` at most: each becomes ``tensor * scale * min(1, max_norm / norm)``, in place or
     in ``out`` (tensors of as many values each, in the same order, of any of the types).  The norm before it, ``scale`` times the 2-norm of all values
     (``scale`` of gradients whose loss was scaled, 1 / the loss's), is returned as a float32 scalar on
-    their device; nothing waits for it."""
+    their device; nothing waits for it.  Changed tensors do not ask for gradients themselves."""
     tensors = _listed(tensors, "tensors")
     at, counts, codes, device, packed = _table(tensors, "tensors")
     to, to_codes = at, codes
@@ -662,6 +666,8 @@ def clip_gradients(tensors, max_norm, scale=1.0, out=None):
         if not (packed and to_packed) and any(a.shape != b.shape or a.stride() != b.stride() for a, b in zip(tensors, out)
                                               if not (a.is_contiguous() and b.is_contiguous())):
             raise ValueError("out must have the tensors' shapes and strides")
+    if any(map(_needs_grad, tensors if out is None else out)):
+        raise ValueError("tensors that are changed must not ask for gradients themselves: detach them")
     stream = _stream(device)
     norm, room, size = _norm_room(tensors[0])
     check(lib.smx_clip_gradients(_of(at), _of(counts), _of(codes), len(tensors), max_norm, scale, _of(to), _of(to_codes),
@@ -677,7 +683,7 @@ class IntegerValues:
     ``scales`` [rows].  Copies (``copy``, ``pickle``, ``torch.save`` and ``torch.load``) are made of these tensors and
     checked like new ones."""
 
-    __slots__ = ("shape", "values", "scales")
+    __slots__ = ("_shape", "_values", "_scales")
 
     def __init__(self, values, scales, shape):
         rows, cols = shape
@@ -689,7 +695,11 @@ class IntegerValues:
             raise ValueError("scales must be contiguous float32 [%d]" % rows)
         if values.device != scales.device:
             raise ValueError("values and scales must be on one device")
-        self.shape, self.values, self.scales = (rows, cols), values, scales
+        self._shape, self._values, self._scales = (rows, cols), values, scales
+
+    shape = property(lambda self: self._shape)
+    values = property(lambda self: self._values)
+    scales = property(lambda self: self._scales)
 
     def __reduce__(self):
         return IntegerValues, (self.values, self.scales, self.shape)
@@ -708,10 +718,10 @@ def quantize_integers(x):
     code, r, c, stride = _rows(x, "x")
     stream = _stream(x.get_device())
     out = IntegerValues.__new__(IntegerValues)
-    out.shape = (r, c)
-    out.values = torch.empty((r, -(-c // 128) * 128), dtype=torch.int8, device=x.device)
-    out.scales = torch.empty(r, dtype=torch.float32, device=x.device)
-    check(lib.smx_integer_quantize(x.data_ptr(), stride, code, r, c, out.values.data_ptr(), out.scales.data_ptr(), stream))
+    out._shape = (r, c)
+    out._values = torch.empty((r, -(-c // 128) * 128), dtype=torch.int8, device=x.device)
+    out._scales = torch.empty(r, dtype=torch.float32, device=x.device)
+    check(lib.smx_integer_quantize(x.data_ptr(), stride, code, r, c, out._values.data_ptr(), out._scales.data_ptr(), stream))
     return out
 
 

@@ -160,6 +160,12 @@ def test_clip_gradients():
                       ([a.clone(), b.int()], "float32, bfloat16 or float16")):
         with pytest.raises(ValueError, match=text):
             node_ops.clip_gradients([a, b], 1.0, out=out)
+    with pytest.raises(ValueError, match="detach"):
+        node_ops.clip_gradients([a, b.clone().requires_grad_()], 1.0)
+    with pytest.raises(ValueError, match="detach"):
+        node_ops.clip_gradients([a], 1.0, out=[a.clone().requires_grad_()])
+    with pytest.raises(ValueError, match="HIP device"):
+        node_ops.clip_gradients([a.clone().requires_grad_()], 1.0, out=[a])
 
 
 def test_clipping_at_the_boundary():
@@ -222,6 +228,12 @@ def test_integers():
                        ((values, torch.zeros(5), (6, 8)), "scales"), ((values, torch.zeros(12)[::2], (6, 8)), "scales")):
         with pytest.raises(ValueError, match=text):
             node_ops.IntegerValues(*args)
+    for name in ("values", "scales", "shape"):
+        with pytest.raises(AttributeError):
+            setattr(w, name, None)
+    for name in ("rows", "num_types", "order", "offsets"):
+        with pytest.raises(AttributeError):
+            setattr(_groups(5, 3), name, None)
     back = pickle.loads(pickle.dumps(w))
     assert back.shape == w.shape and torch.equal(back.values, w.values)
 
