@@ -70,7 +70,8 @@ template <class I, int BITS, bool ONE>
 __global__ void __launch_bounds__(kThreads) k_group_place(const I* __restrict__ types, i64 rows, int kinds, i64 tile,
                                                           const int* __restrict__ counts, int* __restrict__ plan) {
     constexpr int kDigits = BITS == 13 ? kMostKinds + 8 : 1 << BITS;
-    __shared__ __attribute__((aligned(16))) std::uint16_t count[kWaves][kDigits];  // of a round: of each wave, then of the waves before
+    // of a round: of each wave, then of the waves before; a kind's sixteen are 32 bytes
+    __shared__ __attribute__((aligned(16))) std::uint16_t count[kDigits][kWaves];
     __shared__ int base[kDigits];
     __shared__ unsigned long long room[3][kWaves];
     __shared__ int most;  // rows of a kind
@@ -99,10 +100,10 @@ __global__ void __launch_bounds__(kThreads) k_group_place(const I* __restrict__ 
                 same &= kind[k] >> b & 1 ? w : ~w;
             }
             const int before = __popcll(same & ((1ull << lane) - 1));
-            const int had = in[k] ? count[wave][kind[k]] : 0;
+            const int had = in[k] ? count[kind[k]][wave] : 0;
             rank[k] = had + before;
             __builtin_amdgcn_wave_barrier();
-            if (in[k] && before == 0) count[wave][kind[k]] = static_cast<std::uint16_t>(had + __popcll(same));
+            if (in[k] && before == 0) count[kind[k]][wave] = static_cast<std::uint16_t>(had + __popcll(same));
             __builtin_amdgcn_wave_barrier();
         }
         __syncthreads();
@@ -115,12 +116,16 @@ __global__ void __launch_bounds__(kThreads) k_group_place(const I* __restrict__ 
             const int d = c * kThreads + threadIdx.x;
             int sum = 0;
             if (d <= kinds) {
+                uint4* const mine = reinterpret_cast<uint4*>(count[d]);
+                uint4 w[2] = {mine[0], mine[1]};
+                unsigned* const two = reinterpret_cast<unsigned*>(w);
 #pragma unroll
-                for (int w = 0; w < kWaves; ++w) {
-                    const int n = count[w][d];
-                    count[w][d] = static_cast<std::uint16_t>(sum);
-                    sum += n;
+                for (int i = 0; i < kWaves / 2; ++i) {
+                    const unsigned lo = two[i] & 0xffffu, hi = two[i] >> 16;
+                    two[i] = static_cast<unsigned>(sum) | (static_cast<unsigned>(sum) + lo) << 16;
+                    sum += static_cast<int>(lo + hi);
                 }
+                mine[0] = w[0], mine[1] = w[1];
             }
             total[c] = sum;
             if (at > first) continue;
@@ -182,7 +187,7 @@ __global__ void __launch_bounds__(kThreads) k_group_place(const I* __restrict__ 
 #pragma unroll
         for (int k = 0; k < kPerLane; ++k)
             if (in[k])
-                order[base[kind[k]] + count[wave][kind[k]] + rank[k]] = static_cast<int>(at + wave * 64 * kPerLane + 64 * k + lane);
+                order[base[kind[k]] + count[kind[k]][wave] + rank[k]] = static_cast<int>(at + wave * 64 * kPerLane + 64 * k + lane);
         if (at + kRows >= last) return;
         __syncthreads();
 #pragma unroll

@@ -476,9 +476,14 @@ class RowGroups:
         raise TypeError("RowGroups are not copied: make them of the types again (symmetrix.node_ops.group_rows)")
 
 
-@functools.lru_cache(maxsize=None)
-def _plan_order(num_types):
-    return lib.smx_group_plan_order(num_types)
+def _size(function):
+    """A library function of sizes alone, whose answers are kept: the call costs as much as an allocation."""
+    return functools.lru_cache(maxsize=1024)(lambda *sizes: function(*sizes))
+
+
+_plan_order = _size(lib.smx_group_plan_order)
+_group_room, _weights_room, _integer_room = (_size(f) for f in (
+    lib.smx_group_rows_workspace, lib.smx_grouped_linear_by_weights_workspace, lib.smx_integer_linear_workspace))
 
 
 def group_rows(types, num_types):
@@ -492,7 +497,7 @@ def group_rows(types, num_types):
     t = types.shape[0]
     size = _plan_order(num_types) + 4 * t
     plan = torch.empty(size // 4, dtype=torch.int32, device=types.device)
-    work = lib.smx_group_rows_workspace(t, num_types)
+    work = _group_room(t, num_types)
     room = _workspace(work, types)
     check(lib.smx_group_rows(types.data_ptr(), wide, t, num_types, plan.data_ptr(), size, _at(room), work, stream))
     return RowGroups(t, num_types, plan)
@@ -571,7 +576,7 @@ def grouped_linear_gradient(grad, x, w, groups, dtype=None):
                                              code, dx.data_ptr(), w.shape[2], stream))
     if x is not None:
         dw = torch.empty((v, n, k), dtype=dw_dtype, device=grad.device)
-        size = lib.smx_grouped_linear_by_weights_workspace(rows, v, k, n)
+        size = _weights_room(rows, v, k, n)
         room = _workspace(size, grad)
         check(lib.smx_grouped_linear_by_weights(grad.data_ptr(), gs, x.data_ptr(), xs, code, plan, rows, v, k, n,
                                                 _DTYPES[dw_dtype], dw.data_ptr(), k, n * k, _at(room), size, stream))
@@ -758,7 +763,7 @@ def integer_linear(x, w, dtype=None):
     current = _stream(device)
     n = w.shape[0]
     out = x.new_empty((m, n)) if dtype is None else x.new_empty((m, n), dtype=dtype)
-    size = lib.smx_integer_linear_workspace(m, n, k)
+    size = _integer_room(m, n, k)
     room = _workspace(size, x)
     check(lib.smx_integer_linear(x.data_ptr(), stride, code, w.values.data_ptr(), w.scales.data_ptr(), m, n, k, out_code,
                                  out.data_ptr(), n, _at(room), size, current))
