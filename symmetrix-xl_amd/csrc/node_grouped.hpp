@@ -298,7 +298,7 @@ __device__ __forceinline__ void put_tile(const W& w, const acc4 (&acc)[MF][NF], 
 // Rows of 16-bit values that go to LDS by themselves: BM x BN outputs a workgroup, in steps of 64 values of the summed axis.  While one is
 // multiplied, the one after it arrives, over the tile's end into the next tile.
 //
-// 8192 cubed bf16 in 829 us, 1,327 TFLOP/s (a library's product 1,197): a tile of 256 has 2,050 cycles of matrix instructions a step and as
+// 8192 cubed bf16 in 829 us, 1,327 TFLOP/s (a library's product 1,197), the matrix pipe busy 65% of it: a tile of 256 has 2,050 cycles of matrix instructions a step and as
 // many of LDS (192 KB of fragments, 64 KB that arrive), which overlap as far as each fragment is read one ahead of its use.  Steps
 // of 32 with up to five places in LDS, asked for two to four ahead, were slower everywhere (2,048 x 2,048 x 2,048 of two types:
 // 39.4 and 33.9 us): it is not the memory's latency that is waited for.
@@ -533,6 +533,10 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : BM + BN > 12
 // Rows at any alignment, and FP32 ones, which become three bf16 parts on the way: through registers, where a step waits while the one
 // before is multiplied.  Steps are of 64 16-bit or 32 FP32 values; one place in LDS, so that several workgroups share a unit and
 // one brings a step to LDS while another multiplies.
+//
+// FP32: x = x1 + x2 + x3 in bf16, each the rest's nearest, and the six products of parts whose orders of size add up to four at most;
+// what is left out is below 2^-24 of |x||w|.  8,192 x 4,096 x 4,096 in 1,410 us, 195 TFLOP/s (a library's FP32 product 153): the
+// matrix pipe is busy 53% of it, the rest goes to the parts (3.7 vector instructions for each matrix one) and to the one place in LDS.
 template <class T, class O, Way WAY, bool ALIGNED, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, BM == 128 ? 2 : 4) k_grouped_held(Grouped<T, O> p) {
     constexpr Lie LA = WAY == Way::ByWeights ? Lie::Columns : Lie::Rows, LB = WAY == Way::Forward ? Lie::Rows : Lie::Columns;
@@ -747,7 +751,7 @@ __global__ void __launch_bounds__(64 * WM * WN, BM == 128 ? 2 : 4) k_grouped_hel
 }
 
 // The sums of kinds whose rows are cut: rows of workgroups take these kinds in turn and join their runs in order, four neighbouring
-// values a lane.
+// values a lane.  Bytes of the parts bound it: 59 runs of 256 x 512 (31 MB) in 9.9 us.
 template <class O>
 __global__ void __launch_bounds__(256) k_grouped_join(Grouped<O, O> p) {
     const int kinds = p.kinds, lane = threadIdx.x % 64;
@@ -790,6 +794,8 @@ __global__ void __launch_bounds__(256) k_grouped_join(Grouped<O, O> p) {
 }
 
 // Up to 16 rows of a kind: 16 NF outputs a workgroup, for kinds of few rows, whose weights are read once for all of them.
+// KS waves share the summed axis.  The weights' bytes bound it: one row, 2,048 x 4,096 of bf16, 5.8 us (2.9 TB/s, the launch among it);
+// 147 rows of 32 kinds, 1,024 x 2,048 of f16 (134 MB, partly in the last cache), 22.6 us, 5.9 TB/s.
 template <class T, class O, bool DIRECT, int NF, int KS>
 __global__ void __launch_bounds__(64 * KS) k_grouped_rows(Grouped<T, O> p) {
     __shared__ FewRoom<T, NF, KS> room;
