@@ -128,13 +128,17 @@ struct Integers {
     int tiles_m, tiles_n;
 };
 
+// 2^17 products of -128 by itself, which no row brought to integers here has, are the one sum past 2^31 - 1: as -2^31, which no other
+// sum is.
+__device__ __forceinline__ float sum_of(int v) { return v == INT32_MIN ? 0x1p31f : static_cast<float>(v); }
+
 template <class O>
 __device__ __forceinline__ void store_scaled(const Integers<O>& p, int i, int j, i32x4 v, float a) {
     if (i >= p.m) return;
     O* const at = p.out + i * p.out_stride + j;
     float o[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) o[q] = static_cast<float>(v[q]) * a * (j + q < p.n ? p.bs[j + q] : 0.0f);
+    for (int q = 0; q < 4; ++q) o[q] = sum_of(v[q]) * a * (j + q < p.n ? p.bs[j + q] : 0.0f);
     if (j + 4 <= p.n) {
         Pack<O, 4> w;
 #pragma unroll

@@ -131,6 +131,17 @@ def test_longest_sums_are_exact(m):
     assert (got == -float(k * 127 * 127)).all()
 
 
+@pytest.mark.parametrize("m", [3, 100])
+def test_integers_of_another_making(m):
+    """Values down to -128, which rows brought to integers do not reach: the largest sum is 2^31."""
+    k = 1 << 17
+    a, b = (ops.IntegerValues(torch.full((rows, k), -128, dtype=torch.int8, device="cuda"), torch.ones(rows, device="cuda"), (rows, k))
+            for rows in (m, 20))
+    assert (ops.integer_product(a, b) == 2.0 ** 31).all()
+    b.values[:] = 127
+    assert (ops.integer_product(a, b) == -float(k * 128 * 127)).all()
+
+
 def test_finer_than_blocks(gen):
     """What the form is for: rows of normal values, a quarter of the 8-bit blocks' error."""
     x, w = torch.randn(512, 1024, generator=gen, device="cuda"), torch.randn(256, 1024, generator=gen, device="cuda")
