@@ -588,6 +588,8 @@ def grouped_linear_gradient(grad, x, w, groups, dtype=None):
 
 def _packed(t):
     """Whether t's values fill one piece of memory, in whatever order of its axes."""
+    if t.layout is not torch.strided:
+        return False
     if t.is_contiguous():
         return True
     at = 1
@@ -608,7 +610,7 @@ def _table(tensors, name):
     try:
         codes = array.array("i", map(_DTYPES.__getitem__, map(_dtypes_of, tensors)))
         packed = all(map(_T.is_contiguous, tensors))
-    except (KeyError, RuntimeError):
+    except (AttributeError, KeyError, RuntimeError, TypeError):
         raise ValueError("%s must be dense float32, bfloat16 or float16 tensors" % name) from None
     devices = set(map(_T.get_device, tensors))
     if len(devices) != 1:
@@ -654,7 +656,8 @@ def clip_gradients(tensors, max_norm, scale=1.0, out=None):
     """Brings ``tensors`` to a norm of ``max_norm`` at most: each becomes ``tensor * scale * min(1, max_norm / norm)``, in place or
     in ``out`` (tensors of as many values each, in the same order, of any of the types).  The norm before it, ``scale`` times the 2-norm of all values
     (``scale`` of gradients whose loss was scaled, 1 / the loss's), is returned as a float32 scalar on
-    their device; nothing waits for it.  Changed tensors do not ask for gradients themselves."""
+    their device; nothing waits for it.  Changed tensors do not ask for gradients themselves, and a graph that kept one refuses to go
+    back through it."""
     tensors = _listed(tensors, "tensors")
     at, counts, codes, device, packed = _table(tensors, "tensors")
     to, to_codes = at, codes
@@ -675,6 +678,7 @@ def clip_gradients(tensors, max_norm, scale=1.0, out=None):
         raise ValueError("tensors that are changed must not ask for gradients themselves: detach them")
     stream = _stream(device)
     norm, room, size = _norm_room(tensors[0])
+    torch.autograd.graph.increment_version(tensors if out is None else out)
     check(lib.smx_clip_gradients(_of(at), _of(counts), _of(codes), len(tensors), max_norm, scale, _of(to), _of(to_codes),
                                  norm.data_ptr(), room.data_ptr(), size, stream))
     return norm

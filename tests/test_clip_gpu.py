@@ -142,3 +142,26 @@ def test_beyond_32_bits(gen):
     assert ops.gradient_norm([t]).item() == 4.0
     ops.clip_gradients([t], 2.0)
     assert t[-3:].tolist() == [1.0] * 3 and t[0] == 1.0 and t[1 << 31] == 0.0
+
+
+def test_a_graph_notices_clipping(gen):
+    """A tensor that a graph kept is not the one that it kept any more: going back through it is refused, as after torch's own
+    changes in place."""
+    w, g = torch.ones(50, device="cuda", requires_grad=True), torch.randn(50, generator=gen, device="cuda")
+    for out in (None, [torch.empty_like(g)]):
+        kept = g if out is None else out[0]
+        y = (w * kept).sum()
+        ops.gradient_norm([kept])
+        y.backward(retain_graph=True)
+        ops.clip_gradients([g], 0.5, out=out)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+
+
+def test_lists_with_gaps(gen):
+    """A parameter without a gradient has None, which is no tensor."""
+    t = torch.randn(50, generator=gen, device="cuda")
+    for call in (ops.gradient_norm, lambda ts: ops.clip_gradients(ts, 1.0), lambda ts: ops.clip_gradients([t, t], 1.0, out=ts)):
+        for bad in (None, 1.0, t.double(), t.to_sparse()):
+            with pytest.raises(ValueError, match="must be dense float32|must fill their memory"):
+                call([t.clone(), bad])
