@@ -71,7 +71,7 @@ __device__ __forceinline__ Sums<N> sum_before(const Sums<N>& of, unsigned long l
 // leave room for more and shorter loops).  ONE: one workgroup, nothing was counted.
 //
 // Latency bounds it: reads of the counts, one scan over the kinds for offsets, present kinds and tiles of three sizes together, a round
-// of ballots, and the stores.  135 rows of 10 kinds in 6.5 us, 131,071 of 1,009 in 13.9 us (1.5 MB of rows and order).
+// of ballots, and the stores.  135 rows of 89 kinds in 6.5 us, 131,071 of 1,009 in 13.9 us (1.5 MB of rows and order).
 template <class I, int BITS, bool ONE>
 __global__ void __launch_bounds__(kThreads) k_group_place(const I* __restrict__ types, i64 rows, int kinds, i64 tile,
                                                           const int* __restrict__ counts, int* __restrict__ plan) {
