@@ -535,8 +535,9 @@ __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : BM + BN > 12
 // one brings a step to LDS while another multiplies.
 //
 // FP32: x = x1 + x2 + x3 in bf16, each the rest's nearest, and the six products of parts whose orders of size add up to four at most;
-// what is left out is below 2^-24 of |x||w|.  8,192 x 4,096 x 4,096 in 1,410 us, 195 TFLOP/s (a library's FP32 product 153): the
+// what is left out is below 2^-24 of |x||w|.  8,192 x 4,096 x 4,096 in 1,393 us, 197 TFLOP/s (a library's FP32 product 153): the
 // matrix pipe is busy 53% of it, the rest goes to the parts (3.7 vector instructions for each matrix one) and to the one place in LDS.
+// Forming the parts between the last products of the step before took 1,500 us; three workgroups a unit spill (2,344).
 template <class T, class O, Way WAY, bool ALIGNED, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, BM == 128 ? 2 : 4) k_grouped_held(Grouped<T, O> p) {
     constexpr Lie LA = WAY == Way::ByWeights ? Lie::Columns : Lie::Rows, LB = WAY == Way::Forward ? Lie::Rows : Lie::Columns;
@@ -703,7 +704,7 @@ __global__ void __launch_bounds__(64 * WM * WN, BM == 128 ? 2 : 4) k_grouped_hel
             }
             if (more) load();
             if constexpr (SPLIT) {
-                // two columns of fragments at a time, so that the registers are those of three workgroups a unit
+                // two columns of fragments at a time, so that the registers are those of two workgroups a unit
                 constexpr int kAtOnce = NF < 2 ? NF : 2;
 #pragma unroll
                 for (int g0 = 0; g0 < NF; g0 += kAtOnce) {
