@@ -8,7 +8,7 @@
 // well: a scale of its own last place would move quotients that lie next to ties.
 //
 // Sums are of 32-bit integers (v_mfma_i32_16x16x64_i8) and exact up to 2^17 terms (2^17 * 127^2 < 2^31); a product is rounded
-// when its sum becomes FP32 and at each scale, by 2^-24 each, and to the output's type.
+// when its sum becomes FP32 and at each scale (the smaller one first), by 2^-24 each, and to the output's type.
 #include <cmath>
 
 #include "node_tiles.hpp"
@@ -132,13 +132,21 @@ struct Integers {
 // sum is.
 __device__ __forceinline__ float sum_of(int v) { return v == INT32_MIN ? 0x1p31f : static_cast<float>(v); }
 
+// A sum by both scales, by the one of smaller magnitude first: the sum is a whole number, so that nothing is below FP32's normal numbers
+// before the second, and only what is beyond FP32 in the end is beyond it after the first (a row next to FP32's largest number, through
+// small weights).  A scale that is NaN stays one.
+__device__ __forceinline__ float by_scales(int v, float a, float b) {
+    const bool first = __builtin_fabsf(a) < __builtin_fabsf(b);
+    return sum_of(v) * (first ? a : b) * (first ? b : a);
+}
+
 template <class O>
 __device__ __forceinline__ void store_scaled(const Integers<O>& p, int i, int j, i32x4 v, float a) {
     if (i >= p.m) return;
     O* const at = p.out + i * p.out_stride + j;
     float o[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) o[q] = sum_of(v[q]) * a * (j + q < p.n ? p.bs[j + q] : 0.0f);
+    for (int q = 0; q < 4; ++q) o[q] = by_scales(v[q], a, j + q < p.n ? p.bs[j + q] : 0.0f);
     if (j + 4 <= p.n) {
         Pack<O, 4> w;
 #pragma unroll
