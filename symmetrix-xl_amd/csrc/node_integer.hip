@@ -71,9 +71,10 @@ __global__ void __launch_bounds__(256) k_quantize_integers(const T* __restrict__
                 look(held[q]);
             }
         } else {
-            for (int c = 8 * lane; c < cols; c += 8 * LANES) {
-                Eight<T> e = load_pack(row, c, cols);
-                settle(e, c, cols);
+            // (columns are counted without a sign: the step past the last one of 2^31 - 513 is past 2^31 too)
+            for (unsigned c = 8 * lane; c < static_cast<unsigned>(cols); c += 8 * LANES) {
+                Eight<T> e = load_pack(row, static_cast<int>(c), cols);
+                settle(e, static_cast<int>(c), cols);
                 look(e);
             }
         }
@@ -108,10 +109,10 @@ __global__ void __launch_bounds__(256) k_quantize_integers(const T* __restrict__
                 if (c < pitch) put(held[q], c);
             }
         } else {
-            for (int c = 8 * lane; c < pitch; c += 8 * LANES) {
-                Eight<T> e = load_pack(row, c, cols);
-                settle(e, c, cols);
-                put(e, c);
+            for (unsigned c = 8 * lane; c < pitch; c += 8 * LANES) {
+                Eight<T> e = load_pack(row, static_cast<int>(c), cols);
+                settle(e, static_cast<int>(c), cols);
+                put(e, static_cast<int>(c));
             }
         }
     }
