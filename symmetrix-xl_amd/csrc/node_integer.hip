@@ -452,6 +452,19 @@ Integers<O> integers_of(const std::int8_t* a, const float* as, const std::int8_t
     return p;
 }
 
+// f(q) for columns of p that one launch of few rows takes: it has 512 threads for each 16, and a launch fewer than 2^32.
+constexpr i64 kColumnsOnce = 1 << 26;
+
+template <class O, class F>
+void each_slice(const Integers<O>& p, F&& f) {
+    for (i64 j = 0; j < p.n; j += kColumnsOnce) {
+        Integers<O> q = p;
+        q.b += j * p.pitch, q.bs += j, q.out += j;
+        q.n = static_cast<int>(p.n - j < kColumnsOnce ? p.n - j : kColumnsOnce);
+        f(q);
+    }
+}
+
 template <class O>
 void launch_product(const std::int8_t* a, const float* as, const std::int8_t* b, const float* bs, i64 m, i64 n, i64 k, O* out,
                     i64 out_stride, hipStream_t stream) {
@@ -463,8 +476,10 @@ void launch_product(const std::int8_t* a, const float* as, const std::int8_t* b,
     }
     Integers<O> p = integers_of(a, as, b, bs, m, n, k, out, out_stride);
     if (m <= kFewRows) {
-        k_integer_rows<O, 1, 8><<<blocks_for(n, 16), 512, 0, stream>>>(p);
-        SMX_LAUNCH_CHECK("k_integer_rows");
+        each_slice(p, [&](const Integers<O>& q) {
+            k_integer_rows<O, 1, 8><<<blocks_for(q.n, 16), 512, 0, stream>>>(q);
+            SMX_LAUNCH_CHECK("k_integer_rows");
+        });
         return;
     }
     const i64 t = tile_for(m, n), tiles_m = (m + t - 1) / t, tiles_n = (n + t - 1) / t;
@@ -543,10 +558,12 @@ int32_t smx_integer_linear(const void* x, int64_t x_stride, int32_t dtype, const
                 with_dtype(out_dtype, [&](auto o) {
                     using T = decltype(t);
                     using O = decltype(o);
-                    k_integer_raw<T, O, 8><<<blocks_for(n, 16), 512, 0, static_cast<hipStream_t>(stream)>>>(
-                        integers_of<O>(nullptr, nullptr, w_values, w_scales, m, n, k, static_cast<O*>(out), out_stride),
-                        static_cast<const T*>(x), x_stride);
-                    SMX_LAUNCH_CHECK("k_integer_raw");
+                    const auto p = integers_of<O>(nullptr, nullptr, w_values, w_scales, m, n, k, static_cast<O*>(out), out_stride);
+                    each_slice(p, [&](const Integers<O>& q) {
+                        k_integer_raw<T, O, 8><<<blocks_for(q.n, 16), 512, 0, static_cast<hipStream_t>(stream)>>>(
+                            q, static_cast<const T*>(x), x_stride);
+                        SMX_LAUNCH_CHECK("k_integer_raw");
+                    });
                 });
             });
             return;
