@@ -58,15 +58,16 @@ Cut cut_rows(Way way, i64 rows, i64 kinds, i64 n, i64 inner, bool direct, bool s
     Cut c{128, direct, 0, 0, 0};
     const i64 k = kinds < rows ? kinds : rows;
     if (way == Way::Forward && rows <= k * kFewRows) {
-        const i64 units = (kinds + 1 < rows ? kinds + 1 : rows) + rows / 16;
-        if (units * ((n + 15) / 16) < (1LL << 31)) {
-            // Columns and waves of a workgroup: 64 where that still makes two a unit, and the waves such that each has eight steps or more, of
-            // which four are under way (147 rows of 32 types, 1,024 x 2,048: 22.4 us at 64 and 2, 25.7 at 64 and 4, 48.6 at 16 and
-            // 8; 64 of 8, 4,096 squared FP32: 162, 114 and 118; one row, 2,048 x 4,096: 10.4, 10.1 and 8.2, 7.7 at 16 and 4).
-            const i64 steps = ceil_of(inner * (split ? 4 : 2), kStepBytes);
-            c.tile = 16, c.units = static_cast<int>(units);
-            c.columns = units * ceil_of(n, 64) >= 2 * kComputeUnits ? 64 : 16;
-            c.waves = (c.columns == 64 ? 2 : 4) * (steps >= 64 ? 2 : 1);
+        // Columns and waves of a workgroup: 64 where that still makes two a unit, and the waves such that each has eight steps or more, of
+        // which four are under way (147 rows of 32 types, 1,024 x 2,048: 22.4 us at 64 and 2, 25.7 at 64 and 4, 48.6 at 16 and
+        // 8; 64 of 8, 4,096 squared FP32: 162, 114 and 118; one row, 2,048 x 4,096: 10.4, 10.1 and 8.2, 7.7 at 16 and 4).
+        const i64 units = (kinds + 1 < rows ? kinds + 1 : rows) + rows / 16, steps = ceil_of(inner * (split ? 4 : 2), kStepBytes);
+        c.units = static_cast<int>(units);
+        c.columns = units * ceil_of(n, 64) >= 2 * kComputeUnits ? 64 : 16;
+        c.waves = (c.columns == 64 ? 2 : 4) * (steps >= 64 ? 2 : 1);
+        // (a launch has fewer than 2^32 threads; the tiles' are as many as the card holds)
+        if (units * ceil_of(n, c.columns) * 64 * c.waves < (1LL << 32)) {
+            c.tile = 16;
             return c;
         }
     }
