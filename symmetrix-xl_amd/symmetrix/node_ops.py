@@ -678,9 +678,10 @@ def clip_gradients(tensors, max_norm, scale=1.0, out=None):
         raise ValueError("tensors that are changed must not ask for gradients themselves: detach them")
     stream = _stream(device)
     norm, room, size = _norm_room(tensors[0])
-    torch.autograd.graph.increment_version(tensors if out is None else out)
     check(lib.smx_clip_gradients(_of(at), _of(counts), _of(codes), len(tensors), max_norm, scale, _of(to), _of(to_codes),
                                  norm.data_ptr(), room.data_ptr(), size, stream))
+    # (a refused call has changed nothing)
+    torch.autograd.graph.increment_version(tensors if out is None else out)
     return norm
 
 
