@@ -600,6 +600,11 @@ def _packed(t):
     return True
 
 
+def _axes(t):
+    """The sizes and strides of t's axes, of those along which there is anything to step."""
+    return [(n, s) for n, s in zip(t.shape, t.stride()) if n > 1]
+
+
 _dtypes_of, _needs_grad = operator.attrgetter("dtype"), operator.attrgetter("requires_grad")
 _T = torch.Tensor
 
@@ -671,7 +676,7 @@ def clip_gradients(tensors, max_norm, scale=1.0, out=None):
         if to_counts != counts:
             raise ValueError("out must have the tensors' shapes")
         # (contiguous ones of as many values hold them in one order)
-        if not (packed and to_packed) and any(a.shape != b.shape or a.stride() != b.stride() for a, b in zip(tensors, out)
+        if not (packed and to_packed) and any(_axes(a) != _axes(b) for a, b in zip(tensors, out)
                                               if not (a.is_contiguous() and b.is_contiguous())):
             raise ValueError("out must have the tensors' shapes and strides")
     if any(map(_needs_grad, tensors if out is None else out)):

@@ -24,3 +24,20 @@ def test_refused_calls_change_no_version(on_device):
         with pytest.raises(ValueError, match=text):
             call()
     assert a._version == b._version == 0
+
+
+def test_outputs_in_the_tensors_order(monkeypatch):
+    """An axis of one value has any stride: what counts is the order of the values."""
+    calls = []
+    monkeypatch.setattr(node_ops, "_stream", lambda device: calls.append(device) or 0)
+    monkeypatch.setattr(node_ops.lib, "smx_clip_gradients", lambda *args: 0)
+    turned = torch.ones(4, 1, 3).transpose(0, 2)  # [3][1][4], strides 1, 3, 3
+    other = torch.empty_strided((3, 1, 4), (1, 77, 3))
+    assert not turned.is_contiguous() and turned.stride() != other.stride()
+    for to in (other, torch.empty_strided((3, 4), (1, 3)), torch.empty_strided((1, 3, 4), (5, 1, 3))):
+        node_ops.clip_gradients([turned], 1.0, out=[to])
+    assert len(calls) == 3
+    for bad in (torch.ones(3, 1, 4), torch.ones(12), torch.ones(4, 3).t().contiguous()):
+        with pytest.raises(ValueError, match="strides"):
+            node_ops.clip_gradients([turned], 1.0, out=[bad])
+    assert len(calls) == 3
