@@ -77,7 +77,7 @@ Cut cut_rows(Way way, i64 rows, i64 kinds, i64 n, i64 inner, bool direct, bool s
 }
 
 // The weights' gradient of m x n a kind: the tile, the units of rows that the card holds at once, and the least run, so that no more
-// than two rounds are cut (run_of): 0 where that is all rows.
+// than two rounds are cut (run_of): 0 where none can be.
 struct Runs {
     int tile;
     i64 round, least, slots;
@@ -103,7 +103,9 @@ Runs runs_for(i64 rows, i64 kinds, i64 m, i64 n, bool largest) {
         }
         if (cost < least) {
             least = cost;
-            best = {t, round, run < rows ? run : 0, run < rows ? 2 * (rows / run + 1) : 0};
+            // (where a type's tiles fill the card, run_of cuts none: two rounds less one type are no more than one unit)
+            const bool cut = round > 1 && run < rows;
+            best = {t, round, cut ? run : 0, cut ? 2 * (rows / run + 1) : 0};
         }
     }
     return best;
