@@ -223,8 +223,7 @@ SMX_API int64_t smx_integer_stride(int64_t cols);
 SMX_API int32_t smx_integer_quantize(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int64_t cols, int8_t* values,
                                      float* scales, void* stream);
 /* out[i][j] = a_scales[i] b_scales[j] sum over k of a[i][k] b[j][k], a [m][k] and b [n][k] as above, k <= 2^17: the sum is exact and
- * is rounded when it becomes FP32, at either scale (the one of smaller magnitude first: a product that is a number of FP32 is one), and to
- * `dtype`. */
+ * is rounded when it becomes FP32, at either scale (so that a product that is a number of FP32 is one), and to `dtype`. */
 SMX_API int32_t smx_integer_product(const int8_t* a_values, const float* a_scales, const int8_t* b_values, const float* b_scales,
                                     int64_t m, int64_t n, int64_t k, int32_t dtype, void* out, int64_t out_stride, void* stream);
 /* The same with a = x [m][k] of `dtype`, brought to integers within the call; out is out_dtype. */

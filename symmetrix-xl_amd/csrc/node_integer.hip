@@ -8,7 +8,7 @@
 // well: a scale of its own last place would move quotients that lie next to ties.
 //
 // Sums are of 32-bit integers (v_mfma_i32_16x16x64_i8) and exact up to 2^17 terms (2^17 * 127^2 < 2^31); a product is rounded
-// when its sum becomes FP32 and at each scale (the smaller one first), by 2^-24 each, and to the output's type.
+// when its sum becomes FP32 and at each scale, by 2^-24 each, and to the output's type.
 #include <cmath>
 
 #include "node_tiles.hpp"
@@ -133,11 +133,11 @@ struct Integers {
 // sum is.
 __device__ __forceinline__ float sum_of(int v) { return v == INT32_MIN ? 0x1p31f : static_cast<float>(v); }
 
-// A sum by both scales, by the one of smaller magnitude first: the sum is a whole number, so that nothing is below FP32's normal numbers
-// before the second, and only what is beyond FP32 in the end is beyond it after the first (a row next to FP32's largest number, through
-// small weights).  A scale that is NaN stays one.
+// A sum by both scales, by the row's first.  A row next to FP32's largest number, whose scale may take the sum beyond FP32 though small
+// weights bring the product back, has the other's first: beyond FP32 after that is only what is so in the end.  (Neither takes
+// the sum, a whole number, below FP32's normal numbers.)
 __device__ __forceinline__ float by_scales(int v, float a, float b) {
-    const bool first = __builtin_fabsf(a) < __builtin_fabsf(b);
+    const bool first = __builtin_fabsf(a) < 0x1p90f;
     return sum_of(v) * (first ? a : b) * (first ? b : a);
 }
 
