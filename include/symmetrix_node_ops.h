@@ -166,9 +166,11 @@ SMX_API int32_t smx_block_linear(const void* x, int64_t x_stride, int32_t dtype,
 
 /* A plan of `rows` rows by their kind, types[t] in [0, num_types) (int32, or int64 when types_are_64bit); a row of another
  * type is masked.  The plan is device memory (16-byte aligned, smx_group_plan_bytes of it), an input of the products below for
- * the same rows and num_types (with a plan of others they write nothing).  As int32 it holds from byte 16 on the offsets, num_types + 1 of them (of the sorted rows of
- * type z the first is offsets[z] and the one past the last offsets[z + 1]), and from byte smx_group_plan_order on the rows
- * in order: by type, of one type as they come, the masked ones last.  Up to 2^30 rows and 4,096 types. */
+ * the same rows and num_types.  What it is of is known to the device alone: with a plan of others the products return SMX_OK and
+ * write nothing, so an output keeps what it held.  As int32 the plan holds from byte 16 on the offsets, num_types + 1 of them (of
+ * the sorted rows of type z the first is offsets[z] and the one past the last offsets[z + 1]), and from byte
+ * smx_group_plan_order on the rows in order: by type, of one type as they come, the masked ones last.  Up to 2^30 rows and
+ * 4,096 types. */
 SMX_API int64_t smx_group_plan_bytes(int64_t rows, int64_t num_types);
 SMX_API int64_t smx_group_plan_order(int64_t num_types);
 SMX_API int64_t smx_group_rows_workspace(int64_t rows, int64_t num_types);
@@ -177,9 +179,9 @@ SMX_API int32_t smx_group_rows(const void* types, int32_t types_are_64bit, int64
 
 /* out[t] = w[z] x[t] with z the type of row t and w [num_types][outputs][inputs] (w_stride between rows, w_type_stride
  * between types, in values); the rows of masked t are zeros.  Values are `dtype`, out is out_dtype: that or FP32.  Products of FP32
- * values are formed of three bf16 parts of each, to FP32's precision (2^-24 of a product; parts below 2^-126 count as zero, so a
- * value below 2^-102 is off by up to 2^-126).  An infinity or NaN makes the outputs infinite or NaN that it is a term of, and no others.  inputs, outputs
- * <= 2^24. */
+ * values are formed of three bf16 parts of each, to FP32's precision (2^-24 of a product; parts are multiples of 2^-133, so a
+ * value below 2^-110 is off by up to 2^-134).  An infinity or NaN makes the outputs infinite or NaN that it is a term of, and no
+ * others.  inputs, outputs <= 2^24. */
 SMX_API int32_t smx_grouped_linear(const void* x, int64_t x_stride, int32_t dtype, const void* w, int64_t w_stride,
                                    int64_t w_type_stride, const void* plan, int64_t rows, int64_t num_types, int64_t inputs,
                                    int64_t outputs, int32_t out_dtype, void* out, int64_t out_stride, void* stream);
@@ -206,9 +208,10 @@ SMX_API int64_t smx_gradient_norm_workspace(void);
 SMX_API int32_t smx_gradient_norm(const void* const* tensors, const int64_t* counts, const int32_t* dtypes, int64_t num_tensors,
                                   float scale, float* norm, void* workspace, int64_t workspace_bytes, void* stream);
 /* The same, and out[i] = tensors[i] * scale * min(1, max_norm / norm) in out_dtypes[i]: out[i] may be tensors[i] where its type
- * is the same; outputs overlap nothing else.  The factor is FP32, from the norm in FP64.  A norm that is infinite
- * makes every finite value zero and the others NaN, one that is NaN makes all NaN: look at norm.  With a factor of one, values in place
- * are left as they are. */
+ * is the same; outputs overlap nothing else.  The factor is from the norm in FP64 and rounded to FP32's 24 bits
+ * whatever its size, and an output is rounded once more, and to its type; a factor of one changes no value.  A norm that is infinite
+ * makes every finite value zero and the others NaN (a max_norm that is infinite too clips nothing), one that is NaN makes all NaN: look
+ * at norm. */
 SMX_API int32_t smx_clip_gradients(const void* const* tensors, const int64_t* counts, const int32_t* dtypes, int64_t num_tensors,
                                    float max_norm, float scale, void* const* out, const int32_t* out_dtypes, float* norm,
                                    void* workspace, int64_t workspace_bytes, void* stream);
@@ -217,8 +220,8 @@ SMX_API int32_t smx_clip_gradients(const void* const* tensors, const int64_t* co
 
 /* A matrix [rows][cols] in 8-bit integers: values [rows][smx_integer_stride(cols)] (cols rounded up to 128, the rest zeros; 16-byte
  * aligned) and an FP32 scale for each row.  A row's scale is the FP32 product of its largest magnitude and the
- * FP32 number next to 1/127 (0x1.020408p-7), at least 2^-126, and a value the whole number nearest to the exact quotient by the scale, ties to even.  A row with an
- * infinity or NaN has the scale NaN and zeros. */
+ * FP32 number next to 1/127 (0x1.020408p-7), at least 2^-126, and a value the whole number nearest to the exact quotient by the
+ * scale, ties to even.  A row with an infinity or NaN has the scale NaN and zeros. */
 SMX_API int64_t smx_integer_stride(int64_t cols);
 SMX_API int32_t smx_integer_quantize(const void* x, int64_t x_stride, int32_t dtype, int64_t rows, int64_t cols, int8_t* values,
                                      float* scales, void* stream);

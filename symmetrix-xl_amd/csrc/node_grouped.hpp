@@ -298,10 +298,10 @@ __device__ __forceinline__ void put_tile(const W& w, const acc4 (&acc)[MF][NF], 
 // Rows of 16-bit values that go to LDS by themselves: BM x BN outputs a workgroup, in steps of 64 values of the summed axis.  While one is
 // multiplied, the one after it arrives, over the tile's end into the next tile.
 //
-// 8192 cubed bf16 in 829 us, 1,327 TFLOP/s (a library's product 1,197), the matrix pipe busy 65% of it: a tile of 256 has 2,050 cycles of matrix instructions a step and as
-// many of LDS (192 KB of fragments, 64 KB that arrive), which overlap as far as each fragment is read one ahead of its use.  Steps
-// of 32 with up to five places in LDS, asked for two to four ahead, were slower everywhere (2,048 x 2,048 x 2,048 of two types:
-// 39.4 and 33.9 us): it is not the memory's latency that is waited for.
+// 8192 cubed bf16 in 829 us, 1,327 TFLOP/s (a library's product 1,197), the matrix pipe busy 65% of it: a tile of 256 has 2,050
+// cycles of matrix instructions a step and as many of LDS (192 KB of fragments, 64 KB that arrive), which overlap as far as each
+// fragment is read one ahead of its use.  Steps of 32 with up to five places in LDS, asked for two to four ahead, were slower
+// everywhere (2,048 x 2,048 x 2,048 of two types: 39.4 and 33.9 us): it is not the memory's latency that is waited for.
 template <class T, class O, Way WAY, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(64 * WM * WN, BM + BN > 256 ? 1 : BM + BN > 128 ? 2 : 4) k_grouped_tiles(Grouped<T, O> p) {
     static_assert(sizeof(T) == 2);
@@ -794,9 +794,10 @@ __global__ void __launch_bounds__(256) k_grouped_join(Grouped<O, O> p) {
     }
 }
 
-// Up to 16 rows of a kind: 16 NF outputs a workgroup, for kinds of few rows, whose weights are read once for all of them.
-// KS waves share the summed axis.  The weights' bytes bound it: one row, 2,048 x 4,096 of bf16, 5.8 us (2.9 TB/s, the launch among it);
-// 147 rows of 32 kinds, 1,024 x 2,048 of f16 (134 MB, partly in the last cache), 22.6 us, 5.9 TB/s.
+// Up to 16 rows of a kind: 16 NF outputs a workgroup, which reads their weights once for its rows; a kind of more rows has them
+// read, from the caches mostly, for each 16.  KS waves share the summed axis.  The weights' bytes bound it: one row, 2,048 x 4,096
+// of bf16, 5.8 us (2.9 TB/s, the launch among it); 147 rows of 32 kinds, 1,024 x 2,048 of f16 (134 MB, partly in the last cache),
+// 22.6 us, 5.9 TB/s.
 template <class T, class O, bool DIRECT, int NF, int KS>
 __global__ void __launch_bounds__(64 * KS) k_grouped_rows(Grouped<T, O> p) {
     __shared__ FewRoom<T, NF, KS> room;

@@ -50,7 +50,9 @@ __device__ __forceinline__ void fetch(const void* at, unsigned lds) {
 // f(0), ..., f(N - 1) with the number as a constant
 template <int N, class F>
 __device__ __forceinline__ void each_of(F&& f) {
-    [&]<int... I>(std::integer_sequence<int, I...>) __attribute__((always_inline)) { (f(std::integral_constant<int, I>{}), ...); }(std::make_integer_sequence<int, N>{});
+    [&]<int... I>(std::integer_sequence<int, I...>) __attribute__((always_inline)) {
+        (f(std::integral_constant<int, I>{}), ...);
+    }(std::make_integer_sequence<int, N>{});
 }
 __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 

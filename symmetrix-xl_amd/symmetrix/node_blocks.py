@@ -157,8 +157,9 @@ def _energies(h, readout, shift, types, there):
 
 class NodeBlocks(torch.nn.Module):
     """Per-atom energies of ``types`` [atoms] and ``descriptors`` [atoms][descriptors].  Rows are
-    ``dtype``; parameters are float32.  With ``by_species`` a block's weights are a matrix for each type (up to 4,096 types).  An atom whose type is outside [0, num_types) is masked, as in
-    ``node_ops.embed``: its energy is zero, its descriptors are not looked at and nothing is learned from it."""
+    ``dtype``; parameters are float32.  With ``by_species`` a block's weights are a matrix for each type (up to 4,096 types).
+    An atom whose type is outside [0, num_types) is masked, as in ``node_ops.embed``: its energy is zero, its descriptors are
+    not looked at and nothing is learned from it."""
 
     def __init__(self, num_types, num_descriptors, channels=128, blocks=2, dtype=torch.float32, eps=1e-6, by_species=False):
         super().__init__()

@@ -610,8 +610,8 @@ _T = torch.Tensor
 
 
 def _table(tensors, name):
-    """(addresses, counts, type codes, device, whether all are contiguous) of tensors, for the length of a call.  One pass of a built-in over all of
-    them for each: a loop over them in Python took longer than the kernels for a small head's."""
+    """(addresses, counts, type codes, device, whether all are contiguous) of tensors, for the length of a call.  One pass of a
+    built-in over all of them for each: a loop over them in Python took longer than the kernels for a small head's."""
     try:
         codes = array.array("i", map(_DTYPES.__getitem__, map(_dtypes_of, tensors)))
         packed = all(map(_T.is_contiguous, tensors))
@@ -659,10 +659,10 @@ def gradient_norm(tensors, scale=1.0):
 
 def clip_gradients(tensors, max_norm, scale=1.0, out=None):
     """Brings ``tensors`` to a norm of ``max_norm`` at most: each becomes ``tensor * scale * min(1, max_norm / norm)``, in place or
-    in ``out`` (tensors of as many values each, in the same order, of any of the types).  The norm before it, ``scale`` times the 2-norm of all values
-    (``scale`` of gradients whose loss was scaled, 1 / the loss's), is returned as a float32 scalar on
-    their device; nothing waits for it.  Changed tensors do not ask for gradients themselves, and a graph that kept one refuses to go
-    back through it."""
+    in ``out`` (tensors of as many values each, in the same order, of any of the types).  The norm before it, ``scale`` times the
+    2-norm of all values (``scale`` of gradients whose loss was scaled, 1 / the loss's), is returned as a float32 scalar on
+    their device; nothing waits for it.  An infinite ``max_norm`` clips nothing, an infinite norm included.  Changed tensors do not ask
+    for gradients themselves, and a graph that kept one refuses to go back through it."""
     tensors = _listed(tensors, "tensors")
     at, counts, codes, device, packed = _table(tensors, "tensors")
     to, to_codes = at, codes
@@ -728,8 +728,8 @@ torch.serialization.add_safe_globals([IntegerValues])
 
 
 def quantize_integers(x):
-    """``x`` in 8-bit integers: for each row the whole numbers nearest to its values' quotients by a scale, a 127th of
-    the largest magnitude."""
+    """``x`` in 8-bit integers: for each row the whole numbers nearest to its values' quotients by a scale, the FP32 product of
+    the largest magnitude and the FP32 number next to 1/127."""
     code, r, c, stride = _rows(x, "x")
     stream = _stream(x.get_device())
     out = IntegerValues.__new__(IntegerValues)
